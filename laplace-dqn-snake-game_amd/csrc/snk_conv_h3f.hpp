@@ -456,8 +456,8 @@ __global__ __launch_bounds__(512) void conv_h3f_kernel(H3FArgs a_, int S) {
             const int e = min(u * 512 + tid, na4 - 1);
             const int sr = e / (hin2 * 4), pos = (e - sr * hin2 * 4) >> 2;
             const int j = pos / hin, i = pos - j * hin;
-            // channel pairs on v_pk_fma_f32 (two fp32 FMAs per lane and instruction; each
-            // channel's FMA chain and rounding are the scalar form's)
+            // channel pairs as two-vectors (two scalar FMAs each: packed fp32 is off, csrc/Makefile;
+            // each channel's FMA chain and rounding are the scalar form's)
             f32x2 acc01{b1r[0], b1r[1]}, acc23{b1r[2], b1r[3]};
 #pragma unroll
             for (int kk = 0; kk < 9; ++kk) {

@@ -1004,8 +1004,8 @@ static inline int64_t lap_act_lds_floats(const QLayout &L) {
 // Latency matters as much as bandwidth here (the episode tail runs a few live models per
 // launch): conv3's weights arrive by LDS-DMA through a ring of LAP_RING kernel offsets
 // (each weight fetched once, read from LDS by the 16 position groups that share it), and
-// Dense1's stream into a register ring three k-steps deep. The FMAs run on v_pk_fma_f32
-// (two accumulators per instruction) in the scalar form's per-accumulator order, so every
+// Dense1's stream into a register ring three k-steps deep. The FMAs are written
+// on two-vectors (two accumulators each) in the scalar form's per-accumulator order, so every
 // output is bit-identical to an fmaf chain over (kk, ci) / k ascending.
 __global__ __launch_bounds__(256) void lap_act_kernel(QLayout L, const float *__restrict__ W, int64_t ldw, BoardSrc src,
                                                       const uint8_t *__restrict__ fin, uint8_t *__restrict__ act,
