@@ -48,6 +48,10 @@ int snk_device_count(int32_t *n_out);
 int snk_set_device(int32_t device);
 /* hipStream_t to enqueue on; NULL restores the library's own stream */
 int snk_set_stream(void *hip_stream);
+/* this thread's stream selection, exchanged: given = 1 enqueues on hip_stream itself, NULL (HIP's
+ * default stream) included, given = 0 on the library's own stream; old_* receive the selection
+ * that was in force (for a host that lends its own stream to one call) */
+int snk_swap_stream(void *hip_stream, int32_t given, void **old_stream, int32_t *old_given);
 int snk_synchronize(void);
 /* GEMM arithmetic selection, process-wide (no reference counterpart: the
  * reference computes in Flux fp32). Every knob defaults to the production
@@ -222,6 +226,67 @@ int snk_dqn_apply_grad(snk_dqn m);
 /* loss_grad + apply_grad */
 int snk_dqn_update(snk_dqn m, snk_replay rb, const int64_t *idx_dev, int64_t B, double gamma,
                    double *loss_host);
+
+/* ---------------------------------------------------------------- AdamW
+ * Adam with decoupled weight decay over a list of tensors, beside the reference's RMSProp
+ * (utils.jl:429; no reference counterpart). Per element, t the 1-based step and s = grad_scale:
+ *   N = sqrt(sum (s g)^2) over all tensors, c = max_grad_norm / N when N is larger, else 1
+ *   g' = s c g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+ *   p = p - lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + weight_decay p)
+ * computed in fp32 (the norm in fp64), p rounded to its type once.
+ *
+ * State layout: every tensor starts on a multiple of 256 elements, in list order (its start is
+ * snk_adamw_layout's); the places between tensors hold zeros. state_bits 32: m and v are floats.
+ * state_bits 8: blocks of 256 consecutive places share two fp32 scales sm = max|m|, sv = max v;
+ *   m is an int8 a in -127..127, its value sm a|a| / 127^2, a rounded to nearest;
+ *   v is a uint8 b in 0..255, its value sv (b/255)^4, b one of its two neighbours with the chances
+ *   that keep the mean (v changes by 1 - b2 a step, less than half a code: rounding to nearest would
+ *   freeze it), at least 1 where v > 0. The 16 random bits of place i in step t are field i % 4 of
+ *   the counter RNG's hash of (seed, t, i / 4).
+ * The step count lives on the device, so a captured step advances at every replay. A handle's
+ * steps are ordered by the caller (one stream, or events), like every handle's. */
+typedef struct snk_adamw_s *snk_adamw;
+#define SNK_F32 0
+#define SNK_BF16 1
+#define SNK_F16 2
+typedef struct {
+    int32_t struct_size;   /* = sizeof(snk_adamw_cfg_t) = 64 */
+    int32_t param_dtype;   /* SNK_F32 / SNK_BF16 / SNK_F16 */
+    int32_t grad_dtype;    /* SNK_F32 / SNK_BF16 / SNK_F16 */
+    int32_t copy_dtype;    /* 16-bit type of the optional rounded copies of p, or -1 */
+    int32_t state_bits;    /* 32 or 8 */
+    float max_grad_norm;   /* 0: no norm; > 0 (may be inf): norm, clipping, and a step whose norm is
+                              not finite writes nothing and is not counted */
+    double beta1, beta2, eps;
+    uint64_t seed;         /* of the 8-bit rounding */
+    int64_t reserved;      /* 0 */
+} snk_adamw_cfg_t;
+#define SNK_ADAMW_M 0        /* float / int8 [total] */
+#define SNK_ADAMW_V 1        /* float / uint8 [total] */
+#define SNK_ADAMW_M_SCALE 2  /* float [total / 256], 8-bit states */
+#define SNK_ADAMW_V_SCALE 3
+#define SNK_ADAMW_NORM 4     /* float [1], the last step's N (max_grad_norm > 0) */
+/* n tensors of sizes_host[i] >= 0 elements; weight_decay_host[i] >= 0 each. Moments and step start at 0. */
+int snk_adamw_create(snk_adamw *out, int32_t n, const int64_t *sizes_host, const float *weight_decay_host,
+                     const snk_adamw_cfg_t *cfg);
+int snk_adamw_destroy(snk_adamw h);
+/* the tensors' device addresses, contiguous, element-aligned: params (updated), grads, and copies
+ * (NULL unless copy_dtype >= 0). Refused where a tensor that is written overlaps another one.
+ * Enqueued like any work, and kept: later steps (a captured one's replays too) use the last bind. */
+int snk_adamw_bind(snk_adamw h, void *const *params_dev, const void *const *grads_dev, void *const *copies_dev);
+int snk_adamw_step(snk_adamw h, float lr, float grad_scale);
+/* places in the state layout; starts_host (optional, n): each tensor's */
+int snk_adamw_layout(snk_adamw h, int64_t *total_out, int64_t *starts_host);
+int snk_adamw_state_ptr(snk_adamw h, int32_t which, void **dev_out, int64_t *bytes_out);
+/* the moments' values in the state layout, rounded to dtype; either pointer may be NULL */
+int snk_adamw_moments(snk_adamw h, int32_t dtype, void *m_dev, void *v_dev);
+int snk_adamw_get_steps(snk_adamw h, int64_t *steps_out);
+int snk_adamw_set_steps(snk_adamw h, int64_t steps);
+/* q_net is updated by AdamW from now on, in place of RMSProp: snk_dqn_apply_grad, snk_dqn_update
+ * and every trainer path. The layers' weights decay, their biases do not. cfg: param_dtype and
+ * grad_dtype SNK_F32, copy_dtype -1. The model owns the handle (out, optional): it is never
+ * passed to snk_adamw_destroy or snk_adamw_bind. cfg = NULL: back to RMSProp and its old state. */
+int snk_dqn_use_adamw(snk_dqn m, const snk_adamw_cfg_t *cfg, float lr, float weight_decay, snk_adamw *out);
 
 /* ---------------------------------------------------------------- trainer
  * The batched train! loop (utils.jl:420-494) over a batch of envs. */

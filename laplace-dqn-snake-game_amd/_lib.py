@@ -58,6 +58,7 @@ _PROTOS = {
     "snk_device_count": [P(i32)],
     "snk_set_device": [i32],
     "snk_set_stream": [vp],
+    "snk_swap_stream": [vp, i32, P(vp), P(i32)],
     "snk_synchronize": [],
     "snk_set_arith": [i32, i32],
     "snk_get_arith": [i32, P(i32)],
@@ -108,6 +109,16 @@ _PROTOS = {
     "snk_dqn_loss_grad_batch": [vp, vp, vp, vp, vp, vp, vp, i64, f64, P(f64)],
     "snk_dqn_apply_grad": [vp],
     "snk_dqn_update": [vp, vp, vp, i64, f64, P(f64)],
+    "snk_adamw_create": [P(vp), i32, vp, vp, vp],
+    "snk_adamw_destroy": [vp],
+    "snk_adamw_bind": [vp, vp, vp, vp],
+    "snk_adamw_step": [vp, f32, f32],
+    "snk_adamw_layout": [vp, P(i64), vp],
+    "snk_adamw_state_ptr": [vp, i32, P(vp), P(i64)],
+    "snk_adamw_moments": [vp, i32, vp, vp],
+    "snk_adamw_get_steps": [vp, P(i64)],
+    "snk_adamw_set_steps": [vp, i64],
+    "snk_dqn_use_adamw": [vp, vp, f32, f32, P(vp)],
     "snk_abi_sizes": [P(i64), P(i64)],
     "snk_trainer_create": [P(vp), vp, vp, vp, vp],
     "snk_trainer_destroy": [vp],
@@ -144,6 +155,10 @@ _PROTOS = {
     "snk_laplace_sample_params": [vp, vp, u64, i64, vp],
     "snk_laplace_sampling": [vp, vp, vp, i64, u64, i64, P(f32), P(i64), vp, vp],
 }
+
+# element types of the operators on caller's tensors
+SNK_F32, SNK_BF16, SNK_F16 = 0, 1, 2
+DTYPES = {"f32": SNK_F32, "bf16": SNK_BF16, "f16": SNK_F16}
 
 SNK_NET_Q = 0
 SNK_NET_TARGET = 1
@@ -342,6 +357,85 @@ class DeviceArray:
         if getattr(self, "ptr", None) and self.ptr.value and _lib is not None:
             _lib.snk_free(self.ptr)
             self.ptr = None
+
+
+class DeviceView:
+    """Device memory that another object owns (and that this view keeps alive). torch.as_tensor
+    reads and writes it in place."""
+
+    def __init__(self, ptr: int, n: int, dtype: str, owner):
+        self.ptr, self.shape, self.dtype, self.owner = vp(ptr), (int(n),), np.dtype(dtype), owner
+        self.nbytes = int(n) * self.dtype.itemsize
+
+    @property
+    def __cuda_array_interface__(self):
+        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr.value or 0, False), "version": 2}
+
+    def numpy(self) -> np.ndarray:
+        return view_numpy(self.ptr.value, self.shape, self.dtype)
+
+    def upload(self, a) -> None:
+        a = np.ascontiguousarray(a, self.dtype)
+        if a.shape != self.shape:
+            raise ValueError(f"upload: {a.shape} into {self.shape}")
+        call("snk_memcpy_h2d", self.ptr, ptr(a), self.nbytes)
+
+
+class Buffer:
+    """What an operator needs of a caller's device tensor: address, element type, element count,
+    shape, and the torch device it lives on (None: a DeviceArray or DeviceView)."""
+    __slots__ = ("ptr", "dtype", "size", "shape", "device")
+
+
+# numpy has no bfloat16: a uint16 DeviceArray holds its bits
+_NP_TYPES = {"float32": "f32", "float16": "f16", "uint16": "bf16", "int32": "i32", "uint8": "u8", "bool": "u8"}
+_TORCH_TYPES = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16", "torch.int32": "i32",
+                "torch.uint8": "u8", "torch.bool": "u8"}
+
+
+def device_buffer(x, what: str, contiguous: bool = True) -> Buffer:
+    b = Buffer()
+    if isinstance(x, (DeviceArray, DeviceView)):
+        b.ptr, b.shape, b.device = x.ptr.value, x.shape, None
+        kind = _NP_TYPES.get(x.dtype.name)
+        b.size = x.nbytes // x.dtype.itemsize
+    elif hasattr(x, "data_ptr"):
+        if not x.is_cuda:
+            raise ValueError(f"{what}: a tensor on {x.device}, not on the GPU")
+        if contiguous and not x.is_contiguous():
+            raise ValueError(f"{what}: a tensor that is not contiguous")
+        b.ptr, b.shape, b.device, b.size = x.data_ptr(), tuple(x.shape), x.device, x.numel()
+        kind = _TORCH_TYPES.get(str(x.dtype))
+    else:
+        raise TypeError(f"{what}: {type(x).__name__} is neither a DeviceArray nor a torch tensor")
+    if kind is None:
+        raise ValueError(f"{what}: elements of type {x.dtype}")
+    b.dtype = kind
+    return b
+
+
+def same_device(buffers) -> None:
+    """One call's tensors are all DeviceArrays or all on one torch device."""
+    if len({b.device for b in buffers}) > 1:
+        raise ValueError("the tensors of one call live on different devices, or mix DeviceArrays and torch tensors")
+
+
+def call_on(device, name: str, *args) -> None:
+    """call(), on torch's current stream of `device` where the tensors are torch's (their memory is
+    ordered by it); device None: on the library's stream."""
+    if device is None:
+        call(name, *args)
+        return
+    import torch
+    if torch.cuda.current_device() != device.index:
+        raise ValueError(f"the tensors live on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    lib = load()
+    old, given = vp(), i32(0)
+    check(lib.snk_swap_stream(torch.cuda.current_stream().cuda_stream, 1, C.byref(old), C.byref(given)))
+    try:
+        check(getattr(lib, name)(*args))
+    finally:
+        lib.snk_swap_stream(old, given, None, None)
 
 
 def view_numpy(dev_ptr: int, shape, dtype) -> np.ndarray:

@@ -446,6 +446,17 @@ void deep_free(snk_dqn_s *h) {
     h->deep = nullptr;
 }
 
+std::vector<int64_t> deep_sections(const snk_dqn_s *h) {
+    const DeepLayout &D = h->deep->D;
+    std::vector<int64_t> at;
+    for (int l = 0; l < 4; ++l) {
+        at.push_back(D.off_w[l]);
+        at.push_back(D.off_b[l]);
+    }
+    for (int64_t o : {D.off_d1w, D.off_d1b, D.off_d2w, D.off_d2b, D.P}) at.push_back(o);
+    return at;
+}
+
 int64_t deep_ws_gen(const snk_dqn_s *h) { return h->deep ? h->deep->gen : 0; }
 
 void deep_q_changed(snk_dqn_s *h, hipStream_t s) { deep_images(*h->deep, h->theta_q, h->deep->img_q, h->deep->img0_q, s); }
@@ -561,7 +572,10 @@ void deep_loss_grad(snk_dqn_s *h, const BoardSrc &s_src, const BoardSrc &sn_src,
 const double *deep_batch_losses(snk_dqn_s *h) { return h->deep->trn.loss; }
 
 void deep_apply(snk_dqn_s *h, const int64_t *counter, int64_t rate, hipStream_t s) {
-    rmsprop_launch(h->deep->D.P, h->theta_q, h->acc, h->grad, h->lr, h->rho, h->eps, s);
+    if (h->opt)
+        adamw_step(h->opt, h->opt_lr, 1.0f, s);
+    else
+        rmsprop_launch(h->deep->D.P, h->theta_q, h->acc, h->grad, h->lr, h->rho, h->eps, s);
     deep_q_changed(h, s);
     if (counter) deep_sync_target(h, counter, rate, s);
 }

@@ -143,6 +143,12 @@ void dqn_loss_grad(snk_dqn_s *h, const BoardSrc &s_src, const BoardSrc &sn_src, 
     qnet_backward(h->L, h->theta_q, s_src, B, h->trn, h->grad, h->slab, h->slab_cap, s, bo);
 }
 
+void dqn_adamw_apply(snk_dqn_s *h, const int64_t *counter, int64_t rate, hipStream_t s) {
+    adamw_step(h->opt, h->opt_lr, 1.0f, s);
+    dqn_q_changed(h, s);
+    if (counter) dqn_sync_target_launch(h, counter, rate, s);
+}
+
 UpdateTarget dqn_update_target(snk_dqn_s *h, const int64_t *counter, int64_t rate) {
     UpdateTarget u;
     u.theta = h->theta_q;
@@ -229,6 +235,7 @@ extern "C" int snk_dqn_destroy(snk_dqn h) {
     return guard([&] {
         if (!h) return;
         (void)hipStreamSynchronize(stream());
+        adamw_free(h->opt);
         deep_free(h);
         qwork_free(h->act);
         qwork_free(h->tgt);
@@ -480,8 +487,54 @@ extern "C" int snk_dqn_apply_grad(snk_dqn h) {
             deep_apply(h, nullptr, 1, stream());
             return;
         }
+        if (h->opt) {
+            dqn_adamw_apply(h, nullptr, 1, stream());
+            return;
+        }
         const UpdateTarget u = dqn_update_target(h, nullptr, 1);   // RMSProp + forward image, one pass
         grad_update_launch(h->L, nullptr, h->grad, &u, stream());
+    });
+}
+
+extern "C" int snk_dqn_use_adamw(snk_dqn h, const snk_adamw_cfg_t *cfg, float lr, float weight_decay, snk_adamw *out) {
+    return guard([&] {
+        SNK_CHECK(h, SNK_ERR_INVALID, "NULL argument");
+        snk_adamw fresh = nullptr;
+        hipStream_t s = stream();
+        if (cfg) {
+            SNK_CHECK(cfg->param_dtype == SNK_F32 && cfg->grad_dtype == SNK_F32 && cfg->copy_dtype == -1, SNK_ERR_INVALID,
+                      "use_adamw: the model's parameters and gradient are fp32, without copies");
+            SNK_CHECK(lr >= 0 && lr < INFINITY, SNK_ERR_INVALID, "use_adamw: lr %g", lr);
+            const QLayout &L = h->L;
+            const std::vector<int64_t> at =
+                h->deep ? deep_sections(h)
+                        : std::vector<int64_t>{L.off_w1, L.off_b1, L.off_w2, L.off_b2, L.off_w3, L.off_b3, L.off_d1w,
+                                               L.off_d1b, L.off_d2w, L.off_d2b, L.P};
+            std::vector<int64_t> size;
+            std::vector<float> wd;
+            std::vector<void *> p;
+            std::vector<const void *> g;
+            for (size_t i = 0; i + 1 < at.size(); ++i) {
+                size.push_back(at[i + 1] - at[i]);
+                wd.push_back(i % 2 ? 0.0f : weight_decay);   // biases do not decay
+                p.push_back(h->theta_q + at[i]);
+                g.push_back(h->grad + at[i]);
+            }
+            fresh = adamw_create((int32_t)size.size(), size.data(), wd.data(), cfg);
+            try {
+                adamw_bind(fresh, p.data(), g.data(), nullptr, s);
+            } catch (...) {
+                adamw_free(fresh);
+                throw;
+            }
+            adamw_set_owned(fresh);
+        }
+        (void)hipStreamSynchronize(s);
+        adamw_free(h->opt);
+        h->opt = fresh;
+        h->opt_lr = lr;
+        ++h->slab_gen;   // trainer graphs captured with the other optimizer are dropped
+        if (out) *out = fresh;
     });
 }
 

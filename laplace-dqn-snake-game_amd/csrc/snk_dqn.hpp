@@ -1,5 +1,8 @@
 // snk_dqn.hpp — DQNModel handle internals shared by snk_dqn.hip / snk_trainer.hip
 #pragma once
+#include <vector>
+
+#include "snk_optim.hpp"
 #include "snk_qnet.hpp"
 
 namespace snk {
@@ -36,6 +39,9 @@ struct snk_dqn_s {
     uint8_t *jact = nullptr;
     // snk_dqn_create_deep: the deeper bf16 net; L then holds its head offsets and P only
     snk::DeepNet *deep = nullptr;
+    // snk_dqn_use_adamw: updates by AdamW (owned) instead of RMSProp
+    snk_adamw opt = nullptr;
+    float opt_lr = 0.0f;
 };
 
 namespace snk {
@@ -56,6 +62,8 @@ void dqn_loss_grad(snk_dqn_s *h, const BoardSrc &s_src, const BoardSrc &sn_src, 
                    double gamma, hipStream_t s, const LossOpts &o = LossOpts{});
 // RMSProp + forward image (+ target copy when *counter % rate == 0) of an already finished gradient
 UpdateTarget dqn_update_target(snk_dqn_s *h, const int64_t *counter, int64_t rate);
+// the same with h->opt: AdamW, weight images, target copy
+void dqn_adamw_apply(snk_dqn_s *h, const int64_t *counter, int64_t rate, hipStream_t s);
 void dqn_sync_target_launch(snk_dqn_s *h, const int64_t *counter, int64_t rate, hipStream_t s);
 void dqn_permute(snk_dqn_s *h, const float *src, float *dst, bool to_packed, hipStream_t s);
 // q_net parameters changed: rebuild its forward weight image
@@ -75,7 +83,9 @@ const float *deep_forward(snk_dqn_s *h, int32_t which, const BoardSrc &src, int6
 void deep_loss_grad(snk_dqn_s *h, const BoardSrc &s_src, const BoardSrc &sn_src, const HeadArgs &meta, int64_t B,
                     double gamma, hipStream_t s, bool loss_mean);
 const double *deep_batch_losses(snk_dqn_s *h);
-// RMSProp on the finished gradient, weight images, update_target_net! when *counter % rate == 0
+// starts of the packed vector's sections (layer weights and biases in turn), then P
+std::vector<int64_t> deep_sections(const snk_dqn_s *h);
+// RMSProp or AdamW on the finished gradient, weight images, update_target_net! when *counter % rate == 0
 void deep_apply(snk_dqn_s *h, const int64_t *counter, int64_t rate, hipStream_t s);
 
 // generation of every buffer a captured trainer graph points into

@@ -198,6 +198,16 @@ extern "C" int snk_set_stream(void *s) {
     });
 }
 
+extern "C" int snk_swap_stream(void *s, int32_t given, void **old_stream, int32_t *old_given) {
+    return guard([&] {
+        SNK_CHECK(given == 0 || given == 1, SNK_ERR_INVALID, "given = %d is not 0 or 1", given);
+        if (old_stream) *old_stream = reinterpret_cast<void *>(g_user_stream);
+        if (old_given) *old_given = g_user_stream_set ? 1 : 0;
+        g_user_stream = given ? reinterpret_cast<hipStream_t>(s) : nullptr;
+        g_user_stream_set = given != 0;
+    });
+}
+
 extern "C" int snk_set_arith(int32_t knob, int32_t value) {
     return guard([&] {
         SNK_CHECK(knob >= 0 && knob < SNK_ARITH_COUNT, SNK_ERR_INVALID, "unknown arithmetic knob %d", knob);

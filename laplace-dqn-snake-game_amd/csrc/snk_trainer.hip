@@ -108,8 +108,9 @@ static void trainer_iteration(snk_trainer_s *h, bool learn, int n_upd, hipStream
     snk_dqn_s *q = h->dqn;
     const bool upd = learn && n_upd > 0;
     const uint64_t sseed = h->cfg.seed ^ 0x5A4D504C45ULL;
-    chain = chain && upd && !q->deep;
-    next_chain = next_chain && upd && !q->deep;
+    const bool plain_update = q->deep || q->opt;   // not grad_update_kernel's fused RMSProp pass
+    chain = chain && upd && !plain_update;
+    next_chain = next_chain && upd && !plain_update;
     split = split && chain && arith(SNK_ARITH_SPLIT_CHAIN);
     next_split = next_split && next_chain && arith(SNK_ARITH_SPLIT_CHAIN);
     // the first update's sample (counting the n transitions this step stores) rides in a
@@ -175,8 +176,8 @@ static void trainer_iteration(snk_trainer_s *h, bool learn, int n_upd, hipStream
     if (env_head) trace();   // the actions and Q-values the step computed
     if (!upd) return;
     for (int u = 0; u < n_upd; ++u) {
-        // update u > 0 of the non-deep net: drawn by update u-1's grad_update_kernel (PostUpdate::next)
-        if (u > 0 && q->deep) replay_launch_sample(R, h->B, sseed, 0, &h->stats->updates, h->idx, nullptr, s);
+        // update u > 0 of the fused update: drawn by update u-1's grad_update_kernel (PostUpdate::next)
+        if (u > 0 && plain_update) replay_launch_sample(R, h->B, sseed, 0, &h->stats->updates, h->idx, nullptr, s);
         HeadArgs m;
         m.idx = h->idx;
         m.rew = R.reward;
@@ -192,13 +193,19 @@ static void trainer_iteration(snk_trainer_s *h, bool learn, int n_upd, hipStream
                         h->loss_log, h->log_cap, &h->stats->updates, &h->stats->nb, &h->stats->epsilon,
                         h->cfg.decay, h->cfg.epsilon_end, h->ticket, SampleRider{}};
         const bool last = u + 1 == n_upd;
-        if (!q->deep && !last) {   // the next update's replay draw (utils.jl:442), count unchanged
+        if (!plain_update && !last) {   // the next update's replay draw (utils.jl:442), count unchanged
             post.next.count = R.count; post.next.cap = R.cap; post.next.pending = 0; post.next.batch = h->B;
             post.next.seed = sseed; post.next.out = h->idx;
         }
         if (q->deep) {   // the deeper bf16 net: finished gradient, [mean over ranks], RMSProp + images + target
             if (h->comm) comm_allreduce_mean(h->comm, q->grad, q->L.P, s);
             deep_apply(q, &h->stats->nb, h->cfg.target_update_rate, s);
+            post_update_kernel<<<1, 256, 0, s>>>(post);
+            launch_check("post_update_kernel");
+        } else if (q->opt) {   // AdamW: finished gradient, [mean over ranks], step + images + target
+            grad_update_launch(q->L, &pend, q->grad, nullptr, s);
+            if (h->comm) comm_allreduce_mean(h->comm, q->grad, q->L.P, s);
+            dqn_adamw_apply(q, &h->stats->nb, h->cfg.target_update_rate, s);
             post_update_kernel<<<1, 256, 0, s>>>(post);
             launch_check("post_update_kernel");
         } else {
@@ -449,11 +456,12 @@ extern "C" int snk_trainer_set_comm(snk_trainer h, snk_comm comm) {
         hipStream_t s = stream();
         snk_dqn_s *q = h->dqn;
         if (comm) {
-            // replicas start from rank 0's q_net; t_net = q_net; fresh RMSProp state
+            // replicas start from rank 0's q_net; t_net = q_net; fresh optimizer state
             comm_broadcast(comm, q->theta_q, q->L.P, 0, s);
             dqn_q_changed(q, s);
             dqn_sync_target_launch(q, nullptr, 1, s);
             SNK_HIP(hipMemsetAsync(q->acc, 0, q->L.P * sizeof(float), s));
+            if (q->opt) adamw_reset(q->opt, s);
         }
         SNK_HIP(hipStreamSynchronize(s));
         h->comm = comm;   // NULL: detach (updates local again)

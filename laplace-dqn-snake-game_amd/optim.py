@@ -1,0 +1,168 @@
+"""AdamW over a list of device tensors (snk_adamw_*), beside the model's own RMSProp.
+
+Tensors are DeviceArrays (float32, float16, or uint16 holding bfloat16) or contiguous torch GPU
+tensors; work on torch tensors runs on torch's current stream, work on DeviceArrays on the
+library's. One launch covers every tensor, so a step costs the same few launches for ten tensors
+or for hundreds.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _lib
+from ._lib import DeviceView, call, f32, i64, vp
+
+
+class AdamWCfg(C.Structure):
+    """snk_adamw_cfg_t (struct_size set by the constructor: the library's ABI guard)"""
+    _fields_ = [("struct_size", _lib.i32), ("param_dtype", _lib.i32), ("grad_dtype", _lib.i32), ("copy_dtype", _lib.i32),
+                ("state_bits", _lib.i32), ("max_grad_norm", f32), ("beta1", _lib.f64), ("beta2", _lib.f64),
+                ("eps", _lib.f64), ("seed", _lib.u64), ("reserved", i64)]
+
+    def __init__(self, *args, **kw):
+        super().__init__(C.sizeof(self), *args, **kw)
+
+
+def _same(buffers, what):
+    kinds = {b.dtype for b in buffers}
+    if len(kinds) != 1:
+        raise ValueError(f"AdamW: the {what} must share one element type, got {sorted(kinds)}")
+    return _lib.DTYPES[kinds.pop()]
+
+
+class _Handle:
+    """What a user's handle and a model's have in common."""
+
+    _device = None   # the torch device of the tensors, None for DeviceArrays
+    state_bits = 32
+
+    @property
+    def handle(self):
+        return self._h
+
+    def _call(self, name, *args):
+        _lib.call_on(self._device, name, *args)
+
+    @property
+    def steps(self) -> int:
+        """Steps taken (waits for the stream). A skipped step is not counted. Assign to resume."""
+        n = i64(0)
+        self._call("snk_adamw_get_steps", self._h, C.byref(n))
+        return n.value
+
+    @steps.setter
+    def steps(self, n: int) -> None:
+        self._call("snk_adamw_set_steps", self._h, int(n))
+
+    @property
+    def total(self) -> int:
+        """Places in the state layout: every tensor's size rounded up to 256."""
+        n = i64(0)
+        call("snk_adamw_layout", self._h, C.byref(n), None)
+        return n.value
+
+    @property
+    def starts(self) -> list[int]:
+        """Each tensor's first place in the state layout."""
+        n, out = i64(0), (i64 * self._n)()
+        call("snk_adamw_layout", self._h, C.byref(n), out)
+        return list(out)
+
+    def state(self) -> dict[str, DeviceView]:
+        """The state's own device buffers, for checkpoints: m and v (float32, or the int8 / uint8
+        codes with m_scale and v_scale, one a block of 256) and norm, the last step's gradient norm."""
+        names = [("m", 0, "i1" if self.state_bits == 8 else "f4"), ("v", 1, "u1" if self.state_bits == 8 else "f4")]
+        if self.state_bits == 8:
+            names += [("m_scale", 2, "f4"), ("v_scale", 3, "f4")]
+        out = {}
+        for name, which, dt in names + [("norm", 4, "f4")]:
+            p, n = vp(), i64(0)
+            call("snk_adamw_state_ptr", self._h, which, C.byref(p), C.byref(n))
+            out[name] = DeviceView(p.value, n.value // (1 if dt[1] == "1" else 4), dt, self)
+        return out
+
+    def moments(self, m=None, v=None) -> None:
+        """The moments' values, written into m and v: [total] arrays of one type, either may be None."""
+        bufs = [None if x is None else _lib.device_buffer(x, "moments") for x in (m, v)]
+        given = [b for b in bufs if b is not None]
+        if not given:
+            return
+        for b in given:
+            if b.size != self.total:
+                raise ValueError(f"moments: {b.size} elements for {self.total} places")
+        _lib.same_device(given)
+        _lib.call_on(given[0].device, "snk_adamw_moments", self._h, _same(given, "moments"),
+                     *[None if b is None else b.ptr for b in bufs])
+
+
+class AdamW(_Handle):
+    """AdamW(params, grads): params and grads are lists of equal lengths and sizes; they (and
+    copies) are kept alive and used at these addresses by every step until bind() names others.
+
+    weight_decay: one number, or one per tensor. state_bits: 32, or 8 (codes in blocks of 256 with
+    two fp32 scales each, v rounded stochastically with `seed`). max_grad_norm > 0 clips the global
+    gradient norm and skips a step whose norm is not finite. copies: 16-bit tensors that receive the
+    updated parameters too (fp32 master weights with bf16 working weights)."""
+
+    def __init__(self, params, grads, *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01,
+                 state_bits: int = 32, max_grad_norm: float = 0.0, copies=None, seed: int = 0):
+        ps, gs, cs = self._buffers(params, grads, copies)
+        n = len(ps)
+        wd = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+        if len(wd) != n:
+            raise ValueError(f"AdamW: {len(wd)} weight decays for {n} tensors")
+        self.lr, self.state_bits, self._n = float(lr), int(state_bits), n
+        self._sizes = [b.size for b in ps]
+        self._types = (_same(ps, "params"), _same(gs, "grads"), _same(cs, "copies") if cs else -1)
+        cfg = AdamWCfg(*self._types, self.state_bits, float(max_grad_norm), float(betas[0]), float(betas[1]), float(eps),
+                       int(seed), 0)
+        self._device = ps[0].device
+        h = vp()
+        self._call("snk_adamw_create", C.byref(h), n, (i64 * n)(*self._sizes), (f32 * n)(*wd), C.byref(cfg))
+        self._h = h
+        self._bind(ps, gs, cs, (params, grads, copies))
+
+    @staticmethod
+    def _buffers(params, grads, copies):
+        lists = [[_lib.device_buffer(x, "AdamW") for x in xs] for xs in (params, grads, copies or [])]
+        if not lists[0]:
+            raise ValueError("AdamW: no tensors")
+        for other in lists[1:] if copies else lists[1:2]:
+            if [b.size for b in other] != [b.size for b in lists[0]]:
+                raise ValueError("AdamW: params, grads (and copies) need the same sizes")
+        _lib.same_device([b for bufs in lists for b in bufs])
+        return lists
+
+    def _bind(self, ps, gs, cs, keep):
+        n = self._n
+        table = [(vp * n)(*[b.ptr for b in bufs]) if bufs else None for bufs in (ps, gs, cs)]
+        self._device = ps[0].device
+        self._call("snk_adamw_bind", self._h, *table)
+        self._keep = keep
+
+    def bind(self, params, grads, copies=None) -> None:
+        """Other addresses for the same tensors (new gradients, moved parameters)."""
+        ps, gs, cs = self._buffers(params, grads, copies)
+        if [b.size for b in ps] != self._sizes:
+            raise ValueError("AdamW.bind: the sizes are those of the constructor")
+        if (_same(ps, "params"), _same(gs, "grads"), _same(cs, "copies") if cs else -1) != self._types:
+            raise ValueError("AdamW.bind: the element types are those of the constructor")
+        self._bind(ps, gs, cs, (params, grads, copies))
+
+    def step(self, *, lr: float | None = None, grad_scale: float = 1.0) -> None:
+        """One step on the bound gradients times grad_scale (the inverse of a loss scale).
+        Enqueued; nothing waits for it."""
+        self._call("snk_adamw_step", self._h, self.lr if lr is None else lr, grad_scale)
+
+    def __del__(self):
+        if getattr(self, "_h", None) and _lib._lib is not None:
+            _lib._lib.snk_adamw_destroy(self._h)
+            self._h = None
+
+
+class ModelAdamW(_Handle):
+    """The AdamW state of a DQNModel (DQNModel.use_adamw). The model owns it and its apply_grad and
+    update step it; use_rmsprop or another use_adamw ends it, and its state()'s memory with it."""
+
+    def __init__(self, model, handle, lr, state_bits, n):
+        self._model, self._h, self.lr, self.state_bits, self._n = model, handle, float(lr), int(state_bits), int(n)

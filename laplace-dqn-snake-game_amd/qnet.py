@@ -8,11 +8,13 @@ vector loads unchanged (see tests/golden/vanilla_qnet_params.npy).
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 
 import numpy as np
 
 from . import _lib
 from ._lib import DeviceArray, call, ptr, vp
+from .optim import AdamWCfg, ModelAdamW
 
 
 def deep_nparams(board_size: int, n_frames: int) -> int:
@@ -44,6 +46,7 @@ class DQNModel:
         self.board_size, self.n_frames, self.n_actions = int(board_size), int(n_frames), 3
         self.lr, self.rho, self.eps = float(lr), float(rho), float(eps)
         self.deep = bool(deep)
+        self._adamw = None   # weak: the state object refers back to this model
         h = vp()
         call("snk_dqn_create_deep" if self.deep else "snk_dqn_create", C.byref(h), self.board_size, self.n_frames,
              self.lr, self.rho, self.eps, int(seed))
@@ -122,6 +125,29 @@ class DQNModel:
 
     def apply_grad(self) -> None:
         call("snk_dqn_apply_grad", self._h)
+
+    def use_adamw(self, *, lr: float = 5e-4, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
+                  state_bits: int = 32, max_grad_norm: float = 0.0, seed: int = 0) -> ModelAdamW:
+        """Update q_net by AdamW from now on instead of the reference's RMSProp (utils.jl:429):
+        apply_grad, update, and every Trainer on this model. Weights decay, biases do not."""
+        cfg = AdamWCfg(_lib.SNK_F32, _lib.SNK_F32, -1, int(state_bits), float(max_grad_norm), float(betas[0]),
+                       float(betas[1]), float(eps), int(seed), 0)
+        h = vp()
+        call("snk_dqn_use_adamw", self._h, C.byref(cfg), float(lr), float(weight_decay), C.byref(h))
+        self._end_adamw()
+        self._adamw = weakref.ref(opt := ModelAdamW(self, h, lr, state_bits, 12 if self.deep else 10))
+        return opt
+
+    def use_rmsprop(self) -> None:
+        """Back to RMSProp, with its state as it was left. Ends the life of use_adamw's state."""
+        call("snk_dqn_use_adamw", self._h, None, 0.0, 0.0, None)
+        self._end_adamw()
+
+    def _end_adamw(self) -> None:
+        old = self._adamw() if self._adamw else None
+        if old is not None:
+            old._h = None   # the library has freed it: later calls are refused
+        self._adamw = None
 
     def update(self, rpb, idx, B: int, gamma: float = 0.97) -> float:
         loss = C.c_double(0)

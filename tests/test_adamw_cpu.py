@@ -1,0 +1,91 @@
+"""AdamW's refusals that need no device, and its 64-bit reference against itself (CPU)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import adamw_ref
+import snake_amd
+from snake_amd import _lib
+from snake_amd.optim import AdamWCfg
+
+GOOD = dict(param_dtype=0, grad_dtype=0, copy_dtype=-1, state_bits=32, max_grad_norm=0.0, beta1=0.9, beta2=0.999,
+            eps=1e-8, seed=0, reserved=0)
+
+
+def _create(n=1, sizes=(8,), wd=(0.0,), cfg=None, **change):
+    c = AdamWCfg(*{**GOOD, **change}.values()) if cfg is None else cfg
+    h = _lib.vp()
+    st = snake_amd.load().snk_adamw_create(C.byref(h), n, (C.c_int64 * len(sizes))(*sizes), (C.c_float * len(wd))(*wd),
+                                           C.byref(c))
+    return st, snake_amd.load().snk_last_error().decode()
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(param_dtype=3), "type"), (dict(grad_dtype=-1), "type"), (dict(copy_dtype=0), "copy_dtype"),
+    (dict(state_bits=16), "state_bits"), (dict(beta1=1.0), "betas"), (dict(beta2=-0.1), "betas"),
+    (dict(beta1=float("nan")), "betas"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"), (dict(eps=float("inf")), "eps"),
+    (dict(max_grad_norm=-1.0), "max_grad_norm"), (dict(max_grad_norm=float("nan")), "max_grad_norm"),
+    (dict(reserved=1), "reserved"),
+])
+def test_bad_settings_are_refused(change, word):
+    st, msg = _create(**change)
+    assert st == _lib.SNK_ERR_INVALID and word in msg, msg
+
+
+def test_bad_calls_are_refused():
+    lib = snake_amd.load()
+    bad = AdamWCfg(*GOOD.values())
+    bad.struct_size = 60
+    st, msg = _create(cfg=bad)
+    assert st == _lib.SNK_ERR_INVALID and "struct_size" in msg
+    assert C.sizeof(AdamWCfg) == 64
+    assert _create(n=0)[0] == _lib.SNK_ERR_INVALID
+    assert lib.snk_adamw_create(None, 1, None, None, None) == _lib.SNK_ERR_INVALID
+    for name, args in (("snk_adamw_step", (None, 1.0, 1.0)), ("snk_adamw_bind", (None, None, None, None)),
+                       ("snk_adamw_moments", (None, 0, None, None)), ("snk_adamw_get_steps", (None, None)),
+                       ("snk_adamw_set_steps", (None, 1)), ("snk_adamw_layout", (None, None, None)),
+                       ("snk_adamw_state_ptr", (None, 0, None, None)), ("snk_dqn_use_adamw", (None, None, 0.0, 0.0, None))):
+        assert getattr(lib, name)(*args) == _lib.SNK_ERR_INVALID, name
+    assert lib.snk_adamw_destroy(None) == _lib.SNK_OK
+    assert lib.snk_swap_stream(None, 2, None, None) == _lib.SNK_ERR_INVALID
+
+
+def test_host_tensors_are_refused():
+    import torch
+    with pytest.raises(ValueError, match="GPU"):
+        snake_amd.AdamW([torch.zeros(4)], [torch.zeros(4)])
+    with pytest.raises(TypeError):
+        snake_amd.AdamW([np.zeros(4, np.float32)], [np.zeros(4, np.float32)])
+    with pytest.raises(ValueError, match="no tensors"):
+        snake_amd.AdamW([], [])
+
+
+def test_stream_selection_is_exchanged():
+    """snk_swap_stream keeps what snk_set_stream chose (no stream is used here)."""
+    lib = snake_amd.load()
+    old, given = _lib.vp(), C.c_int32(-1)
+    assert lib.snk_swap_stream(_lib.vp(1234), 1, C.byref(old), C.byref(given)) == 0
+    assert given.value == 0 and not old.value
+    assert lib.snk_swap_stream(old, given.value, C.byref(old), C.byref(given)) == 0
+    assert given.value == 1 and old.value == 1234
+    assert lib.snk_swap_stream(None, 0, C.byref(old), C.byref(given)) == 0 and given.value == 0
+
+
+def test_reference_codes_keep_the_mean():
+    """The 8-bit rounding of v is unbiased: over all 65,536 random values the mean of the two
+    neighbours' values is v to 2^-16 of their distance."""
+    part = np.array([1e-9, 1e-4, 0.013, 0.5, 0.97, 1.0])
+    low = np.minimum(np.floor(255 * part ** 0.25), 254)
+    lo, hi = (low / 255) ** 4, ((low + 1) / 255) ** 4
+    ups = np.ceil((part - lo) / (hi - lo) * 65536)   # the r in 0..65535 that go up
+    mean = lo + (hi - lo) * np.minimum(ups, 65536) / 65536
+    assert np.all(np.abs(mean - part) <= (hi - lo) / 65536 + 1e-15)
+
+
+def test_reference_bits_are_the_counter_rng():
+    import devrng
+    seed, t = 0xABCDEF0123, 17
+    got = adamw_ref.bits16(seed, t, 40)
+    for i in (0, 1, 5, 39):
+        assert got[i] == (devrng.rng_hash(seed, t, i // 4) >> (16 * (i % 4))) & 0xFFFF

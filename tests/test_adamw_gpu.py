@@ -1,0 +1,402 @@
+"""AdamW on the GPU against the 64-bit formula (adamw_ref: bounds that count fp32 roundings).
+
+Every step is checked from the state the device itself held before it, so that bounds do not
+accumulate; where a quantity is stored in fewer bits, half a step of that type is added.
+"""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import adamw_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+TT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SIZES = [1, 3, 255, 256, 257, 0, 4095, 4096, 4097, 12289, 2]
+
+
+def flat(tensors, sizes):
+    starts, total = ref.places(sizes)
+    out = np.zeros(total)
+    for x, at, s in zip(tensors, starts, sizes):
+        out[at:at + s] = x.double().cpu().numpy().reshape(-1)
+    return out
+
+
+def spread(values, sizes):
+    starts, total = ref.places(sizes)
+    out = np.zeros(total)
+    for x, at, s in zip(values, starts, sizes):
+        out[at:at + s] = x
+    return out
+
+
+def old_moments(opt):
+    st = {k: x.numpy() for k, x in opt.state().items()}
+    if opt.state_bits == 8:
+        return ref.m_values(st["m"], st["m_scale"]), ref.v_values(st["v"], st["v_scale"]), st
+    return st["m"].astype(np.float64), st["v"].astype(np.float64), st
+
+
+def views(sizes, dtype, gen, std, offset):
+    """Tensors cut out of one buffer with `offset` elements of canary before, between and after."""
+    buf = torch.full((sum(sizes) + offset * (len(sizes) + 1),), 7.0, dtype=dtype, device="cuda")
+    out, at = [], offset
+    for s in sizes:
+        buf[at:at + s] = (torch.randn(s, device="cuda", generator=gen) * std).to(dtype)
+        out.append(buf[at:at + s])
+        at += s + offset
+    return buf, out
+
+
+def canaries(buf, sizes, offset):
+    keep, at = torch.ones_like(buf, dtype=torch.bool), offset
+    for s in sizes:
+        keep[at:at + s] = False
+        at += s + offset
+    return bool((buf[keep] == 7.0).all())
+
+
+def check_step(opt, params, grads, sizes, wds, t, run, *, ptype, lr, b1, b2, eps, scale=1.0, max_norm=0.0, seed=0,
+               copies=None):
+    p, g = flat(params, sizes), flat(grads, sizes)
+    m, v, _ = old_moments(opt)
+    run()
+    want = ref.Step(p, g, m, v, t, lr=lr, b1=b1, b2=b2, eps=eps, wd=spread(wds, sizes), scale=scale, max_norm=max_norm,
+                    state_bits=opt.state_bits)
+    got = flat(params, sizes)
+    tol = want.ep + (ref.HALF[ptype] * (np.abs(want.p) + want.ep) + (2.0 ** -25 if ptype == "f16" else 0)
+                     if ptype != "f32" else 0)
+    assert np.all(np.abs(got - want.p) <= tol), float(np.max(np.abs(got - want.p) / np.maximum(tol, 1e-300)))
+    m2, v2, st = old_moments(opt)
+    if opt.state_bits == 8:
+        want.codes_ok(st["m"], st["m_scale"], st["v"], st["v_scale"], ref.bits16(seed, t, m.size))
+    else:
+        assert np.all(np.abs(m2 - want.m) <= want.em) and np.all(np.abs(v2 - want.v) <= want.ev)
+    if max_norm:
+        assert abs(float(st["norm"][0]) - want.norm) <= 4 * ref.U * want.norm
+    if copies is not None:
+        c = flat(copies, sizes)
+        assert np.all(np.abs(c - got) <= ref.HALF["bf16"] * np.abs(got))
+    assert opt.steps == t
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("ptype,gtype", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"),
+                                         ("f32", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_steps_against_the_formula(snk, bits, ptype, gtype, offset):
+    """Sizes around the block and chunk, aligned or not (offset 1: odd addresses), decay on some
+    tensors only; steps without, under and over the norm limit."""
+    gen = torch.Generator(device="cuda").manual_seed(bits + offset)
+    pbuf, params = views(SIZES, TT[ptype], gen, 0.1, offset)
+    gbuf, grads = views(SIZES, TT[gtype], gen, 0.02, offset)
+    wds = [0.0 if i % 3 else 0.1 for i in range(len(SIZES))]
+    hyper = dict(lr=1e-2, b1=0.9, b2=0.99, eps=1e-8)
+    for max_norm in (0.0, 1.0, 100.0):
+        opt = snk.AdamW(params, grads, lr=1e-2, betas=(0.9, 0.99), weight_decay=wds, state_bits=bits,
+                        max_grad_norm=max_norm, seed=99)
+        for t in (1, 2, 3):
+            for g in grads:
+                g.copy_((torch.randn(g.numel(), device="cuda", generator=gen) * 0.02 *
+                         (torch.rand(g.numel(), device="cuda", generator=gen) > 0.3)).to(g.dtype))
+            check_step(opt, params, grads, SIZES, wds, t, opt.step, ptype=ptype, max_norm=max_norm, seed=99, **hyper)
+    assert canaries(pbuf, SIZES, offset) and canaries(gbuf, SIZES, offset)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_wide_values(snk, bits):
+    """Gradients over 40 orders of magnitude inside one block, large steps counts, other betas."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    n = [1000]
+    p = [torch.randn(1000, device="cuda", generator=gen)]
+    g = [torch.randn(1000, device="cuda", generator=gen) * 10 ** (torch.rand(1000, device="cuda", generator=gen) * 24 - 18)]
+    opt = snk.AdamW(p, g, lr=1e-3, betas=(0.5, 0.9), eps=1e-6, weight_decay=0.0, state_bits=bits, seed=3)
+    opt.steps = 100000
+    for t in (100001, 100002, 100003):
+        check_step(opt, p, g, n, [0.0], t, opt.step, ptype="f32", lr=1e-3, b1=0.5, b2=0.9, eps=1e-6, seed=3)
+
+
+def test_scaled_gradients_and_copies(snk):
+    """fp32 master weights with bf16 copies; gradients of a loss scaled by 1024."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    sizes = [777, 4096, 5]
+    _, p = views(sizes, torch.float32, gen, 0.1, 3)
+    _, g = views(sizes, torch.float16, gen, 3.0, 1)
+    cbuf, c = views(sizes, torch.bfloat16, gen, 0.0, 1)
+    opt = snk.AdamW(p, g, lr=1e-2, weight_decay=0.01, max_grad_norm=0.05, copies=c)
+    for t in (1, 2):
+        check_step(opt, p, g, sizes, [0.01] * 3, t, lambda: opt.step(grad_scale=1 / 1024), ptype="f32", lr=1e-2, b1=0.9,
+                   b2=0.999, eps=1e-8, scale=1 / 1024, max_norm=0.05, copies=c)
+    assert canaries(cbuf, sizes, 1)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_step_with_no_finite_norm_is_skipped(snk, bits, bad):
+    p, g = torch.randn(5000, device="cuda"), torch.randn(5000, device="cuda")
+    opt = snk.AdamW([p], [g], state_bits=bits, max_grad_norm=float("inf"))
+    opt.step()
+    before = [p.clone(), *[torch.as_tensor(x, device="cuda").clone() for k, x in opt.state().items() if k != "norm"]]
+    assert opt.steps == 1
+    g[4321] = bad
+    opt.step()
+    after = [p, *[torch.as_tensor(x, device="cuda") for k, x in opt.state().items() if k != "norm"]]
+    assert opt.steps == 1 and all(torch.equal(a, b) for a, b in zip(before, after))
+    assert not np.isfinite(opt.state()["norm"].numpy()[0])
+    g[4321] = 0.5
+    opt.step()
+    assert opt.steps == 2 and not torch.equal(before[0], p)
+
+
+def test_many_tensors(snk):
+    """Over 128 tensors: the bind takes several launches, the step stays whole."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    sizes = [(i * 37) % 700 for i in range(300)]
+    _, p = views(sizes, torch.float32, gen, 0.1, 1)
+    _, g = views(sizes, torch.float32, gen, 0.1, 1)
+    wds = [0.01 * (i % 2) for i in range(300)]
+    opt = snk.AdamW(p, g, weight_decay=wds, max_grad_norm=1.0)
+    assert opt.starts == ref.places(sizes)[0] and opt.total == ref.places(sizes)[1]
+    for t in (1, 2):
+        check_step(opt, p, g, sizes, wds, t, opt.step, ptype="f32", lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, max_norm=1.0)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_equal_runs_are_equal_bit_for_bit(snk, bits):
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    p0, g = torch.randn(3_000_001, device="cuda", generator=gen), torch.randn(3_000_001, device="cuda", generator=gen)
+    out = []
+    for _ in range(2):
+        p = p0.clone()
+        opt = snk.AdamW([p], [g], state_bits=bits, max_grad_norm=1.0, seed=8)
+        for _ in range(3):
+            opt.step()
+        out.append([p, *[torch.as_tensor(x, device="cuda").clone() for x in opt.state().values()]])
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step(snk, bits):
+    """Replays of a captured step, with eager work and synchronisation between, equal eager steps."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    p0 = torch.randn(70_001, device="cuda", generator=gen)
+    gs = [torch.randn(70_001, device="cuda", generator=gen) for _ in range(5)]
+    runs = []
+    for captured in (False, True):
+        p, g = p0.clone(), torch.zeros_like(p0)
+        opt = snk.AdamW([p], [g], state_bits=bits, max_grad_norm=1.0, seed=1)
+        if captured:
+            graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.graph(graph, stream=side):
+                opt.step()
+        seen = []
+        for i, x in enumerate(gs):
+            g.copy_(x)
+            graph.replay() if captured else opt.step()
+            if i % 2:
+                torch.cuda.synchronize()
+            seen.append(p.clone())
+            p.mul_(0.999)
+        runs.append(seen)
+        assert opt.steps == 5
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_own_stream_and_device_arrays(snk):
+    """DeviceArrays work on the library's stream; torch tensors on torch's current one."""
+    rng = np.random.default_rng(0)
+    p0, g0 = rng.standard_normal(5000).astype(np.float32), rng.standard_normal(5000).astype(np.float32)
+    p, g = snk.DeviceArray.from_host(p0), snk.DeviceArray.from_host(g0)
+    opt = snk.AdamW([p], [g], lr=1e-2, weight_decay=0.1)
+    opt.step()
+    side = torch.cuda.Stream()
+    tp, tg = torch.from_numpy(p0).cuda(), torch.zeros(5000, device="cuda")
+    topt = snk.AdamW([tp], [tg], lr=1e-2, weight_decay=0.1)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)       # the gradient arrives late on the side stream
+        tg.copy_(torch.from_numpy(g0).pin_memory(), non_blocking=True)
+        topt.step()
+    side.synchronize()
+    assert np.array_equal(p.numpy(), tp.cpu().numpy())
+
+
+def test_rebinding(snk):
+    p = [torch.ones(300, device="cuda")]
+    a, b = [torch.full((300,), 1.0, device="cuda")], [torch.full((300,), -1.0, device="cuda")]
+    opt = snk.AdamW(p, a, lr=0.1, betas=(0.0, 0.0), weight_decay=0.0)
+    opt.step()
+    assert torch.allclose(p[0], torch.full_like(p[0], 0.9), rtol=0, atol=1e-6)
+    opt.bind(p, b)
+    opt.step()
+    assert torch.allclose(p[0], torch.full_like(p[0], 1.0), rtol=0, atol=1e-6)
+    with pytest.raises(ValueError):
+        opt.bind([torch.ones(301, device="cuda")], b)
+    with pytest.raises(ValueError):
+        opt.bind([x.half() for x in p], b)
+
+
+def test_overlapping_tensors_are_refused(snk):
+    x, g = torch.zeros(1000, device="cuda"), torch.zeros(1000, device="cuda")
+    for params, grads in (([x[:500], x[499:999]], [g[:500], g[500:1000]]), ([x, x], [g, g]), ([x[:500]], [x[499:999]])):
+        with pytest.raises(snk.SnakeHipError, match="overlaps"):
+            snk.AdamW(params, grads)
+    snk.AdamW([x[:500], x[500:]], [g[:500], g[:500]]).step()     # gradients may share memory
+    c = torch.zeros(1000, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(snk.SnakeHipError, match="overlaps"):
+        snk.AdamW([x[:500], x[500:]], [g[:500], g[500:]], copies=[c[:500], c[400:900]])
+    with pytest.raises(ValueError, match="contiguous"):
+        snk.AdamW([x[::2]], [g[:500]])
+    with pytest.raises(ValueError):
+        snk.AdamW([x], [g[:999]])
+    with pytest.raises(ValueError):
+        snk.AdamW([x, c], [g, g])
+
+
+def test_moments_values(snk):
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    p, g = torch.zeros(1000, device="cuda"), torch.randn(1000, device="cuda", generator=gen)
+    for bits in (32, 8):
+        opt = snk.AdamW([p], [g], state_bits=bits)
+        opt.step()
+        m, v, _ = old_moments(opt)
+        for dt in ("f32", "bf16", "f16"):
+            out = [torch.full((opt.total,), 9.0, dtype=TT[dt], device="cuda") for _ in range(2)]
+            opt.moments(*out)
+            for x, y in zip(out, (m, v)):
+                assert np.all(np.abs(x.double().cpu().numpy() - y) <= (ref.HALF[dt] + 4 * ref.U) * np.abs(y) + 2.0 ** -25 * (dt == "f16"))
+            opt.moments(out[0])
+        with pytest.raises(ValueError):
+            opt.moments(torch.zeros(7, device="cuda"))
+
+
+def test_rounding_keeps_the_mean_of_v(snk):
+    """v decays by 1 % a step with no gradient; nearest codes would never move. Over 400 blocks of
+    one pattern the mean stays within five standard deviations of the exact decay: one step's rounding
+    has at most a quarter of the squared code distance, (4 v / b)^2 / 4, as its variance."""
+    blocks, steps = 400, 30
+    g = torch.linspace(0.3, 1.0, 256, device="cuda").repeat(blocks)
+    p = torch.zeros_like(g)
+    opt = snk.AdamW([p], [g], lr=0.0, betas=(0.0, 0.99), weight_decay=0.0, state_bits=8, seed=11)
+    opt.step()
+    v = [torch.empty(opt.total, device="cuda") for _ in range(2)]
+    opt.moments(*v)
+    start = v[1].view(blocks, 256).double().mean(0)
+    g.zero_()
+    for _ in range(steps):
+        opt.step()
+    opt.moments(*v)
+    got = v[1].view(blocks, 256).double().mean(0)
+    want = start * 0.99 ** steps
+    b = 255 * (want / want.max()) ** 0.25
+    sd = (steps / blocks) ** 0.5 * 0.5 * 4 * start / b
+    assert torch.all((got - want).abs() <= 5 * sd + 1e-5 * want), ((got - want).abs() / sd).max()
+
+
+def test_offsets_past_32_bits(snk):
+    n = 2 ** 31 + 777
+    p = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    g = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    p[-1000:], g[-1000:] = 1.0, 0.5
+    p[:1000], g[:1000] = 1.0, -0.5
+    opt = snk.AdamW([p], [g], lr=0.25, betas=(0.0, 0.0), weight_decay=0.0, state_bits=8)
+    opt.step()
+    assert bool((p[-1000:] == 0.75).all()) and bool((p[:1000] == 1.25).all())
+    assert not bool(p[1000:-1000].any())
+
+
+# ------------------------------------------------------------------ the model's own update
+
+def _replay(snk, n=256, bs=12):
+    g = snk.SnakeGame(bs, 2, n_envs=n, autoreset=True)
+    rb = snk.ReplayBuffer(4096, board_size=bs, n_frames=2)
+    act = snk.DeviceArray(n, np.uint8)
+    for _ in range(8):
+        snk.synth_actions_dev(g, 5, act)
+        snk.step_indices_dev(g, act.ptr, replay=rb)
+    return g, rb
+
+
+@pytest.mark.parametrize("deep", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_model_updates(snk, deep, bits):
+    """apply_grad and update of a model on AdamW: parameters against the formula, weights decaying
+    and biases not, and the forward pass that of the updated parameters."""
+    _, rb = _replay(snk)
+    m = snk.DQNModel(12, 3, n_frames=2, seed=3, deep=deep)
+    start = m.get_params()
+    opt = m.use_adamw(lr=1e-3, weight_decay=0.1, state_bits=bits, max_grad_norm=1.0, seed=21)
+    perm = m.flux_index()
+    sizes = ([576, 32, 9216, 32, 18432, 64, 147456, 64, 49 * 4096, 64, 192, 3] if deep else
+             [288, 16, 4608, 32, 73728, 64, 49 * 4096, 64, 192, 3])
+    assert sum(sizes) == m.P
+    starts, total = ref.places(sizes)
+    assert opt.starts == starts and opt.total == total
+    ends = np.cumsum([0] + sizes)
+
+    def layout(flux):
+        packed = flux[perm].astype(np.float64)
+        return spread([packed[a:b] for a, b in zip(ends, ends[1:])], sizes)
+
+    wd = spread([0.1 if i % 2 == 0 else 0.0 for i in range(len(sizes))], sizes)
+    for t in (1, 2, 3):
+        idx, B = snk.sample(rb, seed=t)
+        p, (mo, vo, _) = layout(m.get_params()), old_moments(opt)
+        m.update(rb, idx, B)
+        want = ref.Step(p, layout(m.grad), mo, vo, t, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=wd, max_norm=1.0,
+                        state_bits=bits)
+        got = layout(m.get_params())
+        assert np.all(np.abs(got - want.p) <= want.ep)
+        assert opt.steps == t
+    x = np.random.default_rng(0).integers(-1, 3, size=(5, 2, 144)).astype(np.float32)
+    q = m(x)
+    m.set_params(m.get_params())          # rebuilds the forward images
+    assert np.array_equal(q, m(x)) and not np.array_equal(start, m.get_params())
+
+
+def test_model_back_to_rmsprop(snk):
+    _, rb = _replay(snk)
+    a, b = (snk.DQNModel(12, 3, n_frames=2, seed=3) for _ in range(2))
+    idx, B = snk.sample(rb, seed=1)
+    for m in (a, b):
+        m.update(rb, idx, B)
+    opt = a.use_adamw(lr=0.0)
+    with pytest.raises(snk.SnakeHipError, match="belongs"):
+        snk._lib.call("snk_adamw_step", opt.handle, 0.1, 1.0)
+    with pytest.raises(snk.SnakeHipError, match="belongs"):
+        snk._lib.call("snk_adamw_destroy", opt.handle)
+    a.use_rmsprop()
+    with pytest.raises(snk.SnakeHipError):
+        opt.steps
+    for m in (a, b):
+        m.update(rb, idx, B)
+    assert np.array_equal(a.get_params(), b.get_params())
+    assert np.array_equal(a.get_params(snk.SNK_NET_OPT_STATE), b.get_params(snk.SNK_NET_OPT_STATE))
+    with pytest.raises(snk.SnakeHipError):
+        a.use_adamw(lr=float("nan"))
+
+
+@pytest.mark.parametrize("deep", [False, True])
+def test_trainer_on_adamw(snk, deep):
+    """Captured training iterations equal eager ones bit for bit; two updates an iteration; the
+    optimizer may change between runs (graphs are captured again)."""
+    out = []
+    for graph in (True, False):
+        model = snk.DQNModel(12, 3, n_frames=2, seed=5, deep=deep)
+        opt = model.use_adamw(lr=1e-3, weight_decay=0.01, max_grad_norm=10.0, state_bits=8, seed=2)
+        tr = snk.Trainer(model=model, game=snk.SnakeGame(12, 2, n_envs=64, autoreset=True), capacity=2048,
+                         updates_per_iter=2, target_update_rate=4, seed=9, graph_unroll=4)
+        snk.fill_buffer_(tr, graph=graph)
+        tr.run(10, graph=graph)
+        assert opt.steps == 20 and tr.stats()["updates"] == 20
+        got = [model.get_params(), model.get_params(snk.SNK_NET_TARGET), tr.losses]
+        model.use_rmsprop()
+        tr.run(5, graph=graph)
+        got.append(model.get_params())
+        out.append(got)
+    assert all(np.array_equal(a, b) for a, b in zip(*out))
+    assert np.all(np.isfinite(out[0][0]))
