@@ -227,6 +227,45 @@ int snk_dqn_apply_grad(snk_dqn m);
 int snk_dqn_update(snk_dqn m, snk_replay rb, const int64_t *idx_dev, int64_t B, double gamma,
                    double *loss_host);
 
+/* ---------------------------------------------------------------- sampling
+ * One index a row from logits, beside epsilon_greedy (utils.jl:153-172; no reference counterpart):
+ * row x[0..n), allowed = not masked and not -inf, w_i = exp((x_i - max x) / temperature), the
+ * allowed entries in order: x descending, equal ones by lower index.
+ *   top_k   keeps the first top_k of the order (<= 0: all)
+ *   top_p   of those, i stays where the mass before it is < top_p times their mass (>= 1: all;
+ *           the first always stays)
+ *   min_p   of all, i stays where w_i >= min_p
+ * Of the entries that every filter keeps, with mass S, the answer is the smallest index i at which
+ * the sum of w_j over the kept j <= i is > u S; its probability is w_i / S. u in [0, 1) is given, one
+ * a row (outside, or NaN: the nearest end). temperature <= 0: the first entry of the order, with
+ * probability 1. No allowed entry: index -1, probability 0. An allowed NaN: -1 and NaN. Infinite
+ * entries share all the mass. What masked places hold does not matter.
+ * Masses are sums of 64-bit integers, units of 2^-(61 - ceil log2 n) of the largest weight but no
+ * finer than 2^-51: the order of the additions does not change the answer. */
+typedef struct {
+    int32_t struct_size;   /* = sizeof(snk_sample_cfg_t) = 56 */
+    int32_t dtype;         /* of the logits: SNK_F32 / SNK_BF16 / SNK_F16 */
+    float temperature;     /* >= 0, finite */
+    int32_t top_k;         /* >= 0 */
+    float top_p, min_p;    /* in [0, 1] */
+    /* per row in place of the numbers above, or NULL */
+    const float *temperature_dev;
+    const int32_t *top_k_dev;
+    const float *top_p_dev, *min_p_dev;
+} snk_sample_cfg_t;
+/* row r's logits start at logits_dev + r * ld elements, its mask (bytes, non-zero = forbidden; NULL:
+ * none) at mask_dev + r * ld_mask; ld, ld_mask >= n, or 0: one row for all. 1 <= n <= 2^24.
+ * idx_dev[rows]; prob_dev[rows] or NULL. ws_dev: snk_sample_workspace's bytes, 16-byte aligned, used
+ * during the call only: two calls in flight need two. */
+int snk_sample_workspace(int64_t rows, int64_t n, int64_t *bytes_out);
+int snk_sample_logits(const void *logits_dev, int64_t rows, int64_t n, int64_t ld, const uint8_t *mask_dev,
+                      int64_t ld_mask, const float *u_dev, const snk_sample_cfg_t *cfg, int32_t *idx_dev,
+                      float *prob_dev, void *ws_dev, int64_t ws_bytes);
+/* the softmax policy over every env's Q values: act_dev [n] action index, drawn with the counter
+ * RNG's u(seed, env, step) as epsilon_greedy draws its own; cfg: dtype SNK_F32, the per-row arrays
+ * may be given */
+int snk_dqn_act_sample(snk_dqn m, snk_env env, const snk_sample_cfg_t *cfg, uint64_t seed, uint8_t *act_dev);
+
 /* ---------------------------------------------------------------- AdamW
  * Adam with decoupled weight decay over a list of tensors, beside the reference's RMSProp
  * (utils.jl:429; no reference counterpart). Per element, t the 1-based step and s = grad_scale:

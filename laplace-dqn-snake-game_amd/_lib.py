@@ -109,6 +109,9 @@ _PROTOS = {
     "snk_dqn_loss_grad_batch": [vp, vp, vp, vp, vp, vp, vp, i64, f64, P(f64)],
     "snk_dqn_apply_grad": [vp],
     "snk_dqn_update": [vp, vp, vp, i64, f64, P(f64)],
+    "snk_sample_workspace": [i64, i64, P(i64)],
+    "snk_sample_logits": [vp, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, i64],
+    "snk_dqn_act_sample": [vp, vp, vp, u64, vp],
     "snk_adamw_create": [P(vp), i32, vp, vp, vp],
     "snk_adamw_destroy": [vp],
     "snk_adamw_bind": [vp, vp, vp, vp],

@@ -268,6 +268,15 @@ static float *which_buf(snk_dqn h, int32_t which) {
     return nullptr;
 }
 
+const float *snk::dqn_q_env(snk_dqn_s *h, int32_t which, snk_env env, hipStream_t s) {
+    const EnvDev &E = env_dev(env);
+    if (h->deep) return deep_forward(h, which, src_env(E), E.n, HEAD_Q, HeadArgs{}, s);
+    qwork_ensure(h->act, h->L, E.n, false);
+    qnet_forward(h->L, which_buf(h, which), which_wt(h, which), src_env(E), E.n, h->act, HEAD_Q, HeadArgs{}, s, -1,
+                 which_wtb(h, which));
+    return h->act.q;
+}
+
 extern "C" int snk_dqn_set_params(snk_dqn h, int32_t which, const float *flux_host) {
     return guard([&] {
         SNK_CHECK(h && flux_host, SNK_ERR_INVALID, "NULL argument");
@@ -334,15 +343,8 @@ extern "C" int snk_dqn_forward_env(snk_dqn h, int32_t which, snk_env env, float 
         const EnvDev &E = env_dev(env);
         SNK_CHECK(E.bs == h->L.bs && E.C == h->L.C, SNK_ERR_INVALID, "env/model geometry mismatch");
         hipStream_t s = stream();
-        if (h->deep) {
-            const float *q = deep_forward(h, which, src_env(E), E.n, HEAD_Q, HeadArgs{}, s);
-            SNK_HIP(hipMemcpyAsync(q_dev, q, E.n * 3 * sizeof(float), hipMemcpyDeviceToDevice, s));
-            return;
-        }
-        qwork_ensure(h->act, h->L, E.n, false);
-        qnet_forward(h->L, which_buf(h, which), which_wt(h, which), src_env(E), E.n, h->act, HEAD_Q, HeadArgs{}, s,
-                     -1, which_wtb(h, which));
-        SNK_HIP(hipMemcpyAsync(q_dev, h->act.q, E.n * 3 * sizeof(float), hipMemcpyDeviceToDevice, s));
+        const float *q = dqn_q_env(h, which, env, s);
+        SNK_HIP(hipMemcpyAsync(q_dev, q, E.n * 3 * sizeof(float), hipMemcpyDeviceToDevice, s));
     });
 }
 

@@ -54,6 +54,8 @@ void replay_launch_sample(const ReplayDev &d, int32_t batch, uint64_t seed, uint
 BoardSrc src_env(const EnvDev &E);
 BoardSrc src_replay(const ReplayDev &R, const int64_t *idx, int chan0);
 BoardSrc src_float(const QLayout &L, const float *x);
+// Q of every env's state, in the model's acting workspace [n][3]
+const float *dqn_q_env(snk_dqn_s *h, int32_t which, snk_env env, hipStream_t s);
 struct LossOpts {
     GradSlabs *defer = nullptr;      // leave K-split slabs and Dense2 to grad_update_launch
     bool loss_mean = true;           // reduce the per-sample losses into h->loss_dev here

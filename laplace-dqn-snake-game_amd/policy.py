@@ -1,0 +1,133 @@
+"""Sampling from logits (snk_sample_logits) and the softmax policy over a Q-net's values, beside
+epsilon_greedy (utils.jl:153-172).
+
+Tensors are DeviceArrays or torch GPU tensors as in optim.py.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from ._lib import DeviceArray, call, f32, i32, i64, vp
+
+
+class SampleCfg(C.Structure):
+    """snk_sample_cfg_t (struct_size set by the constructor: the library's ABI guard)"""
+    _fields_ = [("struct_size", i32), ("dtype", i32), ("temperature", f32), ("top_k", i32), ("top_p", f32), ("min_p", f32),
+                ("temperature_dev", vp), ("top_k_dev", vp), ("top_p_dev", vp), ("min_p_dev", vp)]
+
+    def __init__(self, *args, **kw):
+        super().__init__(C.sizeof(self), *args, **kw)
+
+
+def _rows_of(x, b, what):
+    """(rows, n, row stride in elements) of a 1-D or 2-D tensor whose rows are contiguous."""
+    if len(b.shape) not in (1, 2):
+        raise ValueError(f"{what}: {len(b.shape)} dimensions, expected [n] or [rows, n]")
+    if len(b.shape) == 1:
+        rows, n = 1, b.shape[0]
+    else:
+        rows, n = b.shape
+    if b.device is None:
+        return rows, n, n
+    st = x.stride()
+    if n > 1 and st[-1] != 1:
+        raise ValueError(f"{what}: the last dimension is not contiguous")
+    return rows, n, st[0] if rows > 1 else n
+
+
+def _setting(value, rows, kind, keep, what):
+    """(number, device address) of a setting given as a number or as one value per row."""
+    if isinstance(value, (int, float)):
+        return value, None
+    b = _lib.device_buffer(value, what)
+    if b.dtype != kind or b.size != rows:
+        raise ValueError(f"{what}: expected {rows} values of type {kind}, got {b.size} of {b.dtype}")
+    keep.append(b)
+    return (0 if kind == "i32" else 1.0), b.ptr
+
+
+def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None, out=None, prob=None,
+                  workspace=None):
+    """One index per row of logits [rows, n] (or [n]), drawn with the given u [rows] in [0, 1).
+
+    temperature, top_k, top_p and min_p (include/snakehip.h states the rules) are numbers or one
+    value per row (float32, top_k int32). mask: bytes or bools [rows, n], non-zero forbids. A torch
+    row stride of 0 (expand) shares one row. Returns out [rows] int32 (-1: nothing allowed), made
+    here if not given; prob [rows] float32, if given, receives the probabilities. workspace: a uint8
+    tensor of sample_workspace(rows, n) bytes, made here if not given; calls in flight at the same
+    time need one each."""
+    b = _lib.device_buffer(logits, "logits", contiguous=False)
+    rows, n, ld = _rows_of(logits, b, "logits")
+    if b.dtype not in _lib.DTYPES:
+        raise ValueError(f"logits: elements of type {b.dtype}")
+    ub = _lib.device_buffer(u, "u")
+    keep = [b, ub]
+    if ub.dtype != "f32" or ub.size != rows:
+        raise ValueError(f"u: expected {rows} values of type f32, got {ub.size} of {ub.dtype}")
+    m_ptr, ldm = None, n
+    if mask is not None:
+        mb = _lib.device_buffer(mask, "mask", contiguous=False)
+        mrows, mn, ldm = _rows_of(mask, mb, "mask")
+        if mb.dtype != "u8" or mn != n or mrows not in (1, rows):
+            raise ValueError(f"mask: expected bytes [{rows}, {n}] or [{n}], got {mb.dtype} {list(mb.shape)}")
+        if mrows == 1:
+            ldm = 0
+        m_ptr = mb.ptr
+        keep.append(mb)
+    t, t_dev = _setting(temperature, rows, "f32", keep, "temperature")
+    k, k_dev = _setting(top_k, rows, "i32", keep, "top_k")
+    p, p_dev = _setting(top_p, rows, "f32", keep, "top_p")
+    q, q_dev = _setting(min_p, rows, "f32", keep, "min_p")
+    cfg = SampleCfg(_lib.DTYPES[b.dtype], t, k, p, q, t_dev, k_dev, p_dev, q_dev)
+    if out is None:
+        out = _new(b.device, rows, np.int32)
+    ob = _lib.device_buffer(out, "out")
+    if ob.dtype != "i32" or ob.size != rows:
+        raise ValueError(f"out: expected {rows} values of type i32, got {ob.size} of {ob.dtype}")
+    keep.append(ob)
+    pr = None
+    if prob is not None:
+        pb = _lib.device_buffer(prob, "prob")
+        if pb.dtype != "f32" or pb.size != rows:
+            raise ValueError(f"prob: expected {rows} values of type f32, got {pb.size} of {pb.dtype}")
+        keep.append(pb)
+        pr = pb.ptr
+    need = sample_workspace(rows, n)
+    w_ptr, w_bytes = None, 0
+    if need or workspace is not None:
+        if workspace is None:
+            workspace = _new(b.device, need, np.uint8)
+        wb = _lib.device_buffer(workspace, "workspace")
+        keep.append(wb)
+        w_ptr, w_bytes = wb.ptr, wb.size
+    _lib.same_device(keep)
+    _lib.call_on(b.device, "snk_sample_logits", b.ptr, rows, n, ld, m_ptr, ldm, ub.ptr, C.byref(cfg), ob.ptr, pr, w_ptr,
+                 w_bytes)
+    return out
+
+
+def sample_workspace(rows: int, n: int) -> int:
+    """Bytes of workspace that sample_logits uses for rows x n logits (0: none)."""
+    need = i64(0)
+    call("snk_sample_workspace", rows, n, C.byref(need))
+    return need.value
+
+
+def _new(device, n, dtype):
+    if device is None:
+        return DeviceArray(n, dtype)
+    import torch
+    return torch.empty(n, dtype=torch.int32 if dtype is np.int32 else torch.uint8, device=device)
+
+
+def softmax_actions(game, model, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                    seed: int = 0, act: DeviceArray | None = None) -> np.ndarray:
+    """Boltzmann exploration for every env, in epsilon_greedy's place: action indices drawn from
+    softmax(Q / temperature) under the filters, with the counter RNG's u(seed, env, step)."""
+    act = act if act is not None else DeviceArray(game.n_envs, np.uint8)
+    cfg = SampleCfg(_lib.SNK_F32, temperature, top_k, top_p, min_p, None, None, None, None)
+    call("snk_dqn_act_sample", model.handle, game.handle, C.byref(cfg), int(seed), act.ptr)
+    return act.numpy()

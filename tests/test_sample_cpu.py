@@ -1,0 +1,61 @@
+"""The sampler's refusals that need no device, and its reference against counted cases (CPU)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import sample_ref
+import snake_amd
+from snake_amd import _lib
+from snake_amd.policy import SampleCfg
+
+ONE = 4096   # an address that is never read: every call below is refused before a launch
+
+
+def _call(rows=1, n=8, ld=8, ldm=8, x=ONE, mask=None, u=ONE, idx=ONE, cfg=None, **change):
+    base = dict(dtype=0, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0)
+    cfg = SampleCfg(*{**base, **change}.values()) if cfg is None else cfg
+    lib = snake_amd.load()
+    st = lib.snk_sample_logits(x, rows, n, ld, mask, ldm, u, C.byref(cfg) if cfg else None, idx, None, None, 0)
+    return st, lib.snk_last_error().decode()
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(dtype=7), "type"), (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+    (dict(temperature=float("inf")), "temperature"), (dict(top_k=-1), "top_k"), (dict(top_p=1.5), "top_p"),
+    (dict(top_p=-0.5), "top_p"), (dict(top_p=float("nan")), "top_p"), (dict(min_p=2.0), "min_p"),
+    (dict(min_p=float("nan")), "min_p"), (dict(rows=-1), "rows"), (dict(rows=2 ** 31), "rows"), (dict(n=0), "logits a row"),
+    (dict(n=2 ** 24 + 1, ld=2 ** 25), "logits a row"), (dict(ld=7), "ld"), (dict(ld=-8), "ld"),
+    (dict(mask=ONE, ldm=3), "ld_mask"), (dict(x=None), "NULL"), (dict(u=None), "NULL"), (dict(idx=None), "NULL"),
+    (dict(x=ONE + 2), "aligned"), (dict(x=ONE + 1, dtype=1), "aligned"), (dict(cfg=False), "cfg"),
+])
+def test_bad_calls_are_refused(change, word):
+    st, msg = _call(**change)
+    assert st == _lib.SNK_ERR_INVALID and word in msg, msg
+
+
+def test_struct_size_guard():
+    c = SampleCfg(0, 1.0, 0, 1.0, 0.0)
+    assert C.sizeof(SampleCfg) == 56
+    c.struct_size = 52
+    st, msg = _call(cfg=c)
+    assert st == _lib.SNK_ERR_INVALID and "struct_size" in msg
+    assert snake_amd.load().snk_dqn_act_sample(None, None, C.byref(c), 0, None) == _lib.SNK_ERR_INVALID
+    assert snake_amd.load().snk_sample_workspace(1, 1, None) == _lib.SNK_ERR_INVALID
+
+
+def test_no_rows_is_no_work():
+    assert _call(rows=0, x=None, u=None, idx=None)[0] == _lib.SNK_OK
+
+
+def test_reference_on_counted_cases():
+    x = np.log([1.0, 2.0, 4.0, 1.0])
+    assert [sample_ref.row(x, u)[0] for u in (0.0, 0.124, 0.126, 0.374, 0.376, 0.874, 0.876)] == [0, 0, 1, 1, 2, 2, 3]
+    assert sample_ref.row(x, 0.9, top_k=1)[:2] == (2, 1.0)
+    assert sample_ref.row(x, 0.1, top_k=3)[0] == 0 and sample_ref.row(x, 0.99, top_k=3)[0] == 2    # the tie at 1: index 0
+    assert sample_ref.row(x, 0.1, top_p=0.5)[0] == 2 and sample_ref.row(x, 0.1, top_p=0.51)[0] == 1
+    assert sample_ref.row(x, 0.1, min_p=0.3)[0] == 1
+    assert sample_ref.row(x, 0.999, mask=[0, 0, 1, 1])[0] == 1
+    assert sample_ref.row(x, 0.5, temperature=0.0)[:2] == (2, 1.0)
+    assert sample_ref.row([-np.inf, np.nan], 0.5, mask=[0, 1])[0] == -1
+    assert sample_ref.row([1.0, np.inf, np.inf], 0.6)[:2] == (2, 0.5)

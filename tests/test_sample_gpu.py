@@ -1,0 +1,297 @@
+"""The sampler on the GPU against its definition in 64 bits: equal indices, probabilities to fp32.
+
+A reference answer whose margin (how near u or a filter's limit is to a step of the sums, relative
+to the mass) is under 1e-9 may fall to either side and is left out; with random inputs that is rare,
+and each test asserts how rare. The probability is a quotient of 64-bit sums whose entries are
+rounded to 2^-(61 - log2 n) of the largest weight, rounded to fp32: half a step 2^-24, and 1e-9.
+"""
+import numpy as np
+import pytest
+
+import devrng
+import sample_ref
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+TT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SETTINGS = [dict(), dict(temperature=0.3), dict(top_k=1), dict(top_k=5), dict(top_k=50, top_p=0.8), dict(top_p=0.9),
+            dict(top_p=0.0), dict(min_p=0.1), dict(min_p=1.0), dict(top_k=700, top_p=0.95, min_p=0.01, temperature=1.7),
+            dict(top_p=0.999, temperature=3.0), dict(temperature=0.0)]
+
+
+def check(snk, x, u, mask=None, most_left_out=0, **how):
+    """x [rows, n] torch tensor, how: numbers or arrays of one value per row."""
+    rows, n = x.shape
+    out = torch.full((rows + 2,), -7, dtype=torch.int32, device="cuda")
+    prob = torch.full((rows + 2,), -7.0, device="cuda")
+    dev = {k: torch.as_tensor(v, device="cuda") if isinstance(v, np.ndarray) else v for k, v in how.items()}
+    got = snk.sample_logits(x, u, mask=mask, out=out[1:-1], prob=prob[1:-1], **dev)
+    assert got.data_ptr() == out[1:-1].data_ptr()
+    idx, pr = out.cpu().numpy(), prob.double().cpu().numpy()
+    assert idx[0] == idx[-1] == -7 and pr[0] == pr[-1] == -7
+    xs, us = x.double().cpu().numpy(), u.cpu().numpy()
+    ms = None if mask is None else np.broadcast_to(mask.cpu().numpy(), xs.shape)
+    left_out = 0
+    for r in range(rows):
+        one = {k: v[r] if isinstance(v, np.ndarray) else v for k, v in how.items()}
+        i, p, margin = sample_ref.row(xs[r], us[r], mask=None if ms is None else ms[r], **one)
+        if margin < 1e-9:
+            left_out += 1
+            continue
+        assert idx[1 + r] == i, (r, idx[1 + r], i, margin, one)
+        assert np.isnan(p) == np.isnan(pr[1 + r])
+        if not np.isnan(p):
+            assert abs(pr[1 + r] - p) <= (2.0 ** -24 + 1e-9) * p, (r, pr[1 + r], p)
+    assert left_out <= most_left_out, left_out
+    return idx[1:-1]
+
+
+def logits(rows, n, dtype, seed, std=2.0, stride=None, offset=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    stride = stride or n
+    buf = torch.full((rows * stride + offset,), float("nan"), dtype=TT[dtype], device="cuda")   # never to be read
+    x = buf[offset:offset + rows * stride].view(rows, stride)[:, :n]
+    x.copy_(torch.randn(rows, n, device="cuda", generator=gen) * std)
+    return x, torch.rand(rows, device="cuda", generator=gen)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 8, 9, 31, 63, 64, 65, 200, 511, 512, 513, 1000, 1024, 2047, 4097, 8193, 16385, 50021])
+def test_sizes_and_settings(snk, dtype, n):
+    for k, how in enumerate(SETTINGS):
+        x, u = logits(6, n, dtype, 100 * n + k)
+        # a quarter of 2^-9 steps of bf16 values may tie; the margin of distinct sums is about 1 / n / S
+        check(snk, x, u, most_left_out=1, **how)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,stride,offset", [(7, 9, 1), (100, 101, 1), (700, 703, 3), (5000, 5001, 1), (33000, 33005, 2)])
+def test_strides_and_alignment(snk, dtype, n, stride, offset):
+    """Rows that start at any element; what lies between them is NaN and must not matter."""
+    for how in (dict(), dict(top_k=20), dict(top_p=0.7), dict(min_p=0.05)):
+        x, u = logits(9, n, dtype, n, stride=stride, offset=offset)
+        gen = torch.Generator(device="cuda").manual_seed(n)
+        mask = (torch.rand(9, stride, device="cuda", generator=gen) < 0.3)[:, :n]
+        check(snk, x, u, most_left_out=1, **how)
+        check(snk, x, u, mask=mask.to(torch.uint8) if n % 2 else mask, most_left_out=1, **how)
+        check(snk, x, u, mask=mask[3].contiguous(), most_left_out=1, **how)
+
+
+def test_one_row_for_all(snk):
+    """An expanded row (stride 0), a thousand draws: the drawn shares are those of the weights, since
+    the given u are a grid: an entry of probability p is hit by p 1000 +- 1 of them."""
+    x, _ = logits(1, 300, "f32", 3, std=1.0)
+    u = (torch.arange(1000, device="cuda") + 0.5) / 1000
+    idx = check(snk, x.expand(1000, 300), u)
+    p = torch.softmax(x[0].double(), 0).cpu().numpy()
+    assert np.all(np.abs(np.bincount(idx, minlength=300) - 1000 * p) <= 1 + 1e-6)
+    one = snk.sample_logits(x[0], u[:1])
+    assert int(one[0]) == idx[0]
+
+
+@pytest.mark.parametrize("n", [3, 8, 40, 600, 9000])
+def test_rows_with_nothing_and_odd_values(snk, n):
+    x, u = logits(24, n, "f32", n)
+    mask = torch.zeros(24, n, dtype=torch.uint8, device="cuda")
+    low, inf, nan = torch.finfo(torch.float32).min, float("inf"), float("nan")
+    mask[0] = 1                                # nothing left
+    x[1] = -inf                                # nothing left
+    x[2, :], mask[2, :] = nan, 255             # NaN, all masked
+    x[3, 0], mask[3, 0] = nan, 1               # NaN and infinity in masked places
+    x[4, 0], mask[4, 0] = inf, 1
+    x[5, n // 2] = nan                         # NaN in an allowed place
+    x[6, n - 1] = inf                          # one infinite entry
+    x[7, 0] = x[7, n - 1] = inf                # two
+    x[8] = low                                 # the type's lowest everywhere
+    x[9, 1:] = low                             # ... but for one
+    x[10] = 0.25                               # all equal
+    x[11, ::2], x[11, 1::2] = 0.0, -0.0        # equal zeros
+    mask[12, : n - 1] = 1                      # only the last allowed
+    x[13] = torch.arange(n, device="cuda") * 1e-42    # subnormal
+    x[14] = -inf
+    x[14, n // 2] = -1e30                      # one entry, far down
+    x[15] = torch.where(torch.arange(n, device="cuda") % 3 == 0, 5.0, 1.0)
+    u[16], u[17], u[18], u[19], u[20] = 0.0, 0.99999994, 1.0, nan, -3.0
+    x[21] = 3e38
+    x[22, 0], x[22, 1] = -nan, 1.0             # a NaN of the other sign
+    x[23, 0], x[23, 1:] = -3e38, 3e38
+    for how in (dict(), dict(top_k=2), dict(top_p=0.6), dict(min_p=0.5), dict(temperature=0.0), dict(temperature=1e-30),
+                dict(temperature=1e30), dict(top_k=3, top_p=0.99, min_p=0.001)):
+        check(snk, x, u, mask=mask, most_left_out=24, **how)   # equal entries put limits on exact steps
+    idx = check(snk, x, u, mask=mask, top_p=0.6, most_left_out=24)
+    assert idx[0] == idx[1] == idx[2] == idx[5] == idx[22] == -1 and idx[12] == n - 1 and idx[14] == n // 2 and idx[6] == n - 1
+    assert min(idx[3], idx[4]) >= 1
+    assert idx[7] in (0, n - 1)
+
+
+@pytest.mark.parametrize("n", [6, 300, 3000, 70001])
+def test_settings_of_each_row(snk, n):
+    rng = np.random.default_rng(n)
+    rows = 40
+    x, u = logits(rows, n, "f16", n)
+    how = dict(temperature=rng.uniform(0.2, 2, rows).astype(np.float32), top_k=rng.integers(0, 60, rows).astype(np.int32),
+               top_p=rng.uniform(0.2, 1, rows).astype(np.float32), min_p=rng.uniform(0, 0.2, rows).astype(np.float32))
+    how["top_k"][:4] = [-3, n, n + 9, 2 ** 31 - 1]          # off
+    how["temperature"][4:7] = [0.0, -1.0, np.nan]           # the largest
+    how["top_p"][7:11] = [1.0, 7.0, np.nan, -1.0]
+    how["min_p"][11:14] = [-1.0, np.nan, 9.0]
+    check(snk, x, u, most_left_out=4, **how)
+    for key in how:
+        check(snk, x, u, most_left_out=4, **{key: how[key]})
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("how", [dict(), dict(top_p=0.97), dict(top_k=1500), dict(top_k=64), dict(min_p=1e-4),
+                                 dict(top_k=100000, top_p=0.999)])
+def test_long_rows(snk, dtype, how):
+    for rows, n in ((3, 262144), (2, 1_000_003)):
+        x, u = logits(rows, n, dtype, n, std=1.5)
+        check(snk, x, u, most_left_out=1, **how)
+
+
+def test_the_longest_row(snk):
+    n = 2 ** 24
+    x, u = logits(1, n, "bf16", 1, std=1.0)
+    for how in (dict(top_k=30), dict(top_p=0.5), dict(min_p=0.3)):
+        check(snk, x, u, most_left_out=1, **how)
+    with pytest.raises(snk.SnakeHipError, match="logits a row"):
+        snk.sample_logits(torch.zeros(n + 1, device="cuda"), torch.zeros(1, device="cuda"))
+
+
+def test_many_ties(snk):
+    """Few distinct values: cuts fall inside runs of equal entries, the lower indices stay."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    for n in (8, 100, 511, 5000, 40000):
+        x = torch.randint(0, 4, (16, n), device="cuda", generator=gen).float() * 0.7
+        u = torch.rand(16, device="cuda", generator=gen)
+        for how in (dict(top_k=n // 3 + 1), dict(top_p=0.61803), dict(top_k=n // 2 + 1, top_p=0.7717), dict(min_p=0.2)):
+            check(snk, x, u, most_left_out=1, **how)
+
+
+def test_offsets_past_32_bits(snk):
+    """Rows whose elements lie past 2^32 bytes and past 2^31 elements."""
+    n = 2 ** 20 + 1
+    rows = 2100
+    x = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda").normal_(0, 2)
+    u = torch.rand(rows, device="cuda")
+    for how in (dict(top_k=20), dict()):
+        got = snk.sample_logits(x, u, **how)
+        part = slice(rows - 2, rows)
+        check(snk, x[part], u[part], most_left_out=1, **how)
+        assert torch.equal(got[part], snk.sample_logits(x[part], u[part], **how))
+
+
+@pytest.mark.parametrize("rows,n", [(5, 3), (3, 400), (2, 30000), (70, 9000), (300, 2000)])
+def test_captured_and_on_another_stream(snk, rows, n):
+    """Replays of two captured calls and eager calls between them agree with eager calls."""
+    how = dict(top_k=9, top_p=0.9)
+    x, u = logits(rows, n, "f32", rows)
+    y, v = logits(rows, n, "f32", rows + 1)
+    fresh = [logits(rows, n, "f32", 50 + i) for i in range(4)]
+    graphs = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for a, b in ((x, u), (y, v)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = snk.sample_logits(a, b, **how)
+        graphs.append((g, out))
+    for (fx, fu) in fresh:
+        x.copy_(fx), u.copy_(fu), y.copy_(fx * 0.5), v.copy_(fu)
+        for g, _ in graphs:
+            g.replay()
+        eager = snk.sample_logits(fx, fu, **how), snk.sample_logits(fx * 0.5, fu, **how)
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[0][1], eager[0]) and torch.equal(graphs[1][1], eager[1])
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(5_000_000)
+        x.copy_(fresh[0][0]), u.copy_(fresh[0][1])
+        late = snk.sample_logits(x, u, **how)
+    side.synchronize()
+    assert torch.equal(late, snk.sample_logits(fresh[0][0], fresh[0][1], **how))
+
+
+@pytest.mark.parametrize("n", [3, 500, 20000])
+def test_device_arrays(snk, n):
+    x, u = logits(4, n, "f32", n)
+    a, b = snk.DeviceArray.from_host(x.cpu().numpy()), snk.DeviceArray.from_host(u.cpu().numpy())
+    assert np.array_equal(snk.sample_logits(a, b, top_k=7).numpy(), snk.sample_logits(x, u, top_k=7).cpu().numpy())
+
+
+def test_python_refusals(snk):
+    x, u = logits(4, 100, "f32", 0)
+    for bad in (dict(logits=x.t(), u=u), dict(logits=x, u=u[:3]), dict(logits=x, u=u.double()), dict(logits=x.int(), u=u),
+                dict(logits=x[None], u=u), dict(logits=x, u=u, mask=x), dict(logits=x, u=u, mask=x[:, :9] > 0),
+                dict(logits=x, u=u, out=torch.zeros(4, device="cuda")), dict(logits=x, u=u, prob=u[:2]),
+                dict(logits=x, u=u, temperature=u[:2]), dict(logits=x, u=u, top_k=u)):
+        with pytest.raises(ValueError):
+            snk.sample_logits(**bad)
+    with pytest.raises(snk.SnakeHipError):
+        snk.sample_logits(x, u, top_p=1.01)
+    with pytest.raises(ValueError, match="mix"):
+        snk.sample_logits(x, snk.DeviceArray(4, np.float32))
+
+
+# ------------------------------------------------------------------ the policy over an env batch
+
+@pytest.mark.parametrize("deep", [False, True])
+def test_softmax_actions(snk, deep):
+    n, seed = 300, 77
+    game = snk.SnakeGame(12, 2, n_envs=n, autoreset=True)
+    model = snk.DQNModel(12, 3, n_frames=2, seed=4, deep=deep)
+    act = snk.DeviceArray(n, np.uint8)
+    for t in range(3):
+        q = model.q_env(game)
+        for how in (dict(temperature=0.05), dict(temperature=0.0), dict(temperature=0.1, top_k=2), dict(top_p=0.5)):
+            got = snk.softmax_actions(game, model, seed=seed, act=act, **how)
+            for e in range(n):
+                u = devrng.rng_uniform(devrng.rng_hash(seed, e, t))
+                want, _, margin = sample_ref.row(q[e], u, **how)
+                assert margin < 1e-9 or got[e] == want
+        assert np.array_equal(snk.softmax_actions(game, model, temperature=0.0), snk.epsilon_greedy(game, model, 0.0))
+        snk.step_indices_dev(game, act.ptr)
+
+
+def test_an_iteration_of_both_ends(snk):
+    """Acting by the softmax policy and learning by AdamW, together as a training loop uses them:
+    every action against the definition, every update against the formula."""
+    import adamw_ref
+    n, seed = 128, 5
+    game = snk.SnakeGame(12, 2, n_envs=n, autoreset=True)
+    rb = snk.ReplayBuffer(2048, board_size=12, n_frames=2)
+    model = snk.DQNModel(12, 3, n_frames=2, seed=8)
+    opt = model.use_adamw(lr=1e-3, weight_decay=0.01, max_grad_norm=1.0)
+    sizes = [288, 16, 4608, 32, 73728, 64, 49 * 4096, 64, 192, 3]
+    perm, (starts, total) = model.flux_index(), adamw_ref.places(sizes)
+    ends = np.cumsum([0] + sizes)
+
+    def layout(flux):
+        out = np.zeros(total)
+        for at, a, b in zip(starts, ends, ends[1:]):
+            out[at:at + b - a] = flux[perm][a:b]
+        return out
+
+    wd = layout(np.ones(model.P, np.float32)) * 0
+    for i, (at, s) in enumerate(zip(starts, sizes)):
+        wd[at:at + s] = 0.0 if i % 2 else 0.01
+    act, updates = snk.DeviceArray(n, np.uint8), 0
+    for t in range(6):
+        q = model.q_env(game)
+        got = snk.softmax_actions(game, model, temperature=0.2, top_k=2, seed=seed, act=act)
+        for e in range(n):
+            u = devrng.rng_uniform(devrng.rng_hash(seed, e, t))
+            want, _, margin = sample_ref.row(q[e], u, temperature=0.2, top_k=2)
+            assert margin < 1e-9 or got[e] == want
+        snk.step_indices_dev(game, act.ptr, replay=rb)
+        if t < 2:
+            continue
+        idx, B = snk.sample(rb, seed=t)
+        st = {k: v.numpy() for k, v in opt.state().items()}
+        p = layout(model.get_params())
+        loss = model.update(rb, idx, B)
+        updates += 1
+        want = adamw_ref.Step(p, layout(model.grad), st["m"], st["v"], updates, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=wd,
+                              max_norm=1.0)
+        assert np.all(np.abs(layout(model.get_params()) - want.p) <= want.ep) and np.isfinite(loss)
+    assert opt.steps == updates
