@@ -296,7 +296,7 @@ typedef struct {
     int32_t state_bits;    /* 32 or 8 */
     float max_grad_norm;   /* 0: no norm; > 0 (may be inf): norm, clipping, and a step whose norm is
                               not finite writes nothing and is not counted */
-    double beta1, beta2, eps;
+    double beta1, beta2, eps;   /* in [0, 1), [0, 1), [1e-30, 1e30] */
     uint64_t seed;         /* of the 8-bit rounding */
     int64_t reserved;      /* 0 */
 } snk_adamw_cfg_t;

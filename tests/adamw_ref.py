@@ -54,9 +54,9 @@ class Step:
         c = max_norm / self.norm if max_norm and self.norm > max_norm else 1.0
         gp = g * (float(np.float32(scale)) * c)
         # g': the product's and the factor's rounding (2 U). Old values of 8-bit states: m 4 U (constant,
-        # two products), v 4 U (b^2 is exact, its square,
-        # a constant, two products)
-        old_m, old_v = (0, 0) if state_bits == 32 else (4, 4)
+        # two products), v 12 U ((b / 255): 2 U,
+        # squared 5 U, squared again 11 U, times the scale)
+        old_m, old_v = (0, 0) if state_bits == 32 else (4, 12)
         self.m = b1 * m + (1 - b1) * gp
         self.em = U * ((3 + old_m) * np.abs(b1 * m) + 5 * np.abs((1 - b1) * gp)) + 1e-44
         self.v = b2 * v + (1 - b2) * gp * gp
@@ -95,12 +95,12 @@ class Step:
             lo, hi = (low / 255) ** 4, ((low + 1) / 255) ** 4
             return low + (r < (part - lo) / (hi - lo) * 65536)
         base = np.where(vs > 0, vs, 1)
-        # the chance's own error: levels 3 U each, times level / (hi - lo) <= b / 4: 6 U * 64, in 65536ths: 1.5
-        lowest = v_code((v - ev) / base * (1 - 4 * U), rand + 2)
-        highest = v_code((v + ev) / base * (1 + 4 * U), rand - 2)
+        # the chance's own error: levels 11 U each, times level / (hi - lo) <= b / 4: 22 U * 64, in 65536ths: 5.5
+        lowest = v_code((v - ev) / base * (1 - 4 * U), rand + 8)
+        highest = v_code((v + ev) / base * (1 + 4 * U), rand - 8)
         # a quotient next to a level's edge may be floored to either side
-        lowest = np.minimum(lowest, v_code((v - ev) / base * (1 - 64 * U), rand + 2))
-        highest = np.maximum(highest, v_code((v + ev) / base * (1 + 64 * U), rand - 2))
+        lowest = np.minimum(lowest, v_code((v - ev) / base * (1 - 64 * U), rand + 8))
+        highest = np.maximum(highest, v_code((v + ev) / base * (1 + 64 * U), rand - 8))
         live = v > 0
         lowest, highest = np.where(live, np.maximum(lowest, 1), lowest), np.where(live, np.maximum(highest, 1), highest)
         assert np.all((b >= lowest) & (b <= highest)), "v codes"

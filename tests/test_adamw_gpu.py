@@ -267,8 +267,10 @@ def test_moments_values(snk):
         for dt in ("f32", "bf16", "f16"):
             out = [torch.full((opt.total,), 9.0, dtype=TT[dt], device="cuda") for _ in range(2)]
             opt.moments(*out)
-            for x, y in zip(out, (m, v)):
-                assert np.all(np.abs(x.double().cpu().numpy() - y) <= (ref.HALF[dt] + 4 * ref.U) * np.abs(y) + 2.0 ** -25 * (dt == "f16"))
+            # fp32 values of codes: m 4 U; v 12 U, (b / 255) being 2 U off, squared 5 U, squared again
+            # 11 U, times the scale 12 U
+            for x, y, k in zip(out, (m, v), (4, 12)):
+                assert np.all(np.abs(x.double().cpu().numpy() - y) <= (ref.HALF[dt] + k * ref.U) * np.abs(y) + 2.0 ** -25 * (dt == "f16"))
             opt.moments(out[0])
         with pytest.raises(ValueError):
             opt.moments(torch.zeros(7, device="cuda"))
