@@ -392,8 +392,18 @@ class Buffer:
 
 # numpy has no bfloat16: a uint16 DeviceArray holds its bits
 _NP_TYPES = {"float32": "f32", "float16": "f16", "uint16": "bf16", "int32": "i32", "uint8": "u8", "bool": "u8"}
-_TORCH_TYPES = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16", "torch.int32": "i32",
-                "torch.uint8": "u8", "torch.bool": "u8"}
+_torch = None
+_TORCH_TYPES: dict = {}
+
+
+def torch_module():
+    global _torch
+    if _torch is None:
+        import torch
+        _TORCH_TYPES.update({torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16", torch.int32: "i32",
+                             torch.uint8: "u8", torch.bool: "u8"})
+        _torch = torch
+    return _torch
 
 
 def device_buffer(x, what: str, contiguous: bool = True) -> Buffer:
@@ -403,12 +413,13 @@ def device_buffer(x, what: str, contiguous: bool = True) -> Buffer:
         kind = _NP_TYPES.get(x.dtype.name)
         b.size = x.nbytes // x.dtype.itemsize
     elif hasattr(x, "data_ptr"):
+        torch_module()
         if not x.is_cuda:
             raise ValueError(f"{what}: a tensor on {x.device}, not on the GPU")
         if contiguous and not x.is_contiguous():
             raise ValueError(f"{what}: a tensor that is not contiguous")
-        b.ptr, b.shape, b.device, b.size = x.data_ptr(), tuple(x.shape), x.device, x.numel()
-        kind = _TORCH_TYPES.get(str(x.dtype))
+        b.ptr, b.shape, b.device, b.size = x.data_ptr(), x.shape, x.device, x.numel()
+        kind = _TORCH_TYPES.get(x.dtype)
     else:
         raise TypeError(f"{what}: {type(x).__name__} is neither a DeviceArray nor a torch tensor")
     if kind is None:
@@ -417,10 +428,22 @@ def device_buffer(x, what: str, contiguous: bool = True) -> Buffer:
     return b
 
 
-def same_device(buffers) -> None:
+def vector_ptr(x, what: str, kind: str, size: int, device) -> int:
+    """Address of a contiguous device tensor of `size` elements of one type, on `device`."""
+    b = device_buffer(x, what)
+    if b.dtype != kind or b.size != size:
+        raise ValueError(f"{what}: expected {size} values of type {kind}, got {b.size} of {b.dtype}")
+    if b.device != device:
+        same_device([b, None], device)
+    return b.ptr
+
+
+def same_device(buffers, device="first") -> None:
     """One call's tensors are all DeviceArrays or all on one torch device."""
-    if len({b.device for b in buffers}) > 1:
-        raise ValueError("the tensors of one call live on different devices, or mix DeviceArrays and torch tensors")
+    first = buffers[0].device if device == "first" else device
+    for b in buffers:
+        if b is not None and b.device != first:
+            raise ValueError("the tensors of one call live on different devices, or mix DeviceArrays and torch tensors")
 
 
 def call_on(device, name: str, *args) -> None:
@@ -429,16 +452,23 @@ def call_on(device, name: str, *args) -> None:
     if device is None:
         call(name, *args)
         return
-    import torch
-    if torch.cuda.current_device() != device.index:
-        raise ValueError(f"the tensors live on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    t = torch_module()
+    if t.cuda.current_device() != device.index:
+        raise ValueError(f"the tensors live on {device}, the current device is cuda:{t.cuda.current_device()}")
     lib = load()
     old, given = vp(), i32(0)
-    check(lib.snk_swap_stream(torch.cuda.current_stream().cuda_stream, 1, C.byref(old), C.byref(given)))
+    check(lib.snk_swap_stream(_raw_stream(t, device), 1, C.byref(old), C.byref(given)))
     try:
         check(getattr(lib, name)(*args))
     finally:
         lib.snk_swap_stream(old, given, None, None)
+
+
+def _raw_stream(t, device) -> int:
+    """torch.cuda.current_stream(device).cuda_stream, without its 2.8 us of objects where torch
+    offers the handle itself."""
+    raw = getattr(t._C, "_cuda_getCurrentRawStream", None)
+    return raw(device.index) if raw else t.cuda.current_stream(device).cuda_stream
 
 
 def view_numpy(dev_ptr: int, shape, dtype) -> np.ndarray:

@@ -118,16 +118,27 @@ __device__ __forceinline__ float root(float x) {
     return fmaf(fmaf(-s, s, x), 0.5f * __builtin_amdgcn_rcpf(s), s);
 }
 
+// what a step knows before it starts: its number and 1 / (1 - b^t)
+struct AdamStep {
+    int64_t t;
+    double c1, c2;
+    float ibc1, ibc2;
+};
+__host__ __device__ inline AdamStep next_step(int64_t t, double c1, double c2, const AdamHyper &H) {
+    const double n1 = (1.0 - H.b1d) + H.b1d * c1, n2 = (1.0 - H.b2d) + H.b2d * c2;
+    return AdamStep{t + 1, n1, n2, (float)(1.0 / n1), (float)(1.0 / n2)};
+}
+
 // the step's number and bias corrections, by one thread before the step's launch. In fp64: 1 - b^t
 // loses digits in fp32 while t is small; 1 - b^t = (1 - b) + b (1 - b^(t-1)) needs no power.
 __device__ __forceinline__ void begin_step(AdamCtl *ctl, const AdamHyper &H) {
     if (ctl->skip) return;   // that number has not been used
-    const double c1 = (1.0 - H.b1d) + H.b1d * ctl->c1, c2 = (1.0 - H.b2d) + H.b2d * ctl->c2;
-    ctl->t += 1;
-    ctl->c1 = c1;
-    ctl->c2 = c2;
-    ctl->ibc1 = (float)(1.0 / c1);
-    ctl->ibc2 = (float)(1.0 / c2);
+    const AdamStep n = next_step(ctl->t, ctl->c1, ctl->c2, H);
+    ctl->t = n.t;
+    ctl->c1 = n.c1;
+    ctl->c2 = n.c2;
+    ctl->ibc1 = n.ibc1;
+    ctl->ibc2 = n.ibc2;
 }
 __global__ void adamw_begin_kernel(AdamCtl *__restrict__ ctl, AdamHyper H) { begin_step(ctl, H); }
 
@@ -202,8 +213,20 @@ struct AdamArgs {
     AdamCtl *ctl;
     const double *part;   // n_part partial sums of the norm (0: none)
     int n_part;
+    bool counted;         // the host counts the steps: `step` holds, and ctl is to receive it
+    AdamStep step;
     AdamHyper H;
 };
+
+__device__ __forceinline__ AdamStep this_step(const AdamArgs &A) {
+    if (!A.counted) return AdamStep{A.ctl->t, A.ctl->c1, A.ctl->c2, A.ctl->ibc1, A.ctl->ibc2};
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        A.ctl->t = A.step.t;
+        A.ctl->c1 = A.step.c1;
+        A.ctl->c2 = A.step.c2;
+    }
+    return A.step;
+}
 
 // the factor of the gradients, s c; false where the step is skipped. Workgroup 0 records N.
 __device__ __forceinline__ bool grad_factor(const AdamArgs &A, double *sh, float &gmul) {
@@ -249,7 +272,8 @@ template <class PT, class GT>
 __global__ __launch_bounds__(256) void adamw32_kernel(AdamArgs A) {
     __shared__ double sh[4];
     const AdamChunk T = A.chunks[blockIdx.x];
-    const float ibc1 = A.ctl->ibc1, ibc2 = A.ctl->ibc2;
+    const AdamStep now = this_step(A);
+    const float ibc1 = now.ibc1, ibc2 = now.ibc2;
     float *ms = (float *)A.m + T.place, *vs = (float *)A.v + T.place;
     const int i = threadIdx.x * 4;
     const bool live = i < T.n;
@@ -275,9 +299,10 @@ template <class PT, class GT>
 __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     __shared__ double sh[4];
     const AdamChunk T = A.chunks[blockIdx.x];
-    const float ibc1 = A.ctl->ibc1, ibc2 = A.ctl->ibc2;
+    const AdamStep now = this_step(A);
+    const float ibc1 = now.ibc1, ibc2 = now.ibc2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = threadIdx.x * 4;
-    const uint64_t key = splitmix64(A.H.seed ^ ((uint64_t)A.ctl->t * 0xD1B54A32D192ED03ULL));   // rng_hash's first half
+    const uint64_t key = splitmix64(A.H.seed ^ ((uint64_t)now.t * 0xD1B54A32D192ED03ULL));   // rng_hash's first half
     const uint64_t h = splitmix64(key ^ (uint64_t)((T.place + i) >> 2));
     uint8_t *mcs = (uint8_t *)A.m + T.place, *vcs = (uint8_t *)A.v + T.place;
     float *mss = A.ms + T.place / BLK, *vss = A.vs + T.place / BLK;
@@ -394,6 +419,8 @@ struct snk_adamw_s {
     snk_adamw_cfg_t cfg{};
     int device = 0;
     bool owned = false, bound = false;
+    bool captured = false;   // a step was captured: only the device knows the count
+    AdamStep now{};          // the count until then, without a norm
     std::vector<int64_t> size, start;
     int64_t total = 0, n_chunks = 0;
     DevBuf<AdamTensor> tab;
@@ -441,6 +468,7 @@ void adamw_reset(snk_adamw h, hipStream_t s) {
         zero(h->vs, h->total / BLK * 4);
     }
     zero(h->ctl, sizeof(AdamCtl));
+    h->now = AdamStep{};
 }
 
 snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const snk_adamw_cfg_t *cfg) {
@@ -591,8 +619,21 @@ void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s) {
         }
         A.n_part = parts;
     } else {
-        adamw_begin_kernel<<<1, 1, 0, s>>>(h->ctl, H);
-        launch_check("adamw_begin_kernel");
+        // no norm, so no step is skipped, and the host can count them itself (a launch fewer) as long
+        // as none was captured: replays would not pass by here
+        if (!h->captured) {
+            hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+            SNK_HIP(hipStreamIsCapturing(s, &st));
+            h->captured = st != hipStreamCaptureStatusNone;
+        }
+        if (h->captured || h->n_chunks == 0) {
+            h->captured = true;
+            adamw_begin_kernel<<<1, 1, 0, s>>>(h->ctl, H);
+            launch_check("adamw_begin_kernel");
+        } else {
+            A.counted = true;
+            A.step = h->now = next_step(h->now.t, h->now.c1, h->now.c2, H);
+        }
     }
     if (h->n_chunks == 0) return;
     with_type(c.param_dtype, [&](auto p) {
@@ -701,6 +742,7 @@ extern "C" int snk_adamw_set_steps(snk_adamw h, int64_t steps) {
         ctl.t = steps;
         ctl.c1 = 1.0 - std::pow(h->cfg.beta1, (double)steps);
         ctl.c2 = 1.0 - std::pow(h->cfg.beta2, (double)steps);
+        h->now = AdamStep{steps, ctl.c1, ctl.c2, 0.0f, 0.0f};
         static_assert(offsetof(AdamCtl, norm) == 28, "t, c1, c2 and skip lead the struct");
         SNK_HIP(hipMemcpyAsync(h->ctl.p, &ctl, offsetof(AdamCtl, norm), hipMemcpyHostToDevice, stream()));
         SNK_HIP(hipStreamSynchronize(stream()));

@@ -3,8 +3,12 @@
 //
 // Every filter keeps a prefix of the order (x descending, equal ones by lower index), so a row's
 // answer needs no sort: the prefix is a cut (key kt, nt): the entries above kt and the first nt of
-// the entries equal to it, in index order. Masses are integers (weights rounded to 2^-sh of the
-// largest), so sums in LDS atomics and over any split of the row are exact and always the same.
+// the entries equal to it, in index order. Masses inside a row's cut are integers (weights rounded to
+// 2^-sh of the largest), so sums in LDS atomics are exact and always the same.
+//
+// A row is read once for what decides most rows: the largest logit of every 64 (a bound for top-k and
+// min-p) and, where the whole row's mass counts, the mass of every 512 (sample_scan_kernel). The row's
+// workgroup then reads again only the pieces of 512 that can hold an answer (sample_row_kernel).
 #include <algorithm>
 #include <cmath>
 
@@ -13,7 +17,14 @@
 namespace snk {
 
 constexpr int PIECE = 512;      // consecutive elements a wave reads at once: 8 a lane
+constexpr int GROUP = 64;       // elements of a recorded maximum: 8 lanes' worth
+constexpr int GP = PIECE / GROUP;
 constexpr int BINS = 2048;      // of a level of the radix search: 11 + 11 + 10 bits of the key
+constexpr int RW = 16;          // waves of a row's workgroup
+constexpr int SEGS = 1024;      // most segments the row's masses are kept by
+constexpr int FUSED_N = RW * PIECE;   // rows up to here need no separate scan: a piece a wave
+constexpr int LIST = 2048;      // most candidates held in LDS
+constexpr int PAIRS = 256;      // ... compared each with each
 
 struct SampleArgs {
     const void *x;
@@ -32,6 +43,9 @@ struct SampleArgs {
     uint8_t *act;
     uint64_t seed;
     const int64_t *tptr;
+    // the scan's records (workspace): [rows][pieces] masses, [rows][pieces][GP] maxima
+    double *masses;
+    float *tops;
 };
 
 // a row's settings, the same for all its threads
@@ -40,6 +54,8 @@ struct SampleRow {
     bool greedy;
     int k;        // 1..n
     float p, q, u;
+    // whether the mass of the whole row is needed
+    __device__ __forceinline__ bool whole(int n) const { return k == n && (p < 1.0f || q == 0.0f); }
 };
 __device__ __forceinline__ SampleRow sample_row(const SampleArgs &A, int64_t r) {
     SampleRow s;
@@ -49,7 +65,7 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs &A, int64_t r) 
     const int k = A.k_dev ? A.k_dev[r] : A.top_k;
     s.k = s.greedy ? 1 : k > 0 && k < A.n ? k : A.n;
     const float p = A.p_dev ? A.p_dev[r] : A.top_p, q = A.q_dev ? A.q_dev[r] : A.min_p;
-    s.p = p < 1.0f ? fmaxf(p, 0.0f) : 1.0f;   // NaN: off
+    s.p = p < 1.0f && !s.greedy ? fmaxf(p, 0.0f) : 1.0f;   // NaN: off
     s.q = q > 0.0f ? fminf(q, 1.0f) : 0.0f;
     const float u = A.u ? A.u[r] : rng_uniform(rng_hash(A.seed, (uint64_t)r, (uint64_t)*A.tptr));
     s.u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
@@ -65,15 +81,68 @@ __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// 2^(i/128)
+__device__ const double POW2[128] = {
+    0x1.0000000000000p+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.04315e86e7f85p+0,
+    0x1.059b0d3158574p+0, 0x1.0706b29ddf6dep+0, 0x1.0874518759bc8p+0, 0x1.09e3ecac6f383p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0cc922b7247f7p+0, 0x1.0e3ec32d3d1a2p+0, 0x1.0fb66affed31bp+0,
+    0x1.11301d0125b51p+0, 0x1.12abdc06c31ccp+0, 0x1.1429aaea92de0p+0, 0x1.15a98c8a58e51p+0,
+    0x1.172b83c7d517bp+0, 0x1.18af9388c8deap+0, 0x1.1a35beb6fcb75p+0, 0x1.1bbe084045cd4p+0,
+    0x1.1d4873168b9aap+0, 0x1.1ed5022fcd91dp+0, 0x1.2063b88628cd6p+0, 0x1.21f49917ddc96p+0,
+    0x1.2387a6e756238p+0, 0x1.251ce4fb2a63fp+0, 0x1.26b4565e27cddp+0, 0x1.284dfe1f56381p+0,
+    0x1.29e9df51fdee1p+0, 0x1.2b87fd0dad990p+0, 0x1.2d285a6e4030bp+0, 0x1.2ecafa93e2f56p+0,
+    0x1.306fe0a31b715p+0, 0x1.32170fc4cd831p+0, 0x1.33c08b26416ffp+0, 0x1.356c55f929ff1p+0,
+    0x1.371a7373aa9cbp+0, 0x1.38cae6d05d866p+0, 0x1.3a7db34e59ff7p+0, 0x1.3c32dc313a8e5p+0,
+    0x1.3dea64c123422p+0, 0x1.3fa4504ac801cp+0, 0x1.4160a21f72e2ap+0, 0x1.431f5d950a897p+0,
+    0x1.44e086061892dp+0, 0x1.46a41ed1d0057p+0, 0x1.486a2b5c13cd0p+0, 0x1.4a32af0d7d3dep+0,
+    0x1.4bfdad5362a27p+0, 0x1.4dcb299fddd0dp+0, 0x1.4f9b2769d2ca7p+0, 0x1.516daa2cf6642p+0,
+    0x1.5342b569d4f82p+0, 0x1.551a4ca5d920fp+0, 0x1.56f4736b527dap+0, 0x1.58d12d497c7fdp+0,
+    0x1.5ab07dd485429p+0, 0x1.5c9268a5946b7p+0, 0x1.5e76f15ad2148p+0, 0x1.605e1b976dc09p+0,
+    0x1.6247eb03a5585p+0, 0x1.6434634ccc320p+0, 0x1.6623882552225p+0, 0x1.68155d44ca973p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6c012750bdabfp+0, 0x1.6dfb23c651a2fp+0, 0x1.6ff7df9519484p+0,
+    0x1.71f75e8ec5f74p+0, 0x1.73f9a48a58174p+0, 0x1.75feb564267c9p+0, 0x1.780694fde5d3fp+0,
+    0x1.7a11473eb0187p+0, 0x1.7c1ed0130c132p+0, 0x1.7e2f336cf4e62p+0, 0x1.80427543e1a12p+0,
+    0x1.82589994cce13p+0, 0x1.8471a4623c7adp+0, 0x1.868d99b4492edp+0, 0x1.88ac7d98a6699p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8cf3216b5448cp+0, 0x1.8f1ae99157736p+0, 0x1.9145b0b91ffc6p+0,
+    0x1.93737b0cdc5e5p+0, 0x1.95a44cbc8520fp+0, 0x1.97d829fde4e50p+0, 0x1.9a0f170ca07bap+0,
+    0x1.9c49182a3f090p+0, 0x1.9e86319e32323p+0, 0x1.a0c667b5de565p+0, 0x1.a309bec4a2d33p+0,
+    0x1.a5503b23e255dp+0, 0x1.a799e1330b358p+0, 0x1.a9e6b5579fdbfp+0, 0x1.ac36bbfd3f37ap+0,
+    0x1.ae89f995ad3adp+0, 0x1.b0e07298db666p+0, 0x1.b33a2b84f15fbp+0, 0x1.b59728de5593ap+0,
+    0x1.b7f76f2fb5e47p+0, 0x1.ba5b030a1064ap+0, 0x1.bcc1e904bc1d2p+0, 0x1.bf2c25bd71e09p+0,
+    0x1.c199bdd85529cp+0, 0x1.c40ab5fffd07ap+0, 0x1.c67f12e57d14bp+0, 0x1.c8f6d9406e7b5p+0,
+    0x1.cb720dcef9069p+0, 0x1.cdf0b555dc3fap+0, 0x1.d072d4a07897cp+0, 0x1.d2f87080d89f2p+0,
+    0x1.d5818dcfba487p+0, 0x1.d80e316c98398p+0, 0x1.da9e603db3285p+0, 0x1.dd321f301b460p+0,
+    0x1.dfc97337b9b5fp+0, 0x1.e264614f5a129p+0, 0x1.e502ee78b3ff6p+0, 0x1.e7a51fbc74c83p+0,
+    0x1.ea4afa2a490dap+0, 0x1.ecf482d8e67f1p+0, 0x1.efa1bee615a27p+0, 0x1.f252b376bba97p+0,
+    0x1.f50765b6e4540p+0, 0x1.f7bfdad9cbe14p+0, 0x1.fa7c1819e90d8p+0, 0x1.fd3c22b8f71f1p+0,
+};
+
+// e^((x - top) / T) to 3e-12: a u that falls between the sums of two evaluations that near is a one in
+// 10^5 event over a row of 10^5 entries. 2^(i + j/128 + f/128), |f| <= 1/2: a table in LDS, a cubic,
+// an exponent: 16 instructions, where the library's exp takes three times that.
 struct Weight {
-    double top, inv_t, unit;
+    const double *pow2;   // LDS copy of POW2
+    double top, scale, unit;   // scale = 128 log2(e) / T
     bool hard;   // only entries equal to the largest weigh: temperature 0, or +inf among them
     __device__ __forceinline__ double real(float x) const {
         if (hard) return (double)x == top ? 1.0 : 0.0;
-        return exp(((double)x - top) * inv_t);
+        const double y = fmax(((double)x - top) * scale, -140800.0);   // 2^-1100 and below: 0
+        const double w = rint(y), f = y - w;
+        const int i = (int)w;
+        // (ln 2 / 128)^k / k!
+        double e = fma(f, 0x1.c6b08d704a0bfp-26, 0x1.ebfbdff82c58ep-17);
+        e = fma(f, e, 0x1.62e42fefa39efp-8);
+        const double m = pow2[i & 127];
+        return ldexp(fma(m, f * e, m), i >> 7);
     }
-    __device__ __forceinline__ uint64_t fixed(double w) const { return (uint64_t)rint(w * unit); }
+    // w unit rounded to a whole number: w unit <= 2^51, so that adding 2^52 leaves it in the low bits
+    __device__ __forceinline__ uint64_t fixed(double w) const {
+        return (uint64_t)__double_as_longlong(fma(w, unit, 0x1p52)) & 0xFFFFFFFFFFFFFull;
+    }
 };
+__device__ __forceinline__ Weight weight(const SampleArgs &A, const SampleRow &s, const double *pow2, float top) {
+    return Weight{pow2, (double)top, s.inv_t * 0x1.71547652b82fep+7, A.unit, s.greedy || top == INFINITY};
+}
 
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) pack8 {
@@ -111,6 +180,10 @@ __device__ __forceinline__ V wave_sum(V v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float x) {
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true)));
+}
 
 __device__ __forceinline__ void answer(const SampleArgs &A, int64_t r, int i, double prob) {
     if (A.act) {
@@ -121,9 +194,62 @@ __device__ __forceinline__ void answer(const SampleArgs &A, int64_t r, int i, do
     if (A.prob) A.prob[r] = (float)prob;
 }
 
+// a piece's records: tops[GP], NaN where one is among the 64, and with_mass the sum of the weights
+// relative to the piece's own largest entry
+__device__ __forceinline__ void piece_records(const float *v, bool with_mass, double scale, const double *pow2, float *tops,
+                                              double *mass) {
+    const int lane = threadIdx.x & 63;
+    float top = v[0];
+    bool nan = v[0] != v[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+        nan |= v[e] != v[e];
+        top = fmaxf(top, v[e]);
+    }
+    top = nan ? -INFINITY : top;
+    top = dpp_max<0xB1>(top);    // lanes ^ 1
+    top = dpp_max<0x4E>(top);    // lanes ^ 2
+    top = dpp_max<0x141>(top);   // mirrored in 8
+    const uint64_t nans = __ballot(nan);
+    if ((lane & 7) == 0) tops[lane >> 3] = (nans >> lane) & 255 ? NAN : top;
+    if (!with_mass) return;
+    top = dpp_max<0x140>(top);   // mirrored in 16
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const Weight W{pow2, (double)top, scale, 0.0, top == INFINITY};
+    double m = 0.0;
+    if (top != -INFINITY && !nans) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m += W.real(v[e]);   // -inf: 0
+    }
+    m = wave_sum(m);
+    if (lane == 0) *mass = m;
+}
+
+// ---------------------------------------------------------------- the scan: a wave a piece
+template <class T>
+__global__ __launch_bounds__(256) void sample_scan_kernel(SampleArgs A, int pieces, int64_t total) {
+    __shared__ double pow2[128];
+    if (threadIdx.x < 128) pow2[threadIdx.x] = POW2[threadIdx.x];
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    for (int64_t k = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); k < total;
+         k += (int64_t)gridDim.x * 4) {
+        const int64_t r = k / pieces;
+        const int c = (int)(k - r * pieces);
+        const SampleRow s = sample_row(A, r);
+        float v[8];
+        load8((const T *)A.x + r * A.ld, A.mask ? A.mask + r * A.ld_mask : nullptr, c * PIECE + lane * 8, A.n, v);
+        piece_records(v, s.whole(A.n), s.inv_t * 0x1.71547652b82fep+7, pow2, A.tops + k * GP, A.masses + k);
+    }
+}
+
 // ---------------------------------------------------------------- a thread a row: n <= N
 template <class T, int N>
 __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
+    __shared__ double pow2[128];
+    if (threadIdx.x < 128) pow2[threadIdx.x] = POW2[threadIdx.x];
+    __syncthreads();
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (r >= A.rows) return;
     const SampleRow s = sample_row(A, r);
@@ -141,7 +267,7 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
         answer(A, r, -1, nan ? NAN : 0.0);
         return;
     }
-    const Weight W{(double)top, s.inv_t, A.unit, s.greedy || top == INFINITY};
+    const Weight W = weight(A, s, pow2, top);
     uint64_t w[N], s1 = 0, sum = 0;
     int rank[N];
     bool kept[N];
@@ -181,9 +307,6 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
 }
 
 // ---------------------------------------------------------------- a workgroup a row
-constexpr int RW = 16;          // waves
-constexpr int SEGS = 1024;      // most segments the row's masses are kept by
-
 // exclusive prefix of v over the workgroup's threads; total: of all. sh: RW + 1 values
 template <class V>
 __device__ __forceinline__ V block_scan(V v, V *sh, V &total) {
@@ -203,35 +326,66 @@ __device__ __forceinline__ V block_scan(V v, V *sh, V &total) {
     return sh[wave] + in - v;
 }
 
-template <class T>
+// distance from the top by 64 steps an octave, 2^-12 .. 2^20: a bound that outliers do not spoil
+__device__ __forceinline__ int far_bin(float d) {
+    const int b = (int)(__float_as_uint(d) >> 17) - ((127 - 12) << 6);
+    return min(max(b, 0), BINS - 1);
+}
+
+struct Total {
+    uint32_t count;
+    uint64_t mass;
+};
+
+template <class T, bool FUSED>
 __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
+    __shared__ double pow2[128];
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
     __shared__ uint64_t seg_mass[SEGS];
     __shared__ uint32_t seg_ties[SEGS];
+    __shared__ uint32_t list_key[LIST], list_at[LIST];
     __shared__ uint64_t scan64[RW + 1];
+    __shared__ double scanf[RW + 1];
     __shared__ uint32_t scan32[RW + 1];
+    __shared__ float own_tops[FUSED ? RW * GP : 1];
+    __shared__ double own_masses[FUSED ? RW : 1];
     __shared__ float wave_top[RW];
     __shared__ int wave_nan[RW];
     __shared__ uint64_t found_mass;
-    __shared__ uint32_t found_bin, found_count;
+    __shared__ double found_sum;
+    __shared__ uint32_t found_bin, found_count, listed;
     const int64_t r = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = A.n;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = A.n;
     const SampleRow s = sample_row(A, r);
     const T *x = (const T *)A.x + r * A.ld;
     const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
-    const int pieces = (n + PIECE - 1) / PIECE;
+    const int pieces = (n + PIECE - 1) / PIECE, groups = pieces * GP;
+    if (tid < 128) pow2[tid] = POW2[tid];
+    if (tid == 0) listed = 0;
 
+    const float *tops;
+    const double *masses;
+    if constexpr (FUSED) {
+        __syncthreads();
+        if (wave < pieces) {
+            float v[8];
+            load8(x, mask, wave * PIECE + lane * 8, n, v);
+            piece_records(v, s.whole(n), s.inv_t * 0x1.71547652b82fep+7, pow2, own_tops + wave * GP, own_masses + wave);
+        }
+        __syncthreads();
+        tops = own_tops;
+        masses = own_masses;
+    } else {
+        tops = A.tops + r * pieces * GP;
+        masses = A.masses + r * pieces;
+    }
     float top = -INFINITY;
     bool nan = false;
-    for (int c = wave; c < pieces; c += RW) {
-        float v[8];
-        load8(x, mask, c * PIECE + lane * 8, n, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            nan |= v[e] != v[e];
-            top = fmaxf(top, v[e]);
-        }
+    for (int g = tid; g < groups; g += 1024) {
+        const float t = tops[g];
+        nan |= t != t;
+        top = fmaxf(top, t);
     }
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     nan = __ballot(nan) != 0;
@@ -248,181 +402,391 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
         if (tid == 0) answer(A, r, -1, nan ? NAN : 0.0);
         return;
     }
-    const Weight W{(double)top, s.inv_t, A.unit, s.greedy || top == INFINITY};
+    const Weight W = weight(A, s, pow2, top);
+    const double q = (double)s.q;
+    const int per = (pieces + SEGS - 1) / SEGS, segs = (pieces + per - 1) / per;   // pieces a segment, segments
+
+    // the whole row's mass by segment, from the pieces' masses
+    double seg_sum = 0.0, sum_ex = 0.0, row_sum = 0.0;
+    if (s.whole(n)) {
+        if (tid < segs)
+            for (int c = tid * per; c < min((tid + 1) * per, pieces); ++c) {
+                float t = tops[c * GP];
+#pragma unroll
+                for (int g = 1; g < GP; ++g) t = fmaxf(t, tops[c * GP + g]);
+                if (t != -INFINITY) seg_sum += masses[c] * W.real(t);
+            }
+        sum_ex = block_scan<double>(seg_sum, scanf, row_sum);
+    }
 
     // the cut: keys above kt, and the first nt of those equal to it
     uint32_t kt = 0, nt = 0;
-    // the key at which a prefix of the order ends, three levels of a radix search: by count (the
-    // prefix has k entries) or by mass (the last entry with less than `limit` before it). From
-    // keys >= least. above_*: of the keys over the found one; count_in: of the found one itself.
-    uint64_t above_mass = 0;
-    uint32_t above_count = 0, count_in = 0;
-    auto search = [&](bool by_mass, bool with_mass, uint32_t least, uint32_t k, double limit) {
-        uint32_t prefix = 0;
-        above_mass = 0;
-        above_count = 0;
-        for (int level = 0; level < 3; ++level) {
-            const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
-            for (int b = tid; b < BINS; b += 1024) {
-                mass[b] = 0;
-                count[b] = 0;
-            }
+    double target = 0.0, scale_out = 0.0;   // u S; the probability's 1 / S
+    int seg = 0;
+    uint64_t base = 0;
+    uint32_t ties = 0;
+    const bool cut = s.k < n || s.p < 1.0f, plain = !cut && q == 0.0;
+    double base_real = 0.0;
+    if (plain) {
+        // nothing is filtered: the segment by the pieces' masses
+        target = (double)s.u * row_sum;
+        scale_out = 1.0 / row_sum;
+        if (tid == 0) found_bin = 0;
+        __syncthreads();
+        // the last segment whose prefix is not over the target, of those that weigh anything
+        if (seg_sum > 0.0 && !(sum_ex > target)) atomicMax(&found_bin, (uint32_t)tid);
+        __syncthreads();
+        if (tid == (int)found_bin) found_sum = sum_ex;
+        __syncthreads();
+        seg = (int)found_bin;
+        base_real = found_sum;
+    } else {
+        // candidates: what can be in the cut, by the groups' maxima
+        int far = BINS - 1;   // candidates lie in bins up to here
+        // and, where min-p is not to change the mass that top-p goes by, this near
+        const bool by_q = s.q > 0.0f && s.p >= 1.0f;
+        const float near = by_q ? (float)(-log((double)s.q) / s.inv_t) * 1.0001f + 1e-30f : INFINITY;
+        auto candidate = [&](float v) __attribute__((always_inline)) {
+            const float d = top - v;   // NaN for two infinities: top itself
+            return v != -INFINITY && !(d > near) && far_bin(d > 0.0f ? d : 0.0f) <= far;
+        };
+        bool use_list = true;
+        if (W.hard) {
+            far = 0;
+        } else if (cut) {
+            // the bin that the wanted-th largest maximum falls in: at least that many entries are as near
+            for (int b = tid; b < BINS; b += 1024) count[b] = 0;
             __syncthreads();
+            for (int g = tid; g < groups; g += 1024) {
+                const float t = tops[g];
+                if (t != -INFINITY) atomicAdd(&count[far_bin(top - t)], 1u);
+            }
+            if (tid == 0) found_bin = BINS - 1;
+            __syncthreads();
+            const uint32_t c0 = count[2 * tid], c1 = count[2 * tid + 1];
+            uint32_t all;
+            const uint32_t ex = block_scan<uint32_t>(c0 + c1, scan32, all);
+            // top-p alone: a list that most distributions' nucleus fits into
+            const uint32_t wanted = s.k < n ? (uint32_t)s.k : max(1u, min((uint32_t)LIST / 2, all / 2));
+            if (ex < wanted && ex + c0 + c1 >= wanted) found_bin = ex + c0 >= wanted ? 2 * tid : 2 * tid + 1;
+            __syncthreads();
+            far = (int)found_bin;
+            // fewer groups than wanted entries: everything would be a candidate
+            use_list = all >= wanted || n <= LIST || by_q;
+        }
+        if (use_list) {
             for (int c = wave; c < pieces; c += RW) {
+                const float t = lane < GP ? tops[c * GP + lane] : -INFINITY;
+                const uint64_t some = __ballot(candidate(t));
+                if (!some) continue;
                 float v[8];
                 load8(x, mask, c * PIECE + lane * 8, n, v);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const uint32_t key = key_of(v[e]);
-                    if (key == 0 || key < least || (level > 0 && key >> (shift + bits) != prefix)) continue;
-                    const uint32_t b = (key >> shift) & ((1u << bits) - 1);
-                    atomicAdd(&count[b], 1u);
-                    if (with_mass)
-                        atomicAdd((unsigned long long *)&mass[b], (unsigned long long)W.fixed(W.real(v[e])));
+                    const bool is = candidate(v[e]);
+                    const uint64_t who = __ballot(is);
+                    if (!who) continue;
+                    uint32_t at = 0;
+                    if (lane == 0) at = atomicAdd(&listed, (uint32_t)__popcll(who));
+                    at = __builtin_amdgcn_readfirstlane(at) + (uint32_t)__popcll(who & ((1ull << lane) - 1));
+                    if (is && at < LIST) {
+                        list_key[at] = key_of(v[e]);
+                        list_at[at] = (uint32_t)(c * PIECE + lane * 8 + e);
+                    }
                 }
             }
-            __syncthreads();
-            // bins from the top, two a thread
-            const int b0 = BINS - 1 - 2 * tid, b1 = b0 - 1;
-            const uint64_t m0 = mass[b0], m1 = mass[b1];
-            const uint32_t c0 = count[b0], c1 = count[b1];
-            uint64_t m_all;
-            uint32_t c_all;
-            const uint64_t m_ex = above_mass + block_scan<uint64_t>(m0 + m1, scan64, m_all);
-            const uint32_t c_ex = above_count + block_scan<uint32_t>(c0 + c1, scan32, c_all);
-            auto test = [&](int b, uint64_t m, uint32_t c, uint64_t mb, uint32_t cb) {
-                const bool here = by_mass ? (double)mb < limit && (double)(mb + m) >= limit : cb < k && cb + c >= k;
-                if (here) {   // one bin of one thread
-                    found_bin = (uint32_t)b;
-                    found_mass = mb;
-                    found_count = cb;
-                }
-            };
-            test(b0, m0, c0, m_ex, c_ex);
-            test(b1, m1, c1, m_ex + m0, c_ex + c0);
-            __syncthreads();
-            const uint32_t b = found_bin & (BINS - 1);
-            above_mass = found_mass;
-            above_count = found_count;
-            count_in = count[b];
-            prefix = (prefix << bits) | b;
-            __syncthreads();
         }
-        return prefix;
-    };
-    const bool nucleus = s.p < 1.0f && !s.greedy;
-    uint64_t s1 = 0;
-    if (s.greedy) {
-        kt = key_of(top);
-        nt = 1;
-    } else {
-        bool whole = true;   // no top-k cut
-        if (s.k < n) {
-            // fewer allowed entries than k: nothing to cut
-            uint32_t allowed = 0;
-            for (int c = wave; c < pieces; c += RW) {
-                float v[8];
-                load8(x, mask, c * PIECE + lane * 8, n, v);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) allowed += v[e] != -INFINITY;
+        __syncthreads();
+        uint32_t m = use_list ? listed : LIST + 1;
+        const double limit_row = (double)s.p * row_sum * A.unit;   // top-p alone, in units
+        if (m <= PAIRS) {
+            // each candidate's rank and mass before it, by comparing all pairs: four threads each
+            const int j = tid >> 2;
+            const uint32_t kj = j < (int)m ? list_key[j] : 0, aj = j < (int)m ? list_at[j] : 0;
+            if (tid < (int)m) mass[tid] = W.fixed(W.real(of_key(list_key[tid])));
+            __syncthreads();
+            uint32_t rank = 0;
+            uint64_t before = 0;
+            for (uint32_t i = tid & 3; i < m; i += 4) {
+                const uint32_t ki = list_key[i];
+                const bool first = ki > kj || (ki == kj && list_at[i] < aj);
+                rank += first;
+                before += first ? mass[i] : 0;
             }
-            uint32_t all;
-            block_scan<uint32_t>(allowed, scan32, all);
-            if (all > (uint32_t)s.k) {
-                kt = search(false, nucleus, 0, (uint32_t)s.k, 0.0);
-                nt = (uint32_t)s.k - above_count;
-                s1 = above_mass + nt * W.fixed(W.real(of_key(kt)));
-                whole = false;
+            rank += __shfl_xor(rank, 1);
+            rank += __shfl_xor(rank, 2);
+            before += __shfl_xor(before, 1);
+            before += __shfl_xor(before, 2);
+            const bool own = (tid & 3) == 0 && j < (int)m;
+            const uint64_t wj = j < (int)m ? mass[j] : 0;
+            const bool in_k = own && rank < (uint32_t)s.k;
+            uint64_t s1;
+            block_scan<uint64_t>(in_k ? wj : 0, scan64, s1);
+            // top-p alone: the list has to hold all of the nucleus
+            const bool inside = s.k < n || s.p >= 1.0f || (double)s1 >= limit_row;
+            if (inside) {
+                const double limit = s.k < n ? (double)s.p * (double)s1 : limit_row;
+                const double real = own ? W.real(of_key(kj)) : 0.0;
+                const bool kept = in_k && (s.p >= 1.0f || rank == 0 || (double)before < limit) && real >= q;
+                if (own) seg_mass[j] = kept ? wj : 0;
+                uint64_t sum;
+                block_scan<uint64_t>(kept ? wj : 0, scan64, sum);   // and its barriers
+                uint64_t upto = 0;
+                for (uint32_t i = tid & 3; i < m; i += 4) upto += list_at[i] <= aj ? seg_mass[i] : 0;
+                upto += __shfl_xor(upto, 1);
+                upto += __shfl_xor(upto, 2);
+                const double t = (double)s.u * (double)sum;
+                if (kept && wj && (double)upto > t && !((double)(upto - wj) > t))   // one thread
+                    answer(A, r, (int)aj, real * A.unit / (double)sum);
+                return;
             }
+            __syncthreads();
+            m = LIST + 1;
         }
-        if (nucleus) {
-            if (whole) {
-                uint64_t part = 0;
+        // larger cuts: a radix search over the listed candidates or, where they are too many, the row
+        bool from_list = m <= LIST;
+        auto each = [&](auto &&f) __attribute__((always_inline)) {   // f(x, index) for every candidate, or every entry
+            if (from_list) {
+                for (uint32_t i = tid; i < m; i += 1024) f(of_key(list_key[i]), (int)list_at[i]);
+            } else {
                 for (int c = wave; c < pieces; c += RW) {
                     float v[8];
                     load8(x, mask, c * PIECE + lane * 8, n, v);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (v[e] != -INFINITY) part += W.fixed(W.real(v[e]));
+                    for (int e = 0; e < 8; ++e) f(v[e], c * PIECE + lane * 8 + e);
                 }
-                block_scan<uint64_t>(part, scan64, s1);
             }
-            const double limit = (double)s.p * (double)s1;
-            if (limit <= 0.0) {
-                kt = key_of(top);
-                nt = 1;
-            } else {
-                const uint32_t kk = kt, kn = nt;
-                kt = search(true, true, kk, 0, limit);
-                // tie j stays while above + j w < limit
-                const uint64_t w = W.fixed(W.real(of_key(kt)));
-                const double more = w ? ceil((limit - (double)above_mass) / (double)w) : (double)count_in;
-                nt = (uint32_t)fmin(fmax(more, 1.0), (double)count_in);
-                if (kt == kk) nt = min(nt, kn);
+        };
+        // the key at which a prefix of the order ends, three levels of a radix search: by count (the
+        // prefix has k entries) or by mass (the last entry with less than `limit` before it). From
+        // keys >= least. above_*: of the keys over the found one; count_in: of the found one itself.
+        uint64_t above_mass = 0;
+        uint32_t above_count = 0, count_in = 0;
+        auto search = [&](bool by_mass, bool with_mass, uint32_t least, uint32_t k, double limit) __attribute__((always_inline)) {
+            uint32_t prefix = 0;
+            above_mass = 0;
+            above_count = 0;
+            for (int level = 0; level < 3; ++level) {
+                const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
+                for (int b = tid; b < BINS; b += 1024) {
+                    mass[b] = 0;
+                    count[b] = 0;
+                }
+                __syncthreads();
+                each([&](float v, int) __attribute__((always_inline)) {
+                    const uint32_t key = key_of(v);
+                    if (key == 0 || key < least || (level > 0 && key >> (shift + bits) != prefix)) return;
+                    const uint32_t b = (key >> shift) & ((1u << bits) - 1);
+                    atomicAdd(&count[b], 1u);
+                    if (with_mass) atomicAdd((unsigned long long *)&mass[b], (unsigned long long)W.fixed(W.real(v)));
+                });
+                __syncthreads();
+                // bins from the top, two a thread
+                const int b0 = BINS - 1 - 2 * tid, b1 = b0 - 1;
+                const uint64_t m0 = mass[b0], m1 = mass[b1];
+                const uint32_t c0 = count[b0], c1 = count[b1];
+                uint64_t m_all;
+                uint32_t c_all;
+                const uint64_t m_ex = above_mass + block_scan<uint64_t>(m0 + m1, scan64, m_all);
+                const uint32_t c_ex = above_count + block_scan<uint32_t>(c0 + c1, scan32, c_all);
+                auto test = [&](int b, uint64_t mb, uint32_t cb, uint64_t m_before, uint32_t c_before) __attribute__((always_inline)) {
+                    const bool here = by_mass ? (double)m_before < limit && (double)(m_before + mb) >= limit
+                                              : c_before < k && c_before + cb >= k;
+                    if (here) {   // one bin of one thread
+                        found_bin = (uint32_t)b;
+                        found_mass = m_before;
+                        found_count = c_before;
+                    }
+                };
+                test(b0, m0, c0, m_ex, c_ex);
+                test(b1, m1, c1, m_ex + m0, c_ex + c0);
+                __syncthreads();
+                const uint32_t b = found_bin & (BINS - 1);
+                above_mass = found_mass;
+                above_count = found_count;
+                count_in = count[b];
+                prefix = (prefix << bits) | b;
+                __syncthreads();
+            }
+            return prefix;
+        };
+        auto total_of = [&]() __attribute__((always_inline)) {   // entries and their mass
+            uint32_t c = 0;
+            uint64_t w = 0;
+            each([&](float v, int) __attribute__((always_inline)) {
+                if (v == -INFINITY) return;
+                c += 1;
+                w += W.fixed(W.real(v));
+            });
+            uint64_t w_all;
+            uint32_t c_all;
+            block_scan<uint64_t>(w, scan64, w_all);
+            block_scan<uint32_t>(c, scan32, c_all);
+            return Total{c_all, w_all};
+        };
+        if (W.hard && s.greedy) {
+            kt = key_of(top);
+            nt = 1;
+        } else if (cut) {
+            auto all = total_of();
+            if (from_list && s.k == n && (double)all.mass < limit_row) {   // the nucleus is not inside the list
+                from_list = false;
+                all = total_of();
+            }
+            uint64_t s1 = all.mass;
+            bool k_cut = false;
+            if (s.k < n && all.count > (uint32_t)s.k) {
+                kt = search(false, s.p < 1.0f, 0, (uint32_t)s.k, 0.0);
+                nt = (uint32_t)s.k - above_count;
+                s1 = above_mass + nt * W.fixed(W.real(of_key(kt)));
+                k_cut = true;
+            }
+            if (s.p < 1.0f) {
+                // with a list, the entries behind it count in the limit only
+                const double limit = from_list && s.k == n ? limit_row : (double)s.p * (double)s1;
+                if (limit <= 0.0) {
+                    kt = key_of(top);
+                    nt = 1;
+                } else {
+                    const uint32_t kk = kt, kn = nt;
+                    kt = search(true, true, kk, 0, limit);
+                    // tie j stays while above + j w < limit
+                    const uint64_t w = W.fixed(W.real(of_key(kt)));
+                    const double more = w ? ceil((limit - (double)above_mass) / (double)w) : (double)count_in;
+                    nt = (uint32_t)fmin(fmax(more, 1.0), (double)count_in);
+                    if (k_cut && kt == kk) nt = min(nt, kn);
+                }
             }
         }
-    }
-    const bool cut = kt != 0;
+        const bool bounded = kt != 0;
 
-    // masses by segment, in index order
-    const int per = (pieces + SEGS - 1) / SEGS, segs = (pieces + per - 1) / per;
-    const double q = (double)s.q;
-    for (int g = wave; g < segs; g += RW) {
-        uint64_t m = 0;
-        uint32_t ties = 0;
-        for (int c = g * per; c < min((g + 1) * per, pieces); ++c) {
-            float v[8];
-            load8(x, mask, c * PIECE + lane * 8, n, v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t key = key_of(v[e]);
+        // masses and ties by segment, in index order
+        const double wt = bounded ? W.real(of_key(kt)) : 0.0;
+        const uint64_t wtie = wt >= q ? W.fixed(wt) : 0;
+        if (from_list) {
+            seg_mass[tid] = 0;
+            seg_ties[tid] = 0;
+            __syncthreads();
+            each([&](float v, int i) __attribute__((always_inline)) {
+                const uint32_t key = key_of(v);
+                const int g = i / PIECE / per;
                 if (key > kt) {
-                    const double w = W.real(v[e]);
-                    m += w >= q ? W.fixed(w) : 0;
+                    const double w = W.real(v);
+                    if (w >= q) atomicAdd((unsigned long long *)&seg_mass[g], (unsigned long long)W.fixed(w));
+                } else if (bounded && key == kt) {
+                    atomicAdd(&seg_ties[g], 1u);
                 }
-                ties += cut && key == kt;
+            });
+        } else {
+            for (int g = wave; g < segs; g += RW) {
+                uint64_t w_sum = 0;
+                uint32_t t_sum = 0;
+                for (int c = g * per; c < min((g + 1) * per, pieces); ++c) {
+                    float v[8];
+                    load8(x, mask, c * PIECE + lane * 8, n, v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t key = key_of(v[e]);
+                        if (key > kt) {
+                            const double w = W.real(v[e]);
+                            w_sum += w >= q ? W.fixed(w) : 0;
+                        }
+                        t_sum += bounded && key == kt;
+                    }
+                }
+                w_sum = wave_sum(w_sum);
+                t_sum = wave_sum(t_sum);
+                if (lane == 0) {
+                    seg_mass[g] = w_sum;
+                    seg_ties[g] = t_sum;
+                }
             }
         }
-        m = wave_sum(m);
-        ties = wave_sum(ties);
-        if (lane == 0) {
-            seg_mass[g] = m;
-            seg_ties[g] = ties;
+        __syncthreads();
+        const uint32_t mine = tid < segs ? seg_ties[tid] : 0;
+        uint32_t all_ties;
+        const uint32_t ties_ex = block_scan<uint32_t>(mine, scan32, all_ties);
+        const uint32_t left = nt > ties_ex ? nt - ties_ex : 0;
+        const uint64_t here = (tid < segs ? seg_mass[tid] : 0) + (uint64_t)min(mine, left) * wtie;
+        uint64_t sum;
+        const uint64_t m_ex = block_scan<uint64_t>(here, scan64, sum);
+        target = (double)s.u * (double)sum;
+        scale_out = A.unit / (double)sum;
+        if ((double)(m_ex + here) > target && !((double)m_ex > target)) {   // one thread
+            found_bin = (uint32_t)tid;
+            found_mass = m_ex;
+            found_count = ties_ex;
         }
+        __syncthreads();
+        seg = (int)found_bin;
+        base = found_mass;
+        ties = found_count;
     }
-    __syncthreads();
-    const double wt = cut ? W.real(of_key(kt)) : 0.0;
-    const uint64_t wtie = wt >= q ? W.fixed(wt) : 0;
-    const uint32_t mine = tid < segs ? seg_ties[tid] : 0;
-    uint32_t all_ties;
-    const uint32_t ties_ex = block_scan<uint32_t>(mine, scan32, all_ties);
-    const uint32_t left = nt > ties_ex ? nt - ties_ex : 0;
-    const uint64_t m = (tid < segs ? seg_mass[tid] : 0) + (uint64_t)min(mine, left) * wtie;
-    uint64_t sum;
-    const uint64_t m_ex = block_scan<uint64_t>(m, scan64, sum);
-    const double target = (double)s.u * (double)sum;
-    if ((double)(m_ex + m) > target && !((double)m_ex > target)) {   // one thread
-        found_bin = (uint32_t)tid;
-        found_mass = m_ex;
-        found_count = ties_ex;
-    }
-    __syncthreads();
     if (wave != 0) return;
 
-    // inside the segment
-    uint64_t base = found_mass;
-    uint32_t ties = found_count;
-    const int g = (int)found_bin;
-    for (int c = g * per; c < min((g + 1) * per, pieces); ++c) {
+    // inside the segment, one wave
+    if (plain) {
+        int last = -1;   // if rounding leaves the target just over the segment's end
+        float xl = 0.0f;
+        for (int c = seg * per; c < min((seg + 1) * per, pieces); ++c) {
+            float v[8];
+            const int i = c * PIECE + lane * 8;
+            load8(x, mask, i, n, v);
+            double w8[8], own = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w8[e] = W.real(v[e]);
+                own += w8[e];
+            }
+            const double in = wave_scan(own, lane);
+            double upto = base_real + (in - own);
+            int at = -1;
+            float xa = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                upto += w8[e];
+                if (at < 0 && w8[e] > 0.0 && upto > target) {
+                    at = i + e;
+                    xa = v[e];
+                }
+            }
+            const uint64_t hits = __ballot(at >= 0);
+            if (hits) {
+                if (lane == __ffsll((unsigned long long)hits) - 1) answer(A, r, at, W.real(xa) * scale_out);
+                return;
+            }
+            int mine = -1;
+            float xm = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (w8[e] > 0.0) {
+                    mine = i + e;
+                    xm = v[e];
+                }
+            const uint64_t some = __ballot(mine >= 0);
+            if (some) {
+                const int who = 63 - __clzll((long long)some);
+                last = __shfl(mine, who);
+                xl = __shfl(xm, who);
+            }
+            base_real += __shfl(in, 63);
+        }
+        if (lane == 0) answer(A, r, last, W.real(xl) * scale_out);
+        return;
+    }
+    const bool bounded = kt != 0;
+    const double wt = bounded ? W.real(of_key(kt)) : 0.0;
+    const uint64_t wtie = wt >= q ? W.fixed(wt) : 0;
+    for (int c = seg * per; c < min((seg + 1) * per, pieces); ++c) {
         float v[8];
         const int i = c * PIECE + lane * 8;
         load8(x, mask, i, n, v);
         uint32_t t = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t += cut && key_of(v[e]) == kt;
+        for (int e = 0; e < 8; ++e) t += bounded && key_of(v[e]) == kt;
         const uint32_t t_in = wave_scan(t, lane);
         uint32_t rank = ties + t_in - t;
-        uint64_t w8[8], lane_mass = 0;
+        uint64_t w8[8], own = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint32_t key = key_of(v[e]);
@@ -430,13 +794,13 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
             if (key > kt) {
                 const double w = W.real(v[e]);
                 w8[e] = w >= q ? W.fixed(w) : 0;
-            } else if (cut && key == kt) {
+            } else if (bounded && key == kt) {
                 w8[e] = rank++ < nt ? wtie : 0;
             }
-            lane_mass += w8[e];
+            own += w8[e];
         }
-        const uint64_t in = wave_scan(lane_mass, lane);
-        uint64_t upto = base + in - lane_mass;
+        const uint64_t in = wave_scan(own, lane);
+        uint64_t upto = base + in - own;
         int at = -1;
         float xa = 0.0f;
 #pragma unroll
@@ -449,12 +813,17 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
         }
         const uint64_t hits = __ballot(at >= 0);
         if (hits) {
-            if (lane == __ffsll((unsigned long long)hits) - 1) answer(A, r, at, W.real(xa) * A.unit / (double)sum);
+            if (lane == __ffsll((unsigned long long)hits) - 1) answer(A, r, at, W.real(xa) * scale_out);
             return;
         }
         base += __shfl(in, 63);
         ties += __shfl(t_in, 63);
     }
+}
+
+static void check_shape(int64_t rows, int64_t n) {
+    SNK_CHECK(rows >= 0 && rows < (int64_t)1 << 31, SNK_ERR_INVALID, "sample: %lld rows", (long long)rows);
+    SNK_CHECK(n >= 1 && n <= 1 << 24, SNK_ERR_INVALID, "sample: %lld logits a row, 1 to 2^24 are supported", (long long)n);
 }
 
 static SampleArgs sample_args(const snk_sample_cfg_t *cfg, int64_t rows, int64_t n) {
@@ -464,8 +833,7 @@ static SampleArgs sample_args(const snk_sample_cfg_t *cfg, int64_t rows, int64_t
               cfg->struct_size, (int)sizeof(snk_sample_cfg_t));
     SNK_CHECK(cfg->dtype == SNK_F32 || cfg->dtype == SNK_BF16 || cfg->dtype == SNK_F16, SNK_ERR_INVALID,
               "sample: unknown element type %d", cfg->dtype);
-    SNK_CHECK(rows >= 0 && rows < (int64_t)1 << 31, SNK_ERR_INVALID, "sample: %lld rows", (long long)rows);
-    SNK_CHECK(n >= 1 && n <= 1 << 24, SNK_ERR_INVALID, "sample: %lld logits a row, 1 to 2^24 are supported", (long long)n);
+    check_shape(rows, n);
     SNK_CHECK(cfg->temperature >= 0 && cfg->temperature < INFINITY, SNK_ERR_INVALID, "sample: temperature %g",
               cfg->temperature);
     SNK_CHECK(cfg->top_k >= 0, SNK_ERR_INVALID, "sample: top_k %d is negative", cfg->top_k);
@@ -495,8 +863,15 @@ static void sample_launch_t(const SampleArgs &A, hipStream_t s) {
         sample_few_kernel<T, 4><<<few, 256, 0, s>>>(A);
     else if (A.n <= 8)
         sample_few_kernel<T, 8><<<few, 256, 0, s>>>(A);
-    else
-        sample_row_kernel<T><<<(unsigned)A.rows, 1024, 0, s>>>(A);
+    else if (A.n <= FUSED_N) {
+        sample_row_kernel<T, true><<<(unsigned)A.rows, 1024, 0, s>>>(A);
+    } else {
+        const int pieces = ceil_div(A.n, PIECE);
+        const int64_t total = A.rows * pieces;
+        sample_scan_kernel<T><<<(unsigned)std::min<int64_t>((total + 3) / 4, 4096), 256, 0, s>>>(A, pieces, total);
+        launch_check("sample_scan_kernel");
+        sample_row_kernel<T, false><<<(unsigned)A.rows, 1024, 0, s>>>(A);
+    }
     launch_check("sample kernel");
 }
 
@@ -516,8 +891,9 @@ using namespace snk;
 
 extern "C" int snk_sample_workspace(int64_t rows, int64_t n, int64_t *bytes) {
     return guard([&] {
-        SNK_CHECK(bytes && rows >= 0 && n >= 1, SNK_ERR_INVALID, "bad sample_workspace arguments");
-        *bytes = 0;
+        SNK_CHECK(bytes, SNK_ERR_INVALID, "sample_workspace: NULL argument");
+        check_shape(rows, n);
+        *bytes = n <= FUSED_N ? 0 : rows * ceil_div(n, PIECE) * (8 + 4 * GP);
     });
 }
 
@@ -545,6 +921,8 @@ extern "C" int snk_sample_logits(const void *logits, int64_t rows, int64_t n, in
         A.u = u;
         A.idx = idx;
         A.prob = prob;
+        A.masses = (double *)ws;
+        A.tops = (float *)ws + 2 * rows * ceil_div(n, PIECE);
         sample_launch(A, cfg->dtype, stream());
     });
 }

@@ -33,6 +33,7 @@ def _same(buffers, what):
 class _Handle:
     """What a user's handle and a model's have in common."""
 
+    _total = None
     _device = None   # the torch device of the tensors, None for DeviceArrays
     state_bits = 32
 
@@ -57,9 +58,11 @@ class _Handle:
     @property
     def total(self) -> int:
         """Places in the state layout: every tensor's size rounded up to 256."""
-        n = i64(0)
-        call("snk_adamw_layout", self._h, C.byref(n), None)
-        return n.value
+        if self._total is None:
+            n = i64(0)
+            call("snk_adamw_layout", self._h, C.byref(n), None)
+            self._total = n.value
+        return self._total
 
     @property
     def starts(self) -> list[int]:

@@ -6,6 +6,7 @@ Tensors are DeviceArrays or torch GPU tensors as in optim.py.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 
@@ -20,6 +21,9 @@ class SampleCfg(C.Structure):
 
     def __init__(self, *args, **kw):
         super().__init__(C.sizeof(self), *args, **kw)
+
+
+_CFG = struct.Struct("=iififfQQQQ")   # SampleCfg's bytes
 
 
 def _rows_of(x, b, what):
@@ -38,35 +42,23 @@ def _rows_of(x, b, what):
     return rows, n, st[0] if rows > 1 else n
 
 
-def _setting(value, rows, kind, keep, what):
-    """(number, device address) of a setting given as a number or as one value per row."""
-    if isinstance(value, (int, float)):
-        return value, None
-    b = _lib.device_buffer(value, what)
-    if b.dtype != kind or b.size != rows:
-        raise ValueError(f"{what}: expected {rows} values of type {kind}, got {b.size} of {b.dtype}")
-    keep.append(b)
-    return (0 if kind == "i32" else 1.0), b.ptr
-
-
 def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None, out=None, prob=None,
                   workspace=None):
     """One index per row of logits [rows, n] (or [n]), drawn with the given u [rows] in [0, 1).
 
     temperature, top_k, top_p and min_p (include/snakehip.h states the rules) are numbers or one
-    value per row (float32, top_k int32). mask: bytes or bools [rows, n], non-zero forbids. A torch
-    row stride of 0 (expand) shares one row. Returns out [rows] int32 (-1: nothing allowed), made
-    here if not given; prob [rows] float32, if given, receives the probabilities. workspace: a uint8
-    tensor of sample_workspace(rows, n) bytes, made here if not given; calls in flight at the same
-    time need one each."""
+    value per row (float32, top_k int32). mask: bytes or bools [rows, n], non-zero forbids; [n] is for
+    every row. A torch row stride of 0 (expand) shares one row. Returns out [rows] int32 (-1: nothing
+    allowed), made here if not given; prob [rows] float32, if given, receives the probabilities.
+    workspace: a uint8 tensor of sample_workspace(rows, n) bytes, made here if not given; calls in
+    flight at the same time need one each."""
     b = _lib.device_buffer(logits, "logits", contiguous=False)
+    device = b.device
     rows, n, ld = _rows_of(logits, b, "logits")
-    if b.dtype not in _lib.DTYPES:
+    dtype = _lib.DTYPES.get(b.dtype)
+    if dtype is None:
         raise ValueError(f"logits: elements of type {b.dtype}")
-    ub = _lib.device_buffer(u, "u")
-    keep = [b, ub]
-    if ub.dtype != "f32" or ub.size != rows:
-        raise ValueError(f"u: expected {rows} values of type f32, got {ub.size} of {ub.dtype}")
+    u_ptr = _lib.vector_ptr(u, "u", "f32", rows, device)
     m_ptr, ldm = None, n
     if mask is not None:
         mb = _lib.device_buffer(mask, "mask", contiguous=False)
@@ -75,37 +67,28 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
             raise ValueError(f"mask: expected bytes [{rows}, {n}] or [{n}], got {mb.dtype} {list(mb.shape)}")
         if mrows == 1:
             ldm = 0
+        _lib.same_device([mb], device)
         m_ptr = mb.ptr
-        keep.append(mb)
-    t, t_dev = _setting(temperature, rows, "f32", keep, "temperature")
-    k, k_dev = _setting(top_k, rows, "i32", keep, "top_k")
-    p, p_dev = _setting(top_p, rows, "f32", keep, "top_p")
-    q, q_dev = _setting(min_p, rows, "f32", keep, "min_p")
-    cfg = SampleCfg(_lib.DTYPES[b.dtype], t, k, p, q, t_dev, k_dev, p_dev, q_dev)
+    numbers, arrays = [temperature, top_k, top_p, min_p], [0, 0, 0, 0]
+    for i, (value, what, kind) in enumerate(((temperature, "temperature", "f32"), (top_k, "top_k", "i32"),
+                                             (top_p, "top_p", "f32"), (min_p, "min_p", "f32"))):
+        if not isinstance(value, (float, int)):
+            arrays[i] = _lib.vector_ptr(value, what, kind, rows, device)
+            numbers[i] = 0 if kind == "i32" else 1.0
+    cfg = _CFG.pack(_CFG.size, dtype, *numbers, *arrays)
     if out is None:
-        out = _new(b.device, rows, np.int32)
-    ob = _lib.device_buffer(out, "out")
-    if ob.dtype != "i32" or ob.size != rows:
-        raise ValueError(f"out: expected {rows} values of type i32, got {ob.size} of {ob.dtype}")
-    keep.append(ob)
-    pr = None
-    if prob is not None:
-        pb = _lib.device_buffer(prob, "prob")
-        if pb.dtype != "f32" or pb.size != rows:
-            raise ValueError(f"prob: expected {rows} values of type f32, got {pb.size} of {pb.dtype}")
-        keep.append(pb)
-        pr = pb.ptr
-    need = sample_workspace(rows, n)
+        out = _new(device, rows, np.int32)
+    o_ptr = _lib.vector_ptr(out, "out", "i32", rows, device)
+    p_ptr = None if prob is None else _lib.vector_ptr(prob, "prob", "f32", rows, device)
     w_ptr, w_bytes = None, 0
-    if need or workspace is not None:
+    need = sample_workspace(rows, n)
+    if need:
         if workspace is None:
-            workspace = _new(b.device, need, np.uint8)
+            workspace = _new(device, need, np.uint8)
         wb = _lib.device_buffer(workspace, "workspace")
-        keep.append(wb)
+        _lib.same_device([wb], device)
         w_ptr, w_bytes = wb.ptr, wb.size
-    _lib.same_device(keep)
-    _lib.call_on(b.device, "snk_sample_logits", b.ptr, rows, n, ld, m_ptr, ldm, ub.ptr, C.byref(cfg), ob.ptr, pr, w_ptr,
-                 w_bytes)
+    _lib.call_on(device, "snk_sample_logits", b.ptr, rows, n, ld, m_ptr, ldm, u_ptr, cfg, o_ptr, p_ptr, w_ptr, w_bytes)
     return out
 
 
@@ -119,7 +102,7 @@ def sample_workspace(rows: int, n: int) -> int:
 def _new(device, n, dtype):
     if device is None:
         return DeviceArray(n, dtype)
-    import torch
+    torch = _lib.torch_module()
     return torch.empty(n, dtype=torch.int32 if dtype is np.int32 else torch.uint8, device=device)
 
 
