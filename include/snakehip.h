@@ -240,8 +240,8 @@ int snk_dqn_update(snk_dqn m, snk_replay rb, const int64_t *idx_dev, int64_t B, 
  * a row (outside, or NaN: the nearest end). temperature <= 0: the first entry of the order, with
  * probability 1. No allowed entry: index -1, probability 0. An allowed NaN: -1 and NaN. Infinite
  * entries share all the mass. What masked places hold does not matter.
- * Masses are sums of 64-bit integers, units of 2^-(61 - ceil log2 n) of the largest weight but no
- * finer than 2^-51: the order of the additions does not change the answer. */
+ * Weights and sums are held in 64 bits. An entry lighter than half a unit, 2^-(61 - ceil log2 n) of
+ * the largest weight but no finer than 2^-51, is never drawn. Equal calls give equal answers. */
 typedef struct {
     int32_t struct_size;   /* = sizeof(snk_sample_cfg_t) = 56 */
     int32_t dtype;         /* of the logits: SNK_F32 / SNK_BF16 / SNK_F16 */

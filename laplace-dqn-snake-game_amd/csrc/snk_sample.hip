@@ -7,8 +7,10 @@
 // 2^-sh of the largest), so sums in LDS atomics are exact and always the same.
 //
 // A row is read once for what decides most rows: the largest logit of every 64 (a bound for top-k and
-// min-p) and, where the whole row's mass counts, the mass of every 512 (sample_scan_kernel). The row's
-// workgroup then reads again only the pieces of 512 that can hold an answer (sample_row_kernel).
+// min-p) and, where the whole row's mass counts, the mass of every 2048 (sample_scan_kernel). For
+// top-p alone two more passes over the row find the cut's neighbourhood and the masses above it
+// (sample_bins_kernel, sample_kept_kernel). The row's workgroup (sample_row_kernel) then reads only
+// what can hold the answer. Rows of up to 512 a wave are scanned by that workgroup itself.
 #include <algorithm>
 #include <cmath>
 
@@ -19,13 +21,19 @@ namespace snk {
 constexpr int PIECE = 512;      // consecutive elements a wave reads at once: 8 a lane
 constexpr int GROUP = 64;       // elements of a recorded maximum: 8 lanes' worth
 constexpr int GP = PIECE / GROUP;
+constexpr int BP = 4;           // pieces of a block, the scan's unit of mass
+constexpr int BLOCK = BP * PIECE;
 constexpr int BINS = 2048;      // of a level of the radix search: 11 + 11 + 10 bits of the key
-constexpr int RW = 16;          // waves of a row's workgroup
-constexpr int SEGS = 1024;      // most segments the row's masses are kept by
-constexpr int FUSED_N = RW * PIECE;   // rows up to here need no separate scan: a piece a wave
-constexpr int LIST = 2048;      // most candidates held in LDS
+constexpr int LIST = 1024;      // most candidates held in LDS
 constexpr int PAIRS = 256;      // ... compared each with each
+constexpr int NBINS = 1024;     // of the nucleus' mass over the distance from the top
+constexpr int NLIST = 512;      // most entries of the cut's bin that one split of a row lists
+constexpr int SPLITS = 16;      // most splits of a row
 
+struct SampleHead {             // the nucleus search's result
+    uint64_t above;             // mass over the bin
+    int32_t bin, ok;
+};
 struct SampleArgs {
     const void *x;
     int64_t rows, ld, ld_mask;
@@ -43,9 +51,17 @@ struct SampleArgs {
     uint8_t *act;
     uint64_t seed;
     const int64_t *tptr;
-    // the scan's records (workspace): [rows][pieces] masses, [rows][pieces][GP] maxima
+    // the scan's records (workspace), [rows][blocks]: masses relative to the block's largest entry,
+    // that entry, and the maxima of 64
     double *masses;
-    float *tops;
+    float *block_tops, *tops;
+    // top-p alone: rows row0.. of this launch, each in `splits` parts
+    int64_t row0;
+    int32_t splits;
+    uint64_t *bins, *kept;    // [row][split][NBINS], [row][blocks]
+    uint2 *lists;             // [row][split][NLIST] key, index
+    uint32_t *listed;         // [row][split]
+    SampleHead *heads;        // [row]; nullptr: not run
 };
 
 // a row's settings, the same for all its threads
@@ -56,6 +72,7 @@ struct SampleRow {
     float p, q, u;
     // whether the mass of the whole row is needed
     __device__ __forceinline__ bool whole(int n) const { return k == n && (p < 1.0f || q == 0.0f); }
+    __device__ __forceinline__ bool nucleus(int n) const { return k == n && p < 1.0f; }   // top-p alone
 };
 __device__ __forceinline__ SampleRow sample_row(const SampleArgs &A, int64_t r) {
     SampleRow s;
@@ -119,29 +136,35 @@ __device__ const double POW2[128] = {
 
 // e^((x - top) / T) to 3e-12: a u that falls between the sums of two evaluations that near is a one in
 // 10^5 event over a row of 10^5 entries. 2^(i + j/128 + f/128), |f| <= 1/2: a table in LDS, a cubic,
-// an exponent: 16 instructions, where the library's exp takes three times that.
+// and the exponent added to the table's: 15 instructions, a third of the library's exp. Entries behind
+// 2^-1000 (-inf too) weigh that much: callers leave excluded ones out themselves.
 struct Weight {
     const double *pow2;   // LDS copy of POW2
     double top, scale, unit;   // scale = 128 log2(e) / T
     bool hard;   // only entries equal to the largest weigh: temperature 0, or +inf among them
-    __device__ __forceinline__ double real(float x) const {
-        if (hard) return (double)x == top ? 1.0 : 0.0;
-        const double y = fmax(((double)x - top) * scale, -140800.0);   // 2^-1100 and below: 0
-        const double w = rint(y), f = y - w;
-        const int i = (int)w;
+    __device__ __forceinline__ double soft(float x) const {
+        const double y = fmax(((double)x - top) * scale, -128000.0);
+        const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);   // t's low word: y rounded
+        const int i = (int)(uint32_t)__double_as_longlong(t);
         // (ln 2 / 128)^k / k!
         double e = fma(f, 0x1.c6b08d704a0bfp-26, 0x1.ebfbdff82c58ep-17);
         e = fma(f, e, 0x1.62e42fefa39efp-8);
-        const double m = pow2[i & 127];
-        return ldexp(fma(m, f * e, m), i >> 7);
+        const uint64_t b = (uint64_t)__double_as_longlong(pow2[i & 127]);
+        const double m = __longlong_as_double((long long)(b + ((uint64_t)((uint32_t)(i & ~127) << 13) << 32)));
+        return fma(m, f * e, m);
+    }
+    __device__ __forceinline__ double real(float x) const {
+        if (hard) return (double)x == top ? 1.0 : 0.0;
+        return soft(x);
     }
     // w unit rounded to a whole number: w unit <= 2^51, so that adding 2^52 leaves it in the low bits
     __device__ __forceinline__ uint64_t fixed(double w) const {
         return (uint64_t)__double_as_longlong(fma(w, unit, 0x1p52)) & 0xFFFFFFFFFFFFFull;
     }
 };
+constexpr double LOG2E_128 = 0x1.71547652b82fep+7;
 __device__ __forceinline__ Weight weight(const SampleArgs &A, const SampleRow &s, const double *pow2, float top) {
-    return Weight{pow2, (double)top, s.inv_t * 0x1.71547652b82fep+7, A.unit, s.greedy || top == INFINITY};
+    return Weight{pow2, (double)top, s.inv_t * LOG2E_128, A.unit, s.greedy || top == INFINITY};
 }
 
 template <class T>
@@ -167,22 +190,58 @@ __device__ __forceinline__ void load8(const T *x, const uint8_t *mask, int i, in
     }
 }
 
+// v + v of the lane that CTRL names in the lanes of rows ROWS, v alone in the others
+template <class V, int CTRL, int ROWS>
+__device__ __forceinline__ V dpp_add(V v) {
+    constexpr int N = sizeof(V) / 4;
+    union {
+        V v;
+        int w[N];
+    } a, b;
+    a.v = v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) b.w[i] = __builtin_amdgcn_update_dpp(0, a.w[i], CTRL, ROWS, 0xf, false);
+    return v + b.v;
+}
+// inclusive prefix over the wave, always in the same order: six steps of lane moves, no LDS
 template <class V>
-__device__ __forceinline__ V wave_scan(V v, int lane) {   // inclusive
-    for (int o = 1; o < 64; o <<= 1) {
-        const V y = __shfl_up(v, o);
-        if (lane >= o) v += y;
-    }
-    return v;
+__device__ __forceinline__ V wave_scan(V v) {
+    v = dpp_add<V, 0x111, 0xf>(v);   // row_shr 1, 2, 4, 8: within 16 lanes
+    v = dpp_add<V, 0x112, 0xf>(v);
+    v = dpp_add<V, 0x114, 0xf>(v);
+    v = dpp_add<V, 0x118, 0xf>(v);
+    v = dpp_add<V, 0x142, 0xa>(v);   // row_bcast 15: into rows 1 and 3
+    return dpp_add<V, 0x143, 0xc>(v);   // row_bcast 31: into rows 2 and 3
+}
+template <class V>
+__device__ __forceinline__ V last_lane(V v) {
+    constexpr int N = sizeof(V) / 4;
+    union {
+        V v;
+        int w[N];
+    } a;
+    a.v = v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], 63);
+    return a.v;
 }
 template <class V>
 __device__ __forceinline__ V wave_sum(V v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    return last_lane(wave_scan(v));
 }
 template <int CTRL>
-__device__ __forceinline__ float dpp_max(float x) {
+__device__ __forceinline__ float dpp_max(float x) {   // for lane moves that have a source for every lane
     return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float max8(float x) {   // over each 8 lanes
+    x = dpp_max<0xB1>(x);      // lanes ^ 1
+    x = dpp_max<0x4E>(x);      // lanes ^ 2
+    return dpp_max<0x141>(x);  // mirrored in 8
+}
+__device__ __forceinline__ float max64(float x) {   // of max8's
+    x = dpp_max<0x140>(x);     // mirrored in 16
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
 }
 
 __device__ __forceinline__ void answer(const SampleArgs &A, int64_t r, int i, double prob) {
@@ -194,54 +253,247 @@ __device__ __forceinline__ void answer(const SampleArgs &A, int64_t r, int i, do
     if (A.prob) A.prob[r] = (float)prob;
 }
 
-// a piece's records: tops[GP], NaN where one is among the 64, and with_mass the sum of the weights
-// relative to the piece's own largest entry
-__device__ __forceinline__ void piece_records(const float *v, bool with_mass, double scale, const double *pow2, float *tops,
-                                              double *mass) {
+// records of the P pieces v that a wave holds: the maxima of 64 (NaN where one is among them), the
+// largest entry and, with_mass, the sum of the weights relative to it
+template <int P>
+__device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass, double scale, const double *pow2,
+                                             float *tops, float *top_out, double *mass) {
     const int lane = threadIdx.x & 63;
-    float top = v[0];
-    bool nan = v[0] != v[0];
+    float top = -INFINITY;
+    uint64_t any_nan = 0;
 #pragma unroll
-    for (int e = 1; e < 8; ++e) {
-        nan |= v[e] != v[e];
-        top = fmaxf(top, v[e]);
+    for (int p = 0; p < P; ++p) {
+        float t = v[p][0];
+        bool nan = t != t;
+#pragma unroll
+        for (int e = 1; e < 8; ++e) {
+            nan |= v[p][e] != v[p][e];
+            t = fmaxf(t, v[p][e]);
+        }
+        t = max8(nan ? -INFINITY : t);
+        const uint64_t nans = __ballot(nan);
+        any_nan |= nans;
+        if ((lane & 7) == 0) tops[p * GP + (lane >> 3)] = (nans >> lane) & 255 ? NAN : t;
+        top = fmaxf(top, t);
     }
-    top = nan ? -INFINITY : top;
-    top = dpp_max<0xB1>(top);    // lanes ^ 1
-    top = dpp_max<0x4E>(top);    // lanes ^ 2
-    top = dpp_max<0x141>(top);   // mirrored in 8
-    const uint64_t nans = __ballot(nan);
-    if ((lane & 7) == 0) tops[lane >> 3] = (nans >> lane) & 255 ? NAN : top;
+    if (!with_mass && !top_out) return;
+    top = max64(top);
+    if (top_out && lane == 0) *top_out = any_nan ? NAN : top;
     if (!with_mass) return;
-    top = dpp_max<0x140>(top);   // mirrored in 16
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const Weight W{pow2, (double)top, scale, 0.0, top == INFINITY};
     double m = 0.0;
-    if (top != -INFINITY && !nans) {
+    if (top != -INFINITY && !any_nan) {
+        const Weight W{pow2, (double)top, scale, 0.0, top == INFINITY};
+        if (W.hard) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m += W.real(v[e]);   // -inf: 0
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m += v[p][e] == top ? 1.0 : 0.0;
+        } else {
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m += W.soft(v[p][e]);
+        }
     }
     m = wave_sum(m);
     if (lane == 0) *mass = m;
 }
 
-// ---------------------------------------------------------------- the scan: a wave a piece
+// ---------------------------------------------------------------- the scan: a wave a block
 template <class T>
-__global__ __launch_bounds__(256) void sample_scan_kernel(SampleArgs A, int pieces, int64_t total) {
+__global__ __launch_bounds__(256) void sample_scan_kernel(SampleArgs A, int blocks, int64_t total) {
     __shared__ double pow2[128];
     if (threadIdx.x < 128) pow2[threadIdx.x] = POW2[threadIdx.x];
     __syncthreads();
     const int lane = threadIdx.x & 63;
     for (int64_t k = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); k < total;
          k += (int64_t)gridDim.x * 4) {
-        const int64_t r = k / pieces;
-        const int c = (int)(k - r * pieces);
+        const int64_t r = k / blocks;
+        const int b = (int)(k - r * blocks);
         const SampleRow s = sample_row(A, r);
-        float v[8];
-        load8((const T *)A.x + r * A.ld, A.mask ? A.mask + r * A.ld_mask : nullptr, c * PIECE + lane * 8, A.n, v);
-        piece_records(v, s.whole(A.n), s.inv_t * 0x1.71547652b82fep+7, pow2, A.tops + k * GP, A.masses + k);
+        const T *x = (const T *)A.x + r * A.ld;
+        const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
+        float v[BP][8];
+#pragma unroll
+        for (int p = 0; p < BP; ++p) load8(x, mask, b * BLOCK + p * PIECE + lane * 8, A.n, v[p]);
+        wave_records<BP>(v, s.whole(A.n), s.inv_t * LOG2E_128, pow2, A.tops + k * (BP * GP), A.block_tops + k, A.masses + k);
     }
+}
+
+// exclusive prefix of v over the threads of RW waves; total: of all. sh: RW + 1 values
+template <int RW, class V>
+__device__ __forceinline__ V block_scan(V v, V *sh, V &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const V in = wave_scan(v);
+    __syncthreads();
+    if (lane == 63) sh[wave] = in;
+    __syncthreads();
+    V before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) {
+        const V t = sh[w];
+        before += w < wave ? t : 0;
+        all += t;
+    }
+    total = all;
+    return before + (in - v);
+}
+
+template <int RW, class V>
+__device__ __forceinline__ V block_sum(V v, V *sh) {
+    V all;
+    block_scan<RW, V>(v, sh, all);
+    return all;
+}
+
+// ---------------------------------------------------------------- top-p alone
+// The nucleus' cut is searched by mass over NBINS equal steps of the distance from the top, up to
+// the distance at which an entry is sure to be outside: all entries lighter than e weigh less than
+// n e together, so with n e = (1 - p) S none of them is in the nucleus.
+struct Nucleus {
+    float top, step;    // step: bins a unit of distance
+    double sum;         // S in units
+    bool ok;            // a finite top and a mass to go by
+    __device__ __forceinline__ int bin(float x) const {   // NBINS: outside, or excluded
+        const float b = (top - x) * step;
+        return b < (float)NBINS ? (int)b : NBINS;
+    }
+};
+// by the threads of one wave, from the scan's records of a row
+__device__ __forceinline__ Nucleus nucleus(const SampleArgs &A, const SampleRow &s, const double *pow2, int64_t r, int blocks) {
+    const int lane = threadIdx.x & 63;
+    const float *bt = A.block_tops + r * blocks;
+    float top = -INFINITY;
+    bool nan = false;
+    for (int b = lane; b < blocks; b += 64) {
+        nan |= bt[b] != bt[b];
+        top = fmaxf(top, bt[b]);
+    }
+    top = max64(max8(top));
+    Nucleus N{};
+    N.top = top;
+    N.ok = !__ballot(nan) && fabsf(top) < INFINITY;
+    if (!N.ok) return N;
+    const Weight W = weight(A, s, pow2, top);
+    double sum = 0.0;
+    for (int b = lane; b < blocks; b += 64)
+        if (bt[b] != -INFINITY) sum += A.masses[r * blocks + b] * W.soft(bt[b]);
+    sum = wave_sum(sum);
+    N.sum = sum * A.unit;
+    const double far = log((double)A.n / ((1.0 - (double)s.p) * sum)) * 1.0001 + 1e-6;   // >= 0: sum <= n
+    N.step = (float)(NBINS / far * s.inv_t);
+    N.ok = N.step < INFINITY && N.step > 0.0f;
+    return N;
+}
+
+// a workgroup a split of a row: its mass by bins
+template <class T>
+__global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs A, int blocks) {
+    __shared__ double pow2[128];
+    __shared__ uint64_t mass[NBINS];
+    const int64_t r = A.row0 + blockIdx.x / A.splits;
+    const int part = blockIdx.x % A.splits, tid = threadIdx.x, lane = tid & 63;
+    const SampleRow s = sample_row(A, r);
+    if (!s.nucleus(A.n)) return;
+    if (tid < 128) pow2[tid] = POW2[tid];
+    for (int b = tid; b < NBINS; b += 256) mass[b] = 0;
+    __syncthreads();
+    const Nucleus N = nucleus(A, s, pow2, r, blocks);
+    if (!N.ok) return;
+    const Weight W = weight(A, s, pow2, N.top);
+    const T *x = (const T *)A.x + r * A.ld;
+    const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
+    const int per = (blocks + A.splits - 1) / A.splits, end = min((part + 1) * per, blocks);
+    for (int b = part * per + __builtin_amdgcn_readfirstlane(tid >> 6); b < end; b += 4) {
+        float v[BP][8];
+#pragma unroll
+        for (int p = 0; p < BP; ++p) load8(x, mask, b * BLOCK + p * PIECE + lane * 8, A.n, v[p]);
+#pragma unroll
+        for (int p = 0; p < BP; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = N.bin(v[p][e]);
+                if (k < NBINS)
+                    atomicAdd((unsigned long long *)&mass[k], (unsigned long long)W.fixed(W.soft(v[p][e])));
+            }
+    }
+    __syncthreads();
+    uint64_t *out = A.bins + (int64_t)blockIdx.x * NBINS;
+    for (int b = tid; b < NBINS; b += 256) out[b] = mass[b];
+}
+
+// the same split once more: the cut's bin, the masses of its blocks above that bin (and not under
+// min-p), and the bin's entries
+template <class T>
+__global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs A, int blocks) {
+    __shared__ double pow2[128];
+    __shared__ uint64_t scan[5];
+    __shared__ int cut_bin;
+    __shared__ uint64_t cut_above;
+    __shared__ uint32_t listed;
+    const int64_t local = blockIdx.x / A.splits, r = A.row0 + local;
+    const int part = blockIdx.x % A.splits, tid = threadIdx.x, lane = tid & 63;
+    const SampleRow s = sample_row(A, r);
+    if (!s.nucleus(A.n)) return;
+    if (tid < 128) pow2[tid] = POW2[tid];
+    if (tid == 0) {
+        cut_bin = -1;
+        listed = 0;
+    }
+    __syncthreads();
+    const Nucleus N = nucleus(A, s, pow2, r, blocks);
+    if (N.ok) {
+        // four bins a thread, from the top
+        uint64_t m[4] = {0, 0, 0, 0}, all;
+        for (int k = 0; k < A.splits; ++k) {
+            const uint64_t *in = A.bins + (local * A.splits + k) * NBINS + tid * 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m[j] += in[j];
+        }
+        const double limit = (double)s.p * N.sum;
+        uint64_t above = block_scan<4, uint64_t>(m[0] + m[1] + m[2] + m[3], scan, all);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if ((above == 0 || (double)above < limit) && (double)(above + m[j]) >= limit && m[j]) {   // one bin
+                cut_bin = tid * 4 + j;
+                cut_above = above;
+            }
+            above += m[j];
+        }
+    }
+    __syncthreads();
+    const int cut = cut_bin;
+    if (part == 0 && tid == 0) A.heads[local] = SampleHead{cut < 0 ? 0 : cut_above, cut, cut >= 0};
+    if (cut < 0) return;
+    const Weight W = weight(A, s, pow2, N.top);
+    const double q = (double)s.q;
+    const T *x = (const T *)A.x + r * A.ld;
+    const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
+    const int per = (blocks + A.splits - 1) / A.splits, end = min((part + 1) * per, blocks);
+    uint2 *list = A.lists + (int64_t)blockIdx.x * NLIST;
+    for (int b = part * per + __builtin_amdgcn_readfirstlane(tid >> 6); b < end; b += 4) {
+        float v[BP][8];
+#pragma unroll
+        for (int p = 0; p < BP; ++p) load8(x, mask, b * BLOCK + p * PIECE + lane * 8, A.n, v[p]);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int p = 0; p < BP; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = N.bin(v[p][e]);
+                if (k < cut) {
+                    const double w = W.soft(v[p][e]);
+                    sum += w >= q ? W.fixed(w) : 0;
+                } else if (k == cut) {
+                    const uint32_t at = atomicAdd(&listed, 1u);
+                    if (at < NLIST) list[at] = make_uint2(key_of(v[p][e]), (uint32_t)(b * BLOCK + p * PIECE + lane * 8 + e));
+                }
+            }
+        sum = wave_sum(sum);
+        if (lane == 0) A.kept[local * blocks + b] = sum;
+    }
+    __syncthreads();
+    if (tid == 0) A.listed[blockIdx.x] = listed;
 }
 
 // ---------------------------------------------------------------- a thread a row: n <= N
@@ -307,93 +559,86 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
 }
 
 // ---------------------------------------------------------------- a workgroup a row
-// exclusive prefix of v over the workgroup's threads; total: of all. sh: RW + 1 values
-template <class V>
-__device__ __forceinline__ V block_scan(V v, V *sh, V &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const V in = wave_scan(v, lane);
-    __syncthreads();
-    if (lane == 63) sh[wave] = in;
-    __syncthreads();
-    if (wave == 0) {
-        const V x = lane < RW ? sh[lane] : 0;
-        const V y = wave_scan(x, lane);
-        if (lane < RW) sh[lane] = y - x;
-        if (lane == RW - 1) sh[RW] = y;
-    }
-    __syncthreads();
-    total = sh[RW];
-    return sh[wave] + in - v;
-}
-
 // distance from the top by 64 steps an octave, 2^-12 .. 2^20: a bound that outliers do not spoil
 __device__ __forceinline__ int far_bin(float d) {
     const int b = (int)(__float_as_uint(d) >> 17) - ((127 - 12) << 6);
     return min(max(b, 0), BINS - 1);
 }
-
 struct Total {
     uint32_t count;
     uint64_t mass;
 };
 
-template <class T, bool FUSED>
-__global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
+template <class T, int RW, bool FUSED>
+__global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
+    constexpr int NT = 64 * RW, BT = BINS / NT;   // threads; bins of each
+    constexpr int REC = FUSED ? 1 : BP;           // pieces of a record of mass
     __shared__ double pow2[128];
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
-    __shared__ uint64_t seg_mass[SEGS];
-    __shared__ uint32_t seg_ties[SEGS];
     __shared__ uint32_t list_key[LIST], list_at[LIST];
-    __shared__ uint64_t scan64[RW + 1];
-    __shared__ double scanf[RW + 1];
-    __shared__ uint32_t scan32[RW + 1];
+    __shared__ uint64_t scan64[RW];
+    __shared__ double scanf[RW];
+    __shared__ uint32_t scan32[RW];
     __shared__ float own_tops[FUSED ? RW * GP : 1];
     __shared__ double own_masses[FUSED ? RW : 1];
     __shared__ float wave_top[RW];
     __shared__ int wave_nan[RW];
     __shared__ uint64_t found_mass;
     __shared__ double found_sum;
-    __shared__ uint32_t found_bin, found_count, listed;
-    const int64_t r = blockIdx.x;
+    __shared__ uint32_t found_bin, found_count, listed, grouped;
+    __shared__ double final_sum[4];
+    __shared__ uint64_t final_mass[4];
+    __shared__ uint32_t final_ties[4];
+    __shared__ float final_x[4];
+    __shared__ int final_last[4], final_hit[4];
+    uint64_t *const seg_mass = mass;       // [NT], once the search is over
+    uint32_t *const seg_ties = count;
+    uint32_t *const group_list = (uint32_t *)mass;   // [2 BINS], before it
+    const int64_t r = (FUSED || !A.heads ? 0 : A.row0) + blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = A.n;
     const SampleRow s = sample_row(A, r);
     const T *x = (const T *)A.x + r * A.ld;
     const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
-    const int pieces = (n + PIECE - 1) / PIECE, groups = pieces * GP;
+    const int pieces = (n + PIECE - 1) / PIECE, records = (pieces + REC - 1) / REC, groups = records * REC * GP;
     if (tid < 128) pow2[tid] = POW2[tid];
-    if (tid == 0) listed = 0;
+    if (tid == 0) {
+        listed = 0;
+        grouped = 0;
+    }
 
     const float *tops;
     const double *masses;
     if constexpr (FUSED) {
         __syncthreads();
         if (wave < pieces) {
-            float v[8];
-            load8(x, mask, wave * PIECE + lane * 8, n, v);
-            piece_records(v, s.whole(n), s.inv_t * 0x1.71547652b82fep+7, pow2, own_tops + wave * GP, own_masses + wave);
+            float v[1][8];
+            load8(x, mask, wave * PIECE + lane * 8, n, v[0]);
+            wave_records<1>(v, s.whole(n), s.inv_t * LOG2E_128, pow2, own_tops + wave * GP, nullptr, own_masses + wave);
         }
         __syncthreads();
         tops = own_tops;
         masses = own_masses;
     } else {
-        tops = A.tops + r * pieces * GP;
-        masses = A.masses + r * pieces;
+        tops = A.tops + r * groups;
+        masses = A.masses + r * records;
     }
     float top = -INFINITY;
     bool nan = false;
-    for (int g = tid; g < groups; g += 1024) {
-        const float t = tops[g];
+    const float *const top_src = FUSED ? tops : A.block_tops + r * records;
+    for (int g = tid; g < (FUSED ? groups : records); g += NT) {
+        const float t = top_src[g];
         nan |= t != t;
         top = fmaxf(top, t);
     }
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    top = max64(max8(top));
     nan = __ballot(nan) != 0;
     if (lane == 0) {
         wave_top[wave] = top;
         wave_nan[wave] = nan;
     }
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < RW; ++w) {
         top = fmaxf(top, wave_top[w]);
         nan |= wave_nan[w] != 0;
@@ -404,19 +649,24 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
     }
     const Weight W = weight(A, s, pow2, top);
     const double q = (double)s.q;
-    const int per = (pieces + SEGS - 1) / SEGS, segs = (pieces + per - 1) / per;   // pieces a segment, segments
+    const int per = (records + NT - 1) / NT, segs = (records + per - 1) / per;   // records a segment, segments
 
-    // the whole row's mass by segment, from the pieces' masses
+    // the whole row's mass by segment, from the records
     double seg_sum = 0.0, sum_ex = 0.0, row_sum = 0.0;
     if (s.whole(n)) {
         if (tid < segs)
-            for (int c = tid * per; c < min((tid + 1) * per, pieces); ++c) {
-                float t = tops[c * GP];
+            for (int c = tid * per; c < min((tid + 1) * per, records); ++c) {
+                float t;
+                if constexpr (FUSED) {
+                    t = tops[c * GP];
 #pragma unroll
-                for (int g = 1; g < GP; ++g) t = fmaxf(t, tops[c * GP + g]);
+                    for (int g = 1; g < GP; ++g) t = fmaxf(t, tops[c * GP + g]);
+                } else {
+                    t = A.block_tops[r * records + c];
+                }
                 if (t != -INFINITY) seg_sum += masses[c] * W.real(t);
             }
-        sum_ex = block_scan<double>(seg_sum, scanf, row_sum);
+        sum_ex = block_scan<RW, double>(seg_sum, scanf, row_sum);
     }
 
     // the cut: keys above kt, and the first nt of those equal to it
@@ -428,7 +678,7 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
     const bool cut = s.k < n || s.p < 1.0f, plain = !cut && q == 0.0;
     double base_real = 0.0;
     if (plain) {
-        // nothing is filtered: the segment by the pieces' masses
+        // nothing is filtered: the segment by the records' masses
         target = (double)s.u * row_sum;
         scale_out = 1.0 / row_sum;
         if (tid == 0) found_bin = 0;
@@ -441,113 +691,215 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
         seg = (int)found_bin;
         base_real = found_sum;
     } else {
-        // candidates: what can be in the cut, by the groups' maxima
-        int far = BINS - 1;   // candidates lie in bins up to here
-        // and, where min-p is not to change the mass that top-p goes by, this near
-        const bool by_q = s.q > 0.0f && s.p >= 1.0f;
-        const float near = by_q ? (float)(-log((double)s.q) / s.inv_t) * 1.0001f + 1e-30f : INFINITY;
-        auto candidate = [&](float v) __attribute__((always_inline)) {
-            const float d = top - v;   // NaN for two infinities: top itself
-            return v != -INFINITY && !(d > near) && far_bin(d > 0.0f ? d : 0.0f) <= far;
-        };
-        bool use_list = true;
-        if (W.hard) {
-            far = 0;
-        } else if (cut) {
-            // the bin that the wanted-th largest maximum falls in: at least that many entries are as near
-            for (int b = tid; b < BINS; b += 1024) count[b] = 0;
-            __syncthreads();
-            for (int g = tid; g < groups; g += 1024) {
-                const float t = tops[g];
-                if (t != -INFINITY) atomicAdd(&count[far_bin(top - t)], 1u);
+        const double limit_row = (double)s.p * row_sum * A.unit;   // top-p alone, in units
+        bool use_list = true, binned = false;   // binned: the list is the cut's bin, the rest is above it
+        uint64_t above_list = 0;
+        if (!FUSED && A.heads && s.nucleus(n) && !W.hard) {
+            const int64_t local = blockIdx.x;
+            const SampleHead head = A.heads[local];
+            uint32_t m = 0;
+            bool fits = head.ok != 0;
+            for (int k = 0; k < A.splits && fits; ++k) {
+                const uint32_t c = A.listed[local * A.splits + k];
+                fits = c <= NLIST && m + c <= LIST;
+                if (fits)
+                    for (uint32_t i = tid; i < c; i += NT) {
+                        const uint2 e = A.lists[(local * A.splits + k) * NLIST + i];
+                        list_key[m + i] = e.x;
+                        list_at[m + i] = e.y;
+                    }
+                m += c;
             }
-            if (tid == 0) found_bin = BINS - 1;
-            __syncthreads();
-            const uint32_t c0 = count[2 * tid], c1 = count[2 * tid + 1];
-            uint32_t all;
-            const uint32_t ex = block_scan<uint32_t>(c0 + c1, scan32, all);
-            // top-p alone: a list that most distributions' nucleus fits into
-            const uint32_t wanted = s.k < n ? (uint32_t)s.k : max(1u, min((uint32_t)LIST / 2, all / 2));
-            if (ex < wanted && ex + c0 + c1 >= wanted) found_bin = ex + c0 >= wanted ? 2 * tid : 2 * tid + 1;
-            __syncthreads();
-            far = (int)found_bin;
-            // fewer groups than wanted entries: everything would be a candidate
-            use_list = all >= wanted || n <= LIST || by_q;
-        }
-        if (use_list) {
-            for (int c = wave; c < pieces; c += RW) {
-                const float t = lane < GP ? tops[c * GP + lane] : -INFINITY;
-                const uint64_t some = __ballot(candidate(t));
-                if (!some) continue;
-                float v[8];
-                load8(x, mask, c * PIECE + lane * 8, n, v);
+            binned = fits;
+            use_list = fits;
+            above_list = head.above;
+            if (tid == 0) listed = m;
+        } else {
+            // candidates: what can be in the cut, by the groups' maxima: bins of the distance from the
+            // top up to here, and, where min-p is not to change the mass that top-p goes by, this near
+            int far = BINS - 1;
+            const bool by_q = s.q > 0.0f && s.p >= 1.0f;
+            const float near = by_q ? (float)(-log((double)s.q) / s.inv_t) * 1.0001f + 1e-30f : INFINITY;
+            auto candidate = [&](float v) __attribute__((always_inline)) {
+                const float d = top - v;   // NaN for two infinities: top itself
+                return v != -INFINITY && !(d > near) && far_bin(d > 0.0f ? d : 0.0f) <= far;
+            };
+            if (W.hard) {
+                far = 0;
+            } else if (cut) {
+                // the bin that the wanted-th largest maximum falls in: at least that many entries are as near
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const bool is = candidate(v[e]);
-                    const uint64_t who = __ballot(is);
-                    if (!who) continue;
+                for (int b = 0; b < BT; ++b) count[b * NT + tid] = 0;
+                __syncthreads();
+                for (int g = tid; g < groups; g += NT) {
+                    const float t = tops[g];
+                    if (t != -INFINITY) atomicAdd(&count[far_bin(top - t)], 1u);
+                }
+                if (tid == 0) found_bin = BINS - 1;
+                __syncthreads();
+                uint32_t c[BT], sum = 0, all;
+#pragma unroll
+                for (int b = 0; b < BT; ++b) sum += c[b] = count[tid * BT + b];
+                uint32_t ex = block_scan<RW, uint32_t>(sum, scan32, all);
+                // top-p alone: a list that most distributions' nucleus fits into
+                const uint32_t wanted = s.k < n ? (uint32_t)s.k : max(1u, min((uint32_t)LIST / 2, all / 2));
+#pragma unroll
+                for (int b = 0; b < BT; ++b) {
+                    if (ex < wanted && ex + c[b] >= wanted) found_bin = tid * BT + b;
+                    ex += c[b];
+                }
+                __syncthreads();
+                far = (int)found_bin;
+                // fewer groups than wanted entries: everything would be a candidate
+                use_list = all >= wanted || n <= LIST || by_q;
+            }
+            if (use_list) {
+                for (int g = tid; g < groups; g += NT)
+                    if (candidate(tops[g])) {
+                        const uint32_t at = atomicAdd(&grouped, 1u);
+                        if (at < 2 * BINS) group_list[at] = (uint32_t)g;
+                    }
+                __syncthreads();
+                const uint32_t ng = grouped;
+                use_list = ng <= 2 * BINS;
+                for (uint32_t i0 = wave * 8; use_list && i0 < ng; i0 += RW * 8) {   // a group 8 lanes
+                    const uint32_t i = i0 + (lane >> 3);
+                    const int at0 = i < ng ? (int)group_list[i] * GROUP + (lane & 7) * 8 : n;
+                    float v[8];
+                    load8(x, mask, at0, n, v);
+uint64_t who[8];
+                    uint32_t found = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        who[e] = __ballot(candidate(v[e]));
+                        found += (uint32_t)__popcll(who[e]);
+                    }
+                    if (!found) continue;
                     uint32_t at = 0;
-                    if (lane == 0) at = atomicAdd(&listed, (uint32_t)__popcll(who));
-                    at = __builtin_amdgcn_readfirstlane(at) + (uint32_t)__popcll(who & ((1ull << lane) - 1));
-                    if (is && at < LIST) {
-                        list_key[at] = key_of(v[e]);
-                        list_at[at] = (uint32_t)(c * PIECE + lane * 8 + e);
+                    if (lane == 0) at = atomicAdd(&listed, found);
+                    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t mine = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(who[e] >> 32),
+                                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)who[e], 0));
+                        if ((who[e] >> lane & 1) && mine < LIST) {
+                            list_key[mine] = key_of(v[e]);
+                            list_at[mine] = (uint32_t)(at0 + e);
+                        }
+                        at += (uint32_t)__popcll(who[e]);
                     }
                 }
             }
         }
         __syncthreads();
         uint32_t m = use_list ? listed : LIST + 1;
-        const double limit_row = (double)s.p * row_sum * A.unit;   // top-p alone, in units
         if (m <= PAIRS) {
-            // each candidate's rank and mass before it, by comparing all pairs: four threads each
-            const int j = tid >> 2;
-            const uint32_t kj = j < (int)m ? list_key[j] : 0, aj = j < (int)m ? list_at[j] : 0;
-            if (tid < (int)m) mass[tid] = W.fixed(W.real(of_key(list_key[tid])));
-            __syncthreads();
-            uint32_t rank = 0;
-            uint64_t before = 0;
-            for (uint32_t i = tid & 3; i < m; i += 4) {
-                const uint32_t ki = list_key[i];
-                const bool first = ki > kj || (ki == kj && list_at[i] < aj);
-                rank += first;
-                before += first ? mass[i] : 0;
+            // each candidate's rank and mass before it, by comparing all pairs: four threads a candidate,
+            // sixteen bytes of LDS a comparison, no branches (with them: 350 cycles a comparison)
+            constexpr int AT_ONCE = NT / 4, ROUNDS = PAIRS / AT_ONCE;   // candidates a round
+            uint4 *const cand = (uint4 *)mass;   // key, index, weight
+            if (tid < (int)m) {
+                const uint64_t w = W.fixed(W.real(of_key(list_key[tid])));
+                cand[tid] = make_uint4(list_key[tid], list_at[tid], (uint32_t)w, (uint32_t)(w >> 32));
             }
-            rank += __shfl_xor(rank, 1);
-            rank += __shfl_xor(rank, 2);
-            before += __shfl_xor(before, 1);
-            before += __shfl_xor(before, 2);
-            const bool own = (tid & 3) == 0 && j < (int)m;
-            const uint64_t wj = j < (int)m ? mass[j] : 0;
-            const bool in_k = own && rank < (uint32_t)s.k;
-            uint64_t s1;
-            block_scan<uint64_t>(in_k ? wj : 0, scan64, s1);
+            __syncthreads();
+            uint32_t rank_[ROUNDS];
+            uint64_t before_[ROUNDS], w_[ROUNDS];
+            uint32_t k_[ROUNDS], a_[ROUNDS];
+#pragma unroll
+            for (int o = 0; o < ROUNDS; ++o) {
+                const uint32_t j = o * AT_ONCE + (tid >> 2);
+                rank_[o] = 0;
+                before_[o] = w_[o] = 0;
+                k_[o] = a_[o] = 0;
+                if (o * AT_ONCE >= (int)m) break;
+                if (j < m) {
+                    const uint4 c = cand[j];
+                    k_[o] = c.x;
+                    a_[o] = c.y;
+                    w_[o] = c.z | (uint64_t)c.w << 32;
+                }
+#pragma unroll 4
+                for (uint32_t i = tid & 3; i < m; i += 4) {
+                    const uint4 c = cand[i];
+                    const bool first = (c.x > k_[o]) | ((c.x == k_[o]) & (c.y < a_[o]));
+                    rank_[o] += first;
+                    before_[o] += first ? c.z | (uint64_t)c.w << 32 : 0;
+                }
+                rank_[o] += __shfl_xor(rank_[o], 1);
+                rank_[o] += __shfl_xor(rank_[o], 2);
+                before_[o] += __shfl_xor(before_[o], 1);
+                before_[o] += __shfl_xor(before_[o], 2);
+            }
+            auto own = [&](int o) __attribute__((always_inline)) {   // the thread that answers for a candidate
+                return (tid & 3) == 0 && o * AT_ONCE + (tid >> 2) < (int)m;
+            };
+            uint64_t s1 = 0;
+#pragma unroll
+            for (int o = 0; o < ROUNDS; ++o) s1 += own(o) && rank_[o] < (uint32_t)s.k ? w_[o] : 0;
+            s1 = block_sum<RW, uint64_t>(s1, scan64);
             // top-p alone: the list has to hold all of the nucleus
-            const bool inside = s.k < n || s.p >= 1.0f || (double)s1 >= limit_row;
+            const bool inside = s.k < n || s.p >= 1.0f || (!binned && (double)s1 >= limit_row);
             if (inside) {
                 const double limit = s.k < n ? (double)s.p * (double)s1 : limit_row;
-                const double real = own ? W.real(of_key(kj)) : 0.0;
-                const bool kept = in_k && (s.p >= 1.0f || rank == 0 || (double)before < limit) && real >= q;
-                if (own) seg_mass[j] = kept ? wj : 0;
-                uint64_t sum;
-                block_scan<uint64_t>(kept ? wj : 0, scan64, sum);   // and its barriers
-                uint64_t upto = 0;
-                for (uint32_t i = tid & 3; i < m; i += 4) upto += list_at[i] <= aj ? seg_mass[i] : 0;
-                upto += __shfl_xor(upto, 1);
-                upto += __shfl_xor(upto, 2);
+                uint64_t sum = 0;
+                bool kept[ROUNDS];
+#pragma unroll
+                for (int o = 0; o < ROUNDS; ++o) {
+                    kept[o] = own(o) && rank_[o] < (uint32_t)s.k &&
+                              (s.p >= 1.0f || rank_[o] == 0 || (double)before_[o] < limit) && W.real(of_key(k_[o])) >= q;
+                    if (own(o) && !kept[o]) cand[o * AT_ONCE + (tid >> 2)].z = cand[o * AT_ONCE + (tid >> 2)].w = 0;
+                    sum += kept[o] ? w_[o] : 0;
+                }
+                sum = block_sum<RW, uint64_t>(sum, scan64);   // and its barriers
                 const double t = (double)s.u * (double)sum;
-                if (kept && wj && (double)upto > t && !((double)(upto - wj) > t))   // one thread
-                    answer(A, r, (int)aj, real * A.unit / (double)sum);
+#pragma unroll
+                for (int o = 0; o < ROUNDS; ++o) {
+                    if (o * AT_ONCE >= (int)m) break;
+                    uint64_t upto = 0;
+#pragma unroll 4
+                    for (uint32_t i = tid & 3; i < m; i += 4) {
+                        const uint4 c = cand[i];
+                        upto += c.y <= a_[o] ? c.z | (uint64_t)c.w << 32 : 0;
+                    }
+                    upto += __shfl_xor(upto, 1);
+                    upto += __shfl_xor(upto, 2);
+                    if (kept[o] && w_[o] && (double)upto > t && !((double)(upto - w_[o]) > t))   // one thread
+                        answer(A, r, (int)a_[o], W.real(of_key(k_[o])) * A.unit / (double)sum);
+                }
                 return;
             }
-            __syncthreads();
-            m = LIST + 1;
+            if (binned) {
+                // the cut among the bin's entries: the last one with less than the limit before it
+                if (tid == 0) {
+                    found_bin = 0xFFFFFFFFu;
+                    found_count = 0;
+                }
+                __syncthreads();
+                bool kept[ROUNDS];
+#pragma unroll
+                for (int o = 0; o < ROUNDS; ++o) {
+                    kept[o] = own(o) && ((above_list == 0 && rank_[o] == 0) || (double)(above_list + before_[o]) < limit_row);
+                    if (kept[o]) atomicMin(&found_bin, k_[o]);
+                }
+                __syncthreads();
+                kt = found_bin;
+#pragma unroll
+                for (int o = 0; o < ROUNDS; ++o)
+                    if (kept[o] && k_[o] == kt) atomicAdd(&found_count, 1u);
+                __syncthreads();
+                nt = found_count;
+                __syncthreads();
+            } else {
+                __syncthreads();
+                m = LIST + 1;
+            }
         }
         // larger cuts: a radix search over the listed candidates or, where they are too many, the row
         bool from_list = m <= LIST;
         auto each = [&](auto &&f) __attribute__((always_inline)) {   // f(x, index) for every candidate, or every entry
             if (from_list) {
-                for (uint32_t i = tid; i < m; i += 1024) f(of_key(list_key[i]), (int)list_at[i]);
+                for (uint32_t i = tid; i < m; i += NT) f(of_key(list_key[i]), (int)list_at[i]);
             } else {
                 for (int c = wave; c < pieces; c += RW) {
                     float v[8];
@@ -559,18 +911,19 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
         };
         // the key at which a prefix of the order ends, three levels of a radix search: by count (the
         // prefix has k entries) or by mass (the last entry with less than `limit` before it). From
-        // keys >= least. above_*: of the keys over the found one; count_in: of the found one itself.
+        // keys >= least, with above_mass over all of them. above_*: of the keys over the found one;
+        // count_in: of the found one itself.
         uint64_t above_mass = 0;
         uint32_t above_count = 0, count_in = 0;
         auto search = [&](bool by_mass, bool with_mass, uint32_t least, uint32_t k, double limit) __attribute__((always_inline)) {
             uint32_t prefix = 0;
-            above_mass = 0;
             above_count = 0;
             for (int level = 0; level < 3; ++level) {
                 const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
-                for (int b = tid; b < BINS; b += 1024) {
-                    mass[b] = 0;
-                    count[b] = 0;
+#pragma unroll
+                for (int b = 0; b < BT; ++b) {
+                    mass[b * NT + tid] = 0;
+                    count[b * NT + tid] = 0;
                 }
                 __syncthreads();
                 each([&](float v, int) __attribute__((always_inline)) {
@@ -581,25 +934,31 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
                     if (with_mass) atomicAdd((unsigned long long *)&mass[b], (unsigned long long)W.fixed(W.real(v)));
                 });
                 __syncthreads();
-                // bins from the top, two a thread
-                const int b0 = BINS - 1 - 2 * tid, b1 = b0 - 1;
-                const uint64_t m0 = mass[b0], m1 = mass[b1];
-                const uint32_t c0 = count[b0], c1 = count[b1];
-                uint64_t m_all;
-                uint32_t c_all;
-                const uint64_t m_ex = above_mass + block_scan<uint64_t>(m0 + m1, scan64, m_all);
-                const uint32_t c_ex = above_count + block_scan<uint32_t>(c0 + c1, scan32, c_all);
-                auto test = [&](int b, uint64_t mb, uint32_t cb, uint64_t m_before, uint32_t c_before) __attribute__((always_inline)) {
-                    const bool here = by_mass ? (double)m_before < limit && (double)(m_before + mb) >= limit
-                                              : c_before < k && c_before + cb >= k;
+                // bins from the top, BT a thread
+                uint64_t m_sum = 0, m_all;
+                uint32_t c_sum = 0, c_all;
+#pragma unroll
+                for (int b = 0; b < BT; ++b) {
+                    m_sum += mass[BINS - 1 - tid * BT - b];
+                    c_sum += count[BINS - 1 - tid * BT - b];
+                }
+                uint64_t m_ex = above_mass + block_scan<RW, uint64_t>(m_sum, scan64, m_all);
+                uint32_t c_ex = above_count + block_scan<RW, uint32_t>(c_sum, scan32, c_all);
+#pragma unroll
+                for (int b = 0; b < BT; ++b) {
+                    const int at = BINS - 1 - tid * BT - b;
+                    const uint64_t m_in = m_ex + mass[at];
+                    const uint32_t c_in = c_ex + count[at];
+                    const bool here = by_mass ? (m_ex == 0 || (double)m_ex < limit) && (double)m_in >= limit && m_in > m_ex
+                                              : c_ex < k && c_in >= k;
                     if (here) {   // one bin of one thread
-                        found_bin = (uint32_t)b;
-                        found_mass = m_before;
-                        found_count = c_before;
+                        found_bin = (uint32_t)at;
+                        found_mass = m_ex;
+                        found_count = c_ex;
                     }
-                };
-                test(b0, m0, c0, m_ex, c_ex);
-                test(b1, m1, c1, m_ex + m0, c_ex + c0);
+                    m_ex = m_in;
+                    c_ex = c_in;
+                }
                 __syncthreads();
                 const uint32_t b = found_bin & (BINS - 1);
                 above_mass = found_mass;
@@ -620,22 +979,23 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
             });
             uint64_t w_all;
             uint32_t c_all;
-            block_scan<uint64_t>(w, scan64, w_all);
-            block_scan<uint32_t>(c, scan32, c_all);
+            block_scan<RW, uint64_t>(w, scan64, w_all);
+            block_scan<RW, uint32_t>(c, scan32, c_all);
             return Total{c_all, w_all};
         };
         if (W.hard && s.greedy) {
             kt = key_of(top);
             nt = 1;
-        } else if (cut) {
-            auto all = total_of();
-            if (from_list && s.k == n && (double)all.mass < limit_row) {   // the nucleus is not inside the list
+        } else if (cut && kt == 0) {
+            Total all = total_of();
+            if (from_list && !binned && s.k == n && (double)all.mass < limit_row) {   // the nucleus is not inside the list
                 from_list = false;
                 all = total_of();
             }
             uint64_t s1 = all.mass;
             bool k_cut = false;
             if (s.k < n && all.count > (uint32_t)s.k) {
+                above_mass = 0;
                 kt = search(false, s.p < 1.0f, 0, (uint32_t)s.k, 0.0);
                 nt = (uint32_t)s.k - above_count;
                 s1 = above_mass + nt * W.fixed(W.real(of_key(kt)));
@@ -649,6 +1009,7 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
                     nt = 1;
                 } else {
                     const uint32_t kk = kt, kn = nt;
+                    above_mass = from_list ? above_list : 0;
                     kt = search(true, true, kk, 0, limit);
                     // tie j stays while above + j w < limit
                     const uint64_t w = W.fixed(W.real(of_key(kt)));
@@ -664,24 +1025,27 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
         const double wt = bounded ? W.real(of_key(kt)) : 0.0;
         const uint64_t wtie = wt >= q ? W.fixed(wt) : 0;
         if (from_list) {
-            seg_mass[tid] = 0;
+            uint64_t w = 0;
+            if (binned && tid < segs)
+                for (int c = tid * per; c < min((tid + 1) * per, records); ++c) w += A.kept[(int64_t)blockIdx.x * records + c];
+            seg_mass[tid] = w;
             seg_ties[tid] = 0;
             __syncthreads();
             each([&](float v, int i) __attribute__((always_inline)) {
                 const uint32_t key = key_of(v);
-                const int g = i / PIECE / per;
+                const int g = i / (PIECE * REC) / per;
                 if (key > kt) {
-                    const double w = W.real(v);
-                    if (w >= q) atomicAdd((unsigned long long *)&seg_mass[g], (unsigned long long)W.fixed(w));
+                    const double wr = W.real(v);
+                    if (wr >= q) atomicAdd((unsigned long long *)&seg_mass[g], (unsigned long long)W.fixed(wr));
                 } else if (bounded && key == kt) {
                     atomicAdd(&seg_ties[g], 1u);
                 }
             });
         } else {
+            __syncthreads();
             for (int g = wave; g < segs; g += RW) {
-                uint64_t w_sum = 0;
-                uint32_t t_sum = 0;
-                for (int c = g * per; c < min((g + 1) * per, pieces); ++c) {
+                uint64_t w_sum = 0, t_sum = 0;
+                for (int c = g * per * REC; c < min((g + 1) * per * REC, pieces); ++c) {
                     float v[8];
                     load8(x, mask, c * PIECE + lane * 8, n, v);
 #pragma unroll
@@ -698,18 +1062,18 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
                 t_sum = wave_sum(t_sum);
                 if (lane == 0) {
                     seg_mass[g] = w_sum;
-                    seg_ties[g] = t_sum;
+                    seg_ties[g] = (uint32_t)t_sum;
                 }
             }
         }
         __syncthreads();
         const uint32_t mine = tid < segs ? seg_ties[tid] : 0;
         uint32_t all_ties;
-        const uint32_t ties_ex = block_scan<uint32_t>(mine, scan32, all_ties);
+        const uint32_t ties_ex = block_scan<RW, uint32_t>(mine, scan32, all_ties);
         const uint32_t left = nt > ties_ex ? nt - ties_ex : 0;
         const uint64_t here = (tid < segs ? seg_mass[tid] : 0) + (uint64_t)min(mine, left) * wtie;
         uint64_t sum;
-        const uint64_t m_ex = block_scan<uint64_t>(here, scan64, sum);
+        const uint64_t m_ex = block_scan<RW, uint64_t>(here, scan64, sum);
         target = (double)s.u * (double)sum;
         scale_out = A.unit / (double)sum;
         if ((double)(m_ex + here) > target && !((double)m_ex > target)) {   // one thread
@@ -722,104 +1086,180 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs A) {
         base = found_mass;
         ties = found_count;
     }
-    if (wave != 0) return;
-
-    // inside the segment, one wave
+    // inside the segment: four waves, a piece each
+    const int first = seg * per * REC, end = min((seg + 1) * per * REC, pieces);
     if (plain) {
-        int last = -1;   // if rounding leaves the target just over the segment's end
+        // rounding may leave the target just over the segment's end: the next entry that weighs half a
+        // unit then, or the row's last one; if all from the segment on are lighter, the row's first
+        int last = -1;
         float xl = 0.0f;
-        for (int c = seg * per; c < min((seg + 1) * per, pieces); ++c) {
-            float v[8];
-            const int i = c * PIECE + lane * 8;
-            load8(x, mask, i, n, v);
-            double w8[8], own = 0.0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                w8[e] = W.real(v[e]);
-                own += w8[e];
+        for (int c0 = first;; c0 += 4) {
+            if (c0 >= pieces) {
+                if (last >= 0) break;
+                c0 = 0;
+                target = -1.0;
             }
-            const double in = wave_scan(own, lane);
-            double upto = base_real + (in - own);
+            const int c = c0 + wave, i = c * PIECE + lane * 8;
+            double w8[8], own = 0.0, in = 0.0;
+            float v[8], xm = 0.0f;
+            int mine = -1;
+            const bool works = wave < 4 && c < pieces;
+            if (works) {
+                load8(x, mask, i, n, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w8[e] = W.real(v[e]);
+                    w8[e] = v[e] != -INFINITY && W.fixed(w8[e]) ? w8[e] : 0.0;
+                    own += w8[e];
+                    if (w8[e] > 0.0) {
+                        mine = i + e;
+                        xm = v[e];
+                    }
+                }
+                in = wave_scan(own);
+            }
+            const uint64_t some = __ballot(mine >= 0);
+            const int who = some ? 63 - __clzll((long long)some) : 0;
+            mine = __builtin_amdgcn_readlane(mine, who);
+            xm = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(xm), who));
+            if (wave < 4 && lane == 63) {
+                final_sum[wave] = in;
+                final_last[wave] = some ? mine : -1;
+                final_x[wave] = xm;
+            }
+            __syncthreads();
+            double upto = base_real;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) upto += w < wave ? final_sum[w] : 0.0;
+            upto += in - own;
             int at = -1;
             float xa = 0.0f;
+            if (works) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                upto += w8[e];
-                if (at < 0 && w8[e] > 0.0 && upto > target) {
-                    at = i + e;
-                    xa = v[e];
+                for (int e = 0; e < 8; ++e) {
+                    upto += w8[e];
+                    if (at < 0 && w8[e] > 0.0 && upto > target) {
+                        at = i + e;
+                        xa = v[e];
+                    }
                 }
             }
             const uint64_t hits = __ballot(at >= 0);
-            if (hits) {
-                if (lane == __ffsll((unsigned long long)hits) - 1) answer(A, r, at, W.real(xa) * scale_out);
+            if (wave < 4 && lane == 0) final_hit[wave] = hits ? 1 : 0;
+            __syncthreads();
+            int by = -1;
+#pragma unroll
+            for (int w = 3; w >= 0; --w) by = final_hit[w] ? w : by;
+            if (by >= 0) {
+                if (wave == by && lane == __ffsll((unsigned long long)hits) - 1) answer(A, r, at, W.real(xa) * scale_out);
                 return;
             }
-            int mine = -1;
-            float xm = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (w8[e] > 0.0) {
-                    mine = i + e;
-                    xm = v[e];
+            for (int w = 0; w < 4; ++w) {
+                base_real += final_sum[w];
+                if (final_last[w] >= 0) {
+                    last = final_last[w];
+                    xl = final_x[w];
                 }
-            const uint64_t some = __ballot(mine >= 0);
-            if (some) {
-                const int who = 63 - __clzll((long long)some);
-                last = __shfl(mine, who);
-                xl = __shfl(xm, who);
             }
-            base_real += __shfl(in, 63);
+            __syncthreads();
         }
-        if (lane == 0) answer(A, r, last, W.real(xl) * scale_out);
+        if (tid == 0) answer(A, r, last, W.real(xl) * scale_out);
         return;
     }
     const bool bounded = kt != 0;
     const double wt = bounded ? W.real(of_key(kt)) : 0.0;
     const uint64_t wtie = wt >= q ? W.fixed(wt) : 0;
-    for (int c = seg * per; c < min((seg + 1) * per, pieces); ++c) {
+    for (int c0 = first; c0 < end; c0 += 4) {
+        const int c = c0 + wave, i = c * PIECE + lane * 8;
+        const bool works = wave < 4 && c < end;
         float v[8];
-        const int i = c * PIECE + lane * 8;
-        load8(x, mask, i, n, v);
         uint32_t t = 0;
+        if (works) {
+            load8(x, mask, i, n, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t += bounded && key_of(v[e]) == kt;
-        const uint32_t t_in = wave_scan(t, lane);
+            for (int e = 0; e < 8; ++e) t += bounded && key_of(v[e]) == kt;
+        }
+        const uint32_t t_in = wave_scan(t);
+        if (wave < 4 && lane == 63) final_ties[wave] = t_in;
+        __syncthreads();
         uint32_t rank = ties + t_in - t;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            rank += w < wave ? final_ties[w] : 0;
+            ties += final_ties[w];
+        }
         uint64_t w8[8], own = 0;
+        if (works) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t key = key_of(v[e]);
-            w8[e] = 0;
-            if (key > kt) {
-                const double w = W.real(v[e]);
-                w8[e] = w >= q ? W.fixed(w) : 0;
-            } else if (bounded && key == kt) {
-                w8[e] = rank++ < nt ? wtie : 0;
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t key = key_of(v[e]);
+                w8[e] = 0;
+                if (key > kt) {
+                    const double w = W.real(v[e]);
+                    w8[e] = w >= q ? W.fixed(w) : 0;
+                } else if (bounded && key == kt) {
+                    w8[e] = rank++ < nt ? wtie : 0;
+                }
+                own += w8[e];
             }
-            own += w8[e];
         }
-        const uint64_t in = wave_scan(own, lane);
+        const uint64_t in = wave_scan(own);
+        if (wave < 4 && lane == 63) final_mass[wave] = in;
+        __syncthreads();
         uint64_t upto = base + in - own;
-        int at = -1;
-        float xa = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            upto += w8[e];
-            if (at < 0 && w8[e] && (double)upto > target) {
-                at = i + e;
-                xa = v[e];
+        for (int w = 0; w < 4; ++w) {
+            upto += w < wave ? final_mass[w] : 0;
+            base += final_mass[w];
+        }
+        if (works && !((double)upto > target) && (double)(upto + own) > target) {   // one thread of the row's
+            int at = -1;
+            float xa = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                upto += w8[e];
+                if (at < 0 && w8[e] && (double)upto > target) {
+                    at = i + e;
+                    xa = v[e];
+                }
             }
+            answer(A, r, at, W.real(xa) * scale_out);
         }
-        const uint64_t hits = __ballot(at >= 0);
-        if (hits) {
-            if (lane == __ffsll((unsigned long long)hits) - 1) answer(A, r, at, W.real(xa) * scale_out);
-            return;
-        }
-        base += __shfl(in, 63);
-        ties += __shfl(t_in, 63);
+        if ((double)base > target) return;   // answered
     }
 }
+
+// ---------------------------------------------------------------- launches
+constexpr int64_t MANY_ROWS = 512;   // from here on a row's workgroup has 4 waves instead of 16
+// rows whose workgroup scans them itself: a piece a wave
+static bool fused(int64_t rows, int64_t n) { return n <= (rows >= MANY_ROWS ? 4 : 16) * PIECE; }
+
+// the workspace's parts, in bytes from its start
+struct SampleSpace {
+    int blocks = 0, splits = 0;
+    int64_t chunk = 0;   // rows of a launch of the nucleus kernels
+    int64_t masses = 0, block_tops = 0, tops = 0, bins = 0, kept = 0, lists = 0, listed = 0, heads = 0, bytes = 0;
+    SampleSpace(int64_t rows, int64_t n) {
+        if (n <= 8 || fused(rows, n) || rows == 0) return;
+        blocks = ceil_div(n, BLOCK);
+        splits = (int)std::max<int64_t>(1, std::min<int64_t>({SPLITS, 2048 / rows, (blocks + 3) / 4}));
+        chunk = std::min<int64_t>(rows, 2048 / splits);
+        auto take = [&](int64_t size) {
+            const int64_t at = bytes;
+            bytes += (size + 15) / 16 * 16;
+            return at;
+        };
+        masses = take(rows * blocks * 8);
+        block_tops = take(rows * blocks * 4);
+        tops = take(rows * blocks * BP * GP * 4);
+        bins = take(chunk * splits * NBINS * 8);
+        kept = take(chunk * blocks * 8);
+        lists = take(chunk * splits * NLIST * 8);
+        listed = take(chunk * splits * 4);
+        heads = take(chunk * (int64_t)sizeof(SampleHead));
+    }
+};
 
 static void check_shape(int64_t rows, int64_t n) {
     SNK_CHECK(rows >= 0 && rows < (int64_t)1 << 31, SNK_ERR_INVALID, "sample: %lld rows", (long long)rows);
@@ -857,32 +1297,67 @@ static SampleArgs sample_args(const snk_sample_cfg_t *cfg, int64_t rows, int64_t
 }
 
 template <class T>
-static void sample_launch_t(const SampleArgs &A, hipStream_t s) {
-    const unsigned few = (unsigned)ceil_div(A.rows, 256);
-    if (A.n <= 4)
-        sample_few_kernel<T, 4><<<few, 256, 0, s>>>(A);
-    else if (A.n <= 8)
-        sample_few_kernel<T, 8><<<few, 256, 0, s>>>(A);
-    else if (A.n <= FUSED_N) {
-        sample_row_kernel<T, true><<<(unsigned)A.rows, 1024, 0, s>>>(A);
-    } else {
-        const int pieces = ceil_div(A.n, PIECE);
-        const int64_t total = A.rows * pieces;
-        sample_scan_kernel<T><<<(unsigned)std::min<int64_t>((total + 3) / 4, 4096), 256, 0, s>>>(A, pieces, total);
-        launch_check("sample_scan_kernel");
-        sample_row_kernel<T, false><<<(unsigned)A.rows, 1024, 0, s>>>(A);
+static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
+    if (A.n <= 8) {
+        const unsigned few = (unsigned)ceil_div(A.rows, 256);
+        if (A.n <= 4)
+            sample_few_kernel<T, 4><<<few, 256, 0, s>>>(A);
+        else
+            sample_few_kernel<T, 8><<<few, 256, 0, s>>>(A);
+        launch_check("sample_few_kernel");
+        return;
     }
-    launch_check("sample kernel");
+    const bool many = A.rows >= MANY_ROWS;
+    if (fused(A.rows, A.n)) {
+        if (many)
+            sample_row_kernel<T, 4, true><<<(unsigned)A.rows, 256, 0, s>>>(A);
+        else
+            sample_row_kernel<T, 16, true><<<(unsigned)A.rows, 1024, 0, s>>>(A);
+        launch_check("sample_row_kernel");
+        return;
+    }
+    const SampleSpace S(A.rows, A.n);
+    A.masses = (double *)(ws + S.masses);
+    A.block_tops = (float *)(ws + S.block_tops);
+    A.tops = (float *)(ws + S.tops);
+    const int64_t total = A.rows * S.blocks;
+    sample_scan_kernel<T><<<(unsigned)std::min<int64_t>((total + 3) / 4, 4096), 256, 0, s>>>(A, S.blocks, total);
+    launch_check("sample_scan_kernel");
+    const bool nucleus = (A.p_dev || A.top_p < 1.0f) && (A.k_dev || A.top_k == 0 || A.top_k >= A.n);
+    if (nucleus) {
+        A.splits = S.splits;
+        A.bins = (uint64_t *)(ws + S.bins);
+        A.kept = (uint64_t *)(ws + S.kept);
+        A.lists = (uint2 *)(ws + S.lists);
+        A.listed = (uint32_t *)(ws + S.listed);
+        A.heads = (SampleHead *)(ws + S.heads);
+    }
+    const int64_t chunk = nucleus ? S.chunk : A.rows;
+    for (int64_t r = 0; r < A.rows; r += chunk) {
+        A.row0 = r;
+        const unsigned rows = (unsigned)std::min(chunk, A.rows - r);
+        if (nucleus) {
+            sample_bins_kernel<T><<<rows * S.splits, 256, 0, s>>>(A, S.blocks);
+            launch_check("sample_bins_kernel");
+            sample_kept_kernel<T><<<rows * S.splits, 256, 0, s>>>(A, S.blocks);
+            launch_check("sample_kept_kernel");
+        }
+        if (many)
+            sample_row_kernel<T, 4, false><<<rows, 256, 0, s>>>(A);
+        else
+            sample_row_kernel<T, 16, false><<<rows, 1024, 0, s>>>(A);
+        launch_check("sample_row_kernel");
+    }
 }
 
-static void sample_launch(const SampleArgs &A, int32_t dtype, hipStream_t s) {
+static void sample_launch(const SampleArgs &A, int32_t dtype, void *ws, hipStream_t s) {
     if (A.rows == 0) return;
     if (dtype == SNK_F32)
-        sample_launch_t<float>(A, s);
+        sample_launch_t<float>(A, (uint8_t *)ws, s);
     else if (dtype == SNK_BF16)
-        sample_launch_t<__bf16>(A, s);
+        sample_launch_t<__bf16>(A, (uint8_t *)ws, s);
     else
-        sample_launch_t<_Float16>(A, s);
+        sample_launch_t<_Float16>(A, (uint8_t *)ws, s);
 }
 
 }  // namespace snk
@@ -893,7 +1368,7 @@ extern "C" int snk_sample_workspace(int64_t rows, int64_t n, int64_t *bytes) {
     return guard([&] {
         SNK_CHECK(bytes, SNK_ERR_INVALID, "sample_workspace: NULL argument");
         check_shape(rows, n);
-        *bytes = n <= FUSED_N ? 0 : rows * ceil_div(n, PIECE) * (8 + 4 * GP);
+        *bytes = SampleSpace(rows, n).bytes;
     });
 }
 
@@ -921,9 +1396,7 @@ extern "C" int snk_sample_logits(const void *logits, int64_t rows, int64_t n, in
         A.u = u;
         A.idx = idx;
         A.prob = prob;
-        A.masses = (double *)ws;
-        A.tops = (float *)ws + 2 * rows * ceil_div(n, PIECE);
-        sample_launch(A, cfg->dtype, stream());
+        sample_launch(A, cfg->dtype, ws, stream());
     });
 }
 
@@ -940,6 +1413,6 @@ extern "C" int snk_dqn_act_sample(snk_dqn h, snk_env env, const snk_sample_cfg_t
         A.act = act;
         A.seed = seed;
         A.tptr = &E.ctl->t;
-        sample_launch(A, SNK_F32, s);
+        sample_launch(A, SNK_F32, nullptr, s);   // 3 entries a row: no workspace
     });
 }

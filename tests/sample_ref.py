@@ -2,9 +2,22 @@
 import numpy as np
 
 
+NEAR = 1e-9
+
+
 def row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
-    """(index, probability, margin): margin is how far u, top_p or min_p is from where the answer
-    changes, relative to the row's mass; below ~1e-9 two right evaluations may differ."""
+    """(index, probability, margin): margin is how far u or min_p is from where the answer changes,
+    relative to the row's mass, and 0 where moving the limit of top_p by NEAR of the mass changes it;
+    below NEAR two right evaluations may differ."""
+    i, p, margin = _row(x, u, temperature, top_k, top_p, min_p, mask, 0.0)
+    if top_p < 1:
+        for shift in (-NEAR, NEAR):
+            if _row(x, u, temperature, top_k, top_p, min_p, mask, shift)[0] != i:
+                margin = 0.0
+    return i, p, margin
+
+
+def _row(x, u, temperature, top_k, top_p, min_p, mask, shift):
     x = np.asarray(x, np.float64).copy()
     n = x.size
     if mask is not None:
@@ -35,10 +48,8 @@ def row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
     if p < 1:
         s1 = w.sum()
         before = np.concatenate([[0.0], np.cumsum(w)[:-1]])
-        keep = before < p * s1
+        keep = before < (p + shift) * s1
         keep[0] = True
-        if order.size > 1:
-            margin = min(margin, np.abs(before[1:] - p * s1).min() / s1)
     if q > 0:
         keep &= w >= q
         far = np.abs(w - q)
