@@ -25,7 +25,6 @@ constexpr int BP = 4;           // pieces of a block, the scan's unit of mass
 constexpr int BLOCK = BP * PIECE;
 constexpr int BINS = 2048;      // of a level of the radix search: 11 + 11 + 10 bits of the key
 constexpr int LIST = 1024;      // most candidates held in LDS
-constexpr int PAIRS = 256;      // ... compared each with each
 constexpr int NBINS = 1024;     // of the nucleus' mass over the distance from the top
 constexpr int NLIST = 512;      // most entries of the cut's bin that one split of a row lists
 constexpr int SPLITS = 16;      // most splits of a row
@@ -136,23 +135,25 @@ __device__ const double POW2[128] = {
 
 // e^((x - top) / T) to 3e-12: a u that falls between the sums of two evaluations that near is a one in
 // 10^5 event over a row of 10^5 entries. 2^(i + j/128 + f/128), |f| <= 1/2: a table in LDS, a cubic,
-// and the exponent added to the table's: 15 instructions, a third of the library's exp. Entries behind
+// and the exponent added to the table's: 18 instructions, a third of the library's exp. Entries behind
 // 2^-1000 (-inf too) weigh that much: callers leave excluded ones out themselves.
+typedef const __attribute__((address_space(3))) double *LdsTable;   // no generic pointer's checks per look-up
+__device__ __forceinline__ double exp_128ths(double y, LdsTable pow2) {   // 2^(y / 128)
+    y = fmax(y, -128000.0);
+    const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);   // t's low word: y rounded
+    const int i = __double2loint(t);
+    // (ln 2 / 128)^k / k!
+    double e = fma(f, 0x1.c6b08d704a0bfp-26, 0x1.ebfbdff82c58ep-17);
+    e = fma(f, e, 0x1.62e42fefa39efp-8);
+    const double p = pow2[i & 127];
+    const double m = __hiloint2double(__double2hiint(p) + (int)((uint32_t)(i & ~127) << 13), __double2loint(p));
+    return fma(m, f * e, m);
+}
 struct Weight {
-    const double *pow2;   // LDS copy of POW2
+    LdsTable pow2;        // copy of POW2
     double top, scale, unit;   // scale = 128 log2(e) / T
     bool hard;   // only entries equal to the largest weigh: temperature 0, or +inf among them
-    __device__ __forceinline__ double soft(float x) const {
-        const double y = fmax(((double)x - top) * scale, -128000.0);
-        const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);   // t's low word: y rounded
-        const int i = (int)(uint32_t)__double_as_longlong(t);
-        // (ln 2 / 128)^k / k!
-        double e = fma(f, 0x1.c6b08d704a0bfp-26, 0x1.ebfbdff82c58ep-17);
-        e = fma(f, e, 0x1.62e42fefa39efp-8);
-        const uint64_t b = (uint64_t)__double_as_longlong(pow2[i & 127]);
-        const double m = __longlong_as_double((long long)(b + ((uint64_t)((uint32_t)(i & ~127) << 13) << 32)));
-        return fma(m, f * e, m);
-    }
+    __device__ __forceinline__ double soft(float x) const { return exp_128ths(((double)x - top) * scale, pow2); }
     __device__ __forceinline__ double real(float x) const {
         if (hard) return (double)x == top ? 1.0 : 0.0;
         return soft(x);
@@ -163,7 +164,7 @@ struct Weight {
     }
 };
 constexpr double LOG2E_128 = 0x1.71547652b82fep+7;
-__device__ __forceinline__ Weight weight(const SampleArgs &A, const SampleRow &s, const double *pow2, float top) {
+__device__ __forceinline__ Weight weight(const SampleArgs &A, const SampleRow &s, LdsTable pow2, float top) {
     return Weight{pow2, (double)top, s.inv_t * LOG2E_128, A.unit, s.greedy || top == INFINITY};
 }
 
@@ -171,24 +172,59 @@ template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) pack8 {
     T v[8];
 };
-// elements i..i+7 of a row, -inf where masked or behind the end; -0 becomes +0 (they are equal)
+// Elements i..i+7 of a row of n >= 8, -inf where masked or behind the end; -0 becomes +0 (they are
+// equal). In two steps, so that several loads are in flight before one is waited for: the load, of a
+// whole vector inside the row whatever i is, and the values, by single elements where it was moved.
 template <class T>
-__device__ __forceinline__ void load8(const T *x, const uint8_t *mask, int i, int n, float *v) {
-    if (i + 8 <= n) {
-        const pack8<T> q = *reinterpret_cast<const pack8<T> *>(x + i);
+struct Raw8 {
+    pack8<T> q;
+    pack8<uint8_t> m;
+    __device__ __forceinline__ void load(const T *x, const uint8_t *mask, int i, int n) {
+        const int at = min(i, n - 8);
+        q = *reinterpret_cast<const pack8<T> *>(x + at);
+        if (mask) m = *reinterpret_cast<const pack8<uint8_t> *>(mask + at);
+    }
+    __device__ __forceinline__ void values(const T *x, const uint8_t *mask, int i, int n, float *v) const {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = (float)q.v[k] + 0.0f;
         if (mask) {
-            const pack8<uint8_t> m = *reinterpret_cast<const pack8<uint8_t> *>(mask + i);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = m.v[k] ? -INFINITY : v[k];
         }
-    } else {
+        if (__any(i + 8 > n)) {   // a row's last vectors
+            if (i + 8 > n)
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            v[k] = i + k < n && !(mask && mask[i + k]) ? (float)x[i + k] + 0.0f : -INFINITY;
+                for (int k = 0; k < 8; ++k)
+                    v[k] = i + k < n && !(mask && mask[i + k]) ? (float)x[i + k] + 0.0f : -INFINITY;
+        }
     }
+};
+template <class T>
+__device__ __forceinline__ void load8(const T *x, const uint8_t *mask, int i, int n, float *v) {
+    Raw8<T> r;
+    r.load(x, mask, i, n);
+    r.values(x, mask, i, n, v);
 }
+template <class T>
+__device__ __forceinline__ void load_block(const T *x, const uint8_t *mask, int i, int n, float (*v)[8]) {
+    Raw8<T> r[BP];
+#pragma unroll
+    for (int p = 0; p < BP; ++p) r[p].load(x, mask, i + p * PIECE, n);
+#pragma unroll
+    for (int p = 0; p < BP; ++p) r[p].values(x, mask, i + p * PIECE, n, v[p]);
+}
+// one element, likewise
+template <class T>
+struct Raw1 {
+    T q;
+    uint8_t m;
+    __device__ __forceinline__ void load(const T *x, const uint8_t *mask, int i, int n) {
+        const int at = min(i, n - 1);
+        q = x[at];
+        m = mask ? mask[at] : 0;
+    }
+    __device__ __forceinline__ float value(int i, int n) const { return i < n && !m ? (float)q + 0.0f : -INFINITY; }
+};
 
 // v + v of the lane that CTRL names in the lanes of rows ROWS, v alone in the others
 template <class V, int CTRL, int ROWS>
@@ -214,7 +250,7 @@ __device__ __forceinline__ V wave_scan(V v) {
     return dpp_add<V, 0x143, 0xc>(v);   // row_bcast 31: into rows 2 and 3
 }
 template <class V>
-__device__ __forceinline__ V last_lane(V v) {
+__device__ __forceinline__ V read_lane(V v, int lane) {   // lane: the same on every lane
     constexpr int N = sizeof(V) / 4;
     union {
         V v;
@@ -222,8 +258,12 @@ __device__ __forceinline__ V last_lane(V v) {
     } a;
     a.v = v;
 #pragma unroll
-    for (int i = 0; i < N; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], 63);
+    for (int i = 0; i < N; ++i) a.w[i] = __builtin_amdgcn_readlane(a.w[i], lane);
     return a.v;
+}
+template <class V>
+__device__ __forceinline__ V last_lane(V v) {
+    return read_lane(v, 63);
 }
 template <class V>
 __device__ __forceinline__ V wave_sum(V v) {
@@ -256,7 +296,7 @@ __device__ __forceinline__ void answer(const SampleArgs &A, int64_t r, int i, do
 // records of the P pieces v that a wave holds: the maxima of 64 (NaN where one is among them), the
 // largest entry and, with_mass, the sum of the weights relative to it
 template <int P>
-__device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass, double scale, const double *pow2,
+__device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass, double scale, LdsTable pow2,
                                              float *tops, float *top_out, double *mass) {
     const int lane = threadIdx.x & 63;
     float top = -INFINITY;
@@ -282,17 +322,17 @@ __device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass
     if (!with_mass) return;
     double m = 0.0;
     if (top != -INFINITY && !any_nan) {
-        const Weight W{pow2, (double)top, scale, 0.0, top == INFINITY};
-        if (W.hard) {
+        if (top == INFINITY) {
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) m += v[p][e] == top ? 1.0 : 0.0;
         } else {
+            const double wide = (double)top;   // subtracted, not folded into a fused product: exact for equal entries
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) m += W.soft(v[p][e]);
+                for (int e = 0; e < 8; ++e) m += exp_128ths(((double)v[p][e] - wide) * scale, pow2);
         }
     }
     m = wave_sum(m);
@@ -314,9 +354,8 @@ __global__ __launch_bounds__(256) void sample_scan_kernel(SampleArgs A, int bloc
         const T *x = (const T *)A.x + r * A.ld;
         const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
         float v[BP][8];
-#pragma unroll
-        for (int p = 0; p < BP; ++p) load8(x, mask, b * BLOCK + p * PIECE + lane * 8, A.n, v[p]);
-        wave_records<BP>(v, s.whole(A.n), s.inv_t * LOG2E_128, pow2, A.tops + k * (BP * GP), A.block_tops + k, A.masses + k);
+        load_block(x, mask, b * BLOCK + lane * 8, A.n, v);
+        wave_records<BP>(v, s.whole(A.n), s.inv_t * LOG2E_128, (LdsTable)pow2, A.tops + k * (BP * GP), A.block_tops + k, A.masses + k);
     }
 }
 
@@ -328,15 +367,17 @@ __device__ __forceinline__ V block_scan(V v, V *sh, V &total) {
     __syncthreads();
     if (lane == 63) sh[wave] = in;
     __syncthreads();
-    V before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < RW; ++w) {
-        const V t = sh[w];
-        before += w < wave ? t : 0;
-        all += t;
+    // every wave scans the waves' sums itself, within 16 lanes
+    V sums = lane < RW ? sh[lane] : 0;
+    sums = dpp_add<V, 0x111, 0xf>(sums);
+    sums = dpp_add<V, 0x112, 0xf>(sums);
+    if (RW > 4) {
+        sums = dpp_add<V, 0x114, 0xf>(sums);
+        sums = dpp_add<V, 0x118, 0xf>(sums);
     }
-    total = all;
-    return before + (in - v);
+    total = read_lane(sums, RW - 1);
+    const int w = __builtin_amdgcn_readfirstlane(wave);
+    return (w ? read_lane(sums, w - 1) : V(0)) + (in - v);
 }
 
 template <int RW, class V>
@@ -360,7 +401,7 @@ struct Nucleus {
     }
 };
 // by the threads of one wave, from the scan's records of a row
-__device__ __forceinline__ Nucleus nucleus(const SampleArgs &A, const SampleRow &s, const double *pow2, int64_t r, int blocks) {
+__device__ __forceinline__ Nucleus nucleus(const SampleArgs &A, const SampleRow &s, LdsTable pow2, int64_t r, int blocks) {
     const int lane = threadIdx.x & 63;
     const float *bt = A.block_tops + r * blocks;
     float top = -INFINITY;
@@ -374,7 +415,7 @@ __device__ __forceinline__ Nucleus nucleus(const SampleArgs &A, const SampleRow 
     N.top = top;
     N.ok = !__ballot(nan) && fabsf(top) < INFINITY;
     if (!N.ok) return N;
-    const Weight W = weight(A, s, pow2, top);
+    const Weight W = weight(A, s, (LdsTable)pow2, top);
     double sum = 0.0;
     for (int b = lane; b < blocks; b += 64)
         if (bt[b] != -INFINITY) sum += A.masses[r * blocks + b] * W.soft(bt[b]);
@@ -398,16 +439,15 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs A, int bloc
     if (tid < 128) pow2[tid] = POW2[tid];
     for (int b = tid; b < NBINS; b += 256) mass[b] = 0;
     __syncthreads();
-    const Nucleus N = nucleus(A, s, pow2, r, blocks);
+    const Nucleus N = nucleus(A, s, (LdsTable)pow2, r, blocks);
     if (!N.ok) return;
-    const Weight W = weight(A, s, pow2, N.top);
+    const Weight W = weight(A, s, (LdsTable)pow2, N.top);
     const T *x = (const T *)A.x + r * A.ld;
     const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
     const int per = (blocks + A.splits - 1) / A.splits, end = min((part + 1) * per, blocks);
     for (int b = part * per + __builtin_amdgcn_readfirstlane(tid >> 6); b < end; b += 4) {
         float v[BP][8];
-#pragma unroll
-        for (int p = 0; p < BP; ++p) load8(x, mask, b * BLOCK + p * PIECE + lane * 8, A.n, v[p]);
+        load_block(x, mask, b * BLOCK + lane * 8, A.n, v);
 #pragma unroll
         for (int p = 0; p < BP; ++p)
 #pragma unroll
@@ -441,7 +481,7 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs A, int bloc
         listed = 0;
     }
     __syncthreads();
-    const Nucleus N = nucleus(A, s, pow2, r, blocks);
+    const Nucleus N = nucleus(A, s, (LdsTable)pow2, r, blocks);
     if (N.ok) {
         // four bins a thread, from the top
         uint64_t m[4] = {0, 0, 0, 0}, all;
@@ -465,7 +505,7 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs A, int bloc
     const int cut = cut_bin;
     if (part == 0 && tid == 0) A.heads[local] = SampleHead{cut < 0 ? 0 : cut_above, cut, cut >= 0};
     if (cut < 0) return;
-    const Weight W = weight(A, s, pow2, N.top);
+    const Weight W = weight(A, s, (LdsTable)pow2, N.top);
     const double q = (double)s.q;
     const T *x = (const T *)A.x + r * A.ld;
     const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
@@ -473,8 +513,7 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs A, int bloc
     uint2 *list = A.lists + (int64_t)blockIdx.x * NLIST;
     for (int b = part * per + __builtin_amdgcn_readfirstlane(tid >> 6); b < end; b += 4) {
         float v[BP][8];
-#pragma unroll
-        for (int p = 0; p < BP; ++p) load8(x, mask, b * BLOCK + p * PIECE + lane * 8, A.n, v[p]);
+        load_block(x, mask, b * BLOCK + lane * 8, A.n, v);
         uint64_t sum = 0;
 #pragma unroll
         for (int p = 0; p < BP; ++p)
@@ -519,7 +558,7 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
         answer(A, r, -1, nan ? NAN : 0.0);
         return;
     }
-    const Weight W = weight(A, s, pow2, top);
+    const Weight W = weight(A, s, (LdsTable)pow2, top);
     uint64_t w[N], s1 = 0, sum = 0;
     int rank[N];
     bool kept[N];
@@ -586,7 +625,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
     __shared__ int wave_nan[RW];
     __shared__ uint64_t found_mass;
     __shared__ double found_sum;
-    __shared__ uint32_t found_bin, found_count, listed, grouped;
+    __shared__ uint32_t found_bin, found_count, listed;
     __shared__ double final_sum[4];
     __shared__ uint64_t final_mass[4];
     __shared__ uint32_t final_ties[4];
@@ -594,7 +633,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
     __shared__ int final_last[4], final_hit[4];
     uint64_t *const seg_mass = mass;       // [NT], once the search is over
     uint32_t *const seg_ties = count;
-    uint32_t *const group_list = (uint32_t *)mass;   // [2 BINS], before it
+    uint32_t *const group_list = (uint32_t *)mass;   // [LIST], before it
     const int64_t r = (FUSED || !A.heads ? 0 : A.row0) + blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = A.n;
     const SampleRow s = sample_row(A, r);
@@ -602,10 +641,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
     const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
     const int pieces = (n + PIECE - 1) / PIECE, records = (pieces + REC - 1) / REC, groups = records * REC * GP;
     if (tid < 128) pow2[tid] = POW2[tid];
-    if (tid == 0) {
-        listed = 0;
-        grouped = 0;
-    }
+    if (tid == 0) listed = 0;
 
     const float *tops;
     const double *masses;
@@ -614,7 +650,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         if (wave < pieces) {
             float v[1][8];
             load8(x, mask, wave * PIECE + lane * 8, n, v[0]);
-            wave_records<1>(v, s.whole(n), s.inv_t * LOG2E_128, pow2, own_tops + wave * GP, nullptr, own_masses + wave);
+            wave_records<1>(v, s.whole(n), s.inv_t * LOG2E_128, (LdsTable)pow2, own_tops + wave * GP, nullptr, own_masses + wave);
         }
         __syncthreads();
         tops = own_tops;
@@ -623,6 +659,9 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         tops = A.tops + r * groups;
         masses = A.masses + r * records;
     }
+    const int share = (groups + NT - 1) / NT, g0 = tid * share, g1 = min(g0 + share, groups);   // consecutive groups a thread
+    const float t_first = g0 < groups ? tops[g0] : -INFINITY;
+    auto top_of = [&](int g) __attribute__((always_inline)) { return g == g0 ? t_first : tops[g]; };
     float top = -INFINITY;
     bool nan = false;
     const float *const top_src = FUSED ? tops : A.block_tops + r * records;
@@ -647,7 +686,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         if (tid == 0) answer(A, r, -1, nan ? NAN : 0.0);
         return;
     }
-    const Weight W = weight(A, s, pow2, top);
+    const Weight W = weight(A, s, (LdsTable)pow2, top);
     const double q = (double)s.q;
     const int per = (records + NT - 1) / NT, segs = (records + per - 1) / per;   // records a segment, segments
 
@@ -697,23 +736,25 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         if (!FUSED && A.heads && s.nucleus(n) && !W.hard) {
             const int64_t local = blockIdx.x;
             const SampleHead head = A.heads[local];
-            uint32_t m = 0;
             bool fits = head.ok != 0;
-            for (int k = 0; k < A.splits && fits; ++k) {
-                const uint32_t c = A.listed[local * A.splits + k];
-                fits = c <= NLIST && m + c <= LIST;
-                if (fits)
-                    for (uint32_t i = tid; i < c; i += NT) {
+            if (fits) {   // SPLITS <= 64: a lane a split, every wave for itself
+                const uint32_t c = lane < A.splits ? A.listed[local * A.splits + lane] : 0;
+                const uint32_t in = wave_scan(c), m = last_lane(in);
+                fits = !__ballot(c > NLIST) && m <= LIST;
+                for (int k = wave; k < A.splits && fits; k += RW) {
+                    const uint32_t ck = (uint32_t)__builtin_amdgcn_readlane((int)c, k);
+                    const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)in, k) - ck;
+                    for (uint32_t i = lane; i < ck; i += 64) {
                         const uint2 e = A.lists[(local * A.splits + k) * NLIST + i];
-                        list_key[m + i] = e.x;
-                        list_at[m + i] = e.y;
+                        list_key[at + i] = e.x;
+                        list_at[at + i] = e.y;
                     }
-                m += c;
+                }
+                if (tid == 0) listed = m;
             }
             binned = fits;
             use_list = fits;
             above_list = head.above;
-            if (tid == 0) listed = m;
         } else {
             // candidates: what can be in the cut, by the groups' maxima: bins of the distance from the
             // top up to here, and, where min-p is not to change the mass that top-p goes by, this near
@@ -731,8 +772,8 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
 #pragma unroll
                 for (int b = 0; b < BT; ++b) count[b * NT + tid] = 0;
                 __syncthreads();
-                for (int g = tid; g < groups; g += NT) {
-                    const float t = tops[g];
+                for (int g = g0; g < g1; ++g) {
+                    const float t = top_of(g);
                     if (t != -INFINITY) atomicAdd(&count[far_bin(top - t)], 1u);
                 }
                 if (tid == 0) found_bin = BINS - 1;
@@ -754,149 +795,171 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
                 use_list = all >= wanted || n <= LIST || by_q;
             }
             if (use_list) {
-                for (int g = tid; g < groups; g += NT)
-                    if (candidate(tops[g])) {
-                        const uint32_t at = atomicAdd(&grouped, 1u);
-                        if (at < 2 * BINS) group_list[at] = (uint32_t)g;
-                    }
+                // the groups that hold candidates, in order
+                uint32_t c = 0, ng;
+                for (int g = g0; g < g1; ++g) c += candidate(top_of(g));
+                uint32_t to = block_scan<RW, uint32_t>(c, scan32, ng);
+                use_list = ng <= LIST;   // each holds one at least
+                if (use_list && c)
+                    for (int g = g0; g < g1; ++g)
+                        if (candidate(top_of(g))) group_list[to++] = (uint32_t)g;
                 __syncthreads();
-                const uint32_t ng = grouped;
-                use_list = ng <= 2 * BINS;
-                for (uint32_t i0 = wave * 8; use_list && i0 < ng; i0 += RW * 8) {   // a group 8 lanes
-                    const uint32_t i = i0 + (lane >> 3);
-                    const int at0 = i < ng ? (int)group_list[i] * GROUP + (lane & 7) * 8 : n;
-                    float v[8];
-                    load8(x, mask, at0, n, v);
-uint64_t who[8];
-                    uint32_t found = 0;
+                // their candidates, in order: a wave a group, its groups consecutive, up to DEEP in flight
+                uint32_t m_before = 0;
+                constexpr int DEEP = RW == 16 ? 4 : 8;
+                const int deep = (int)min((uint32_t)DEEP, (ng + RW - 1) / RW);
+                for (uint32_t i0 = 0; use_list && i0 < ng; i0 += RW * deep) {
+                    Raw1<T> raw[DEEP];
+                    float v[DEEP];
+                    int at0[DEEP];
+                    uint64_t who[DEEP];
+                    uint32_t own = 0;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        who[e] = __ballot(candidate(v[e]));
-                        found += (uint32_t)__popcll(who[e]);
+                    for (int o = 0; o < DEEP; ++o) {
+                        const uint32_t i = i0 + wave * deep + o;
+                        at0[o] = o < deep && i < ng ? (int)group_list[i] * GROUP + lane : n;
                     }
-                    if (!found) continue;
-                    uint32_t at = 0;
-                    if (lane == 0) at = atomicAdd(&listed, found);
-                    at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t mine = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(who[e] >> 32),
-                                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)who[e], 0));
-                        if ((who[e] >> lane & 1) && mine < LIST) {
-                            list_key[mine] = key_of(v[e]);
-                            list_at[mine] = (uint32_t)(at0 + e);
+                    for (int o = 0; o < DEEP; ++o) raw[o].load(x, mask, at0[o], n);
+#pragma unroll
+                    for (int o = 0; o < DEEP; ++o) {
+                        v[o] = raw[o].value(at0[o], n);
+                        who[o] = __ballot(candidate(v[o]));
+                        own += (uint32_t)__popcll(who[o]);
+                    }
+                    if (lane == 0) scan32[wave] = own;
+                    __syncthreads();
+                    uint32_t owns = lane < RW ? scan32[lane] : 0;
+                    owns = wave_scan(owns);
+                    uint32_t at = m_before + (wave ? read_lane(owns, wave - 1) : 0);
+                    m_before += read_lane(owns, RW - 1);
+#pragma unroll
+                    for (int o = 0; o < DEEP; ++o) {
+                        const uint32_t mine = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(who[o] >> 32),
+                                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)who[o], 0));
+                        if ((who[o] >> lane & 1) && mine < LIST) {
+                            list_key[mine] = key_of(v[o]);
+                            list_at[mine] = (uint32_t)at0[o];
                         }
-                        at += (uint32_t)__popcll(who[e]);
+                        at += (uint32_t)__popcll(who[o]);
                     }
+                    __syncthreads();
                 }
+                if (tid == 0) listed = m_before;
             }
         }
         __syncthreads();
         uint32_t m = use_list ? listed : LIST + 1;
-        if (m <= PAIRS) {
-            // each candidate's rank and mass before it, by comparing all pairs: four threads a candidate,
-            // sixteen bytes of LDS a comparison, no branches (with them: 350 cycles a comparison)
+        if (m <= 64 && !s.nucleus(n)) {
+            // a candidate a lane, in index order: its rank and the mass before it, by every wave over its
+            // share of the others, then the answer by one wave's prefix sums
+            const bool is = lane < (int)m;
+            const uint32_t key = is ? list_key[lane] : 0;
+            const double real = is ? W.real(of_key(key)) : 0.0;
+            const uint64_t w = is ? W.fixed(real) : 0;
+            bool kept = is;
+            if (s.k < n) {
+                uint32_t rank = 0;
+                uint64_t before = 0;
+                for (int i = wave; i < (int)m; i += RW) {
+                    const uint32_t ki = read_lane(key, i);
+                    const bool first = (ki > key) | ((ki == key) & (i < lane));
+                    const uint64_t wi = read_lane(w, i);
+                    rank += first;
+                    before += first ? wi : 0;
+                }
+                count[tid] = rank;
+                mass[tid] = before;
+                __syncthreads();
+                if (wave != 0) return;
+#pragma unroll
+                for (int v = 1; v < RW; ++v) {
+                    rank += count[v * 64 + lane];
+                    before += mass[v * 64 + lane];
+                }
+                kept = is && rank < (uint32_t)s.k;
+                if (s.p < 1.0f) {
+                    const double limit = (double)s.p * (double)wave_sum<uint64_t>(kept ? w : 0);
+                    kept = kept && (rank == 0 || (double)before < limit);
+                }
+            }
+            if (wave != 0) return;
+            const uint64_t own = kept && real >= q ? w : 0, upto = wave_scan(own), sum = last_lane(upto);
+            const double t = (double)s.u * (double)sum;
+            if (own && (double)upto > t && !((double)(upto - own) > t))   // one lane
+                answer(A, r, (int)list_at[lane], real * A.unit / (double)sum);
+            return;
+        }
+        bool from_list = m <= LIST;
+        constexpr int PAIRS = NT >= 512 ? 256 : 128;
+        if (cut && m <= PAIRS) {
+            // each candidate's rank and the mass before it, by comparing all pairs: four threads a
+            // candidate, sixteen bytes of LDS a comparison, no branches (350 cycles a comparison with them)
             constexpr int AT_ONCE = NT / 4, ROUNDS = PAIRS / AT_ONCE;   // candidates a round
             uint4 *const cand = (uint4 *)mass;   // key, index, weight
             if (tid < (int)m) {
                 const uint64_t w = W.fixed(W.real(of_key(list_key[tid])));
                 cand[tid] = make_uint4(list_key[tid], list_at[tid], (uint32_t)w, (uint32_t)(w >> 32));
             }
+            if (tid == 0) {
+                found_bin = 0xFFFFFFFFu;
+                found_count = 0;
+            }
             __syncthreads();
-            uint32_t rank_[ROUNDS];
-            uint64_t before_[ROUNDS], w_[ROUNDS];
-            uint32_t k_[ROUNDS], a_[ROUNDS];
+            uint32_t rank[ROUNDS], key[ROUNDS];
+            uint64_t before[ROUNDS], s1 = 0;
+            bool own[ROUNDS];   // the thread that answers for a candidate
 #pragma unroll
             for (int o = 0; o < ROUNDS; ++o) {
                 const uint32_t j = o * AT_ONCE + (tid >> 2);
-                rank_[o] = 0;
-                before_[o] = w_[o] = 0;
-                k_[o] = a_[o] = 0;
-                if (o * AT_ONCE >= (int)m) break;
-                if (j < m) {
-                    const uint4 c = cand[j];
-                    k_[o] = c.x;
-                    a_[o] = c.y;
-                    w_[o] = c.z | (uint64_t)c.w << 32;
-                }
+                rank[o] = key[o] = 0;
+                before[o] = 0;
+                own[o] = (tid & 3) == 0 && j < m;
+                if (o * AT_ONCE >= (int)m) continue;
+                const uint4 me = cand[min(j, m - 1)];
+                key[o] = me.x;
 #pragma unroll 4
                 for (uint32_t i = tid & 3; i < m; i += 4) {
                     const uint4 c = cand[i];
-                    const bool first = (c.x > k_[o]) | ((c.x == k_[o]) & (c.y < a_[o]));
-                    rank_[o] += first;
-                    before_[o] += first ? c.z | (uint64_t)c.w << 32 : 0;
+                    const bool first = (c.x > me.x) | ((c.x == me.x) & (c.y < me.y));
+                    rank[o] += first;
+                    before[o] += first ? c.z | (uint64_t)c.w << 32 : 0;
                 }
-                rank_[o] += __shfl_xor(rank_[o], 1);
-                rank_[o] += __shfl_xor(rank_[o], 2);
-                before_[o] += __shfl_xor(before_[o], 1);
-                before_[o] += __shfl_xor(before_[o], 2);
+                rank[o] += __shfl_xor(rank[o], 1);
+                rank[o] += __shfl_xor(rank[o], 2);
+                before[o] += __shfl_xor(before[o], 1);
+                before[o] += __shfl_xor(before[o], 2);
+                s1 += own[o] && rank[o] < (uint32_t)s.k ? me.z | (uint64_t)me.w << 32 : 0;
             }
-            auto own = [&](int o) __attribute__((always_inline)) {   // the thread that answers for a candidate
-                return (tid & 3) == 0 && o * AT_ONCE + (tid >> 2) < (int)m;
-            };
-            uint64_t s1 = 0;
-#pragma unroll
-            for (int o = 0; o < ROUNDS; ++o) s1 += own(o) && rank_[o] < (uint32_t)s.k ? w_[o] : 0;
-            s1 = block_sum<RW, uint64_t>(s1, scan64);
-            // top-p alone: the list has to hold all of the nucleus
-            const bool inside = s.k < n || s.p >= 1.0f || (!binned && (double)s1 >= limit_row);
+            double limit = limit_row;
+            bool inside = true;
+            if (!binned && s.p < 1.0f) {
+                s1 = block_sum<RW, uint64_t>(s1, scan64);
+                // top-p alone: the list has to hold all of the nucleus
+                inside = s.k < n || (double)s1 >= limit_row;
+                if (s.k < n) limit = (double)s.p * (double)s1;
+            }
             if (inside) {
-                const double limit = s.k < n ? (double)s.p * (double)s1 : limit_row;
-                uint64_t sum = 0;
                 bool kept[ROUNDS];
 #pragma unroll
                 for (int o = 0; o < ROUNDS; ++o) {
-                    kept[o] = own(o) && rank_[o] < (uint32_t)s.k &&
-                              (s.p >= 1.0f || rank_[o] == 0 || (double)before_[o] < limit) && W.real(of_key(k_[o])) >= q;
-                    if (own(o) && !kept[o]) cand[o * AT_ONCE + (tid >> 2)].z = cand[o * AT_ONCE + (tid >> 2)].w = 0;
-                    sum += kept[o] ? w_[o] : 0;
-                }
-                sum = block_sum<RW, uint64_t>(sum, scan64);   // and its barriers
-                const double t = (double)s.u * (double)sum;
-#pragma unroll
-                for (int o = 0; o < ROUNDS; ++o) {
-                    if (o * AT_ONCE >= (int)m) break;
-                    uint64_t upto = 0;
-#pragma unroll 4
-                    for (uint32_t i = tid & 3; i < m; i += 4) {
-                        const uint4 c = cand[i];
-                        upto += c.y <= a_[o] ? c.z | (uint64_t)c.w << 32 : 0;
-                    }
-                    upto += __shfl_xor(upto, 1);
-                    upto += __shfl_xor(upto, 2);
-                    if (kept[o] && w_[o] && (double)upto > t && !((double)(upto - w_[o]) > t))   // one thread
-                        answer(A, r, (int)a_[o], W.real(of_key(k_[o])) * A.unit / (double)sum);
-                }
-                return;
-            }
-            if (binned) {
-                // the cut among the bin's entries: the last one with less than the limit before it
-                if (tid == 0) {
-                    found_bin = 0xFFFFFFFFu;
-                    found_count = 0;
-                }
-                __syncthreads();
-                bool kept[ROUNDS];
-#pragma unroll
-                for (int o = 0; o < ROUNDS; ++o) {
-                    kept[o] = own(o) && ((above_list == 0 && rank_[o] == 0) || (double)(above_list + before_[o]) < limit_row);
-                    if (kept[o]) atomicMin(&found_bin, k_[o]);
+                    kept[o] = own[o] && rank[o] < (uint32_t)s.k &&
+                              (s.p >= 1.0f || (above_list == 0 && rank[o] == 0) || (double)(above_list + before[o]) < limit);
+                    if (kept[o]) atomicMin(&found_bin, key[o]);
                 }
                 __syncthreads();
                 kt = found_bin;
 #pragma unroll
                 for (int o = 0; o < ROUNDS; ++o)
-                    if (kept[o] && k_[o] == kt) atomicAdd(&found_count, 1u);
+                    if (kept[o] && key[o] == kt) atomicAdd(&found_count, 1u);
                 __syncthreads();
                 nt = found_count;
-                __syncthreads();
             } else {
-                __syncthreads();
-                m = LIST + 1;
+                from_list = false;
             }
+            __syncthreads();
         }
         // larger cuts: a radix search over the listed candidates or, where they are too many, the row
-        bool from_list = m <= LIST;
         auto each = [&](auto &&f) __attribute__((always_inline)) {   // f(x, index) for every candidate, or every entry
             if (from_list) {
                 for (uint32_t i = tid; i < m; i += NT) f(of_key(list_key[i]), (int)list_at[i]);
@@ -1020,6 +1083,36 @@ uint64_t who[8];
             }
         }
         const bool bounded = kt != 0;
+
+        if (from_list && !binned) {
+            // the list is in index order and holds all that is kept: its prefix sums answer
+            const uint32_t share = (m + NT - 1) / NT, i0 = min(tid * share, m), i1 = min(i0 + share, m);
+            uint32_t t = 0, all_ties;
+            for (uint32_t i = i0; i < i1; ++i) t += bounded && list_key[i] == kt;
+            uint32_t rank = block_scan<RW, uint32_t>(t, scan32, all_ties);
+            const uint32_t rank0 = rank;
+            auto kept_weight = [&](uint32_t i) __attribute__((always_inline)) -> uint64_t {
+                const uint32_t key = list_key[i];
+                if (key < kt || (bounded && key == kt && rank++ >= nt)) return 0;
+                const double w = W.real(of_key(key));
+                return w >= q ? W.fixed(w) : 0;
+            };
+            uint64_t own = 0, sum;
+            for (uint32_t i = i0; i < i1; ++i) own += kept_weight(i);
+            uint64_t upto = block_scan<RW, uint64_t>(own, scan64, sum);
+            const double t_sum = (double)s.u * (double)sum;
+            if (own && !((double)upto > t_sum) && (double)(upto + own) > t_sum) {   // one thread
+                rank = rank0;
+                for (uint32_t i = i0; i < i1; ++i) {
+                    upto += kept_weight(i);
+                    if ((double)upto > t_sum) {
+                        answer(A, r, (int)list_at[i], W.real(of_key(list_key[i])) * A.unit / (double)sum);
+                        break;
+                    }
+                }
+            }
+            return;
+        }
 
         // masses and ties by segment, in index order
         const double wt = bounded ? W.real(of_key(kt)) : 0.0;
@@ -1343,7 +1436,7 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
             launch_check("sample_kept_kernel");
         }
         if (many)
-            sample_row_kernel<T, 4, false><<<rows, 256, 0, s>>>(A);
+            sample_row_kernel<T, 8, false><<<rows, 512, 0, s>>>(A);
         else
             sample_row_kernel<T, 16, false><<<rows, 1024, 0, s>>>(A);
         launch_check("sample_row_kernel");
