@@ -77,7 +77,7 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs &A, int64_t r) 
     SampleRow s;
     const float t = A.t_dev ? A.t_dev[r] : A.temperature;
     s.greedy = !(t > 0.0f);
-    s.inv_t = s.greedy ? 0.0 : 1.0 / (double)t;
+    s.inv_t = s.greedy ? 1.0 : fmax(1.0 / (double)t, 1e-300);   // t = inf: all alike, -inf still nothing
     const int k = A.k_dev ? A.k_dev[r] : A.top_k;
     s.k = s.greedy ? 1 : k > 0 && k < A.n ? k : A.n;
     const float p = A.p_dev ? A.p_dev[r] : A.top_p, q = A.q_dev ? A.q_dev[r] : A.min_p;
@@ -90,70 +90,76 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs &A, int64_t r) 
 
 // order-preserving key of an allowed logit; 0 for -inf (excluded)
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);   // -0 becomes +0: they are equal
     return x == -INFINITY ? 0u : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// 2^(i/128)
-__device__ const double POW2[128] = {
-    0x1.0000000000000p+0, 0x1.0163da9fb3335p+0, 0x1.02c9a3e778061p+0, 0x1.04315e86e7f85p+0,
-    0x1.059b0d3158574p+0, 0x1.0706b29ddf6dep+0, 0x1.0874518759bc8p+0, 0x1.09e3ecac6f383p+0,
-    0x1.0b5586cf9890fp+0, 0x1.0cc922b7247f7p+0, 0x1.0e3ec32d3d1a2p+0, 0x1.0fb66affed31bp+0,
-    0x1.11301d0125b51p+0, 0x1.12abdc06c31ccp+0, 0x1.1429aaea92de0p+0, 0x1.15a98c8a58e51p+0,
-    0x1.172b83c7d517bp+0, 0x1.18af9388c8deap+0, 0x1.1a35beb6fcb75p+0, 0x1.1bbe084045cd4p+0,
-    0x1.1d4873168b9aap+0, 0x1.1ed5022fcd91dp+0, 0x1.2063b88628cd6p+0, 0x1.21f49917ddc96p+0,
-    0x1.2387a6e756238p+0, 0x1.251ce4fb2a63fp+0, 0x1.26b4565e27cddp+0, 0x1.284dfe1f56381p+0,
-    0x1.29e9df51fdee1p+0, 0x1.2b87fd0dad990p+0, 0x1.2d285a6e4030bp+0, 0x1.2ecafa93e2f56p+0,
-    0x1.306fe0a31b715p+0, 0x1.32170fc4cd831p+0, 0x1.33c08b26416ffp+0, 0x1.356c55f929ff1p+0,
-    0x1.371a7373aa9cbp+0, 0x1.38cae6d05d866p+0, 0x1.3a7db34e59ff7p+0, 0x1.3c32dc313a8e5p+0,
-    0x1.3dea64c123422p+0, 0x1.3fa4504ac801cp+0, 0x1.4160a21f72e2ap+0, 0x1.431f5d950a897p+0,
-    0x1.44e086061892dp+0, 0x1.46a41ed1d0057p+0, 0x1.486a2b5c13cd0p+0, 0x1.4a32af0d7d3dep+0,
-    0x1.4bfdad5362a27p+0, 0x1.4dcb299fddd0dp+0, 0x1.4f9b2769d2ca7p+0, 0x1.516daa2cf6642p+0,
-    0x1.5342b569d4f82p+0, 0x1.551a4ca5d920fp+0, 0x1.56f4736b527dap+0, 0x1.58d12d497c7fdp+0,
-    0x1.5ab07dd485429p+0, 0x1.5c9268a5946b7p+0, 0x1.5e76f15ad2148p+0, 0x1.605e1b976dc09p+0,
-    0x1.6247eb03a5585p+0, 0x1.6434634ccc320p+0, 0x1.6623882552225p+0, 0x1.68155d44ca973p+0,
-    0x1.6a09e667f3bcdp+0, 0x1.6c012750bdabfp+0, 0x1.6dfb23c651a2fp+0, 0x1.6ff7df9519484p+0,
-    0x1.71f75e8ec5f74p+0, 0x1.73f9a48a58174p+0, 0x1.75feb564267c9p+0, 0x1.780694fde5d3fp+0,
-    0x1.7a11473eb0187p+0, 0x1.7c1ed0130c132p+0, 0x1.7e2f336cf4e62p+0, 0x1.80427543e1a12p+0,
-    0x1.82589994cce13p+0, 0x1.8471a4623c7adp+0, 0x1.868d99b4492edp+0, 0x1.88ac7d98a6699p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.8cf3216b5448cp+0, 0x1.8f1ae99157736p+0, 0x1.9145b0b91ffc6p+0,
-    0x1.93737b0cdc5e5p+0, 0x1.95a44cbc8520fp+0, 0x1.97d829fde4e50p+0, 0x1.9a0f170ca07bap+0,
-    0x1.9c49182a3f090p+0, 0x1.9e86319e32323p+0, 0x1.a0c667b5de565p+0, 0x1.a309bec4a2d33p+0,
-    0x1.a5503b23e255dp+0, 0x1.a799e1330b358p+0, 0x1.a9e6b5579fdbfp+0, 0x1.ac36bbfd3f37ap+0,
-    0x1.ae89f995ad3adp+0, 0x1.b0e07298db666p+0, 0x1.b33a2b84f15fbp+0, 0x1.b59728de5593ap+0,
-    0x1.b7f76f2fb5e47p+0, 0x1.ba5b030a1064ap+0, 0x1.bcc1e904bc1d2p+0, 0x1.bf2c25bd71e09p+0,
-    0x1.c199bdd85529cp+0, 0x1.c40ab5fffd07ap+0, 0x1.c67f12e57d14bp+0, 0x1.c8f6d9406e7b5p+0,
-    0x1.cb720dcef9069p+0, 0x1.cdf0b555dc3fap+0, 0x1.d072d4a07897cp+0, 0x1.d2f87080d89f2p+0,
-    0x1.d5818dcfba487p+0, 0x1.d80e316c98398p+0, 0x1.da9e603db3285p+0, 0x1.dd321f301b460p+0,
-    0x1.dfc97337b9b5fp+0, 0x1.e264614f5a129p+0, 0x1.e502ee78b3ff6p+0, 0x1.e7a51fbc74c83p+0,
-    0x1.ea4afa2a490dap+0, 0x1.ecf482d8e67f1p+0, 0x1.efa1bee615a27p+0, 0x1.f252b376bba97p+0,
-    0x1.f50765b6e4540p+0, 0x1.f7bfdad9cbe14p+0, 0x1.fa7c1819e90d8p+0, 0x1.fd3c22b8f71f1p+0,
+// The bits of 2^(j/128) less j 2^45: adding i 2^45, i = 128 e + j, gives those of 2^(e + j/128)
+// without splitting i
+__device__ const uint64_t POW2[128] = {
+    0x3ff0000000000000ull, 0x3feff63da9fb3335ull, 0x3fefec9a3e778061ull, 0x3fefe315e86e7f85ull,
+    0x3fefd9b0d3158574ull, 0x3fefd06b29ddf6deull, 0x3fefc74518759bc8ull, 0x3fefbe3ecac6f383ull,
+    0x3fefb5586cf9890full, 0x3fefac922b7247f7ull, 0x3fefa3ec32d3d1a2ull, 0x3fef9b66affed31bull,
+    0x3fef9301d0125b51ull, 0x3fef8abdc06c31ccull, 0x3fef829aaea92de0ull, 0x3fef7a98c8a58e51ull,
+    0x3fef72b83c7d517bull, 0x3fef6af9388c8deaull, 0x3fef635beb6fcb75ull, 0x3fef5be084045cd4ull,
+    0x3fef54873168b9aaull, 0x3fef4d5022fcd91dull, 0x3fef463b88628cd6ull, 0x3fef3f49917ddc96ull,
+    0x3fef387a6e756238ull, 0x3fef31ce4fb2a63full, 0x3fef2b4565e27cddull, 0x3fef24dfe1f56381ull,
+    0x3fef1e9df51fdee1ull, 0x3fef187fd0dad990ull, 0x3fef1285a6e4030bull, 0x3fef0cafa93e2f56ull,
+    0x3fef06fe0a31b715ull, 0x3fef0170fc4cd831ull, 0x3feefc08b26416ffull, 0x3feef6c55f929ff1ull,
+    0x3feef1a7373aa9cbull, 0x3feeecae6d05d866ull, 0x3feee7db34e59ff7ull, 0x3feee32dc313a8e5ull,
+    0x3feedea64c123422ull, 0x3feeda4504ac801cull, 0x3feed60a21f72e2aull, 0x3feed1f5d950a897ull,
+    0x3feece086061892dull, 0x3feeca41ed1d0057ull, 0x3feec6a2b5c13cd0ull, 0x3feec32af0d7d3deull,
+    0x3feebfdad5362a27ull, 0x3feebcb299fddd0dull, 0x3feeb9b2769d2ca7ull, 0x3feeb6daa2cf6642ull,
+    0x3feeb42b569d4f82ull, 0x3feeb1a4ca5d920full, 0x3feeaf4736b527daull, 0x3feead12d497c7fdull,
+    0x3feeab07dd485429ull, 0x3feea9268a5946b7ull, 0x3feea76f15ad2148ull, 0x3feea5e1b976dc09ull,
+    0x3feea47eb03a5585ull, 0x3feea34634ccc320ull, 0x3feea23882552225ull, 0x3feea155d44ca973ull,
+    0x3feea09e667f3bcdull, 0x3feea012750bdabfull, 0x3fee9fb23c651a2full, 0x3fee9f7df9519484ull,
+    0x3fee9f75e8ec5f74ull, 0x3fee9f9a48a58174ull, 0x3fee9feb564267c9ull, 0x3feea0694fde5d3full,
+    0x3feea11473eb0187ull, 0x3feea1ed0130c132ull, 0x3feea2f336cf4e62ull, 0x3feea427543e1a12ull,
+    0x3feea589994cce13ull, 0x3feea71a4623c7adull, 0x3feea8d99b4492edull, 0x3feeaac7d98a6699ull,
+    0x3feeace5422aa0dbull, 0x3feeaf3216b5448cull, 0x3feeb1ae99157736ull, 0x3feeb45b0b91ffc6ull,
+    0x3feeb737b0cdc5e5ull, 0x3feeba44cbc8520full, 0x3feebd829fde4e50ull, 0x3feec0f170ca07baull,
+    0x3feec49182a3f090ull, 0x3feec86319e32323ull, 0x3feecc667b5de565ull, 0x3feed09bec4a2d33ull,
+    0x3feed503b23e255dull, 0x3feed99e1330b358ull, 0x3feede6b5579fdbfull, 0x3feee36bbfd3f37aull,
+    0x3feee89f995ad3adull, 0x3feeee07298db666ull, 0x3feef3a2b84f15fbull, 0x3feef9728de5593aull,
+    0x3feeff76f2fb5e47ull, 0x3fef05b030a1064aull, 0x3fef0c1e904bc1d2ull, 0x3fef12c25bd71e09ull,
+    0x3fef199bdd85529cull, 0x3fef20ab5fffd07aull, 0x3fef27f12e57d14bull, 0x3fef2f6d9406e7b5ull,
+    0x3fef3720dcef9069ull, 0x3fef3f0b555dc3faull, 0x3fef472d4a07897cull, 0x3fef4f87080d89f2ull,
+    0x3fef5818dcfba487ull, 0x3fef60e316c98398ull, 0x3fef69e603db3285ull, 0x3fef7321f301b460ull,
+    0x3fef7c97337b9b5full, 0x3fef864614f5a129ull, 0x3fef902ee78b3ff6ull, 0x3fef9a51fbc74c83ull,
+    0x3fefa4afa2a490daull, 0x3fefaf482d8e67f1ull, 0x3fefba1bee615a27ull, 0x3fefc52b376bba97ull,
+    0x3fefd0765b6e4540ull, 0x3fefdbfdad9cbe14ull, 0x3fefe7c1819e90d8ull, 0x3feff3c22b8f71f1ull,
 };
 
 // e^((x - top) / T) to 3e-12: a u that falls between the sums of two evaluations that near is a one in
 // 10^5 event over a row of 10^5 entries. 2^(i + j/128 + f/128), |f| <= 1/2: a table in LDS, a cubic,
-// and the exponent added to the table's: 18 instructions, a third of the library's exp. Entries behind
-// 2^-1000 (-inf too) weigh that much: callers leave excluded ones out themselves.
-typedef const __attribute__((address_space(3))) double *LdsTable;   // no generic pointer's checks per look-up
-__device__ __forceinline__ double exp_128ths(double y, LdsTable pow2) {   // 2^(y / 128)
-    y = fmax(y, -128000.0);
-    const double t = y + 0x1.8p52, f = y - (t - 0x1.8p52);   // t's low word: y rounded
+// and the exponent added to the table's: 15 instructions, a quarter of the library's exp. Entries
+// behind 2^-1000 (-inf too) weigh that much: callers leave excluded ones out themselves.
+typedef const __attribute__((address_space(3))) uint64_t *LdsTable;   // no generic pointer's checks per look-up
+struct Scale {
+    double scale, low;   // 128 log2(e) / T, and the distance at which the weight is 2^-1000
+};
+__device__ __forceinline__ double exp_weight(double d, Scale S, LdsTable pow2) {   // 2^(d scale / 128), d <= 0
+    d = fmax(d, S.low);
+    const double t = fma(d, S.scale, 0x1.8p52), f = fma(d, S.scale, 0x1.8p52 - t);   // t's low word: d scale rounded
     const int i = __double2loint(t);
     // (ln 2 / 128)^k / k!
     double e = fma(f, 0x1.c6b08d704a0bfp-26, 0x1.ebfbdff82c58ep-17);
     e = fma(f, e, 0x1.62e42fefa39efp-8);
-    const double p = pow2[i & 127];
-    const double m = __hiloint2double(__double2hiint(p) + (int)((uint32_t)(i & ~127) << 13), __double2loint(p));
+    const uint64_t p = pow2[i & 127];
+    const double m = __hiloint2double((int)((uint32_t)(p >> 32) + ((uint32_t)i << 13)), (int)(uint32_t)p);
     return fma(m, f * e, m);
 }
 struct Weight {
     LdsTable pow2;        // copy of POW2
-    double top, scale, unit;   // scale = 128 log2(e) / T
+    double top;
+    Scale scale;
+    double unit;
     bool hard;   // only entries equal to the largest weigh: temperature 0, or +inf among them
-    __device__ __forceinline__ double soft(float x) const { return exp_128ths(((double)x - top) * scale, pow2); }
+    __device__ __forceinline__ double soft(float x) const { return exp_weight((double)x - top, scale, pow2); }
     __device__ __forceinline__ double real(float x) const {
         if (hard) return (double)x == top ? 1.0 : 0.0;
         return soft(x);
@@ -163,17 +169,19 @@ struct Weight {
         return (uint64_t)__double_as_longlong(fma(w, unit, 0x1p52)) & 0xFFFFFFFFFFFFFull;
     }
 };
-constexpr double LOG2E_128 = 0x1.71547652b82fep+7;
+__device__ __forceinline__ Scale scale_of(const SampleRow &s) {
+    const double scale = s.inv_t * 0x1.71547652b82fep+7;
+    return Scale{scale, -128000.0 / scale};
+}
 __device__ __forceinline__ Weight weight(const SampleArgs &A, const SampleRow &s, LdsTable pow2, float top) {
-    return Weight{pow2, (double)top, s.inv_t * LOG2E_128, A.unit, s.greedy || top == INFINITY};
+    return Weight{pow2, (double)top, scale_of(s), A.unit, s.greedy || top == INFINITY};
 }
 
 template <class T>
 struct __attribute__((packed, aligned(sizeof(T)))) pack8 {
     T v[8];
 };
-// Elements i..i+7 of a row of n >= 8, -inf where masked or behind the end; -0 becomes +0 (they are
-// equal). In two steps, so that several loads are in flight before one is waited for: the load, of a
+// Elements i..i+7 of a row of n >= 8, -inf where masked or behind the end. In two steps, so that several loads are in flight before one is waited for: the load, of a
 // whole vector inside the row whatever i is, and the values, by single elements where it was moved.
 template <class T>
 struct Raw8 {
@@ -186,7 +194,7 @@ struct Raw8 {
     }
     __device__ __forceinline__ void values(const T *x, const uint8_t *mask, int i, int n, float *v) const {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (float)q.v[k] + 0.0f;
+        for (int k = 0; k < 8; ++k) v[k] = (float)q.v[k];
         if (mask) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = m.v[k] ? -INFINITY : v[k];
@@ -195,7 +203,7 @@ struct Raw8 {
             if (i + 8 > n)
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                    v[k] = i + k < n && !(mask && mask[i + k]) ? (float)x[i + k] + 0.0f : -INFINITY;
+                    v[k] = i + k < n && !(mask && mask[i + k]) ? (float)x[i + k] : -INFINITY;
         }
     }
 };
@@ -223,7 +231,7 @@ struct Raw1 {
         q = x[at];
         m = mask ? mask[at] : 0;
     }
-    __device__ __forceinline__ float value(int i, int n) const { return i < n && !m ? (float)q + 0.0f : -INFINITY; }
+    __device__ __forceinline__ float value(int i, int n) const { return i < n && !m ? (float)q : -INFINITY; }
 };
 
 // v + v of the lane that CTRL names in the lanes of rows ROWS, v alone in the others
@@ -296,7 +304,7 @@ __device__ __forceinline__ void answer(const SampleArgs &A, int64_t r, int i, do
 // records of the P pieces v that a wave holds: the maxima of 64 (NaN where one is among them), the
 // largest entry and, with_mass, the sum of the weights relative to it
 template <int P>
-__device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass, double scale, LdsTable pow2,
+__device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass, Scale scale, LdsTable pow2,
                                              float *tops, float *top_out, double *mass) {
     const int lane = threadIdx.x & 63;
     float top = -INFINITY;
@@ -332,7 +340,7 @@ __device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass
 #pragma unroll
             for (int p = 0; p < P; ++p)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) m += exp_128ths(((double)v[p][e] - wide) * scale, pow2);
+                for (int e = 0; e < 8; ++e) m += exp_weight((double)v[p][e] - wide, scale, pow2);
         }
     }
     m = wave_sum(m);
@@ -342,7 +350,7 @@ __device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass
 // ---------------------------------------------------------------- the scan: a wave a block
 template <class T>
 __global__ __launch_bounds__(256) void sample_scan_kernel(SampleArgs A, int blocks, int64_t total) {
-    __shared__ double pow2[128];
+    __shared__ uint64_t pow2[128];
     if (threadIdx.x < 128) pow2[threadIdx.x] = POW2[threadIdx.x];
     __syncthreads();
     const int lane = threadIdx.x & 63;
@@ -355,7 +363,7 @@ __global__ __launch_bounds__(256) void sample_scan_kernel(SampleArgs A, int bloc
         const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
         float v[BP][8];
         load_block(x, mask, b * BLOCK + lane * 8, A.n, v);
-        wave_records<BP>(v, s.whole(A.n), s.inv_t * LOG2E_128, (LdsTable)pow2, A.tops + k * (BP * GP), A.block_tops + k, A.masses + k);
+        wave_records<BP>(v, s.whole(A.n), scale_of(s), (LdsTable)pow2, A.tops + k * (BP * GP), A.block_tops + k, A.masses + k);
     }
 }
 
@@ -427,54 +435,64 @@ __device__ __forceinline__ Nucleus nucleus(const SampleArgs &A, const SampleRow 
     return N;
 }
 
-// a workgroup a split of a row: its mass by bins
+// a workgroup a split of a row, a wave a piece: its mass by bins
+constexpr int NW = 16, NTH = 64 * NW;
+static_assert(NBINS == NTH && NW % BP == 0, "a bin a thread, whole blocks a round");
 template <class T>
-__global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs A, int blocks) {
-    __shared__ double pow2[128];
+__global__ __launch_bounds__(1024) void sample_bins_kernel(SampleArgs A, int blocks) {
+    __shared__ uint64_t pow2[128];
     __shared__ uint64_t mass[NBINS];
     const int64_t r = A.row0 + blockIdx.x / A.splits;
     const int part = blockIdx.x % A.splits, tid = threadIdx.x, lane = tid & 63;
     const SampleRow s = sample_row(A, r);
     if (!s.nucleus(A.n)) return;
+    const T *x = (const T *)A.x + r * A.ld;
+    const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
+    const int per = (blocks + A.splits - 1) / A.splits * BP, end = min((part + 1) * per, blocks * BP);   // pieces
+    int c = part * per + __builtin_amdgcn_readfirstlane(tid >> 6);
+    Raw8<T> raw;   // of the next piece: in flight during all that follows
+    if (c < end) raw.load(x, mask, c * PIECE + lane * 8, A.n);
     if (tid < 128) pow2[tid] = POW2[tid];
-    for (int b = tid; b < NBINS; b += 256) mass[b] = 0;
+    mass[tid] = 0;
     __syncthreads();
     const Nucleus N = nucleus(A, s, (LdsTable)pow2, r, blocks);
     if (!N.ok) return;
     const Weight W = weight(A, s, (LdsTable)pow2, N.top);
-    const T *x = (const T *)A.x + r * A.ld;
-    const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
-    const int per = (blocks + A.splits - 1) / A.splits, end = min((part + 1) * per, blocks);
-    for (int b = part * per + __builtin_amdgcn_readfirstlane(tid >> 6); b < end; b += 4) {
-        float v[BP][8];
-        load_block(x, mask, b * BLOCK + lane * 8, A.n, v);
+    for (; c < end; c += NW) {
+        float v[8];
+        raw.values(x, mask, c * PIECE + lane * 8, A.n, v);
+        if (c + NW < end) raw.load(x, mask, (c + NW) * PIECE + lane * 8, A.n);
 #pragma unroll
-        for (int p = 0; p < BP; ++p)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int k = N.bin(v[p][e]);
-                if (k < NBINS)
-                    atomicAdd((unsigned long long *)&mass[k], (unsigned long long)W.fixed(W.soft(v[p][e])));
-            }
+        for (int e = 0; e < 8; ++e) {
+            const int k = N.bin(v[e]);
+            if (k < NBINS) atomicAdd((unsigned long long *)&mass[k], (unsigned long long)W.fixed(W.soft(v[e])));
+        }
     }
     __syncthreads();
-    uint64_t *out = A.bins + (int64_t)blockIdx.x * NBINS;
-    for (int b = tid; b < NBINS; b += 256) out[b] = mass[b];
+    A.bins[(int64_t)blockIdx.x * NBINS + tid] = mass[tid];
 }
 
 // the same split once more: the cut's bin, the masses of its blocks above that bin (and not under
 // min-p), and the bin's entries
 template <class T>
-__global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs A, int blocks) {
-    __shared__ double pow2[128];
-    __shared__ uint64_t scan[5];
+__global__ __launch_bounds__(1024) void sample_kept_kernel(SampleArgs A, int blocks) {
+    __shared__ uint64_t pow2[128];
+    __shared__ uint64_t scan[NW];
     __shared__ int cut_bin;
     __shared__ uint64_t cut_above;
     __shared__ uint32_t listed;
     const int64_t local = blockIdx.x / A.splits, r = A.row0 + local;
     const int part = blockIdx.x % A.splits, tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const SampleRow s = sample_row(A, r);
     if (!s.nucleus(A.n)) return;
+    const T *x = (const T *)A.x + r * A.ld;
+    const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
+    const int per = (blocks + A.splits - 1) / A.splits * BP, end = min((part + 1) * per, blocks * BP);
+    Raw8<T> raw;
+    if (part * per + wave < end) raw.load(x, mask, (part * per + wave) * PIECE + lane * 8, A.n);
+    uint64_t m = 0, all;   // the bin of this thread, from the top
+    for (int k = 0; k < A.splits; ++k) m += A.bins[(local * A.splits + k) * NBINS + tid];
     if (tid < 128) pow2[tid] = POW2[tid];
     if (tid == 0) {
         cut_bin = -1;
@@ -483,22 +501,11 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs A, int bloc
     __syncthreads();
     const Nucleus N = nucleus(A, s, (LdsTable)pow2, r, blocks);
     if (N.ok) {
-        // four bins a thread, from the top
-        uint64_t m[4] = {0, 0, 0, 0}, all;
-        for (int k = 0; k < A.splits; ++k) {
-            const uint64_t *in = A.bins + (local * A.splits + k) * NBINS + tid * 4;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) m[j] += in[j];
-        }
         const double limit = (double)s.p * N.sum;
-        uint64_t above = block_scan<4, uint64_t>(m[0] + m[1] + m[2] + m[3], scan, all);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if ((above == 0 || (double)above < limit) && (double)(above + m[j]) >= limit && m[j]) {   // one bin
-                cut_bin = tid * 4 + j;
-                cut_above = above;
-            }
-            above += m[j];
+        const uint64_t above = block_scan<NW, uint64_t>(m, scan, all);
+        if ((above == 0 || (double)above < limit) && (double)(above + m) >= limit && m) {   // one bin
+            cut_bin = tid;
+            cut_above = above;
         }
     }
     __syncthreads();
@@ -507,29 +514,36 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs A, int bloc
     if (cut < 0) return;
     const Weight W = weight(A, s, (LdsTable)pow2, N.top);
     const double q = (double)s.q;
-    const T *x = (const T *)A.x + r * A.ld;
-    const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
-    const int per = (blocks + A.splits - 1) / A.splits, end = min((part + 1) * per, blocks);
     uint2 *list = A.lists + (int64_t)blockIdx.x * NLIST;
-    for (int b = part * per + __builtin_amdgcn_readfirstlane(tid >> 6); b < end; b += 4) {
-        float v[BP][8];
-        load_block(x, mask, b * BLOCK + lane * 8, A.n, v);
+    for (int c0 = part * per; c0 < end; c0 += NW) {
+        const int c = c0 + wave, i = c * PIECE + lane * 8;
         uint64_t sum = 0;
-#pragma unroll
-        for (int p = 0; p < BP; ++p)
+        if (c < end) {
+            float v[8];
+            raw.values(x, mask, i, A.n, v);
+            if (c + NW < end) raw.load(x, mask, i + NW * PIECE, A.n);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int k = N.bin(v[p][e]);
+                const int k = N.bin(v[e]);
                 if (k < cut) {
-                    const double w = W.soft(v[p][e]);
+                    const double w = W.soft(v[e]);
                     sum += w >= q ? W.fixed(w) : 0;
                 } else if (k == cut) {
                     const uint32_t at = atomicAdd(&listed, 1u);
-                    if (at < NLIST) list[at] = make_uint2(key_of(v[p][e]), (uint32_t)(b * BLOCK + p * PIECE + lane * 8 + e));
+                    if (at < NLIST) list[at] = make_uint2(key_of(v[e]), (uint32_t)(i + e));
                 }
             }
+        }
         sum = wave_sum(sum);
-        if (lane == 0) A.kept[local * blocks + b] = sum;
+        __syncthreads();
+        if (lane == 0) scan[wave] = sum;
+        __syncthreads();
+        if (tid < NW / BP && c0 + tid * BP < end) {
+            uint64_t block = 0;
+#pragma unroll
+            for (int p = 0; p < BP; ++p) block += scan[tid * BP + p];
+            A.kept[local * blocks + c0 / BP + tid] = block;
+        }
     }
     __syncthreads();
     if (tid == 0) A.listed[blockIdx.x] = listed;
@@ -538,7 +552,7 @@ __global__ __launch_bounds__(256) void sample_kept_kernel(SampleArgs A, int bloc
 // ---------------------------------------------------------------- a thread a row: n <= N
 template <class T, int N>
 __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
-    __shared__ double pow2[128];
+    __shared__ uint64_t pow2[128];
     if (threadIdx.x < 128) pow2[threadIdx.x] = POW2[threadIdx.x];
     __syncthreads();
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -550,7 +564,7 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        v[i] = i < A.n && !(mask && mask[i]) ? (float)x[i] + 0.0f : -INFINITY;
+        v[i] = i < A.n && !(mask && mask[i]) ? (float)x[i] : -INFINITY;
         nan |= v[i] != v[i];
         top = fmaxf(top, v[i]);
     }
@@ -612,7 +626,7 @@ template <class T, int RW, bool FUSED>
 __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
     constexpr int NT = 64 * RW, BT = BINS / NT;   // threads; bins of each
     constexpr int REC = FUSED ? 1 : BP;           // pieces of a record of mass
-    __shared__ double pow2[128];
+    __shared__ uint64_t pow2[128];
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
     __shared__ uint32_t list_key[LIST], list_at[LIST];
@@ -650,7 +664,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         if (wave < pieces) {
             float v[1][8];
             load8(x, mask, wave * PIECE + lane * 8, n, v[0]);
-            wave_records<1>(v, s.whole(n), s.inv_t * LOG2E_128, (LdsTable)pow2, own_tops + wave * GP, nullptr, own_masses + wave);
+            wave_records<1>(v, s.whole(n), scale_of(s), (LdsTable)pow2, own_tops + wave * GP, nullptr, own_masses + wave);
         }
         __syncthreads();
         tops = own_tops;
@@ -1336,7 +1350,7 @@ struct SampleSpace {
     SampleSpace(int64_t rows, int64_t n) {
         if (n <= 8 || fused(rows, n) || rows == 0) return;
         blocks = ceil_div(n, BLOCK);
-        splits = (int)std::max<int64_t>(1, std::min<int64_t>({SPLITS, 2048 / rows, (blocks + 3) / 4}));
+        splits = (int)std::max<int64_t>(1, std::min<int64_t>({SPLITS, 1024 / rows, (blocks + 3) / 4}));
         chunk = std::min<int64_t>(rows, 2048 / splits);
         auto take = [&](int64_t size) {
             const int64_t at = bytes;
@@ -1430,9 +1444,9 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
         A.row0 = r;
         const unsigned rows = (unsigned)std::min(chunk, A.rows - r);
         if (nucleus) {
-            sample_bins_kernel<T><<<rows * S.splits, 256, 0, s>>>(A, S.blocks);
+            sample_bins_kernel<T><<<rows * S.splits, NTH, 0, s>>>(A, S.blocks);
             launch_check("sample_bins_kernel");
-            sample_kept_kernel<T><<<rows * S.splits, 256, 0, s>>>(A, S.blocks);
+            sample_kept_kernel<T><<<rows * S.splits, NTH, 0, s>>>(A, S.blocks);
             launch_check("sample_kept_kernel");
         }
         if (many)
