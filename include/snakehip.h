@@ -255,8 +255,8 @@ typedef struct {
 } snk_sample_cfg_t;
 /* row r's logits start at logits_dev + r * ld elements, its mask (bytes, non-zero = forbidden; NULL:
  * none) at mask_dev + r * ld_mask; ld, ld_mask >= n, or 0: one row for all. 1 <= n <= 2^24.
- * idx_dev[rows]; prob_dev[rows] or NULL. ws_dev: snk_sample_workspace's bytes, 16-byte aligned, used
- * during the call only: two calls in flight need two. */
+ * idx_dev[rows]; prob_dev[rows] or NULL. ws_dev: snk_sample_workspace's bytes (0 for n <= 2048),
+ * 16-byte aligned, used during the call only: two calls in flight need two. */
 int snk_sample_workspace(int64_t rows, int64_t n, int64_t *bytes_out);
 int snk_sample_logits(const void *logits_dev, int64_t rows, int64_t n, int64_t ld, const uint8_t *mask_dev,
                       int64_t ld_mask, const float *u_dev, const snk_sample_cfg_t *cfg, int32_t *idx_dev,
@@ -296,7 +296,7 @@ typedef struct {
     int32_t state_bits;    /* 32 or 8 */
     float max_grad_norm;   /* 0: no norm; > 0 (may be inf): norm, clipping, and a step whose norm is
                               not finite writes nothing and is not counted */
-    double beta1, beta2, eps;   /* in [0, 1), [0, 1), [1e-30, 1e30] */
+    double beta1, beta2, eps;   /* in [0, 1), [0, 1), [1e-30, 1e30] (8-bit states: from 1e-12) */
     uint64_t seed;         /* of the 8-bit rounding */
     int64_t reserved;      /* 0 */
 } snk_adamw_cfg_t;

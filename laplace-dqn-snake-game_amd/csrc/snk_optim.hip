@@ -11,6 +11,7 @@
 #include <cstddef>
 #include <cstring>
 #include <memory>
+#include <type_traits>
 #include <vector>
 
 #include "snk_optim.hpp"
@@ -20,6 +21,10 @@ namespace snk {
 constexpr int BLK = 256;        // elements of a wave's block = the 8-bit states' block
 constexpr int CH = 1024;        // elements of a workgroup's chunk
 constexpr int NORM_WG = 2048;   // most workgroups (= partial sums) of the norm pass
+// From this many bytes of parameters, gradients and moments on, a step reads and writes past the
+// caches: nothing of them lives there until the next step, and what is written evicts nothing that is
+// still to be read. 32-bit states: 159 us against 180 at 537 MB, 78 against 68 at 268 MB.
+constexpr int64_t NT_FROM = 320ll << 20;
 constexpr int FEW_PARTS = 256;  // partial sums that every workgroup of the step adds up itself
 
 struct AdamTensor {
@@ -41,6 +46,8 @@ struct alignas(16) AdamCtl {
     int32_t skip;         // the last step's N was not finite
     float norm;           // the last step's N
     float ibc1, ibc2;     // 1 / (1 - b^t)
+    float gmul;           // the factor of the gradients, where adamw_parts_kernel found it
+    int32_t pad[3];
 };
 struct AdamHyper {
     double b1d, b2d;
@@ -49,56 +56,74 @@ struct AdamHyper {
     uint64_t seed;
 };
 
-// four consecutive elements at an element-aligned address: one 16- or 8-byte access (unaligned
-// global accesses are legal on gfx950), so views that start anywhere take the same path
+// An address that was itself loaded is generic to the compiler (flat accesses, waited for with LDS's):
+// these go to global memory. N consecutive elements at an element-aligned address are one 16- or
+// 8-byte access (unaligned global accesses are legal on gfx950), so views that start anywhere take
+// the same path.
+#define SNK_GLOBAL __attribute__((address_space(1)))
 template <class T, int N>
-struct __attribute__((packed, aligned(sizeof(T)))) pack {
-    T v[N];
+struct Pack {
+    typedef typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type Bits;
+    typedef Bits Vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    Vec q;
+    // NT: not kept in the caches (read or written once a step, and more of it than they hold)
+    template <bool NT = false>
+    __device__ __forceinline__ void load(const T *p) {
+        q = NT ? __builtin_nontemporal_load((const SNK_GLOBAL Vec *)p) : *(const SNK_GLOBAL Vec *)p;
+    }
+    template <bool NT = false>
+    __device__ __forceinline__ void store(T *p) const {
+        if (NT)
+            __builtin_nontemporal_store(q, (SNK_GLOBAL Vec *)p);
+        else
+            *(SNK_GLOBAL Vec *)p = q;
+    }
+    __device__ __forceinline__ float get(int k) const { return (float)__builtin_bit_cast(T, (Bits)q[k]); }
+    __device__ __forceinline__ void set(int k, float x) { q[k] = __builtin_bit_cast(Bits, (T)x); }   // to nearest even
 };
-template <class T, class I>
+template <bool NT, class T, class I>
 __device__ __forceinline__ void load4(const T *p, I i, I n, float *x) {
     if (i + 4 <= n) {
-        const pack<T, 4> q = *reinterpret_cast<const pack<T, 4> *>(p + i);
+        Pack<T, 4> q;
+        q.template load<NT>(p + i);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = (float)q.v[k];
+        for (int k = 0; k < 4; ++k) x[k] = q.get(k);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = i + k < n ? (float)p[i + k] : 0.0f;
+        for (int k = 0; k < 4; ++k) x[k] = i + k < n ? (float)((const SNK_GLOBAL T *)p)[i + k] : 0.0f;
     }
 }
-template <class T, class I>
+template <bool NT, class T, class I>
 __device__ __forceinline__ void store4(T *p, I i, I n, const float *x) {
     if (i + 4 <= n) {
-        pack<T, 4> q;
+        Pack<T, 4> q;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) q.v[k] = (T)x[k];   // round to nearest even
-        *reinterpret_cast<pack<T, 4> *>(p + i) = q;
+        for (int k = 0; k < 4; ++k) q.set(k, x[k]);
+        q.template store<NT>(p + i);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (i + k < n) p[i + k] = (T)x[k];
+            if (i + k < n) ((SNK_GLOBAL T *)p)[i + k] = (T)x[k];
     }
 }
 
 // largest of 64 non-negative floats (0 where a lane has no partner)
 __device__ __forceinline__ float wave_max_nonneg(float x) {
-    auto step = [&](auto ctrl, auto mask) {
-        const float y = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value,
-                                                                   decltype(mask)::value, 0xf, false));
-        x = fmaxf(x, y);
+    auto step = [&](auto ctrl) {
+        x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true)));
     };
-    step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});   // row_shr 1, 2, 4, 8
-    step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
-    step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
-    step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
-    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});   // row_bcast 15, 31
-    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+    step(std::integral_constant<int, 0x111>{});   // row_shr 1, 2, 4, 8
+    step(std::integral_constant<int, 0x112>{});
+    step(std::integral_constant<int, 0x114>{});
+    step(std::integral_constant<int, 0x118>{});
+    step(std::integral_constant<int, 0x142>{});   // row_bcast 15, 31
+    step(std::integral_constant<int, 0x143>{});
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
 // the values the 8-bit codes stand for
-__device__ __forceinline__ float m_value(int a, float scale) {
-    return (float)(a * abs(a)) * (1.0f / 16129.0f) * scale;
+__device__ __forceinline__ float m_value(float a, float scale) {   // a |a| / 127^2 (a |a| is exact)
+    return a * fabsf(a) * (1.0f / 16129.0f) * scale;
 }
 __device__ __forceinline__ float v_level(float b) {   // (b / 255)^4
     const float r = b * (1.0f / 255.0f), r2 = r * r;
@@ -178,15 +203,15 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(const AdamChunk *__rest
         const GT *g_next = (const GT *)chunks[next].g;
         const int n_next = chunks[next].n;
         if (n == CH) {
-            pack<GT, V> q[N];
+            Pack<GT, V> q[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) q[j] = *reinterpret_cast<const pack<GT, V> *>(g + (j * 64 + lane) * V);
+            for (int j = 0; j < N; ++j) q[j].load(g + (j * 64 + lane) * V);
 #pragma unroll
             for (int j = 0; j < N; ++j)
 #pragma unroll
-                for (int e = 0; e < V; ++e) add((float)q[j].v[e]);
+                for (int e = 0; e < V; ++e) add(q[j].get(e));
         } else {
-            for (int k = lane; k < n; k += 64) add((float)g[k]);
+            for (int k = lane; k < n; k += 64) add((float)((const SNK_GLOBAL GT *)g)[k]);
         }
         g = g_next;
         n = n_next;
@@ -197,13 +222,22 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(const AdamChunk *__rest
         if (blockIdx.x == 0) begin_step(ctl, H);
     }
 }
-// many partial sums to one
-__global__ __launch_bounds__(256) void adamw_parts_kernel(double *__restrict__ part, int n) {
+// N and the factor of the gradients, s c; false where the step is to be skipped
+__device__ __forceinline__ bool clip_factor(const AdamHyper &H, double sum, float &norm, float &gmul) {
+    const double N = sqrt(sum);
+    norm = (float)N;
+    gmul = H.gscale;
+    if (N > (double)H.max_norm) gmul = (float)((double)H.gscale * ((double)H.max_norm / N));
+    return N < INFINITY;   // false for NaN too
+}
+// ... once for the whole step, where the partial sums are many
+__global__ __launch_bounds__(256) void adamw_parts_kernel(const double *__restrict__ part, int n, AdamCtl *__restrict__ ctl,
+                                                          AdamHyper H) {
     __shared__ double sh[4];
     double sum = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) sum += part[i];
     sum = sum256(sum, sh);
-    if (threadIdx.x == 0) part[0] = sum;   // after every read: sum256's barrier
+    if (threadIdx.x == 0) ctl->skip = clip_factor(H, sum, ctl->norm, ctl->gmul) ? 0 : 1;
 }
 
 struct AdamArgs {
@@ -211,7 +245,7 @@ struct AdamArgs {
     void *m, *v;
     float *ms, *vs;
     AdamCtl *ctl;
-    const double *part;   // n_part partial sums of the norm (0: none)
+    const double *part;   // n_part partial sums of the norm (0: no norm, -1: ctl has its results)
     int n_part;
     bool counted;         // the host counts the steps: `step` holds, and ctl is to receive it
     AdamStep step;
@@ -232,43 +266,46 @@ __device__ __forceinline__ AdamStep this_step(const AdamArgs &A) {
 __device__ __forceinline__ bool grad_factor(const AdamArgs &A, double *sh, float &gmul) {
     gmul = A.H.gscale;
     if (A.n_part == 0) return true;
-    double sum = (int)threadIdx.x < A.n_part ? A.part[threadIdx.x] : 0.0;
-    sum = A.n_part == 1 ? A.part[0] : sum256(sum, sh);
-    const double N = sqrt(sum);
-    const bool fine = N < INFINITY;   // false for NaN too
-    if (N > (double)A.H.max_norm) gmul = (float)((double)A.H.gscale * ((double)A.H.max_norm / N));
+    if (A.n_part < 0) {
+        gmul = A.ctl->gmul;
+        return A.ctl->skip == 0;
+    }
+    const double sum = sum256((int)threadIdx.x < A.n_part ? A.part[threadIdx.x] : 0.0, sh);
+    float norm;
+    const bool fine = clip_factor(A.H, sum, norm, gmul);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
-        A.ctl->norm = (float)N;
+        A.ctl->norm = norm;
         A.ctl->skip = fine ? 0 : 1;
     }
     return fine;
 }
 
-// one element: new moments in m, v; the new parameter is returned. EXACT: the step's quotient
-// correctly rounded (HBM hides it with 32-bit moments), or within 2 ulp by the hardware's reciprocal
+// one element: new moments in m, v; the new parameter is returned. EXACT: the step's root and quotient
+// correctly rounded (HBM hides them with 32-bit moments), or within an ulp each by the hardware's own,
+// which take a subnormal v for 0: nothing beside an eps of 1e-12 and more
 template <bool EXACT>
 __device__ __forceinline__ float adamw_one(const AdamHyper &H, float gmul, float ibc1, float ibc2, float wd, float p,
                                            float g, float &m, float &v) {
     g *= gmul;
     m = H.b1 * m + H.omb1 * g;
     v = H.b2 * v + H.omb2 * (g * g);
-    const float den = __builtin_sqrtf(v * ibc2) + H.eps;
+    const float den = (EXACT ? __builtin_sqrtf(v * ibc2) : __builtin_amdgcn_sqrtf(v * ibc2)) + H.eps;
     const float step = EXACT ? (m * ibc1) / den : (m * ibc1) * __builtin_amdgcn_rcpf(den);
     return p - H.lr * (step + wd * p);
 }
 
-template <class PT>
+template <class PT, bool NT>
 __device__ __forceinline__ void store_params(const AdamChunk &T, int copy_dtype, int i, const float *p) {
-    store4((PT *)T.p, i, T.n, p);
+    store4<NT>((PT *)T.p, i, T.n, p);
     if (T.c) {
         if (copy_dtype == SNK_BF16)
-            store4((__bf16 *)T.c, i, T.n, p);
+            store4<NT>((__bf16 *)T.c, i, T.n, p);
         else
-            store4((_Float16 *)T.c, i, T.n, p);
+            store4<NT>((_Float16 *)T.c, i, T.n, p);
     }
 }
 
-template <class PT, class GT>
+template <class PT, class GT, bool NT>
 __global__ __launch_bounds__(256) void adamw32_kernel(AdamArgs A) {
     __shared__ double sh[4];
     const AdamChunk T = A.chunks[blockIdx.x];
@@ -277,25 +314,22 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamArgs A) {
     float *ms = (float *)A.m + T.place, *vs = (float *)A.v + T.place;
     const int i = threadIdx.x * 4;
     const bool live = i < T.n;
-    float p[4], g[4], gmul;
-    float4 m, v;
+    float p[4], g[4], m[4], v[4], gmul;
     if (live) {
-        load4((const PT *)T.p, i, T.n, p);
-        load4((const GT *)T.g, i, T.n, g);
-        m = *(float4 *)(ms + i);   // padded: always whole
-        v = *(float4 *)(vs + i);
+        load4<NT>((const PT *)T.p, i, T.n, p);
+        load4<NT>((const GT *)T.g, i, T.n, g);
+        load4<NT>(ms, i, BLK * 4, m);   // padded: always whole
+        load4<NT>(vs, i, BLK * 4, v);
     }
     if (!grad_factor(A, sh, gmul) || !live) return;
-    p[0] = adamw_one<true>(A.H, gmul, ibc1, ibc2, T.wd, p[0], g[0], m.x, v.x);
-    p[1] = adamw_one<true>(A.H, gmul, ibc1, ibc2, T.wd, p[1], g[1], m.y, v.y);
-    p[2] = adamw_one<true>(A.H, gmul, ibc1, ibc2, T.wd, p[2], g[2], m.z, v.z);
-    p[3] = adamw_one<true>(A.H, gmul, ibc1, ibc2, T.wd, p[3], g[3], m.w, v.w);
-    *(float4 *)(ms + i) = m;
-    *(float4 *)(vs + i) = v;
-    store_params<PT>(T, A.H.copy_dtype, i, p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) p[e] = adamw_one<true>(A.H, gmul, ibc1, ibc2, T.wd, p[e], g[e], m[e], v[e]);
+    store4<NT>(ms, i, BLK * 4, m);
+    store4<NT>(vs, i, BLK * 4, v);
+    store_params<PT, NT>(T, A.H.copy_dtype, i, p);
 }
 
-template <class PT, class GT>
+template <class PT, class GT, bool NT>
 __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     __shared__ double sh[4];
     const AdamChunk T = A.chunks[blockIdx.x];
@@ -310,10 +344,10 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     float p[4], g[4], gmul, ms0 = 0.0f, vs0 = 0.0f;
     uint32_t mc = 0, vc = 0;
     if (live) {
-        load4((const PT *)T.p, i, T.n, p);
-        load4((const GT *)T.g, i, T.n, g);
-        mc = *(const uint32_t *)(mcs + i);
-        vc = *(const uint32_t *)(vcs + i);
+        load4<NT>((const PT *)T.p, i, T.n, p);
+        load4<NT>((const GT *)T.g, i, T.n, g);
+        mc = NT ? __builtin_nontemporal_load((const uint32_t *)(mcs + i)) : *(const uint32_t *)(mcs + i);
+        vc = NT ? __builtin_nontemporal_load((const uint32_t *)(vcs + i)) : *(const uint32_t *)(vcs + i);
         ms0 = mss[wave];
         vs0 = vss[wave];
     }
@@ -321,13 +355,13 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     float m[4], v[4], mmax = 0.0f, vmax = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {   // places behind the tensor's end hold zeros and read g = 0
-        m[e] = m_value((int)(int8_t)(mc >> (8 * e)), ms0);
+        m[e] = m_value((float)(int8_t)(mc >> (8 * e)), ms0);
         v[e] = v_level((float)((vc >> (8 * e)) & 255u)) * vs0;
         p[e] = adamw_one<false>(A.H, gmul, ibc1, ibc2, T.wd, p[e], g[e], m[e], v[e]);
         mmax = fmaxf(mmax, fabsf(m[e]));
         vmax = fmaxf(vmax, v[e]);
     }
-    store_params<PT>(T, A.H.copy_dtype, i, p);
+    store_params<PT, NT>(T, A.H.copy_dtype, i, p);
     mmax = wave_max_nonneg(mmax);
     vmax = wave_max_nonneg(vmax);
     // the codes as correctly rounded quotients and roots give them (the same arithmetic anywhere gives
@@ -336,22 +370,47 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     const float km = mmax < 0x1p-100f ? 0x1p100f : 1.0f, kv = vmax < 0x1p-100f ? 0x1p100f : 1.0f;
     const float dm = mmax > 0.0f ? mmax * km : 1.0f, dv = vmax > 0.0f ? vmax * kv : 1.0f;
     const float im = 1.0f / dm, iv = 1.0f / dv;
+    float least[4];   // the code of v's least value above 0: a v that came back as 0 would leave m / eps
+#pragma unroll
+    for (int e = 0; e < 4; ++e) least[e] = v[e] > 0.0f ? 1.0f : 0.0f;
+    if (km != 1.0f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m[e] *= km;
+    if (kv != 1.0f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= kv;
     uint32_t mo = 0, vo = 0;
+    float a[4], far = 0.0f, all = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int a = (int)rintf(127.0f * root(quotient(fabsf(m[e]) * km, dm, im)));
-        mo |= (uint32_t)((m[e] < 0.0f ? -a : a) & 255) << (8 * e);
+        const float x = 127.0f * __builtin_amdgcn_sqrtf(fabsf(m[e]) * im);   // within 127 2^-22 of the true one
+        a[e] = rintf(x);
+        far = fmaxf(far, fabsf(x - a[e]));
+        all += x - a[e];   // NaN where an x is
+    }
+    // 1 wave in 20: what is next to a half (and a NaN, whose code is 0), again in full
+    if (__builtin_amdgcn_ballot_w64(!(fmaf(0.0f, all, far) < 0.4999f)))
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = rintf(127.0f * root(quotient(fabsf(m[e]), dm, im)));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        mo = __builtin_amdgcn_cvt_pk_u8_f32(copysignf(a[e], m[e]) + 128.0f, e, mo);
         // next to a level either floor leads to that level, so the hardware's roots (1 ulp) do here
-        const float part = quotient(v[e] * kv, dv, iv);
+        const float part = quotient(v[e], dv, iv);
         const float low = fminf(floorf(255.0f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(part))), 254.0f);
         const float lo = v_level(low), hi = v_level(low + 1.0f);
         const float r = (float)((uint32_t)(h >> (16 * e)) & 0xFFFFu) * 0x1p-16f;
-        uint32_t b = (uint32_t)low + (r * (hi - lo) < part - lo ? 1u : 0u);
-        if (v[e] > 0.0f && b == 0) b = 1;   // never back as 0: m / eps would follow
-        vo |= (b & 255u) << (8 * e);
+        const float b = r * (hi - lo) < part - lo ? low + 1.0f : low;
+        vo = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(b, least[e]), e, vo);
     }
-    *(uint32_t *)(mcs + i) = mo;
-    *(uint32_t *)(vcs + i) = vo;
+    mo ^= 0x80808080u;   // a + 128 as a signed byte
+    if (NT) {
+        __builtin_nontemporal_store(mo, (uint32_t *)(mcs + i));
+        __builtin_nontemporal_store(vo, (uint32_t *)(vcs + i));
+    } else {
+        *(uint32_t *)(mcs + i) = mo;
+        *(uint32_t *)(vcs + i) = vo;
+    }
     if (lane == 0) {
         mss[wave] = mmax;
         vss[wave] = vmax;
@@ -370,15 +429,15 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(AdamArgs A, int64_t 
             const float ms = A.ms[i / BLK], vs = A.vs[i / BLK];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                m[e] = m_value((int)(int8_t)(mc >> (8 * e)), ms);
+                m[e] = m_value((float)(int8_t)(mc >> (8 * e)), ms);
                 v[e] = v_level((float)((vc >> (8 * e)) & 255u)) * vs;
             }
         } else {
-            load4((const float *)A.m, i, total, m);
-            load4((const float *)A.v, i, total, v);
+            load4<false>((const float *)A.m, i, total, m);
+            load4<false>((const float *)A.v, i, total, v);
         }
-        if (mo) store4(mo, i, total, m);
-        if (vo) store4(vo, i, total, v);
+        if (mo) store4<false>(mo, i, total, m);
+        if (vo) store4<false>(vo, i, total, v);
     }
 }
 
@@ -483,7 +542,8 @@ snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const s
               cfg->state_bits);
     SNK_CHECK(cfg->beta1 >= 0 && cfg->beta1 < 1 && cfg->beta2 >= 0 && cfg->beta2 < 1, SNK_ERR_INVALID,
               "AdamW: betas (%g, %g) outside [0, 1)", cfg->beta1, cfg->beta2);
-    SNK_CHECK(cfg->eps >= 1e-30 && cfg->eps <= 1e30, SNK_ERR_INVALID, "AdamW: eps %g outside [1e-30, 1e30]", cfg->eps);
+    const double least = cfg->state_bits == 8 ? 1e-12 : 1e-30;
+    SNK_CHECK(cfg->eps >= least && cfg->eps <= 1e30, SNK_ERR_INVALID, "AdamW: eps %g outside [%g, 1e30]", cfg->eps, least);
     SNK_CHECK(cfg->max_grad_norm >= 0, SNK_ERR_INVALID, "AdamW: max_grad_norm %g is negative", cfg->max_grad_norm);
     SNK_CHECK(cfg->reserved == 0, SNK_ERR_INVALID, "AdamW: reserved must be 0");
     auto h = std::make_unique<snk_adamw_s>();
@@ -613,9 +673,9 @@ void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s) {
         });
         launch_check("adamw_norm_kernel");
         if (parts > FEW_PARTS) {
-            adamw_parts_kernel<<<1, 256, 0, s>>>(h->part, parts);
+            adamw_parts_kernel<<<1, 256, 0, s>>>(h->part, parts, h->ctl, H);
             launch_check("adamw_parts_kernel");
-            parts = 1;
+            parts = -1;
         }
         A.n_part = parts;
     } else {
@@ -636,14 +696,20 @@ void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s) {
         }
     }
     if (h->n_chunks == 0) return;
+    const bool nt = h->total * (dtype_size(c.param_dtype) + dtype_size(c.grad_dtype) + c.state_bits / 4) >= NT_FROM;
     with_type(c.param_dtype, [&](auto p) {
         with_type(c.grad_dtype, [&](auto g) {
             using PT = decltype(p);
             using GT = decltype(g);
-            if (c.state_bits == 8)
-                adamw8_kernel<PT, GT><<<(unsigned)h->n_chunks, 256, 0, s>>>(A);
+            const unsigned grid = (unsigned)h->n_chunks;
+            if (c.state_bits == 8 && nt)
+                adamw8_kernel<PT, GT, true><<<grid, 256, 0, s>>>(A);
+            else if (c.state_bits == 8)
+                adamw8_kernel<PT, GT, false><<<grid, 256, 0, s>>>(A);
+            else if (nt)
+                adamw32_kernel<PT, GT, true><<<grid, 256, 0, s>>>(A);
             else
-                adamw32_kernel<PT, GT><<<(unsigned)h->n_chunks, 256, 0, s>>>(A);
+                adamw32_kernel<PT, GT, false><<<grid, 256, 0, s>>>(A);
         });
     });
     launch_check("adamw_kernel");

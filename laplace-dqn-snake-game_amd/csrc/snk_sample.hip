@@ -65,7 +65,7 @@ struct SampleArgs {
 
 // a row's settings, the same for all its threads
 struct SampleRow {
-    double inv_t;
+    double t, inv_t;
     bool greedy;
     int k;        // 1..n
     float p, q, u;
@@ -77,7 +77,8 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs &A, int64_t r) 
     SampleRow s;
     const float t = A.t_dev ? A.t_dev[r] : A.temperature;
     s.greedy = !(t > 0.0f);
-    s.inv_t = s.greedy ? 1.0 : fmax(1.0 / (double)t, 1e-300);   // t = inf: all alike, -inf still nothing
+    s.t = s.greedy ? 1.0 : fmin((double)t, 1e300);   // t = inf: all alike, -inf still nothing
+    s.inv_t = 1.0 / s.t;
     const int k = A.k_dev ? A.k_dev[r] : A.top_k;
     s.k = s.greedy ? 1 : k > 0 && k < A.n ? k : A.n;
     const float p = A.p_dev ? A.p_dev[r] : A.top_p, q = A.q_dev ? A.q_dev[r] : A.min_p;
@@ -170,8 +171,7 @@ struct Weight {
     }
 };
 __device__ __forceinline__ Scale scale_of(const SampleRow &s) {
-    const double scale = s.inv_t * 0x1.71547652b82fep+7;
-    return Scale{scale, -128000.0 / scale};
+    return Scale{s.inv_t * 0x1.71547652b82fep+7, s.t * -693.0};
 }
 __device__ __forceinline__ Weight weight(const SampleArgs &A, const SampleRow &s, LdsTable pow2, float top) {
     return Weight{pow2, (double)top, scale_of(s), A.unit, s.greedy || top == INFINITY};
@@ -429,8 +429,9 @@ __device__ __forceinline__ Nucleus nucleus(const SampleArgs &A, const SampleRow 
         if (bt[b] != -INFINITY) sum += A.masses[r * blocks + b] * W.soft(bt[b]);
     sum = wave_sum(sum);
     N.sum = sum * A.unit;
-    const double far = log((double)A.n / ((1.0 - (double)s.p) * sum)) * 1.0001 + 1e-6;   // >= 0: sum <= n
-    N.step = (float)(NBINS / far * s.inv_t);
+    // the hardware's log2 (1 ulp), a little further out; its argument is at least 1: sum <= n
+    const float far = __builtin_amdgcn_logf((float)A.n / ((float)(1.0 - (double)s.p) * (float)sum)) * 0.69315f + 1e-3f;
+    N.step = NBINS / far * (float)s.inv_t;
     N.ok = N.step < INFINITY && N.step > 0.0f;
     return N;
 }
@@ -492,7 +493,16 @@ __global__ __launch_bounds__(1024) void sample_kept_kernel(SampleArgs A, int blo
     Raw8<T> raw;
     if (part * per + wave < end) raw.load(x, mask, (part * per + wave) * PIECE + lane * 8, A.n);
     uint64_t m = 0, all;   // the bin of this thread, from the top
-    for (int k = 0; k < A.splits; ++k) m += A.bins[(local * A.splits + k) * NBINS + tid];
+    const uint64_t *bins = A.bins + local * A.splits * NBINS + tid;
+    if (A.splits == 1) {
+        m = bins[0];
+    } else {   // all loads in flight at once: 10,000 cycles one after another
+        uint64_t part_mass[SPLITS];
+#pragma unroll
+        for (int k = 0; k < SPLITS; ++k) part_mass[k] = bins[min(k, A.splits - 1) * NBINS];
+#pragma unroll
+        for (int k = 0; k < SPLITS; ++k) m += k < A.splits ? part_mass[k] : 0;
+    }
     if (tid < 128) pow2[tid] = POW2[tid];
     if (tid == 0) {
         cut_bin = -1;
@@ -774,7 +784,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             // top up to here, and, where min-p is not to change the mass that top-p goes by, this near
             int far = BINS - 1;
             const bool by_q = s.q > 0.0f && s.p >= 1.0f;
-            const float near = by_q ? (float)(-log((double)s.q) / s.inv_t) * 1.0001f + 1e-30f : INFINITY;
+            const float near = by_q ? (__builtin_amdgcn_logf(s.q) * -0.69315f + 1e-4f) * (float)s.t : INFINITY;
             auto candidate = [&](float v) __attribute__((always_inline)) {
                 const float d = top - v;   // NaN for two infinities: top itself
                 return v != -INFINITY && !(d > near) && far_bin(d > 0.0f ? d : 0.0f) <= far;

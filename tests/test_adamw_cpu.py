@@ -25,7 +25,7 @@ def _create(n=1, sizes=(8,), wd=(0.0,), cfg=None, **change):
     (dict(param_dtype=3), "type"), (dict(grad_dtype=-1), "type"), (dict(copy_dtype=0), "copy_dtype"),
     (dict(state_bits=16), "state_bits"), (dict(beta1=1.0), "betas"), (dict(beta2=-0.1), "betas"),
     (dict(beta1=float("nan")), "betas"), (dict(eps=0.0), "eps"), (dict(eps=1e-60), "eps"), (dict(eps=float("inf")), "eps"),
-    (dict(max_grad_norm=-1.0), "max_grad_norm"), (dict(max_grad_norm=float("nan")), "max_grad_norm"),
+    (dict(state_bits=8, eps=1e-13), "eps"), (dict(eps=2e30), "eps"), (dict(max_grad_norm=-1.0), "max_grad_norm"), (dict(max_grad_norm=float("nan")), "max_grad_norm"),
     (dict(reserved=1), "reserved"),
 ])
 def test_bad_settings_are_refused(change, word):
