@@ -81,21 +81,22 @@ struct Pack {
     __device__ __forceinline__ float get(int k) const { return (float)__builtin_bit_cast(T, (Bits)q[k]); }
     __device__ __forceinline__ void set(int k, float x) { q[k] = __builtin_bit_cast(Bits, (T)x); }   // to nearest even
 };
+// four elements from place i of n, zeros behind the end; WHOLE: none lies there. Not converted yet: what
+// is loaded next should not wait for this.
 template <bool NT, class T, class I>
-__device__ __forceinline__ void load4(const T *p, I i, I n, float *x) {
-    if (i + 4 <= n) {
-        Pack<T, 4> q;
+__device__ __forceinline__ Pack<T, 4> load4(const T *p, I i, I n, bool whole) {
+    Pack<T, 4> q;
+    if (whole) {
         q.template load<NT>(p + i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = q.get(k);
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = i + k < n ? (float)((const SNK_GLOBAL T *)p)[i + k] : 0.0f;
+        for (int k = 0; k < 4; ++k) q.q[k] = i + k < n ? ((const SNK_GLOBAL typename Pack<T, 4>::Bits *)p)[i + k] : 0;
     }
+    return q;
 }
 template <bool NT, class T, class I>
-__device__ __forceinline__ void store4(T *p, I i, I n, const float *x) {
-    if (i + 4 <= n) {
+__device__ __forceinline__ void store4(T *p, I i, I n, bool whole, const float *x) {
+    if (whole) {
         Pack<T, 4> q;
 #pragma unroll
         for (int k = 0; k < 4; ++k) q.set(k, x[k]);
@@ -107,10 +108,12 @@ __device__ __forceinline__ void store4(T *p, I i, I n, const float *x) {
     }
 }
 
-// largest of 64 non-negative floats (0 where a lane has no partner)
-__device__ __forceinline__ float wave_max_nonneg(float x) {
-    auto step = [&](auto ctrl) {
-        x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true)));
+// largest of 64 non-negative floats, which order as their bits do
+__device__ __forceinline__ float wave_max_nonneg(float f) {
+    uint32_t x = __float_as_uint(f);
+    auto step = [&](auto ctrl) {   // 0 where a lane has no partner
+        const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true);
+        x = x > y ? x : y;
     };
     step(std::integral_constant<int, 0x111>{});   // row_shr 1, 2, 4, 8
     step(std::integral_constant<int, 0x112>{});
@@ -118,7 +121,7 @@ __device__ __forceinline__ float wave_max_nonneg(float x) {
     step(std::integral_constant<int, 0x118>{});
     step(std::integral_constant<int, 0x142>{});   // row_bcast 15, 31
     step(std::integral_constant<int, 0x143>{});
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+    return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)x, 63));
 }
 
 // the values the 8-bit codes stand for
@@ -135,12 +138,21 @@ __device__ __forceinline__ float quotient(float x, float d, float inv_d) {
     const float q = x * inv_d;
     return fmaf(fmaf(-q, d, x), inv_d, q);
 }
-// sqrt(x), rounded correctly but for one x in millions: the hardware's root (1 ulp) and a Newton step
-// on its exact residual. Below 2^-100 the answer is that of 2^-100: no code of either moment sees it.
-__device__ __forceinline__ float root(float x) {
-    x = fmaxf(x, 0x1p-100f);
-    const float s = __builtin_amdgcn_sqrtf(x);
-    return fmaf(fmaf(-s, s, x), 0.5f * __builtin_amdgcn_rcpf(s), s);
+// 1 / d, rounded correctly (but for a d whose significand is all ones): the hardware's (1 ulp) and a
+// Newton step. d in the middle of fp32's range.
+__device__ __forceinline__ float reciprocal(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, r, 1.0f), r, r);
+}
+// a wave's largest value d >= 0 and the values brought there where they are not: far from an overflow of
+// 1 / d and an underflow of what counts beside d
+__device__ __forceinline__ void to_middle(float &d, float *x) {
+    if (d >= 0x1p-100f && d <= 0x1p100f) return;
+    asm volatile("");   // a branch that is hardly ever taken, not eight selects
+    const float k = d < 1.0f ? 0x1p100f : 0x1p-100f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] *= k;
+    d = d > 0.0f ? d * k : 1.0f;
 }
 
 // what a step knows before it starts: its number and 1 / (1 - b^t)
@@ -295,90 +307,101 @@ __device__ __forceinline__ float adamw_one(const AdamHyper &H, float gmul, float
 }
 
 template <class PT, bool NT>
-__device__ __forceinline__ void store_params(const AdamChunk &T, int copy_dtype, int i, const float *p) {
-    store4<NT>((PT *)T.p, i, T.n, p);
+__device__ __forceinline__ void store_params(const AdamChunk &T, int copy_dtype, int i, bool whole, const float *p) {
+    store4<NT>((PT *)T.p, i, T.n, whole, p);
     if (T.c) {
         if (copy_dtype == SNK_BF16)
-            store4<NT>((__bf16 *)T.c, i, T.n, p);
+            store4<NT>((__bf16 *)T.c, i, T.n, whole, p);
         else
-            store4<NT>((_Float16 *)T.c, i, T.n, p);
+            store4<NT>((_Float16 *)T.c, i, T.n, whole, p);
     }
 }
 
+// Waves behind the chunk's end read its last 256 places too, so that no load waits for a test, and
+// leave before the first store.
 template <class PT, class GT, bool NT>
 __global__ __launch_bounds__(256) void adamw32_kernel(AdamArgs A) {
     __shared__ double sh[4];
     const AdamChunk T = A.chunks[blockIdx.x];
     const AdamStep now = this_step(A);
     const float ibc1 = now.ibc1, ibc2 = now.ibc2;
+    const int lane = threadIdx.x & 63, mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int last = (T.n - 1) / BLK, wave = mine < last ? mine : last;
+    const int i = wave * BLK + lane * 4;
+    const bool whole = (wave + 1) * BLK <= T.n;
     float *ms = (float *)A.m + T.place, *vs = (float *)A.v + T.place;
-    const int i = threadIdx.x * 4;
-    const bool live = i < T.n;
-    float p[4], g[4], m[4], v[4], gmul;
-    if (live) {
-        load4<NT>((const PT *)T.p, i, T.n, p);
-        load4<NT>((const GT *)T.g, i, T.n, g);
-        load4<NT>(ms, i, BLK * 4, m);   // padded: always whole
-        load4<NT>(vs, i, BLK * 4, v);
-    }
-    if (!grad_factor(A, sh, gmul) || !live) return;
+    Pack<float, 4> mq, vq;
+    mq.template load<NT>(ms + i);   // padded: always whole
+    vq.template load<NT>(vs + i);
+    const Pack<PT, 4> pq = load4<NT>((const PT *)T.p, i, T.n, whole);
+    const Pack<GT, 4> gq = load4<NT>((const GT *)T.g, i, T.n, whole);
+    float gmul;
+    if (!grad_factor(A, sh, gmul) || mine > last) return;
+    float p[4], m[4], v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) p[e] = adamw_one<true>(A.H, gmul, ibc1, ibc2, T.wd, p[e], g[e], m[e], v[e]);
-    store4<NT>(ms, i, BLK * 4, m);
-    store4<NT>(vs, i, BLK * 4, v);
-    store_params<PT, NT>(T, A.H.copy_dtype, i, p);
+    for (int e = 0; e < 4; ++e) {
+        m[e] = mq.get(e);
+        v[e] = vq.get(e);
+        p[e] = adamw_one<true>(A.H, gmul, ibc1, ibc2, T.wd, pq.get(e), gq.get(e), m[e], v[e]);
+        mq.set(e, m[e]);
+        vq.set(e, v[e]);
+    }
+    mq.template store<NT>(ms + i);
+    vq.template store<NT>(vs + i);
+    store_params<PT, NT>(T, A.H.copy_dtype, i, whole, p);
 }
 
 template <class PT, class GT, bool NT>
 __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     __shared__ double sh[4];
+    __shared__ float level[256];   // v's: 12 multiplications an element that one read and one pair of reads do
     const AdamChunk T = A.chunks[blockIdx.x];
     const AdamStep now = this_step(A);
     const float ibc1 = now.ibc1, ibc2 = now.ibc2;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = threadIdx.x * 4;
+    const int lane = threadIdx.x & 63, mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int last = (T.n - 1) / BLK, wave = mine < last ? mine : last;
+    const int i = wave * BLK + lane * 4;
+    const bool whole = (wave + 1) * BLK <= T.n;
     const uint64_t key = splitmix64(A.H.seed ^ ((uint64_t)now.t * 0xD1B54A32D192ED03ULL));   // rng_hash's first half
-    const uint64_t h = splitmix64(key ^ (uint64_t)((T.place + i) >> 2));
-    uint8_t *mcs = (uint8_t *)A.m + T.place, *vcs = (uint8_t *)A.v + T.place;
-    float *mss = A.ms + T.place / BLK, *vss = A.vs + T.place / BLK;
-    const bool live = wave * BLK < T.n;   // whole waves: a block's places are all stored
-    float p[4], g[4], gmul, ms0 = 0.0f, vs0 = 0.0f;
-    uint32_t mc = 0, vc = 0;
-    if (live) {
-        load4<NT>((const PT *)T.p, i, T.n, p);
-        load4<NT>((const GT *)T.g, i, T.n, g);
-        mc = NT ? __builtin_nontemporal_load((const uint32_t *)(mcs + i)) : *(const uint32_t *)(mcs + i);
-        vc = NT ? __builtin_nontemporal_load((const uint32_t *)(vcs + i)) : *(const uint32_t *)(vcs + i);
-        ms0 = mss[wave];
-        vs0 = vss[wave];
+    const int64_t block = T.place / BLK + wave;
+    SNK_GLOBAL uint32_t *mcs = (SNK_GLOBAL uint32_t *)A.m + block * 64, *vcs = (SNK_GLOBAL uint32_t *)A.v + block * 64;
+    uint32_t mc, vc;
+    if (NT) {
+        mc = __builtin_nontemporal_load(mcs + lane);
+        vc = __builtin_nontemporal_load(vcs + lane);
+    } else {
+        mc = mcs[lane];
+        vc = vcs[lane];
     }
-    if (!grad_factor(A, sh, gmul) || !live) return;
-    float m[4], v[4], mmax = 0.0f, vmax = 0.0f;
+    const Pack<PT, 4> pq = load4<NT>((const PT *)T.p, i, T.n, whole);
+    const Pack<GT, 4> gq = load4<NT>((const GT *)T.g, i, T.n, whole);
+    const float ms0 = A.ms[block], vs0 = A.vs[block];
+    level[threadIdx.x] = v_level((float)threadIdx.x);
+    const uint64_t h = splitmix64(key ^ (uint64_t)(block * 64 + lane));
+    float gmul;
+    const bool go = grad_factor(A, sh, gmul);
+    __syncthreads();
+    if (!go || mine > last) return;
+    float p[4], m[4], v[4], mmax = 0.0f, vmax = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {   // places behind the tensor's end hold zeros and read g = 0
         m[e] = m_value((float)(int8_t)(mc >> (8 * e)), ms0);
-        v[e] = v_level((float)((vc >> (8 * e)) & 255u)) * vs0;
-        p[e] = adamw_one<false>(A.H, gmul, ibc1, ibc2, T.wd, p[e], g[e], m[e], v[e]);
+        v[e] = level[(vc >> (8 * e)) & 255u] * vs0;
+        p[e] = adamw_one<false>(A.H, gmul, ibc1, ibc2, T.wd, pq.get(e), gq.get(e), m[e], v[e]);
         mmax = fmaxf(mmax, fabsf(m[e]));
         vmax = fmaxf(vmax, v[e]);
     }
-    store_params<PT, NT>(T, A.H.copy_dtype, i, p);
+    store_params<PT, NT>(T, A.H.copy_dtype, i, whole, p);
     mmax = wave_max_nonneg(mmax);
     vmax = wave_max_nonneg(vmax);
-    // the codes as correctly rounded quotients and roots give them (the same arithmetic anywhere gives
-    // the same codes), at a third of the divide's cost: one reciprocal a wave, of a scale brought up
-    // first where it would overflow. 0.38 ms against 0.58 with the compiler's divides (133 M, bf16).
-    const float km = mmax < 0x1p-100f ? 0x1p100f : 1.0f, kv = vmax < 0x1p-100f ? 0x1p100f : 1.0f;
-    const float dm = mmax > 0.0f ? mmax * km : 1.0f, dv = vmax > 0.0f ? vmax * kv : 1.0f;
-    const float im = 1.0f / dm, iv = 1.0f / dv;
-    float least[4];   // the code of v's least value above 0: a v that came back as 0 would leave m / eps
+    // The codes as correctly rounded quotients and roots give them (the same arithmetic anywhere gives
+    // the same codes): by one reciprocal a wave, of a scale in the middle of fp32's range.
+    float least[4], dm = mmax, dv = vmax;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) least[e] = v[e] > 0.0f ? 1.0f : 0.0f;
-    if (km != 1.0f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m[e] *= km;
-    if (kv != 1.0f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= kv;
+    for (int e = 0; e < 4; ++e) least[e] = __builtin_amdgcn_fmed3f(ceilf(v[e]), 0.0f, 1.0f);
+    to_middle(dm, m);
+    to_middle(dv, v);
+    const float im = reciprocal(dm), iv = reciprocal(dv);
     uint32_t mo = 0, vo = 0;
     float a[4], far = 0.0f, all = 0.0f;
 #pragma unroll
@@ -391,29 +414,30 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     // 1 wave in 20: what is next to a half (and a NaN, whose code is 0), again in full
     if (__builtin_amdgcn_ballot_w64(!(fmaf(0.0f, all, far) < 0.4999f)))
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = rintf(127.0f * root(quotient(fabsf(m[e]), dm, im)));
+        for (int e = 0; e < 4; ++e) a[e] = rintf(127.0f * __builtin_sqrtf(fmaxf(fabsf(m[e]) / dm, 0.0f)));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         mo = __builtin_amdgcn_cvt_pk_u8_f32(copysignf(a[e], m[e]) + 128.0f, e, mo);
-        // next to a level either floor leads to that level, so the hardware's roots (1 ulp) do here
+        // next to a level either floor leads to that level, so the hardware's roots (1 ulp) do here. What
+        // is above 0 never becomes 0 (m / eps would follow): its lower level is at least the first.
         const float part = quotient(v[e], dv, iv);
-        const float low = fminf(floorf(255.0f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(part))), 254.0f);
-        const float lo = v_level(low), hi = v_level(low + 1.0f);
+        const float low = __builtin_amdgcn_fmed3f(floorf(255.0f * __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(part))), least[e], 254.0f);
+        const int l = (int)low;
+        const float lo = level[l], hi = level[l + 1];
         const float r = (float)((uint32_t)(h >> (16 * e)) & 0xFFFFu) * 0x1p-16f;
-        const float b = r * (hi - lo) < part - lo ? low + 1.0f : low;
-        vo = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(b, least[e]), e, vo);
+        vo = __builtin_amdgcn_cvt_pk_u8_f32(r * (hi - lo) < part - lo ? low + 1.0f : low, e, vo);
     }
     mo ^= 0x80808080u;   // a + 128 as a signed byte
     if (NT) {
-        __builtin_nontemporal_store(mo, (uint32_t *)(mcs + i));
-        __builtin_nontemporal_store(vo, (uint32_t *)(vcs + i));
+        __builtin_nontemporal_store(mo, mcs + lane);
+        __builtin_nontemporal_store(vo, vcs + lane);
     } else {
-        *(uint32_t *)(mcs + i) = mo;
-        *(uint32_t *)(vcs + i) = vo;
+        mcs[lane] = mo;
+        vcs[lane] = vo;
     }
     if (lane == 0) {
-        mss[wave] = mmax;
-        vss[wave] = vmax;
+        A.ms[block] = mmax;
+        A.vs[block] = vmax;
     }
 }
 
@@ -422,6 +446,7 @@ template <class OT, bool EIGHT>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(AdamArgs A, int64_t total, OT *__restrict__ mo,
                                                             OT *__restrict__ vo) {
     for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < total; i += (int64_t)gridDim.x * 1024) {
+        const bool whole = i + 4 <= total;
         float m[4], v[4];
         if (EIGHT) {
             const uint32_t mc = *(const uint32_t *)((const uint8_t *)A.m + i);
@@ -433,11 +458,16 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(AdamArgs A, int64_t 
                 v[e] = v_level((float)((vc >> (8 * e)) & 255u)) * vs;
             }
         } else {
-            load4<false>((const float *)A.m, i, total, m);
-            load4<false>((const float *)A.v, i, total, v);
+            const Pack<float, 4> mq = load4<false>((const float *)A.m, i, total, whole);
+            const Pack<float, 4> vq = load4<false>((const float *)A.v, i, total, whole);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m[e] = mq.get(e);
+                v[e] = vq.get(e);
+            }
         }
-        if (mo) store4<false>(mo, i, total, m);
-        if (vo) store4<false>(vo, i, total, v);
+        if (mo) store4<false>(mo, i, total, whole, m);
+        if (vo) store4<false>(vo, i, total, whole, v);
     }
 }
 
