@@ -311,13 +311,14 @@ int snk_adamw_create(snk_adamw *out, int32_t n, const int64_t *sizes_host, const
 int snk_adamw_destroy(snk_adamw h);
 /* the tensors' device addresses, contiguous, element-aligned: params (updated), grads, and copies
  * (NULL unless copy_dtype >= 0). Refused where a tensor that is written overlaps another one.
- * Enqueued like any work, and kept: later steps (a captured one's replays too) use the last bind. */
+ * Enqueued like any work, and kept: later steps (an earlier captured one's replays too) use the last
+ * bind. Refused, as snk_adamw_create is, while the stream is being captured. */
 int snk_adamw_bind(snk_adamw h, void *const *params_dev, const void *const *grads_dev, void *const *copies_dev);
 int snk_adamw_step(snk_adamw h, float lr, float grad_scale);
 /* places in the state layout; starts_host (optional, n): each tensor's */
 int snk_adamw_layout(snk_adamw h, int64_t *total_out, int64_t *starts_host);
 int snk_adamw_state_ptr(snk_adamw h, int32_t which, void **dev_out, int64_t *bytes_out);
-/* the moments' values in the state layout, rounded to dtype; either pointer may be NULL */
+/* the moments' values in the state layout, rounded to dtype, into two arrays; either may be NULL */
 int snk_adamw_moments(snk_adamw h, int32_t dtype, void *m_dev, void *v_dev);
 int snk_adamw_get_steps(snk_adamw h, int64_t *steps_out);
 int snk_adamw_set_steps(snk_adamw h, int64_t steps);

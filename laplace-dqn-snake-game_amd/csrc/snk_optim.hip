@@ -25,6 +25,7 @@ constexpr int NORM_WG = 2048;   // most workgroups (= partial sums) of the norm 
 // caches: nothing of them lives there until the next step, and what is written evicts nothing that is
 // still to be read. 32-bit states: 159 us against 180 at 537 MB, 78 against 68 at 268 MB.
 constexpr int64_t NT_FROM = 320ll << 20;
+constexpr int64_t GRID = 1 << 23;   // chunks of one launch: the card's grids end at 2^32 threads
 constexpr int FEW_PARTS = 256;  // partial sums that every workgroup of the step adds up itself
 
 struct AdamTensor {
@@ -542,6 +543,13 @@ static void check_device(snk_adamw h) {
               dev);
 }
 
+// what a replay would not do again, and what would leave addresses that no replay has brought yet
+static void check_not_captured(hipStream_t s, const char *what) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    SNK_HIP(hipStreamIsCapturing(s, &st));
+    SNK_CHECK(st == hipStreamCaptureStatusNone, SNK_ERR_STATE, "AdamW: %s while the stream is being captured", what);
+}
+
 namespace snk {
 
 void adamw_reset(snk_adamw h, hipStream_t s) {
@@ -576,6 +584,8 @@ snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const s
     SNK_CHECK(cfg->eps >= least && cfg->eps <= 1e30, SNK_ERR_INVALID, "AdamW: eps %g outside [%g, 1e30]", cfg->eps, least);
     SNK_CHECK(cfg->max_grad_norm >= 0, SNK_ERR_INVALID, "AdamW: max_grad_norm %g is negative", cfg->max_grad_norm);
     SNK_CHECK(cfg->reserved == 0, SNK_ERR_INVALID, "AdamW: reserved must be 0");
+    hipStream_t s = stream();
+    check_not_captured(s, "a handle is made");
     auto h = std::make_unique<snk_adamw_s>();
     h->cfg = *cfg;
     SNK_HIP(hipGetDevice(&h->device));
@@ -604,7 +614,6 @@ snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const s
     }
     h->part = DevBuf<double>(NORM_WG);
     h->ctl = DevBuf<AdamCtl>(1);
-    hipStream_t s = stream();
     if (!chunks.empty())
         SNK_HIP(hipMemcpyAsync(h->chunks, chunks.data(), chunks.size() * sizeof(AdamChunk), hipMemcpyHostToDevice, s));
     adamw_reset(h.get(), s);
@@ -618,6 +627,7 @@ void adamw_set_owned(snk_adamw h) { h->owned = true; }
 void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void *const *copies, hipStream_t s) {
     const int n = (int)h->size.size();
     SNK_CHECK(params && grads, SNK_ERR_INVALID, "adamw_bind: NULL argument");
+    check_not_captured(s, "tensors are bound");
     SNK_CHECK((copies != nullptr) == (h->cfg.copy_dtype >= 0), SNK_ERR_INVALID,
               "adamw_bind: copies go with a copy_dtype, and only with one");
     struct Span {
@@ -727,22 +737,24 @@ void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s) {
     }
     if (h->n_chunks == 0) return;
     const bool nt = h->total * (dtype_size(c.param_dtype) + dtype_size(c.grad_dtype) + c.state_bits / 4) >= NT_FROM;
-    with_type(c.param_dtype, [&](auto p) {
-        with_type(c.grad_dtype, [&](auto g) {
-            using PT = decltype(p);
-            using GT = decltype(g);
-            const unsigned grid = (unsigned)h->n_chunks;
-            if (c.state_bits == 8 && nt)
-                adamw8_kernel<PT, GT, true><<<grid, 256, 0, s>>>(A);
-            else if (c.state_bits == 8)
-                adamw8_kernel<PT, GT, false><<<grid, 256, 0, s>>>(A);
-            else if (nt)
-                adamw32_kernel<PT, GT, true><<<grid, 256, 0, s>>>(A);
-            else
-                adamw32_kernel<PT, GT, false><<<grid, 256, 0, s>>>(A);
+    for (int64_t at = 0; at < h->n_chunks; at += GRID, A.chunks += GRID) {
+        with_type(c.param_dtype, [&](auto p) {
+            with_type(c.grad_dtype, [&](auto g) {
+                using PT = decltype(p);
+                using GT = decltype(g);
+                const unsigned grid = (unsigned)std::min(GRID, h->n_chunks - at);
+                if (c.state_bits == 8 && nt)
+                    adamw8_kernel<PT, GT, true><<<grid, 256, 0, s>>>(A);
+                else if (c.state_bits == 8)
+                    adamw8_kernel<PT, GT, false><<<grid, 256, 0, s>>>(A);
+                else if (nt)
+                    adamw32_kernel<PT, GT, true><<<grid, 256, 0, s>>>(A);
+                else
+                    adamw32_kernel<PT, GT, false><<<grid, 256, 0, s>>>(A);
+            });
         });
-    });
-    launch_check("adamw_kernel");
+        launch_check("adamw_kernel");
+    }
 }
 
 }  // namespace snk
@@ -807,6 +819,7 @@ extern "C" int snk_adamw_moments(snk_adamw h, int32_t dtype, void *m_dev, void *
         SNK_CHECK(h && dtype_ok(dtype), SNK_ERR_INVALID, "bad adamw_moments arguments");
         check_device(h);
         if (h->total == 0 || (!m_dev && !v_dev)) return;
+        SNK_CHECK(m_dev != v_dev, SNK_ERR_INVALID, "adamw_moments: both moments into one array");
         const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(h->total, 1024), 4096);
         with_type(dtype, [&](auto o) {
             using OT = decltype(o);

@@ -54,8 +54,8 @@ struct SampleArgs {
     // that entry, and the maxima of 64
     double *masses;
     float *block_tops, *tops;
-    // top-p alone: rows row0.. of this launch, each in `splits` parts
-    int64_t row0;
+    int64_t row0;   // the first row of this launch
+    // top-p alone: each row in `splits` parts
     int32_t splits;
     uint64_t *bins, *kept;    // [row][split][NBINS], [row][blocks]
     uint2 *lists;             // [row][split][NLIST] key, index
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
     uint64_t *const seg_mass = mass;       // [NT], once the search is over
     uint32_t *const seg_ties = count;
     uint32_t *const group_list = (uint32_t *)mass;   // [LIST], before it
-    const int64_t r = (FUSED || !A.heads ? 0 : A.row0) + blockIdx.x;
+    const int64_t r = A.row0 + blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = A.n;
     const SampleRow s = sample_row(A, r);
     const T *x = (const T *)A.x + r * A.ld;
@@ -1348,6 +1348,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
 }
 
 // ---------------------------------------------------------------- launches
+constexpr int64_t GRID = 1 << 22;      // rows of one launch: the card's grids end at 2^32 threads
 constexpr int64_t MANY_ROWS = 512;   // from here on a row's workgroup has 4 waves instead of 16
 // rows whose workgroup scans them itself: a piece a wave
 static bool fused(int64_t rows, int64_t n) { return n <= (rows >= MANY_ROWS ? 4 : 16) * PIECE; }
@@ -1426,11 +1427,14 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
     }
     const bool many = A.rows >= MANY_ROWS;
     if (fused(A.rows, A.n)) {
-        if (many)
-            sample_row_kernel<T, 4, true><<<(unsigned)A.rows, 256, 0, s>>>(A);
-        else
-            sample_row_kernel<T, 16, true><<<(unsigned)A.rows, 1024, 0, s>>>(A);
-        launch_check("sample_row_kernel");
+        for (; A.row0 < A.rows; A.row0 += GRID) {
+            const unsigned rows = (unsigned)std::min(GRID, A.rows - A.row0);
+            if (many)
+                sample_row_kernel<T, 4, true><<<rows, 256, 0, s>>>(A);
+            else
+                sample_row_kernel<T, 16, true><<<rows, 1024, 0, s>>>(A);
+            launch_check("sample_row_kernel");
+        }
         return;
     }
     const SampleSpace S(A.rows, A.n);
@@ -1449,10 +1453,9 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
         A.listed = (uint32_t *)(ws + S.listed);
         A.heads = (SampleHead *)(ws + S.heads);
     }
-    const int64_t chunk = nucleus ? S.chunk : A.rows;
-    for (int64_t r = 0; r < A.rows; r += chunk) {
-        A.row0 = r;
-        const unsigned rows = (unsigned)std::min(chunk, A.rows - r);
+    const int64_t chunk = nucleus ? S.chunk : GRID;
+    for (; A.row0 < A.rows; A.row0 += chunk) {
+        const unsigned rows = (unsigned)std::min(chunk, A.rows - A.row0);
         if (nucleus) {
             sample_bins_kernel<T><<<rows * S.splits, NTH, 0, s>>>(A, S.blocks);
             launch_check("sample_bins_kernel");

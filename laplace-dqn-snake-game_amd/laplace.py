@@ -168,7 +168,7 @@ def compute_D(tr, K: int = 1000, thin: int = 10, burn_in: int = 50_000, graph: b
     else:
         raise ValueError(f"unknown schedule {schedule!r}")
     if reset_optimizer:
-        model.set_params(np.zeros(model.P, np.float32), _lib.SNK_NET_OPT_STATE)
+        model.reset_optimizer()
 
     def updates(nb_from: int, nb_to: int) -> None:          # updates nb_from .. nb_to (inclusive)
         if nb_to < nb_from:

@@ -84,6 +84,13 @@ class _Handle:
             out[name] = DeviceView(p.value, n.value // (1 if dt[1] == "1" else 4), dt, self)
         return out
 
+    def reset(self) -> None:
+        """Zero moments, step 0."""
+        for name, view in self.state().items():
+            if name != "norm" and view.nbytes:
+                self._call("snk_memset", view.ptr, 0, view.nbytes)
+        self.steps = 0
+
     def moments(self, m=None, v=None) -> None:
         """The moments' values, written into m and v: [total] arrays of one type, either may be None."""
         bufs = [None if x is None else _lib.device_buffer(x, "moments") for x in (m, v)]
@@ -109,6 +116,7 @@ class AdamW(_Handle):
 
     def __init__(self, params, grads, *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01,
                  state_bits: int = 32, max_grad_norm: float = 0.0, copies=None, seed: int = 0):
+        keep = params, grads, copies = self._lists(params, grads, copies)
         ps, gs, cs = self._buffers(params, grads, copies)
         n = len(ps)
         wd = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
@@ -123,7 +131,11 @@ class AdamW(_Handle):
         h = vp()
         self._call("snk_adamw_create", C.byref(h), n, (i64 * n)(*self._sizes), (f32 * n)(*wd), C.byref(cfg))
         self._h = h
-        self._bind(ps, gs, cs, (params, grads, copies))
+        self._bind(ps, gs, cs, keep)
+
+    @staticmethod
+    def _lists(*lists):   # of our own: what they hold has to live as long as its addresses are used
+        return tuple(None if xs is None else tuple(xs) for xs in lists)
 
     @staticmethod
     def _buffers(params, grads, copies):
@@ -144,13 +156,15 @@ class AdamW(_Handle):
         self._keep = keep
 
     def bind(self, params, grads, copies=None) -> None:
-        """Other addresses for the same tensors (new gradients, moved parameters)."""
+        """Other addresses for the same tensors (new gradients, moved parameters). Not while a graph is
+        captured; graphs captured before use the new addresses from then on."""
+        keep = params, grads, copies = self._lists(params, grads, copies)
         ps, gs, cs = self._buffers(params, grads, copies)
         if [b.size for b in ps] != self._sizes:
             raise ValueError("AdamW.bind: the sizes are those of the constructor")
         if (_same(ps, "params"), _same(gs, "grads"), _same(cs, "copies") if cs else -1) != self._types:
             raise ValueError("AdamW.bind: the element types are those of the constructor")
-        self._bind(ps, gs, cs, (params, grads, copies))
+        self._bind(ps, gs, cs, keep)
 
     def step(self, *, lr: float | None = None, grad_scale: float = 1.0) -> None:
         """One step on the bound gradients times grad_scale (the inverse of a loss scale).

@@ -46,7 +46,7 @@ class DQNModel:
         self.board_size, self.n_frames, self.n_actions = int(board_size), int(n_frames), 3
         self.lr, self.rho, self.eps = float(lr), float(rho), float(eps)
         self.deep = bool(deep)
-        self._adamw = None   # weak: the state object refers back to this model
+        self._adamw = self._adamw_args = None   # the state object, weakly: it refers back to this model
         h = vp()
         call("snk_dqn_create_deep" if self.deep else "snk_dqn_create", C.byref(h), self.board_size, self.n_frames,
              self.lr, self.rho, self.eps, int(seed))
@@ -135,8 +135,24 @@ class DQNModel:
         h = vp()
         call("snk_dqn_use_adamw", self._h, C.byref(cfg), float(lr), float(weight_decay), C.byref(h))
         self._end_adamw()
-        self._adamw = weakref.ref(opt := ModelAdamW(self, h, lr, state_bits, 12 if self.deep else 10))
+        self._adamw_args = (h, lr, state_bits, 12 if self.deep else 10)
+        return self.adamw
+
+    @property
+    def adamw(self) -> ModelAdamW | None:
+        """use_adamw's state, None under RMSProp."""
+        opt = self._adamw() if self._adamw else None
+        if opt is None and self._adamw_args:
+            opt = ModelAdamW(self, *self._adamw_args)
+            self._adamw = weakref.ref(opt)
         return opt
+
+    def reset_optimizer(self) -> None:
+        """The optimizer in force as it was at first: RMSProp's accumulators or AdamW's moments zero."""
+        if self._adamw_args:
+            self.adamw.reset()
+        else:
+            self.set_params(np.zeros(self.P, np.float32), _lib.SNK_NET_OPT_STATE)
 
     def use_rmsprop(self) -> None:
         """Back to RMSProp, with its state as it was left. Ends the life of use_adamw's state."""
@@ -147,7 +163,7 @@ class DQNModel:
         old = self._adamw() if self._adamw else None
         if old is not None:
             old._h = None   # the library has freed it: later calls are refused
-        self._adamw = None
+        self._adamw = self._adamw_args = None
 
     def update(self, rpb, idx, B: int, gamma: float = 0.97) -> float:
         loss = C.c_double(0)

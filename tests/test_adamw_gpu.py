@@ -402,3 +402,103 @@ def test_trainer_on_adamw(snk, deep):
         out.append(got)
     assert all(np.array_equal(a, b) for a, b in zip(*out))
     assert np.all(np.isfinite(out[0][0]))
+
+
+def test_lists_of_the_caller_may_change(snk):
+    """Generators are taken, and what the caller's lists lose later is kept."""
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    ps = [torch.randn(5000, device="cuda", generator=gen) for _ in range(3)]
+    gs = [torch.randn(5000, device="cuda", generator=gen) for _ in range(3)]
+    want = [p.clone() for p in ps]
+    same = snk.AdamW(want, [g.clone() for g in gs])
+    opt = snk.AdamW((p for p in ps), gs)
+    del gs[:]
+    others = [torch.full((5000,), 7.0, device="cuda") for _ in range(12)]   # may take freed places
+    same.step()
+    opt.step()
+    assert all(torch.equal(a, b) for a, b in zip(ps, want))
+    assert all(bool((x == 7.0).all()) for x in others)
+
+
+def test_refused_under_capture(snk):
+    """A handle is made and tensors are bound outside a capture; the capture goes on."""
+    p, g, q = (torch.ones(300, device="cuda") for _ in range(3))
+    opt = snk.AdamW([p], [g])
+    model = snk.DQNModel(12, 3, n_frames=2)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        with pytest.raises(snk.SnakeHipError, match="captured"):
+            snk.AdamW([q], [g])
+        with pytest.raises(snk.SnakeHipError, match="captured"):
+            opt.bind([q], [g])
+        opt.step()
+    assert opt.steps == 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert opt.steps == 1 and bool((p < 1).all()) and bool((q == 1).all())
+    assert model.use_adamw().steps == 0
+
+
+def test_moments_into_one_array_are_refused(snk):
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = snk.AdamW([p], [g])
+    x = torch.empty(opt.total, device="cuda")
+    with pytest.raises(snk.SnakeHipError, match="one array"):
+        opt.moments(x, x)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_reset_optimizer(snk, bits):
+    """reset() and DQNModel.reset_optimizer start the optimizer in force again, the state object lost or not."""
+    model = snk.DQNModel(12, 3, n_frames=2, seed=3)
+    assert model.adamw is None
+    opt = model.use_adamw(lr=1e-3, state_bits=bits)
+    assert model.adamw is opt
+    gen = np.random.default_rng(1)
+    start, grad = model.get_params(), gen.standard_normal(model.P).astype(np.float32)
+
+    def step():
+        model.set_params(start)
+        model.set_params(grad, snk.SNK_NET_GRAD)
+        model.apply_grad()
+        return model.get_params()
+
+    first, second = step(), step()
+    assert not np.array_equal(first, second)
+    opt.reset()
+    assert opt.steps == 0 and not opt.state()["m"].numpy().any()
+    assert np.array_equal(step(), first)
+    del opt
+    model.reset_optimizer()
+    assert model.adamw.steps == 0
+    assert np.array_equal(step(), first)
+    model.use_rmsprop()
+    assert model.adamw is None
+    first, second = step(), step()
+    model.reset_optimizer()
+    assert np.array_equal(step(), first) and not np.array_equal(first, second)
+
+
+def test_more_elements_than_one_grid(snk):
+    """Places past 2^34: the tail of a tensor moves as a small tensor of its own does."""
+    big, tail = (1 << 34) + 1000, 3048   # the tail starts on a block
+    if torch.cuda.mem_get_info()[0] < 140 << 30:
+        pytest.skip("needs 140 GB of free memory")
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    p, g = (torch.zeros(big, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    p[-tail:] = torch.randn(tail, device="cuda", generator=gen)
+    g[-tail:] = torch.randn(tail, device="cuda", generator=gen)
+    p2, g2 = p[-tail:].clone(), g[-tail:].clone()
+    a = snk.AdamW([p], [g], state_bits=8, lr=1e-2)
+    b = snk.AdamW([p2], [g2], state_bits=8, lr=1e-2)
+    a.step()
+    b.step()
+    assert torch.equal(p[-tail:], p2) and not bool(p[:1 << 20].any())
+    x, y = a.state(), b.state()
+    for name in ("m", "m_scale", "v_scale"):
+        small = torch.as_tensor(y[name], device="cuda")
+        assert torch.equal(torch.as_tensor(x[name], device="cuda")[-small.numel():], small), name
+    assert a.steps == 1
+    del a, p, g
+    torch.cuda.empty_cache()

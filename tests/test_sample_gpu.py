@@ -323,3 +323,18 @@ def test_an_iteration_of_both_ends(snk):
                               max_norm=1.0)
         assert np.all(np.abs(layout(model.get_params()) - want.p) <= want.ep) and np.isfinite(loss)
     assert opt.steps == updates
+
+
+@pytest.mark.parametrize("n", [9, 2049])
+def test_more_rows_than_one_grid(snk, n):
+    """Rows past 2^22, which take a second launch, answer as a call of their own."""
+    rows, last = (1 << 22) + 300, 400
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(n, device="cuda", generator=gen).to(torch.float16)
+    u = torch.rand(rows, device="cuda", generator=gen)
+    prob, want_prob = torch.empty(rows, device="cuda"), torch.empty(last, device="cuda")
+    got = snk.sample_logits(x.expand(rows, n), u, prob=prob)
+    want = snk.sample_logits(x.expand(last, n), u[-last:].contiguous(), prob=want_prob)
+    assert torch.equal(got[-last:], want) and torch.equal(prob[-last:], want_prob)
+    want = snk.sample_logits(x.expand(last, n), u[:last].contiguous(), prob=want_prob)
+    assert torch.equal(got[:last], want) and torch.equal(prob[:last], want_prob)
