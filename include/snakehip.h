@@ -255,7 +255,7 @@ typedef struct {
 } snk_sample_cfg_t;
 /* row r's logits start at logits_dev + r * ld elements, its mask (bytes, non-zero = forbidden; NULL:
  * none) at mask_dev + r * ld_mask; ld, ld_mask >= n, or 0: one row for all. 1 <= n <= 2^24.
- * idx_dev[rows]; prob_dev[rows] or NULL. ws_dev: snk_sample_workspace's bytes (0 for n <= 2048),
+ * idx_dev[rows]; prob_dev[rows] or NULL. ws_dev: snk_sample_workspace's bytes (0 for n <= 4096),
  * 16-byte aligned, used during the call only: two calls in flight need two. */
 int snk_sample_workspace(int64_t rows, int64_t n, int64_t *bytes_out);
 int snk_sample_logits(const void *logits_dev, int64_t rows, int64_t n, int64_t ld, const uint8_t *mask_dev,

@@ -6,13 +6,16 @@
 // the entries equal to it, in index order. Masses inside a row's cut are integers (weights rounded to
 // 2^-sh of the largest), so sums in LDS atomics are exact and always the same.
 //
-// A row is read once for what decides most rows: the largest logit of every 64 (a bound for top-k and
+// Rows of up to 8 entries take a thread each (sample_few_kernel), of up to 4,096 the registers of one to
+// four waves (sample_wave_kernel).
+// A longer row is read once for what decides most rows: the largest logit of every 64 (a bound for top-k and
 // min-p) and, where the whole row's mass counts, the mass of every 2048 (sample_scan_kernel). For
 // top-p alone two more passes over the row find the cut's neighbourhood and the masses above it
 // (sample_bins_kernel, sample_kept_kernel). The row's workgroup (sample_row_kernel) then reads only
-// what can hold the answer. Rows of up to 512 a wave are scanned by that workgroup itself.
+// what can hold the answer. A few rows of up to 8,192 are scanned by that workgroup itself.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "snk_dqn.hpp"
 
@@ -177,45 +180,45 @@ __device__ __forceinline__ Weight weight(const SampleArgs &A, const SampleRow &s
     return Weight{pow2, (double)top, scale_of(s), A.unit, s.greedy || top == INFINITY};
 }
 
-template <class T>
-struct __attribute__((packed, aligned(sizeof(T)))) pack8 {
-    T v[8];
+template <class T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Packed {
+    T v[V];
 };
-// Elements i..i+7 of a row of n >= 8, -inf where masked or behind the end. In two steps, so that several loads are in flight before one is waited for: the load, of a
+// Elements i..i+V-1 of a row of n >= V, -inf where masked or behind the end. In two steps, so that several loads are in flight before one is waited for: the load, of a
 // whole vector inside the row whatever i is, and the values, by single elements where it was moved.
-template <class T>
-struct Raw8 {
-    pack8<T> q;
-    pack8<uint8_t> m;
+template <class T, int V = 8>
+struct Raw {
+    Packed<T, V> q;
+    Packed<uint8_t, V> m;
     __device__ __forceinline__ void load(const T *x, const uint8_t *mask, int i, int n) {
-        const int at = min(i, n - 8);
-        q = *reinterpret_cast<const pack8<T> *>(x + at);
-        if (mask) m = *reinterpret_cast<const pack8<uint8_t> *>(mask + at);
+        const int at = min(i, n - V);
+        q = *reinterpret_cast<const Packed<T, V> *>(x + at);
+        if (mask) m = *reinterpret_cast<const Packed<uint8_t, V> *>(mask + at);
     }
     __device__ __forceinline__ void values(const T *x, const uint8_t *mask, int i, int n, float *v) const {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (float)q.v[k];
+        for (int k = 0; k < V; ++k) v[k] = (float)q.v[k];
         if (mask) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = m.v[k] ? -INFINITY : v[k];
+            for (int k = 0; k < V; ++k) v[k] = m.v[k] ? -INFINITY : v[k];
         }
-        if (__any(i + 8 > n)) {   // a row's last vectors
-            if (i + 8 > n)
+        if (__any(i + V > n)) {   // a row's last vectors
+            if (i + V > n)
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < V; ++k)
                     v[k] = i + k < n && !(mask && mask[i + k]) ? (float)x[i + k] : -INFINITY;
         }
     }
 };
 template <class T>
 __device__ __forceinline__ void load8(const T *x, const uint8_t *mask, int i, int n, float *v) {
-    Raw8<T> r;
+    Raw<T> r;
     r.load(x, mask, i, n);
     r.values(x, mask, i, n, v);
 }
 template <class T>
 __device__ __forceinline__ void load_block(const T *x, const uint8_t *mask, int i, int n, float (*v)[8]) {
-    Raw8<T> r[BP];
+    Raw<T> r[BP];
 #pragma unroll
     for (int p = 0; p < BP; ++p) r[p].load(x, mask, i + p * PIECE, n);
 #pragma unroll
@@ -451,7 +454,7 @@ __global__ __launch_bounds__(1024) void sample_bins_kernel(SampleArgs A, int blo
     const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
     const int per = (blocks + A.splits - 1) / A.splits * BP, end = min((part + 1) * per, blocks * BP);   // pieces
     int c = part * per + __builtin_amdgcn_readfirstlane(tid >> 6);
-    Raw8<T> raw;   // of the next piece: in flight during all that follows
+    Raw<T> raw;   // of the next piece: in flight during all that follows
     if (c < end) raw.load(x, mask, c * PIECE + lane * 8, A.n);
     if (tid < 128) pow2[tid] = POW2[tid];
     mass[tid] = 0;
@@ -490,7 +493,7 @@ __global__ __launch_bounds__(1024) void sample_kept_kernel(SampleArgs A, int blo
     const T *x = (const T *)A.x + r * A.ld;
     const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
     const int per = (blocks + A.splits - 1) / A.splits * BP, end = min((part + 1) * per, blocks * BP);
-    Raw8<T> raw;
+    Raw<T> raw;
     if (part * per + wave < end) raw.load(x, mask, (part * per + wave) * PIECE + lane * 8, A.n);
     uint64_t m = 0, all;   // the bin of this thread, from the top
     const uint64_t *bins = A.bins + local * A.splits * NBINS + tid;
@@ -619,6 +622,286 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
         }
     }
     answer(A, r, at, W.real(xa) * A.unit / (double)sum);
+}
+
+// ---------------------------------------------------------------- 64 E NW threads' registers a row
+// Comparisons with others that cost what one bit of a search by mass does. 65,536 rows, top-p 0.9, fp32
+// (28 bits): n = 16 54 us by pairs and 190 by bits, n = 64 130 and 190; bf16 (13 bits): n = 48 104 and
+// 111, n = 64 130 and 111.
+constexpr int PAIRS_A_BIT = 4;
+// low bits that the keys of the type's positive values share, and those of its negative ones
+template <class T>
+constexpr int KEY_SHIFT = sizeof(T) == 4 ? 0 : std::is_same<T, __bf16>::value ? 16 : 13;
+
+// Thread l of the row's holds the elements E l..E l + E - 1, so that a prefix over the row is E additions
+// and one over the lanes. The cut's key is built from its highest bit that the row's keys differ in: by
+// how many entries are not below it (top-k: E comparisons and bit counts), or by their mass (top-p).
+// NW waves a row: alone (four rows a workgroup), or a workgroup, whose waves add up through LDS.
+// Bound by its instructions, 20 an element for the weight and the prefix and 2 (top-k) or 5 (top-p) an
+// element a bit. 65,536 rows of 1,024 bf16: 133 us whole, 225 top-k 40, 315 top-p 0.9 (a workgroup
+// with bins and lists in LDS a row: 366, 1,097, 1,622); 256 rows: 10 us, of which 6 are the launch.
+template <class T, int E, int NW>
+__global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void sample_wave_kernel(SampleArgs A) {
+    constexpr int V = E < 8 ? E : 8, SHIFT = KEY_SHIFT<T>, ROWS = NW == 1 ? 4 : 1;
+    __shared__ uint64_t pow2[128];
+    __shared__ uint64_t slots[2][NW];   // one sum's while the last one's are read
+    __shared__ float tops[NW];
+    __shared__ uint32_t leasts[NW];
+    __shared__ uint32_t list_key[ROWS][64], list_at[ROWS][64];
+    if (threadIdx.x < 128) pow2[threadIdx.x] = POW2[threadIdx.x];
+    __syncthreads();
+    const int lane = threadIdx.x & 63, n = A.n, in_group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = NW == 1 ? 0 : in_group, i0 = (wave * 64 + lane) * E;
+    const int64_t r = A.row0 + (int64_t)blockIdx.x * ROWS + (NW == 1 ? in_group : 0);
+    if (r >= A.rows) return;
+    const T *x = (const T *)A.x + r * A.ld;
+    const uint8_t *mask = A.mask ? A.mask + r * A.ld_mask : nullptr;
+    Raw<T, V> raw[E / V];
+#pragma unroll
+    for (int p = 0; p < E / V; ++p) raw[p].load(x, mask, i0 + p * V, n);
+    const SampleRow s = sample_row(A, r);
+    float v[E];
+#pragma unroll
+    for (int p = 0; p < E / V; ++p) raw[p].values(x, mask, i0 + p * V, n, v + p * V);
+    uint32_t key[E];   // above SHIFT; 0: excluded
+    float most = -INFINITY;
+    uint32_t least = 0xFFFFFFFFu;
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        nan |= v[e] != v[e];
+        most = fmaxf(most, v[e]);
+        key[e] = key_of(v[e]) >> SHIFT;
+        least = min(least, key[e] - 1);   // 0 becomes the largest
+    }
+    float top = max64(max8(most));
+    nan = __ballot(nan) != 0;
+    const bool cut = s.k < n || s.p < 1.0f;
+    if (cut)
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) least = min(least, (uint32_t)__shfl_xor((int)least, o));
+    if constexpr (NW > 1) {
+        if (lane == 0) {
+            tops[wave] = nan ? NAN : top;
+            leasts[wave] = least;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int o = 0; o < NW; ++o) {
+            const float t = tops[o];
+            nan |= t != t;
+            top = fmaxf(top, t);
+            least = min(least, leasts[o]);
+        }
+    }
+    if (nan || top == -INFINITY) {   // all of the row's waves
+        if (threadIdx.x % (64 * NW) == 0) answer(A, r, -1, nan ? NAN : 0.0);
+        return;
+    }
+    const Weight W = weight(A, s, (LdsTable)pow2, top);
+    auto logit = [&](uint32_t k) __attribute__((always_inline)) {
+        return of_key(k << SHIFT | (SHIFT && !(k >> (31 - SHIFT)) ? (1u << SHIFT) - 1 : 0u));
+    };
+    uint64_t w[E];
+    uint32_t heavy = 0;   // what min-p keeps, a bit an element
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const double real = key[e] ? W.real(v[e]) : 0.0;
+        w[e] = W.fixed(real);
+        heavy |= real >= (double)s.q ? 1u << e : 0u;
+        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // four at once: more only hold registers
+    }
+    int turn = 0;
+    auto over_waves = [&](uint64_t mine, uint64_t &before) __attribute__((always_inline)) {   // mine: the wave's
+        before = 0;
+        if constexpr (NW == 1) return mine;
+        if (lane == 0) slots[turn][wave] = mine;
+        __syncthreads();
+        uint64_t all = 0;
+#pragma unroll
+        for (int o = 0; o < NW; ++o) {
+            const uint64_t m = slots[turn][o];
+            before += o < wave ? m : 0;
+            all += m;
+        }
+        turn ^= 1;
+        return read_lane(all, 0);
+    };
+    auto not_below = [&](uint32_t at) __attribute__((always_inline)) {
+        int c = 0;
+        uint64_t before;
+#pragma unroll
+        for (int e = 0; e < E; ++e) c += __popcll(__ballot(key[e] >= at));
+        return (int)over_waves((uint64_t)c, before);
+    };
+    auto mass_not_below = [&](uint32_t at) __attribute__((always_inline)) {
+        uint64_t m = 0, before;
+#pragma unroll
+        for (int e = 0; e < E; ++e) m += key[e] >= at ? w[e] : 0;
+        return over_waves(wave_sum(m), before);
+    };
+    auto key_weight = [&](uint32_t k) __attribute__((always_inline)) { return W.fixed(W.real(logit(k))); };
+    // the first k of a wave's entries, one a lane in index order (key 0: none), their top-p and the
+    // answer: each entry's rank and the mass before it by comparing it with the m others
+    auto by_pairs = [&](uint32_t own_key, uint64_t own_w, bool over, int at, int m) __attribute__((always_inline)) {
+        uint32_t ahead = 0;
+        uint64_t mass = 0;
+        for (int i = 0; i < m; ++i) {
+            const uint32_t ki = read_lane(own_key, i);
+            const bool before = (ki > own_key) | ((ki == own_key) & (i < lane));
+            const uint64_t wi = read_lane(own_w, i);
+            ahead += before;
+            mass += before ? wi : 0;
+        }
+        bool kept = own_key && ahead < (uint32_t)s.k;
+        const double limit = (double)s.p * (double)wave_sum<uint64_t>(kept ? own_w : 0);
+        kept = kept && (s.p >= 1.0f || ahead == 0 || (double)mass < limit);
+        const uint64_t w = kept && over ? own_w : 0, upto = wave_scan(w), sum = last_lane(upto);
+        const double target = (double)s.u * (double)sum;
+        if (w && (double)upto > target && !((double)(upto - w) > target))   // one lane
+            answer(A, r, at, W.real(logit(own_key)) * A.unit / (double)sum);
+    };
+    // the cut: keys above kt, and the first nt of those equal to it
+    uint32_t kt = 0, nt = 0;
+    if (cut) {
+        const uint32_t first = key_of(top) >> SHIFT;
+        const uint32_t differ = (uint32_t)__builtin_amdgcn_readfirstlane((int)(first ^ (least + 1)));
+        const int bits = differ ? 32 - __clz((int)differ) : 0;
+        const uint32_t common = bits == 32 ? 0u : first >> bits << bits;
+        if constexpr (E == 1 && NW == 1)
+            if (s.p < 1.0f && n < PAIRS_A_BIT * bits) {
+                by_pairs(key[0], w[0], heavy & 1, i0, n);
+                return;
+            }
+        bool k_cut = false;
+        if (s.k < n && not_below(1) > s.k) {
+            k_cut = true;
+            kt = common;
+            int above = 0;
+            for (int b = bits - 1; b >= 0; --b) {
+                const uint32_t at = kt | 1u << b;
+                const int c = not_below(at);
+                if (c == s.k) {   // no tie is split
+                    kt = at - 1;
+                    above = c;
+                    break;
+                }
+                if (c > s.k)
+                    kt = at;
+                else
+                    above = c;   // at last: the entries over the key that the lower bits fill up to
+            }
+            nt = (uint32_t)(s.k - above);
+        }
+        if (E * NW > 1 && k_cut && s.k <= 64 && s.p < 1.0f) {
+            // top-p over a wave's worth of entries: listed in index order, for one wave
+            uint32_t ties = 0, mine = 0;
+            uint64_t before;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ties += key[e] == kt;
+            uint32_t upto = wave_scan(ties);
+            if constexpr (NW > 1) {
+                over_waves(last_lane(upto), before);
+                upto += (uint32_t)before;
+            }
+            uint32_t rank = upto - ties, in = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const bool is = key[e] > kt || (key[e] == kt && rank < nt);
+                rank += key[e] == kt;
+                in |= is ? 1u << e : 0u;
+            }
+            mine = (uint32_t)__popc(in);
+            upto = wave_scan(mine);
+            if constexpr (NW > 1) {
+                over_waves(last_lane(upto), before);
+                upto += (uint32_t)before;
+            }
+            uint32_t to = upto - mine;
+            const int row = NW == 1 ? in_group : 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (in >> e & 1) {   // k in all
+                    list_key[row][to] = key[e];
+                    list_at[row][to++] = (uint32_t)(i0 + e);
+                }
+            if constexpr (NW > 1) {
+                __syncthreads();
+                if (wave != 0) return;
+            } else {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the wave's own writes, then its reads
+            }
+            const uint32_t k = lane < s.k ? list_key[row][lane] : 0;
+            const double real = k ? W.real(logit(k)) : 0.0;
+            by_pairs(k, W.fixed(real), real >= (double)s.q, lane < s.k ? (int)list_at[row][lane] : -1, s.k);
+            return;
+        }
+        if (s.p < 1.0f) {
+            const uint64_t s1 = mass_not_below(kt + 1) + (nt ? nt * key_weight(kt) : 0);
+            const double limit = (double)s.p * (double)s1;
+            if (limit <= 0.0) {
+                kt = first;
+                nt = 1;
+            } else {
+                uint32_t t = common;
+                uint64_t above = 0;
+                for (int b = bits - 1; b >= 0; --b) {
+                    const uint32_t at = t | 1u << b;
+                    if (k_cut && at <= kt) {
+                        t = at;
+                        continue;
+                    }
+                    const uint64_t m = mass_not_below(at);
+                    if ((double)m >= limit)
+                        t = at;
+                    else
+                        above = m;
+                }
+                // tie j stays while above + j w < limit
+                const uint64_t wt = key_weight(t);
+                const double more = wt ? ceil((limit - (double)above) / (double)wt) : (double)n;
+                const uint32_t stay = (uint32_t)fmin(fmax(more, 1.0), (double)n);
+                nt = k_cut && t == kt ? min(stay, nt) : stay;
+                kt = t;
+            }
+        }
+    }
+    uint32_t rank = 0;
+    if (nt) {
+        uint32_t ties = 0;
+        uint64_t before;
+#pragma unroll
+        for (int e = 0; e < E; ++e) ties += key[e] == kt;
+        const uint32_t upto = wave_scan(ties);
+        over_waves(last_lane(upto), before);
+        rank = (uint32_t)before + upto - ties;
+    }
+    uint64_t own = 0, before;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        bool kept = key[e] > kt;
+        if (nt && key[e] == kt) kept = rank++ < nt;
+        w[e] = kept && (heavy >> e & 1) ? w[e] : 0;
+        own += w[e];
+    }
+    uint64_t upto = wave_scan(own);
+    const uint64_t sum = over_waves(last_lane(upto), before);
+    upto += before;
+    const double target = (double)s.u * (double)sum;
+    if (own && (double)upto > target && !((double)(upto - own) > target)) {   // one lane of the row's
+        upto -= own;
+        int at = -1;
+        uint32_t ka = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            upto += w[e];
+            if (at < 0 && w[e] && (double)upto > target) {
+                at = i0 + e;
+                ka = key[e];
+            }
+        }
+        answer(A, r, at, W.real(logit(ka)) * A.unit / (double)sum);
+    }
 }
 
 // ---------------------------------------------------------------- a workgroup a row
@@ -915,7 +1198,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             return;
         }
         bool from_list = m <= LIST;
-        constexpr int PAIRS = NT >= 512 ? 256 : 128;
+        constexpr int PAIRS = 256;
         if (cut && m <= PAIRS) {
             // each candidate's rank and the mass before it, by comparing all pairs: four threads a
             // candidate, sixteen bytes of LDS a comparison, no branches (350 cycles a comparison with them)
@@ -1348,10 +1631,16 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
 }
 
 // ---------------------------------------------------------------- launches
-constexpr int64_t GRID = 1 << 22;      // rows of one launch: the card's grids end at 2^32 threads
-constexpr int64_t MANY_ROWS = 512;   // from here on a row's workgroup has 4 waves instead of 16
+// Rows up to here are held in registers: sixteen entries a lane of four waves. Twice that, sixteen waves
+// (8,192 fp32, 8 rows): 20 us top-k 40 and 35 top-p 0.9, against 12 and 33 by the groups' maxima.
+constexpr int WAVE_N = 4096;
+constexpr int64_t GRID = 1 << 22;    // rows of one launch: the card's grids end at 2^32 threads
+// From here on the card has rows enough: 513 to 1,024 entries take one wave a row instead of four (bf16,
+// top-p 0.9: 4,096 rows 26 us against 45, 128 rows 13 against 10), longer rows' workgroups 8 waves
+// instead of 16.
+constexpr int64_t MANY_ROWS = 512;
 // rows whose workgroup scans them itself: a piece a wave
-static bool fused(int64_t rows, int64_t n) { return n <= (rows >= MANY_ROWS ? 4 : 16) * PIECE; }
+static bool fused(int64_t rows, int64_t n) { return rows < MANY_ROWS && n <= 16 * PIECE; }
 
 // the workspace's parts, in bytes from its start
 struct SampleSpace {
@@ -1359,7 +1648,7 @@ struct SampleSpace {
     int64_t chunk = 0;   // rows of a launch of the nucleus kernels
     int64_t masses = 0, block_tops = 0, tops = 0, bins = 0, kept = 0, lists = 0, listed = 0, heads = 0, bytes = 0;
     SampleSpace(int64_t rows, int64_t n) {
-        if (n <= 8 || fused(rows, n) || rows == 0) return;
+        if (n <= WAVE_N || fused(rows, n) || rows == 0) return;
         blocks = ceil_div(n, BLOCK);
         splits = (int)std::max<int64_t>(1, std::min<int64_t>({SPLITS, 1024 / rows, (blocks + 3) / 4}));
         chunk = std::min<int64_t>(rows, 2048 / splits);
@@ -1426,15 +1715,35 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
         return;
     }
     const bool many = A.rows >= MANY_ROWS;
-    if (fused(A.rows, A.n)) {
+    // a top-k that the groups' maxima bound, so that its candidates are few: 8 rows of 4,096, top-k 40,
+    // 11 us against 15, with top-p 0.9 11 against 17
+    const bool by_groups = !many && A.n > 2048 && !A.k_dev && A.top_k > 0 && A.top_k <= A.n / GROUP;
+    if (A.n <= WAVE_N && !by_groups) {
         for (; A.row0 < A.rows; A.row0 += GRID) {
-            const unsigned rows = (unsigned)std::min(GRID, A.rows - A.row0);
-            if (many)
-                sample_row_kernel<T, 4, true><<<rows, 256, 0, s>>>(A);
+            const unsigned rows = (unsigned)std::min(GRID, A.rows - A.row0), fours = (rows + 3) / 4;
+            if (A.n <= 64)
+                sample_wave_kernel<T, 1, 1><<<fours, 256, 0, s>>>(A);
+            else if (A.n <= 128)
+                sample_wave_kernel<T, 2, 1><<<fours, 256, 0, s>>>(A);
+            else if (A.n <= 256)
+                sample_wave_kernel<T, 4, 1><<<fours, 256, 0, s>>>(A);
+            else if (A.n <= 512)
+                sample_wave_kernel<T, 8, 1><<<fours, 256, 0, s>>>(A);
+            else if (A.n <= 1024 && many)
+                sample_wave_kernel<T, 16, 1><<<fours, 256, 0, s>>>(A);
+            else if (A.n <= 1024)
+                sample_wave_kernel<T, 4, 4><<<rows, 256, 0, s>>>(A);
+            else if (A.n <= 2048)
+                sample_wave_kernel<T, 8, 4><<<rows, 256, 0, s>>>(A);
             else
-                sample_row_kernel<T, 16, true><<<rows, 1024, 0, s>>>(A);
-            launch_check("sample_row_kernel");
+                sample_wave_kernel<T, 16, 4><<<rows, 256, 0, s>>>(A);
+            launch_check("sample_wave_kernel");
         }
+        return;
+    }
+    if (fused(A.rows, A.n)) {
+        sample_row_kernel<T, 16, true><<<(unsigned)A.rows, 1024, 0, s>>>(A);
+        launch_check("sample_row_kernel");
         return;
     }
     const SampleSpace S(A.rows, A.n);

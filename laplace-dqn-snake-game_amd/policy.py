@@ -81,7 +81,7 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     o_ptr = _lib.vector_ptr(out, "out", "i32", rows, device)
     p_ptr = None if prob is None else _lib.vector_ptr(prob, "prob", "f32", rows, device)
     w_ptr, w_bytes = None, 0
-    need = sample_workspace(rows, n) if n > 2048 else 0
+    need = sample_workspace(rows, n) if n > 4096 else 0
     if need:
         if workspace is None:
             workspace = _new(device, need, np.uint8)

@@ -338,3 +338,39 @@ def test_more_rows_than_one_grid(snk, n):
     assert torch.equal(got[-last:], want) and torch.equal(prob[-last:], want_prob)
     want = snk.sample_logits(x.expand(last, n), u[:last].contiguous(), prob=want_prob)
     assert torch.equal(got[:last], want) and torch.equal(prob[:last], want_prob)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [10, 16, 40, 128, 129, 256, 257, 1023, 1025, 2048, 2049, 3333, 4095, 4096])
+def test_rows_in_registers(snk, dtype, n):
+    """Few rows and many, of the sizes at which a row's share of waves changes; what is not the row's is NaN."""
+    for k, how in enumerate(SETTINGS + [dict(top_k=33, top_p=0.6), dict(top_k=64, top_p=0.99, min_p=0.02), dict(top_k=9, temperature=9.0)]):
+        x, u = logits(6, n, dtype, 7 * n + k, stride=n + 3, offset=1)
+        check(snk, x, u, most_left_out=1, **how)
+        x, u = logits(700, n, dtype, 9 * n + k)
+        x[5] = -torch.inf
+        x[6, : n // 2] = torch.inf
+        x[7] = 0.25
+        x[8, n // 3] = torch.nan
+        x[9, n - 1] = -torch.inf
+        x[10, 1:] = -torch.inf
+        mask = torch.rand(700, n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(n)) < 0.3
+        mask[11, : n // 2] = True
+        got = snk.sample_logits(x, u, mask=mask, **how)
+        rows = slice(0, 24)
+        assert torch.equal(got[rows], snk.sample_logits(x[rows], u[rows], mask=mask[rows], **how)), how
+        check(snk, x[rows], u[rows], mask=mask[rows], most_left_out=2, **how)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [20, 64, 500, 900, 2000, 4000])
+def test_ties_at_the_cut(snk, dtype, n):
+    """Few distinct values of either sign: cuts that split a run of equal entries, in index order."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    x = (torch.randint(-3, 4, (600, n), device="cuda", generator=gen) * 0.5).to(TT[dtype])
+    u = torch.rand(600, device="cuda", generator=gen)
+    for how in (dict(top_k=7), dict(top_k=n // 2), dict(top_p=0.4), dict(top_p=0.9, min_p=0.1), dict(top_k=60, top_p=0.7),
+                dict(top_k=n // 2 + 1, top_p=0.5)):
+        got = snk.sample_logits(x, u, **how)
+        assert torch.equal(got[:20], snk.sample_logits(x[:20], u[:20], **how)), how
+        check(snk, x[:20], u[:20], most_left_out=1, **how)
