@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import threading
 
 import numpy as np
 
@@ -430,7 +431,10 @@ def device_buffer(x, what: str, contiguous: bool = True) -> Buffer:
 
 def vector_ptr(x, what: str, kind: str, size: int, device) -> int:
     """Address of a contiguous device tensor of `size` elements of one type, on `device`."""
-    b = device_buffer(x, what)
+    if device is not None and hasattr(x, "data_ptr") and _TORCH_TYPES.get(x.dtype) == kind and x.numel() == size \
+            and x.device == device and x.is_contiguous():
+        return x.data_ptr()
+    b = device_buffer(x, what)   # says what is wrong
     if b.dtype != kind or b.size != size:
         raise ValueError(f"{what}: expected {size} values of type {kind}, got {b.size} of {b.dtype}")
     if b.device != device:
@@ -452,23 +456,38 @@ def call_on(device, name: str, *args) -> None:
     if device is None:
         call(name, *args)
         return
-    t = torch_module()
-    if t.cuda.current_device() != device.index:
-        raise ValueError(f"the tensors live on {device}, the current device is cuda:{t.cuda.current_device()}")
-    lib = load()
-    old, given = vp(), i32(0)
-    check(lib.snk_swap_stream(_raw_stream(t, device), 1, C.byref(old), C.byref(given)))
+    if not _torch_calls:
+        _torch_calls.extend(_find_torch_calls())
+    current, raw_stream = _torch_calls
+    index = device.index
+    if current() != index:
+        raise ValueError(f"the tensors live on {device}, the current device is cuda:{current()}")
+    lib = _lib or load()
+    try:
+        old, given, p_old, p_given = _slots.of_thread
+    except AttributeError:
+        old, given = vp(), i32(0)
+        _slots.of_thread = old, given, C.byref(old), C.byref(given)
+        _, _, p_old, p_given = _slots.of_thread
+    check(lib.snk_swap_stream(raw_stream(index), 1, p_old, p_given))
+    old, given = old.value, given.value
     try:
         check(getattr(lib, name)(*args))
     finally:
         lib.snk_swap_stream(old, given, None, None)
 
 
-def _raw_stream(t, device) -> int:
-    """torch.cuda.current_stream(device).cuda_stream, without its 2.8 us of objects where torch
-    offers the handle itself."""
-    raw = getattr(t._C, "_cuda_getCurrentRawStream", None)
-    return raw(device.index) if raw else t.cuda.current_stream(device).cuda_stream
+_slots = threading.local()   # where snk_swap_stream writes: made once a thread
+_torch_calls: list = []
+
+
+def _find_torch_calls():
+    """torch's current device and current stream's handle, without the objects (2.8 us a call) where
+    torch offers them so."""
+    t = torch_module()
+    device = getattr(t._C, "_cuda_getDevice", None) or t.cuda.current_device
+    stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (lambda i: t.cuda.current_stream(i).cuda_stream)
+    return device, stream
 
 
 def view_numpy(dev_ptr: int, shape, dtype) -> np.ndarray:

@@ -34,7 +34,7 @@ def _rows_of(x, b, what):
         rows, n = 1, b.shape[0]
     else:
         rows, n = b.shape
-    if b.device is None:
+    if b.device is None or x.is_contiguous():
         return rows, n, n
     st = x.stride()
     if n > 1 and st[-1] != 1:
