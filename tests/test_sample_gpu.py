@@ -374,3 +374,20 @@ def test_ties_at_the_cut(snk, dtype, n):
         got = snk.sample_logits(x, u, **how)
         assert torch.equal(got[:20], snk.sample_logits(x[:20], u[:20], **how)), how
         check(snk, x[:20], u[:20], most_left_out=1, **how)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("n", [8192, 8193, 20011, 32767, 32768, 32769])
+def test_rows_scanned_by_their_workgroup(snk, dtype, n):
+    """Up to 32,768 entries, four pieces of 512 a wave, the row's end inside any of them; as many rows
+    take the scan's own launch."""
+    for k, how in enumerate(SETTINGS):
+        x, u = logits(520, n, dtype, n + k, stride=n + 1, offset=1)
+        x[3] = -torch.inf
+        x[4, 1000:] = -torch.inf
+        x[5, :-1] = -torch.inf
+        mask = torch.rand(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(n)) < 0.3
+        few = slice(0, 9)
+        check(snk, x[few], u[few], mask=mask, most_left_out=1, **how)
+        got = snk.sample_logits(x, u, mask=mask, **how)
+        assert (got[few] != snk.sample_logits(x[few], u[few], mask=mask, **how)).sum() <= 1, how   # sums in another order
