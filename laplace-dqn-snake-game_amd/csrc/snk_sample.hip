@@ -351,6 +351,10 @@ __device__ __forceinline__ void wave_records(const float (*v)[8], bool with_mass
 }
 
 // ---------------------------------------------------------------- the scan: a wave a block
+// 2,048 entries a wave, four 16-byte loads a lane in flight before the first is waited for. With masses
+// the weights bound it, 23 fp64 instructions an entry: 256 rows of 131,072 bf16 in 26 us, 2.6 TB/s,
+// 22 us of them issue. Without (top-k, min-p alone) the reads: 512 rows of 32,003 bf16 8-10 us, 3.2 TB/s
+// and more. The next block read ahead cost more in waves a SIMD than it hid.
 template <class T>
 __global__ __launch_bounds__(256) void sample_scan_kernel(SampleArgs A, int blocks, int64_t total) {
     __shared__ uint64_t pow2[128];
@@ -439,7 +443,9 @@ __device__ __forceinline__ Nucleus nucleus(const SampleArgs &A, const SampleRow 
     return N;
 }
 
-// a workgroup a split of a row, a wave a piece: its mass by bins
+// A workgroup a split of a row, a wave a piece: its mass by bins. Rows are split until the card has 1,024
+// workgroups, a row into 16 at most (8 rows of 131,072 fp32: 6.7 us, the kernel after it 9.6). Bound by
+// the LDS atomics of neighbours that meet in one bin and, with few rows, by one wave's chain of steps.
 constexpr int NW = 16, NTH = 64 * NW;
 static_assert(NBINS == NTH && NW % BP == 0, "a bin a thread, whole blocks a round");
 template <class T>
@@ -563,6 +569,8 @@ __global__ __launch_bounds__(1024) void sample_kept_kernel(SampleArgs A, int blo
 }
 
 // ---------------------------------------------------------------- a thread a row: n <= N
+// Everything in registers, ranks by all pairs. 65,536 rows of 3 fp32: 4.0 us, 0.3 TB/s: a launch's own
+// 3.6 us; a wave a row (the next kernel) 23 us.
 template <class T, int N>
 __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
     __shared__ uint64_t pow2[128];
@@ -915,6 +923,9 @@ struct Total {
     uint64_t mass;
 };
 
+// Bound by its chain of a dozen dependent steps between barriers, not by what it reads: 256 rows of
+// 131,072 bf16, whole, 7.8 us; 128 of 50,021, top-k 40, 9.5; 8 of 131,072 fp32 after the nucleus search
+// 12; 512 of 32,003, min-p 0.05, with 8 waves each 16 (with 16 waves 20).
 // OWN: pieces a wave scans here, 0: sample_scan_kernel's records
 template <class T, int RW, int OWN>
 __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
