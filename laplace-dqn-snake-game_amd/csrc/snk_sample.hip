@@ -918,6 +918,9 @@ __device__ __forceinline__ int far_bin(float d) {
     const int b = (int)(__float_as_uint(d) >> 17) - ((127 - 12) << 6);
     return min(max(b, 0), BINS - 1);
 }
+__device__ __forceinline__ float far_edge(int b) {   // all in bins up to b are nearer, and nothing else is
+    return b < BINS - 1 ? __uint_as_float((uint32_t)(b + 1 + ((127 - 12) << 6)) << 17) : INFINITY;
+}
 struct Total {
     uint32_t count;
     uint64_t mass;
@@ -925,7 +928,7 @@ struct Total {
 
 // Bound by its chain of a dozen dependent steps between barriers, not by what it reads: 256 rows of
 // 131,072 bf16, whole, 7.8 us; 128 of 50,021, top-k 40, 9.5; 8 of 131,072 fp32 after the nucleus search
-// 12; 512 of 32,003, min-p 0.05, with 8 waves each 16 (with 16 waves 20).
+// 12; 512 of 32,003, min-p 0.05, with 8 waves each 14 (4 us more with 16).
 // OWN: pieces a wave scans here, 0: sample_scan_kernel's records
 template <class T, int RW, int OWN>
 __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
@@ -1078,15 +1081,12 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         } else {
             // candidates: what can be in the cut, by the groups' maxima: bins of the distance from the
             // top up to here, and, where min-p is not to change the mass that top-p goes by, this near
-            int far = BINS - 1;
             const bool by_q = s.q > 0.0f && s.p >= 1.0f;
             const float near = by_q ? (__builtin_amdgcn_logf(s.q) * -0.69315f + 1e-4f) * (float)s.t : INFINITY;
-            auto candidate = [&](float v) __attribute__((always_inline)) {
-                const float d = top - v;   // NaN for two infinities: top itself
-                return v != -INFINITY && !(d > near) && far_bin(d > 0.0f ? d : 0.0f) <= far;
-            };
+            float edge = near;   // candidates are nearer; NaN for two infinities: top itself
+            auto candidate = [&](float v) __attribute__((always_inline)) { return !(top - v >= edge); };
             if (W.hard) {
-                far = 0;
+                edge = far_edge(0);
             } else if (cut) {
                 // the bin that the wanted-th largest maximum falls in: at least that many entries are as near
 #pragma unroll
@@ -1110,7 +1110,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
                     ex += c[b];
                 }
                 __syncthreads();
-                far = (int)found_bin;
+                edge = fminf(near, far_edge((int)found_bin));
                 // fewer groups than wanted entries: everything would be a candidate
                 use_list = all >= wanted || n <= LIST || by_q;
             }
@@ -1208,6 +1208,31 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             const double t = (double)s.u * (double)sum;
             if (own && (double)upto > t && !((double)(upto - own) > t))   // one lane
                 answer(A, r, (int)list_at[lane], real * A.unit / (double)sum);
+            return;
+        }
+        if (!cut && m <= LIST) {
+            // min-p alone: prefix sums of the list, by one wave without a barrier
+            if (wave != 0) return;
+            const uint32_t share = (m + 63) / 64, i0 = min(lane * share, m), i1 = min(i0 + share, m);
+            auto kept_weight = [&](uint32_t i) __attribute__((always_inline)) -> uint64_t {
+                const double w = W.real(of_key(list_key[i]));
+                return w >= q ? W.fixed(w) : 0;
+            };
+            uint64_t own = 0;
+            for (uint32_t i = i0; i < i1; ++i) own += kept_weight(i);
+            uint64_t upto = wave_scan(own);
+            const uint64_t sum = last_lane(upto);
+            const double t = (double)s.u * (double)sum;
+            if (own && (double)upto > t && !((double)(upto - own) > t)) {   // one lane
+                upto -= own;
+                for (uint32_t i = i0; i < i1; ++i) {
+                    upto += kept_weight(i);
+                    if ((double)upto > t) {
+                        answer(A, r, (int)list_at[i], W.real(of_key(list_key[i])) * A.unit / (double)sum);
+                        break;
+                    }
+                }
+            }
             return;
         }
         bool from_list = m <= LIST;
@@ -1648,12 +1673,16 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
 // (8,192 fp32, 8 rows): 20 us top-k 40 and 35 top-p 0.9, against 12 and 33 by the groups' maxima.
 constexpr int WAVE_N = 4096;
 constexpr int64_t GRID = 1 << 22;    // rows of one launch: the card's grids end at 2^32 threads
-// From here on the card has rows enough: 513 to 1,024 entries take one wave a row instead of four (bf16,
-// top-p 0.9: 4,096 rows 26 us against 45, 128 rows 13 against 10), longer rows' workgroups 8 waves
-// instead of 16.
-constexpr int64_t MANY_ROWS = 512;
+// A CU holds one row's workgroup of 16 waves, two of 8 or four of 4; more rows than 256 CUs hold at once
+// take smaller ones. bf16 rows of 16,384: 511 rows, top-k 40, 13.6 us by 8 waves each and 14.9 by 16, whole
+// 16.1 and 17.9; 1,000 rows 19.6 by 4 and 23.5 by 8, whole 23.1 and 27.7 (min-p over longer rows loses a
+// tenth: 640 rows of 32,000 34 and 31).
+constexpr int64_t ROWS_OF_16 = 256, ROWS_OF_8 = 512;
+// From here on rows of 513 to 1,024 entries take one wave instead of four: bf16, top-p 0.9, 4,096 rows
+// 26 us against 45, 1,024 rows 14 against 17, 511 rows 14 against 12.
+constexpr int64_t ONE_WAVE_FROM = 768;
 // rows whose workgroup scans them itself: a piece a wave
-static bool fused(int64_t rows, int64_t n) { return rows < MANY_ROWS && n <= 16 * PIECE; }
+static bool fused(int64_t rows, int64_t n) { return rows <= ROWS_OF_16 && n <= 16 * PIECE; }
 
 // the workspace's parts, in bytes from its start
 struct SampleSpace {
@@ -1727,7 +1756,7 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
         launch_check("sample_few_kernel");
         return;
     }
-    const bool many = A.rows >= MANY_ROWS;
+    const bool many = A.rows > ROWS_OF_16;
     // a top-k that the groups' maxima bound, so that its candidates are few: 8 rows of 4,096, top-k 40,
     // 11 us against 15, with top-p 0.9 11 against 17
     const bool by_groups = !many && A.n > 2048 && !A.k_dev && A.top_k > 0 && A.top_k <= A.n / GROUP;
@@ -1742,7 +1771,7 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
                 sample_wave_kernel<T, 4, 1><<<fours, 256, 0, s>>>(A);
             else if (A.n <= 512)
                 sample_wave_kernel<T, 8, 1><<<fours, 256, 0, s>>>(A);
-            else if (A.n <= 1024 && many)
+            else if (A.n <= 1024 && A.rows >= ONE_WAVE_FROM)
                 sample_wave_kernel<T, 16, 1><<<fours, 256, 0, s>>>(A);
             else if (A.n <= 1024)
                 sample_wave_kernel<T, 4, 4><<<rows, 256, 0, s>>>(A);
@@ -1761,8 +1790,8 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
         return;
     }
     // up to 32,768, four pieces a wave, where top-p alone does not need its passes over the scan's
-    // records: bf16 rows of 16,384, top-k 40, 8 rows 10.7 us against 12.7 with the scan's own launch,
-    // 500 rows 15.4 against 18.4 (640 rows with 16 waves each 21.8, with 8 and the scan 19.2)
+    // records: 8 bf16 rows of 16,384, top-k 40, 10.7 us against 12.7 with the scan's own launch, 256 rows
+    // of 32,000 10.1 against 12.8
     if (!many && A.n <= 16 * BLOCK && !nucleus) {
         sample_row_kernel<T, 16, BP><<<(unsigned)A.rows, 1024, 0, s>>>(A);
         launch_check("sample_row_kernel");
@@ -1792,7 +1821,9 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
             sample_kept_kernel<T><<<rows * S.splits, NTH, 0, s>>>(A, S.blocks);
             launch_check("sample_kept_kernel");
         }
-        if (many)
+        if (A.rows > ROWS_OF_8)
+            sample_row_kernel<T, 4, 0><<<rows, 256, 0, s>>>(A);
+        else if (many)
             sample_row_kernel<T, 8, 0><<<rows, 512, 0, s>>>(A);
         else
             sample_row_kernel<T, 16, 0><<<rows, 1024, 0, s>>>(A);

@@ -391,3 +391,15 @@ def test_rows_scanned_by_their_workgroup(snk, dtype, n):
         check(snk, x[few], u[few], mask=mask, most_left_out=1, **how)
         got = snk.sample_logits(x, u, mask=mask, **how)
         assert (got[few] != snk.sample_logits(x[few], u[few], mask=mask, **how)).sum() <= 1, how   # sums in another order
+
+
+@pytest.mark.parametrize("n", [700, 1024, 4097, 9000, 40000])
+def test_rows_by_the_card(snk, n):
+    """The numbers of rows at which a row's workgroup shrinks give the same answers."""
+    x, u = logits(1030, n, "bf16", n)
+    mask = torch.rand(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(n)) < 0.1
+    for how in (dict(), dict(top_k=40), dict(top_p=0.9), dict(top_k=30, top_p=0.9), dict(min_p=0.02), dict(top_k=90, min_p=0.1)):
+        calls = [snk.sample_logits(x[:rows], u[:rows], mask=mask, **how)[:250] for rows in (250, 256, 257, 512, 513, 767, 768, 1030)]
+        check(snk, x[:10], u[:10], mask=mask, most_left_out=1, **how)
+        for got in calls[1:]:
+            assert (got != calls[0]).sum() <= 1, how   # whole rows' masses are added in another order
