@@ -92,7 +92,8 @@ class _Handle:
         self.steps = 0
 
     def moments(self, m=None, v=None) -> None:
-        """The moments' values, written into m and v: [total] arrays of one type, either may be None."""
+        """The moments' values, written into m and v: [total] arrays of one type, either may be None,
+        DeviceArrays or torch tensors as the parameters are (a model's: DeviceArrays)."""
         bufs = [None if x is None else _lib.device_buffer(x, "moments") for x in (m, v)]
         given = [b for b in bufs if b is not None]
         if not given:
@@ -100,9 +101,8 @@ class _Handle:
         for b in given:
             if b.size != self.total:
                 raise ValueError(f"moments: {b.size} elements for {self.total} places")
-        _lib.same_device(given)
-        _lib.call_on(given[0].device, "snk_adamw_moments", self._h, _same(given, "moments"),
-                     *[None if b is None else b.ptr for b in bufs])
+        _lib.same_device(given, self._device)   # another kind's stream would not wait for the steps
+        self._call("snk_adamw_moments", self._h, _same(given, "moments"), *[None if b is None else b.ptr for b in bufs])
 
 
 class AdamW(_Handle):

@@ -502,3 +502,49 @@ def test_more_elements_than_one_grid(snk):
     assert a.steps == 1
     del a, p, g
     torch.cuda.empty_cache()
+
+
+def test_moments_of_the_parameters_kind(snk):
+    """DeviceArrays are written on the library's stream, torch tensors on torch's: they are not mixed."""
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = snk.AdamW([p], [g])
+    with pytest.raises(ValueError, match="mix"):
+        opt.moments(snk.DeviceArray(opt.total, np.float32))
+    held = snk.DQNModel(12, 3, n_frames=2).use_adamw()
+    with pytest.raises(ValueError, match="mix"):
+        held.moments(torch.empty(held.total, device="cuda"))
+    out = snk.DeviceArray(held.total, np.float32)
+    held.moments(out)
+    assert not out.numpy().any()
+
+
+@pytest.mark.parametrize("param,grad,bits,copies,n", [
+    ("f32", "bf16", 32, "f16", 25_000_003), ("f32", "f32", 32, None, 25_000_003), ("bf16", "f32", 32, None, 25_000_003),
+    ("f16", "f16", 32, None, 30_000_001), ("bf16", "bf16", 8, None, 57_000_001), ("f32", "f16", 8, "bf16", 45_000_001),
+    ("f16", "f32", 8, None, 45_000_001)])
+def test_large_steps(snk, param, grad, bits, copies, n):
+    """More bytes than the caches hold take the accesses past them: the same bits as the halves, stepped
+    by handles of their own, get (but for v's codes, whose rounding goes by the place)."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    sizes = [n // 2 - 5, n - n // 2 + 5]
+    pb, ps = views(sizes, TT[param], gen, 0.1, 3)
+    gb, gs = views(sizes, TT[grad], gen, 0.01, 1)
+    cs = None if copies is None else [torch.zeros(s, dtype=TT[copies], device="cuda") for s in sizes]
+    halves = [[p.clone(), g.clone(), None if cs is None else torch.zeros_like(cs[i])] for i, (p, g) in enumerate(zip(ps, gs))]
+    how = dict(state_bits=bits, lr=1e-2, weight_decay=0.1, seed=3)
+    opt = snk.AdamW(ps, gs, copies=cs, **how)
+    opts = [snk.AdamW([p], [g], copies=None if c is None else [c], **how) for p, g, c in halves]
+    for steps in range(2 if bits == 32 else 1):
+        opt.step()
+        for o in opts:
+            o.step()
+    st = {k: torch.as_tensor(x, device="cuda") for k, x in opt.state().items()}
+    for i, (half, o) in enumerate(zip(halves, opts)):
+        assert torch.equal(ps[i], half[0])
+        assert cs is None or torch.equal(cs[i], half[2])
+        for k, x in o.state().items():
+            x = torch.as_tensor(x, device="cuda")
+            at = opt.starts[i] // (256 if "scale" in k else 1)
+            if k != "norm" and (k != "v" or bits == 32):
+                assert torch.equal(st[k][at:at + x.numel()], x), k
+    assert canaries(pb, sizes, 3) and canaries(gb, sizes, 1)
