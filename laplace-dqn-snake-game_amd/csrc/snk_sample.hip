@@ -27,7 +27,7 @@ constexpr int GP = PIECE / GROUP;
 constexpr int BP = 4;           // pieces of a block, the scan's unit of mass
 constexpr int BLOCK = BP * PIECE;
 constexpr int BINS = 2048;      // of a level of the radix search: 11 + 11 + 10 bits of the key
-constexpr int LIST = 1024;      // most candidates held in LDS
+constexpr int NUCLEUS_LIST = 512;   // candidates that top-p alone lists where no other search was run
 constexpr int NBINS = 1024;     // of the nucleus' mass over the distance from the top
 constexpr int NLIST = 512;      // most entries of the cut's bin that one split of a row lists
 constexpr int SPLITS = 16;      // most splits of a row
@@ -921,10 +921,6 @@ __device__ __forceinline__ int far_bin(float d) {
 __device__ __forceinline__ float far_edge(int b) {   // all in bins up to b are nearer, and nothing else is
     return b < BINS - 1 ? __uint_as_float((uint32_t)(b + 1 + ((127 - 12) << 6)) << 17) : INFINITY;
 }
-struct Total {
-    uint32_t count;
-    uint64_t mass;
-};
 
 // Bound by its chain of a dozen dependent steps between barriers, not by what it reads: 256 rows of
 // 131,072 bf16, whole, 7.8 us; 128 of 50,021, top-k 40, 9.5; 8 of 131,072 fp32 after the nucleus search
@@ -935,6 +931,9 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
     constexpr bool FUSED = OWN > 0;
     constexpr int NT = 64 * RW, BT = BINS / NT;   // threads; bins of each
     constexpr int REC = FUSED ? OWN : BP;         // pieces of a record of mass
+    // most candidates held in LDS, as many as leave room for the workgroups that the registers allow
+    constexpr int LIST = RW == 16 ? 4096 : RW == 8 ? 2048 : 1024;
+    static_assert(LIST * 4 <= BINS * 8, "group_list lies in mass");
     __shared__ uint64_t pow2[128];
     __shared__ uint64_t mass[BINS];
     __shared__ uint32_t count[BINS];
@@ -1085,36 +1084,106 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             const float near = by_q ? (__builtin_amdgcn_logf(s.q) * -0.69315f + 1e-4f) * (float)s.t : INFINITY;
             float edge = near;   // candidates are nearer; NaN for two infinities: top itself
             auto candidate = [&](float v) __attribute__((always_inline)) { return !(top - v >= edge); };
+            bool dense = false;   // candidates in most groups
             if (W.hard) {
                 edge = far_edge(0);
             } else if (cut) {
-                // the bin that the wanted-th largest maximum falls in: at least that many entries are as near
+                // the bin that the wanted-th largest of the counted maxima falls in: at least that many
+                // entries are as near
+                uint32_t all, wanted;
+                auto clear_counts = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                for (int b = 0; b < BT; ++b) count[b * NT + tid] = 0;
-                __syncthreads();
+                    for (int b = 0; b < BT; ++b) count[b * NT + tid] = 0;
+                    __syncthreads();
+                };
+                auto edge_by_counts = [&]() __attribute__((always_inline)) {
+                    if (tid == 0) found_bin = BINS - 1;
+                    __syncthreads();
+                    uint32_t c[BT], sum = 0;
+#pragma unroll
+                    for (int b = 0; b < BT; ++b) sum += c[b] = count[tid * BT + b];
+                    uint32_t ex = block_scan<RW, uint32_t>(sum, scan32, all);
+                    // top-p alone: a list that most distributions' nucleus fits into
+                    wanted = s.k < n ? (uint32_t)s.k : max(1u, min((uint32_t)NUCLEUS_LIST, all / 2));
+#pragma unroll
+                    for (int b = 0; b < BT; ++b) {
+                        if (ex < wanted && ex + c[b] >= wanted) found_bin = tid * BT + b;
+                        ex += c[b];
+                    }
+                    __syncthreads();
+                    return fminf(near, far_edge((int)found_bin));
+                };
+                clear_counts();
                 for (int g = g0; g < g1; ++g) {
                     const float t = top_of(g);
                     if (t != -INFINITY) atomicAdd(&count[far_bin(top - t)], 1u);
                 }
-                if (tid == 0) found_bin = BINS - 1;
-                __syncthreads();
-                uint32_t c[BT], sum = 0, all;
+                edge = edge_by_counts();
+                // Too few groups for that many entries, or so few that their maxima leave more than the
+                // list holds: of A groups, W with a larger maximum, -A ln(1 - W/A) entries are expected.
+                // Then by the maxima of 8, read again: one row of 131,072, top-k 2,000, 39 us against 115 by a
+                // radix search over the row, of 50,000, top-k 700 and top-p 0.9, 41 against 109.
+                if (s.k < n && n > LIST && wanted <= LIST &&
+                    (all <= wanted || (float)all * __logf(1.0f - (float)wanted / (float)all) < -0.85f * LIST)) {
+                    dense = true;
+                    clear_counts();
+                    for (int c = wave * BP; c < pieces; c += RW * BP) {
+                        float v[BP][8];
+                        load_pieces<BP>(x, mask, c * PIECE + lane * 8, n, v);
 #pragma unroll
-                for (int b = 0; b < BT; ++b) sum += c[b] = count[tid * BT + b];
-                uint32_t ex = block_scan<RW, uint32_t>(sum, scan32, all);
-                // top-p alone: a list that most distributions' nucleus fits into
-                const uint32_t wanted = s.k < n ? (uint32_t)s.k : max(1u, min((uint32_t)LIST / 2, all / 2));
+                        for (int p = 0; p < BP; ++p) {
+                            float t = v[p][0];
 #pragma unroll
-                for (int b = 0; b < BT; ++b) {
-                    if (ex < wanted && ex + c[b] >= wanted) found_bin = tid * BT + b;
-                    ex += c[b];
+                            for (int e = 1; e < 8; ++e) t = fmaxf(t, v[p][e]);
+                            if (t != -INFINITY) atomicAdd(&count[far_bin(top - t)], 1u);
+                        }
+                    }
+                    edge = edge_by_counts();
                 }
-                __syncthreads();
-                edge = fminf(near, far_edge((int)found_bin));
-                // fewer groups than wanted entries: everything would be a candidate
+                // fewer maxima than wanted entries: everything would be a candidate
                 use_list = all >= wanted || n <= LIST || by_q;
             }
-            if (use_list) {
+            if (use_list && dense) {
+                // a run of pieces a wave: its candidates counted, then listed
+                const int run = (pieces + RW - 1) / RW, c0 = wave * run, c1 = min(c0 + run, pieces);
+                auto each_piece = [&](auto &&f) __attribute__((always_inline)) {   // f(8 entries, the first's index)
+                    for (int c = c0; c < c1; c += BP) {
+                        float v[BP][8];
+                        load_pieces<BP>(x, mask, c * PIECE + lane * 8, n, v);
+#pragma unroll
+                        for (int p = 0; p < BP; ++p)
+                            if (c + p < c1) f(v[p], (c + p) * PIECE + lane * 8);
+                    }
+                };
+                uint32_t own = 0;
+                each_piece([&](const float *v, int) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) own += candidate(v[e]);
+                });
+                own = wave_sum(own);
+                if (lane == 0) scan32[wave] = own;
+                __syncthreads();
+                const uint32_t owns = wave_scan(lane < RW ? scan32[lane] : 0u);
+                uint32_t at = wave ? read_lane(owns, wave - 1) : 0;
+                if (tid == 0) listed = read_lane(owns, RW - 1);
+                each_piece([&](const float *v, int i) __attribute__((always_inline)) {
+                    uint32_t in = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) in += candidate(v[e]);
+                    const uint32_t upto = wave_scan(in);
+                    uint32_t to = at + upto - in;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (candidate(v[e])) {
+                            if (to < LIST) {
+                                list_key[to] = key_of(v[e]);
+                                list_at[to] = (uint32_t)(i + e);
+                            }
+                            ++to;
+                        }
+                    at += last_lane(upto);
+                });
+            } else if (use_list) {
                 // the groups that hold candidates, in order
                 uint32_t c = 0, ng;
                 for (int g = g0; g < g1; ++g) c += candidate(top_of(g));
@@ -1321,8 +1390,9 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         // prefix has k entries) or by mass (the last entry with less than `limit` before it). From
         // keys >= least, with above_mass over all of them. above_*: of the keys over the found one;
         // count_in: of the found one itself.
-        uint64_t above_mass = 0;
+        uint64_t above_mass = 0, all_mass = 0;
         uint32_t above_count = 0, count_in = 0;
+        bool found = true;   // false: by count, and there are no more than k entries; all_mass is theirs
         auto search = [&](bool by_mass, bool with_mass, uint32_t least, uint32_t k, double limit) __attribute__((always_inline)) {
             uint32_t prefix = 0;
             above_count = 0;
@@ -1352,6 +1422,12 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
                 }
                 uint64_t m_ex = above_mass + block_scan<RW, uint64_t>(m_sum, scan64, m_all);
                 uint32_t c_ex = above_count + block_scan<RW, uint32_t>(c_sum, scan32, c_all);
+                if (!by_mass && level == 0 && c_all <= k) {   // for all threads
+                    found = false;
+                    all_mass = m_all;
+                    __syncthreads();
+                    return 0u;
+                }
 #pragma unroll
                 for (int b = 0; b < BT; ++b) {
                     const int at = BINS - 1 - tid * BT - b;
@@ -1377,37 +1453,34 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             }
             return prefix;
         };
-        auto total_of = [&]() __attribute__((always_inline)) {   // entries and their mass
-            uint32_t c = 0;
+        auto mass_of_all = [&]() __attribute__((always_inline)) {
             uint64_t w = 0;
             each([&](float v, int) __attribute__((always_inline)) {
-                if (v == -INFINITY) return;
-                c += 1;
-                w += W.fixed(W.real(v));
+                if (v != -INFINITY) w += W.fixed(W.real(v));
             });
-            uint64_t w_all;
-            uint32_t c_all;
-            block_scan<RW, uint64_t>(w, scan64, w_all);
-            block_scan<RW, uint32_t>(c, scan32, c_all);
-            return Total{c_all, w_all};
+            return block_sum<RW, uint64_t>(w, scan64);
         };
         if (W.hard && s.greedy) {
             kt = key_of(top);
             nt = 1;
         } else if (cut && kt == 0) {
-            Total all = total_of();
-            if (from_list && !binned && s.k == n && (double)all.mass < limit_row) {   // the nucleus is not inside the list
-                from_list = false;
-                all = total_of();
-            }
-            uint64_t s1 = all.mass;
+            uint64_t s1 = 0;
             bool k_cut = false;
-            if (s.k < n && all.count > (uint32_t)s.k) {
-                above_mass = 0;
+            if (s.k < n) {
                 kt = search(false, s.p < 1.0f, 0, (uint32_t)s.k, 0.0);
-                nt = (uint32_t)s.k - above_count;
-                s1 = above_mass + nt * W.fixed(W.real(of_key(kt)));
-                k_cut = true;
+                k_cut = found;
+                if (k_cut) {
+                    nt = (uint32_t)s.k - above_count;
+                    s1 = above_mass + nt * W.fixed(W.real(of_key(kt)));
+                } else {
+                    s1 = all_mass;
+                }
+            } else {
+                s1 = mass_of_all();
+                if (from_list && !binned && (double)s1 < limit_row) {   // the nucleus is not inside the list
+                    from_list = false;
+                    s1 = mass_of_all();
+                }
             }
             if (s.p < 1.0f) {
                 // with a list, the entries behind it count in the limit only

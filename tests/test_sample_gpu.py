@@ -403,3 +403,22 @@ def test_rows_by_the_card(snk, n):
         check(snk, x[:10], u[:10], mask=mask, most_left_out=1, **how)
         for got in calls[1:]:
             assert (got != calls[0]).sum() <= 1, how   # whole rows' masses are added in another order
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [4097, 8192, 12345, 33000, 70001])
+def test_large_top_k(snk, dtype, n):
+    """Cuts that the maxima of 64 do not bound: by the maxima of 8, or by the whole row."""
+    for rows in (5, 300, 600):
+        x, u = logits(rows, n, dtype, n + rows)
+        x[1] = -torch.inf
+        x[2, 3000:] = -torch.inf
+        x[3] = torch.round(x[3])                 # many ties
+        x[4, ::2] = x[4, 0]
+        mask = torch.rand(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(n)) < 0.2
+        part = slice(0, 6)
+        for how in (dict(top_k=n // 64 + 1), dict(top_k=n // 64 - 3, top_p=0.9), dict(top_k=700), dict(top_k=1000, top_p=0.7),
+                    dict(top_k=1990, min_p=0.003), dict(top_k=2000, top_p=0.95, min_p=0.001), dict(top_k=4050), dict(top_k=n - 1)):
+            got = snk.sample_logits(x, u, mask=mask, **how)
+            assert torch.equal(got[part], snk.sample_logits(x[part], u[part], mask=mask, **how)), how
+            check(snk, x[part], u[part], mask=mask, most_left_out=2, **how)
