@@ -1081,7 +1081,8 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             // candidates: what can be in the cut, by the groups' maxima: bins of the distance from the
             // top up to here, and, where min-p is not to change the mass that top-p goes by, this near
             const bool by_q = s.q > 0.0f && s.p >= 1.0f;
-            const float near = by_q ? (__builtin_amdgcn_logf(s.q) * -0.69315f + 1e-4f) * (float)s.t : INFINITY;
+            // (never 0, however low the temperature: the top itself is nearer)
+            const float near = by_q ? fmaxf((__builtin_amdgcn_logf(s.q) * -0.69315f + 1e-4f) * (float)s.t, 0x1p-120f) : INFINITY;
             float edge = near;   // candidates are nearer; NaN for two infinities: top itself
             auto candidate = [&](float v) __attribute__((always_inline)) { return !(top - v >= edge); };
             bool dense = false;   // candidates in most groups

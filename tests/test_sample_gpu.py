@@ -422,3 +422,18 @@ def test_large_top_k(snk, dtype, n):
             got = snk.sample_logits(x, u, mask=mask, **how)
             assert torch.equal(got[part], snk.sample_logits(x[part], u[part], mask=mask, **how)), how
             check(snk, x[part], u[part], mask=mask, most_left_out=2, **how)
+
+
+@pytest.mark.parametrize("n", [3, 40, 600, 3000, 4097, 20000, 70001])
+def test_temperatures_at_the_ends(snk, n):
+    """The least and the largest temperatures that fp32 holds, under every filter."""
+    for t in (1e-45, 1e-38, 1e-20, 1e20, 3e38):
+        for how in (dict(), dict(min_p=0.3), dict(min_p=1.0), dict(top_k=3, min_p=0.3), dict(top_p=0.5), dict(top_k=2, top_p=0.5)):
+            for rows in (4, 300):
+                x, u = logits(rows, n, "f32", n)
+                got = snk.sample_logits(x, u, temperature=t, **how)
+                assert int(got.min()) >= 0 and int(got.max()) < n, (t, how)
+                if t < 1:
+                    assert torch.equal(got.long(), x.argmax(1)), (t, how)
+                else:
+                    check(snk, x[:4], u[:4], temperature=t, most_left_out=4, **how)
