@@ -637,6 +637,10 @@ __global__ __launch_bounds__(256) void sample_few_kernel(SampleArgs A) {
 // (28 bits): n = 16 54 us by pairs and 190 by bits, n = 64 130 and 190; bf16 (13 bits): n = 48 104 and
 // 111, n = 64 130 and 111.
 constexpr int PAIRS_A_BIT = 4;
+// Every so many bits of an fp32 search by mass, those that the keys still in question share are set at
+// once: 32,768 rows, top-p 0.9, n = 128 69 us against 115, n = 1,024 214 against 253. 16-bit keys have too
+// few bits for that (bf16, n = 1,024: 181 and 168).
+constexpr int NARROW = 4;
 // low bits that the keys of the type's positive values share, and those of its negative ones
 template <class T>
 constexpr int KEY_SHIFT = sizeof(T) == 4 ? 0 : std::is_same<T, __bf16>::value ? 16 : 13;
@@ -748,6 +752,27 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void sample_wave_kernel(Sa
         for (int e = 0; e < E; ++e) m += key[e] >= at ? w[e] : 0;
         return over_waves(wave_sum(m), before);
     };
+    // the row's largest and smallest of two values a lane
+    auto span_over_waves = [&](uint32_t &most, uint32_t &least) __attribute__((always_inline)) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            most = max(most, (uint32_t)__shfl_xor((int)most, o));
+            least = min(least, (uint32_t)__shfl_xor((int)least, o));
+        }
+        if constexpr (NW > 1) {
+            if (lane == 0) slots[turn][wave] = (uint64_t)most << 32 | least;
+            __syncthreads();
+#pragma unroll
+            for (int o = 0; o < NW; ++o) {
+                const uint64_t m = slots[turn][o];
+                most = max(most, (uint32_t)(m >> 32));
+                least = min(least, (uint32_t)m);
+            }
+            turn ^= 1;
+        }
+        most = (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
+        least = (uint32_t)__builtin_amdgcn_readfirstlane((int)least);
+    };
     auto key_weight = [&](uint32_t k) __attribute__((always_inline)) { return W.fixed(W.real(logit(k))); };
     // the first k of a wave's entries, one a lane in index order (key 0: none), their top-p and the
     // answer: each entry's rank and the mass before it by comparing it with the m others
@@ -851,8 +876,9 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void sample_wave_kernel(Sa
                 kt = first;
                 nt = 1;
             } else {
-                uint32_t t = common;
-                uint64_t above = 0;
+                uint32_t t = common, over = first + 1;   // the cut's key is one of t..over - 1
+                uint64_t above = 0;                      // mass from `over` on
+                int steps = 0;
                 for (int b = bits - 1; b >= 0; --b) {
                     const uint32_t at = t | 1u << b;
                     if (k_cut && at <= kt) {
@@ -860,10 +886,25 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void sample_wave_kernel(Sa
                         continue;
                     }
                     const uint64_t m = mass_not_below(at);
-                    if ((double)m >= limit)
+                    if ((double)m >= limit) {
                         t = at;
-                    else
+                    } else {
                         above = m;
+                        over = at;
+                    }
+                    if (SHIFT == 0 && ++steps % NARROW == 0) {
+                        uint32_t most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const bool in = key[e] >= t && key[e] < over;
+                            most = max(most, in ? key[e] : 0u);
+                            least = min(least, in ? key[e] : 0xFFFFFFFFu);
+                        }
+                        span_over_waves(most, least);
+                        const uint32_t differ = most ^ least;
+                        b = differ ? 32 - __clz((int)differ) : 0;
+                        t = most >> b << b;   // a key is in question always, and four bits are known: b <= 28
+                    }
                 }
                 // tie j stays while above + j w < limit
                 const uint64_t wt = key_weight(t);
