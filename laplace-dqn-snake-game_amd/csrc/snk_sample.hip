@@ -1899,6 +1899,14 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
         return;
     }
     const bool nucleus = (A.p_dev || A.top_p < 1.0f) && (A.k_dev || A.top_k == 0 || A.top_k >= A.n);
+    if constexpr (sizeof(T) == 2)
+        if (fused(A.rows, A.n) && nucleus && !A.k_dev) {
+            // top-p alone has no bound by the groups: in the registers of sixteen waves, 128 rows of 8,192
+            // bf16 23 us against 34, fp16 25 (fp32's keys have twice the bits: 37 against 34)
+            sample_wave_kernel<T, 8, 16><<<(unsigned)A.rows, 1024, 0, s>>>(A);
+            launch_check("sample_wave_kernel");
+            return;
+        }
     if (fused(A.rows, A.n)) {
         sample_row_kernel<T, 16, 1><<<(unsigned)A.rows, 1024, 0, s>>>(A);
         launch_check("sample_row_kernel");
