@@ -20,7 +20,7 @@ namespace snk {
 
 constexpr int BLK = 256;        // elements of a wave's block = the 8-bit states' block
 constexpr int CH = 1024;        // elements of a workgroup's chunk
-constexpr int NORM_WG = 2048;   // most workgroups (= partial sums) of the norm pass
+constexpr int NORM_WG = 1024;   // most workgroups (= partial sums) of the norm pass
 // From this many bytes of parameters, gradients and moments on, a step reads and writes past the
 // caches: nothing of them lives there until the next step, and what is written evicts nothing that is
 // still to be read. 32-bit states: 159 us against 180 at 537 MB, 78 against 68 at 268 MB.
@@ -180,7 +180,7 @@ __device__ __forceinline__ void begin_step(AdamCtl *ctl, const AdamHyper &H) {
 }
 __global__ void adamw_begin_kernel(AdamCtl *__restrict__ ctl, AdamHyper H) { begin_step(ctl, H); }
 
-// sum of a value over a workgroup of 256, in one order, a wave's by lane moves; sh: 4 values
+// sum of a value over a workgroup of W waves, in one order, a wave's by lane moves; sh: W values
 template <int CTRL, int ROWS>
 __device__ __forceinline__ double plus_lane(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -188,7 +188,8 @@ __device__ __forceinline__ double plus_lane(double v) {
     const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
     return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ double sum256(double v, double *sh) {
+template <int W>
+__device__ __forceinline__ double sum_group(double v, double *sh) {
     v = plus_lane<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8: within 16 lanes
     v = plus_lane<0x112, 0xf>(v);
     v = plus_lane<0x114, 0xf>(v);
@@ -197,20 +198,24 @@ __device__ __forceinline__ double sum256(double v, double *sh) {
     v = plus_lane<0x143, 0xc>(v);
     if ((threadIdx.x & 63) == 63) sh[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+    double sum = sh[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) sum += sh[w];
+    return sum;
 }
 
 // N: partial sums of (s g)^2 in fp64 (fp32 squares overflow above 1.8e19 and lose the small ones).
 // A wave a chunk, 16 elements a lane in 16-byte reads, the next chunk's record read ahead; bound by
 // HBM's reads of g (133 M bf16: 73 us, 3.7 TB/s). The partials are added by the step itself or by adamw_parts_kernel: a count of
-// arrivals costs more, 25 ns a workgroup (27 us for 1,079 of them).
-template <class GT>
-__global__ __launch_bounds__(256) void adamw_norm_kernel(const AdamChunk *__restrict__ chunks, int64_t n_chunks,
+// arrivals costs more, 25 ns a workgroup (27 us for 1,079 of them). W waves a workgroup.
+template <class GT, int W>
+__global__ __launch_bounds__(64 * W) void adamw_norm_kernel(const AdamChunk *__restrict__ chunks, int64_t n_chunks,
                                                          double *__restrict__ part, AdamCtl *__restrict__ ctl, AdamHyper H) {
     constexpr int V = 16 / sizeof(GT), N = CH / (64 * V);
-    __shared__ double sh[4];
+    __shared__ double sh[W];
     const int lane = threadIdx.x & 63;
-    const int64_t first = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), stride = (int64_t)gridDim.x * 4;
+    const int64_t first = (int64_t)blockIdx.x * W + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t stride = (int64_t)gridDim.x * W;
     double sum = 0.0;
     const float gs = H.gscale;
     auto add = [&](float g) {
@@ -241,7 +246,7 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(const AdamChunk *__rest
         g = g_next;
         n = n_next;
     }
-    sum = sum256(sum, sh);
+    sum = sum_group<W>(sum, sh);
     if (threadIdx.x == 0) {
         part[blockIdx.x] = sum;
         if (blockIdx.x == 0) begin_step(ctl, H);
@@ -261,7 +266,7 @@ __global__ __launch_bounds__(256) void adamw_parts_kernel(const double *__restri
     __shared__ double sh[4];
     double sum = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) sum += part[i];
-    sum = sum256(sum, sh);
+    sum = sum_group<4>(sum, sh);
     if (threadIdx.x == 0) ctl->skip = clip_factor(H, sum, ctl->norm, ctl->gmul) ? 0 : 1;
 }
 
@@ -288,14 +293,17 @@ __device__ __forceinline__ AdamStep this_step(const AdamArgs &A) {
 }
 
 // the factor of the gradients, s c; false where the step is skipped. Workgroup 0 records N.
-__device__ __forceinline__ bool grad_factor(const AdamArgs &A, double *sh, float &gmul) {
+__device__ __forceinline__ double own_part(const AdamArgs &A) {   // before what takes longer to arrive
+    return (int)threadIdx.x < A.n_part ? A.part[threadIdx.x] : 0.0;
+}
+__device__ __forceinline__ bool grad_factor(const AdamArgs &A, double part, double *sh, float &gmul) {
     gmul = A.H.gscale;
     if (A.n_part == 0) return true;
     if (A.n_part < 0) {
         gmul = A.ctl->gmul;
         return A.ctl->skip == 0;
     }
-    const double sum = sum256((int)threadIdx.x < A.n_part ? A.part[threadIdx.x] : 0.0, sh);
+    const double sum = sum_group<4>(part, sh);
     float norm;
     const bool fine = clip_factor(A.H, sum, norm, gmul);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -344,13 +352,14 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamArgs A) {
     const int i = wave * BLK + lane * 4;
     const bool whole = (wave + 1) * BLK <= T.n;
     float *ms = (float *)A.m + T.place, *vs = (float *)A.v + T.place;
+    const double part = own_part(A);
     Pack<float, 4> mq, vq;
     mq.template load<NT>(ms + i);   // padded: always whole
     vq.template load<NT>(vs + i);
     const Pack<PT, 4> pq = load4<NT>((const PT *)T.p, i, T.n, whole);
     const Pack<GT, 4> gq = load4<NT>((const GT *)T.g, i, T.n, whole);
     float gmul;
-    if (!grad_factor(A, sh, gmul) || mine > last) return;
+    if (!grad_factor(A, part, sh, gmul) || mine > last) return;
     float p[4], m[4], v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -383,6 +392,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     const uint64_t key = splitmix64(A.H.seed ^ ((uint64_t)now.t * 0xD1B54A32D192ED03ULL));   // rng_hash's first half
     const int64_t block = T.place / BLK + wave;
     SNK_GLOBAL uint32_t *mcs = (SNK_GLOBAL uint32_t *)A.m + block * 64, *vcs = (SNK_GLOBAL uint32_t *)A.v + block * 64;
+    const double part = own_part(A);
     uint32_t mc, vc;
     if (NT) {
         mc = __builtin_nontemporal_load(mcs + lane);
@@ -397,7 +407,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     level[threadIdx.x] = v_level((float)threadIdx.x);
     const uint64_t h = splitmix64(key ^ (uint64_t)(block * 64 + lane));
     float gmul;
-    const bool go = grad_factor(A, sh, gmul);
+    const bool go = grad_factor(A, part, sh, gmul);
     __syncthreads();
     if (!go || mine > last) return;
     float p[4], m[4], v[4], mmax = 0.0f, vmax = 0.0f;
@@ -723,10 +733,17 @@ void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s) {
     H.copy_dtype = c.copy_dtype;
     H.seed = c.seed;
     if (c.max_grad_norm > 0 && h->n_chunks > 0) {
-        const int64_t waves = (h->n_chunks + 3) / 4;   // in workgroups of four
-        int parts = (int)std::min<int64_t>(waves, waves <= 4 * FEW_PARTS ? FEW_PARTS : NORM_WG);
+        // a chunk a wave as long as the step can add the partial sums itself: workgroups of four waves,
+        // or of eight (1.1 M elements: 14.6 us a step against 15.7; 490 k: 10.0 against 9.8)
+        const bool eight = h->n_chunks > 4 * FEW_PARTS;
+        const int64_t groups = eight ? (h->n_chunks + 7) / 8 : (h->n_chunks + 3) / 4;
+        int parts = (int)std::min<int64_t>(groups, groups <= 2 * FEW_PARTS ? FEW_PARTS : NORM_WG);
         with_type(c.grad_dtype, [&](auto g) {
-            adamw_norm_kernel<decltype(g)><<<(unsigned)parts, 256, 0, s>>>(h->chunks, h->n_chunks, h->part, h->ctl, H);
+            using GT = decltype(g);
+            if (eight)
+                adamw_norm_kernel<GT, 8><<<(unsigned)parts, 512, 0, s>>>(h->chunks, h->n_chunks, h->part, h->ctl, H);
+            else
+                adamw_norm_kernel<GT, 4><<<(unsigned)parts, 256, 0, s>>>(h->chunks, h->n_chunks, h->part, h->ctl, H);
         });
         launch_check("adamw_norm_kernel");
         if (parts > FEW_PARTS) {
