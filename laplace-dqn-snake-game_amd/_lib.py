@@ -456,8 +456,9 @@ def call_on(device, name: str, *args) -> None:
     if device is None:
         call(name, *args)
         return
-    if not _torch_calls:
-        _torch_calls.extend(_find_torch_calls())
+    global _torch_calls
+    if _torch_calls is None:
+        _torch_calls = _find_torch_calls()   # the same for every thread that gets here
     current, raw_stream = _torch_calls
     index = device.index
     if current() != index:
@@ -478,7 +479,7 @@ def call_on(device, name: str, *args) -> None:
 
 
 _slots = threading.local()   # where snk_swap_stream writes: made once a thread
-_torch_calls: list = []
+_torch_calls = None
 
 
 def _find_torch_calls():

@@ -24,6 +24,8 @@ class SampleCfg(C.Structure):
 
 
 _CFG = struct.Struct("=iififfQQQQ")   # SampleCfg's bytes
+_SETTINGS = (("temperature", "f32"), ("top_k", "i32"), ("top_p", "f32"), ("min_p", "f32"))
+_NONE = (0, 0, 0, 0)
 
 
 def _rows_of(x, b, what):
@@ -69,10 +71,11 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
             ldm = 0
         _lib.same_device([mb], device)
         m_ptr = mb.ptr
-    numbers, arrays = [temperature, top_k, top_p, min_p], [0, 0, 0, 0]
-    for i, (value, what, kind) in enumerate(((temperature, "temperature", "f32"), (top_k, "top_k", "i32"),
-                                             (top_p, "top_p", "f32"), (min_p, "min_p", "f32"))):
-        if not isinstance(value, (float, int)):
+    numbers, arrays = [temperature, top_k, top_p, min_p], _NONE
+    for i, value in enumerate(numbers):
+        if value.__class__ is not float and not isinstance(value, (float, int)):
+            what, kind = _SETTINGS[i]
+            arrays = list(arrays)
             arrays[i] = _lib.vector_ptr(value, what, kind, rows, device)
             numbers[i] = 0 if kind == "i32" else 1.0
     cfg = _CFG.pack(_CFG.size, dtype, *numbers, *arrays)

@@ -437,3 +437,42 @@ def test_temperatures_at_the_ends(snk, n):
                     assert torch.equal(got.long(), x.argmax(1)), (t, how)
                 else:
                     check(snk, x[:4], u[:4], temperature=t, most_left_out=4, **how)
+
+
+def test_threads_at_once(snk):
+    """Two operators on threads and streams of their own: each call keeps its thread's stream."""
+    import threading
+    x, u = logits(64, 3000, "bf16", 1)
+    p0, g = torch.randn(50_001, device="cuda"), torch.randn(50_001, device="cuda")
+    want_index, want_p = snk.sample_logits(x, u, top_k=20, top_p=0.9), p0.clone()
+    same = snk.AdamW([want_p], [g], state_bits=8)
+    for _ in range(20):
+        same.step()
+    torch.cuda.synchronize()
+    errors = []
+
+    def run(which):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                if which % 2:
+                    for _ in range(50):
+                        got = snk.sample_logits(x, u, top_k=20, top_p=0.9)
+                    stream.synchronize()
+                    assert torch.equal(got, want_index)
+                else:
+                    p = p0.clone()
+                    opt = snk.AdamW([p], [g], state_bits=8)
+                    for _ in range(20):
+                        opt.step()
+                    stream.synchronize()
+                    assert torch.equal(p, want_p)
+        except BaseException as e:   # noqa: BLE001 - reported by the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
