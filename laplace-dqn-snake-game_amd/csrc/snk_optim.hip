@@ -240,8 +240,21 @@ __global__ __launch_bounds__(64 * W) void adamw_norm_kernel(const AdamChunk *__r
             for (int j = 0; j < N; ++j)
 #pragma unroll
                 for (int e = 0; e < V; ++e) add(q[j].get(e));
-        } else {
-            for (int k = lane; k < n; k += 64) add((float)((const SNK_GLOBAL GT *)g)[k]);
+        } else {   // whole vectors and the rest, all in flight at once
+            Pack<GT, V> q[N];
+            const int rest = n % V;
+            GT x{};
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                q[j].q = 0;
+                if ((j * 64 + lane + 1) * V <= n) q[j].load(g + (j * 64 + lane) * V);
+            }
+            if (lane < rest) x = ((const SNK_GLOBAL GT *)g)[n - rest + lane];
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) add(q[j].get(e));
+            add((float)x);
         }
         g = g_next;
         n = n_next;
