@@ -32,9 +32,11 @@ constexpr int NBINS = 1024;     // of the nucleus' mass over the distance from t
 constexpr int NLIST = 512;      // most entries of the cut's bin that one split of a row lists
 constexpr int SPLITS = 16;      // most splits of a row
 
-struct SampleHead {             // the nucleus search's result
-    uint64_t above;             // mass over the bin
-    int32_t bin, ok;
+struct SampleHead {             // the nucleus search's results
+    double sum;                 // by sample_bins_kernel: the row's mass in units, the largest entry,
+    float top, step;            // bins a unit of distance
+    int32_t fine, ok;           // a finite top and a mass to go by; a bin was found
+    uint64_t above;             // by sample_kept_kernel: mass over the bin
 };
 struct SampleArgs {
     const void *x;
@@ -466,6 +468,13 @@ __global__ __launch_bounds__(1024) void sample_bins_kernel(SampleArgs A, int blo
     mass[tid] = 0;
     __syncthreads();
     const Nucleus N = nucleus(A, s, (LdsTable)pow2, r, blocks);
+    if (part == 0 && tid == 0) {
+        SampleHead &head = A.heads[r - A.row0];
+        head.sum = N.sum;
+        head.top = N.top;
+        head.step = N.step;
+        head.fine = N.ok;
+    }
     if (!N.ok) return;
     const Weight W = weight(A, s, (LdsTable)pow2, N.top);
     for (; c < end; c += NW) {
@@ -503,6 +512,8 @@ __global__ __launch_bounds__(1024) void sample_kept_kernel(SampleArgs A, int blo
     if (part * per + wave < end) raw.load(x, mask, (part * per + wave) * PIECE + lane * 8, A.n);
     uint64_t m = 0, all;   // the bin of this thread, from the top
     const uint64_t *bins = A.bins + local * A.splits * NBINS + tid;
+    const SampleHead &head = A.heads[local];
+    const Nucleus N{head.top, head.step, head.sum, head.fine != 0};
     if (A.splits == 1) {
         m = bins[0];
     } else {   // all loads in flight at once: 10,000 cycles one after another
@@ -518,7 +529,6 @@ __global__ __launch_bounds__(1024) void sample_kept_kernel(SampleArgs A, int blo
         listed = 0;
     }
     __syncthreads();
-    const Nucleus N = nucleus(A, s, (LdsTable)pow2, r, blocks);
     if (N.ok) {
         const double limit = (double)s.p * N.sum;
         const uint64_t above = block_scan<NW, uint64_t>(m, scan, all);
@@ -529,7 +539,10 @@ __global__ __launch_bounds__(1024) void sample_kept_kernel(SampleArgs A, int blo
     }
     __syncthreads();
     const int cut = cut_bin;
-    if (part == 0 && tid == 0) A.heads[local] = SampleHead{cut < 0 ? 0 : cut_above, cut, cut >= 0};
+    if (part == 0 && tid == 0) {   // what no other workgroup reads yet
+        A.heads[local].above = cut < 0 ? 0 : cut_above;
+        A.heads[local].ok = cut >= 0;
+    }
     if (cut < 0) return;
     const Weight W = weight(A, s, (LdsTable)pow2, N.top);
     const double q = (double)s.q;
@@ -1005,6 +1018,19 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
     const int pieces = (n + PIECE - 1) / PIECE, records = (pieces + REC - 1) / REC, groups = records * REC * GP;
     if (tid < 128) pow2[tid] = POW2[tid];
     if (tid == 0) listed = 0;
+    const int per = (records + NT - 1) / NT, segs = (records + per - 1) / per;   // records a segment, segments
+
+    // the nucleus search's results: loaded before what takes longer
+    const int64_t local = blockIdx.x;
+    SampleHead head{};
+    uint32_t in_split = 0;
+    uint64_t kept_above = 0;
+    if (!FUSED && A.heads && s.nucleus(n)) {
+        head = A.heads[local];
+        in_split = lane < A.splits ? A.listed[local * A.splits + lane] : 0;
+        if (tid < segs)
+            for (int c = tid * per; c < min((tid + 1) * per, records); ++c) kept_above += A.kept[local * records + c];
+    }
 
     const float *tops;
     const double *masses;
@@ -1051,11 +1077,10 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
     }
     const Weight W = weight(A, s, (LdsTable)pow2, top);
     const double q = (double)s.q;
-    const int per = (records + NT - 1) / NT, segs = (records + per - 1) / per;   // records a segment, segments
 
     // the whole row's mass by segment, from the records
     double seg_sum = 0.0, sum_ex = 0.0, row_sum = 0.0;
-    if (s.whole(n)) {
+    if (s.whole(n) && !head.ok) {
         if (tid < segs)
             for (int c = tid * per; c < min((tid + 1) * per, records); ++c) {
                 float t;
@@ -1093,15 +1118,13 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         seg = (int)found_bin;
         base_real = found_sum;
     } else {
-        const double limit_row = (double)s.p * row_sum * A.unit;   // top-p alone, in units
+        const double limit_row = (double)s.p * (head.ok ? head.sum : row_sum * A.unit);   // top-p alone, in units
         bool use_list = true, binned = false;   // binned: the list is the cut's bin, the rest is above it
         uint64_t above_list = 0;
         if (!FUSED && A.heads && s.nucleus(n) && !W.hard) {
-            const int64_t local = blockIdx.x;
-            const SampleHead head = A.heads[local];
             bool fits = head.ok != 0;
             if (fits) {   // SPLITS <= 64: a lane a split, every wave for itself
-                const uint32_t c = lane < A.splits ? A.listed[local * A.splits + lane] : 0;
+                const uint32_t c = in_split;
                 const uint32_t in = wave_scan(c), m = last_lane(in);
                 fits = !__ballot(c > NLIST) && m <= LIST;
                 for (int k = wave; k < A.splits && fits; k += RW) {
@@ -1349,9 +1372,10 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         bool from_list = m <= LIST;
         constexpr int PAIRS = 256;
         if (cut && m <= PAIRS) {
-            // each candidate's rank and the mass before it, by comparing all pairs: four threads a
-            // candidate, sixteen bytes of LDS a comparison, no branches (350 cycles a comparison with them)
-            constexpr int AT_ONCE = NT / 4, ROUNDS = PAIRS / AT_ONCE;   // candidates a round
+            // each candidate's rank and the mass before it, by comparing all pairs: four to sixteen threads
+            // a candidate, sixteen bytes of LDS a comparison, no branches (350 cycles a comparison with them)
+            constexpr int AT_ONCE = NT / 4, ROUNDS = PAIRS / AT_ONCE;   // candidates a round, of four threads
+            const int shift = m * 16 <= NT ? 4 : m * 8 <= NT ? 3 : 2, others = 1 << shift, mine = tid & (others - 1);
             uint4 *const cand = (uint4 *)mass;   // key, index, weight
             if (tid < (int)m) {
                 const uint64_t w = W.fixed(W.real(of_key(list_key[tid])));
@@ -1367,24 +1391,24 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             bool own[ROUNDS];   // the thread that answers for a candidate
 #pragma unroll
             for (int o = 0; o < ROUNDS; ++o) {
-                const uint32_t j = o * AT_ONCE + (tid >> 2);
+                const uint32_t j = o * AT_ONCE + (tid >> shift);
                 rank[o] = key[o] = 0;
                 before[o] = 0;
-                own[o] = (tid & 3) == 0 && j < m;
+                own[o] = mine == 0 && j < m;
                 if (o * AT_ONCE >= (int)m) continue;
                 const uint4 me = cand[min(j, m - 1)];
                 key[o] = me.x;
 #pragma unroll 4
-                for (uint32_t i = tid & 3; i < m; i += 4) {
+                for (uint32_t i = mine; i < m; i += others) {
                     const uint4 c = cand[i];
                     const bool first = (c.x > me.x) | ((c.x == me.x) & (c.y < me.y));
                     rank[o] += first;
                     before[o] += first ? c.z | (uint64_t)c.w << 32 : 0;
                 }
-                rank[o] += __shfl_xor(rank[o], 1);
-                rank[o] += __shfl_xor(rank[o], 2);
-                before[o] += __shfl_xor(before[o], 1);
-                before[o] += __shfl_xor(before[o], 2);
+                for (int d = 1; d < others; d <<= 1) {
+                    rank[o] += __shfl_xor(rank[o], d);
+                    before[o] += __shfl_xor(before[o], d);
+                }
                 s1 += own[o] && rank[o] < (uint32_t)s.k ? me.z | (uint64_t)me.w << 32 : 0;
             }
             double limit = limit_row;
@@ -1578,10 +1602,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
         const double wt = bounded ? W.real(of_key(kt)) : 0.0;
         const uint64_t wtie = wt >= q ? W.fixed(wt) : 0;
         if (from_list) {
-            uint64_t w = 0;
-            if (binned && tid < segs)
-                for (int c = tid * per; c < min((tid + 1) * per, records); ++c) w += A.kept[(int64_t)blockIdx.x * records + c];
-            seg_mass[tid] = w;
+            seg_mass[tid] = binned ? kept_above : 0;
             seg_ties[tid] = 0;
             __syncthreads();
             each([&](float v, int i) __attribute__((always_inline)) {
