@@ -446,7 +446,7 @@ __device__ __forceinline__ Nucleus nucleus(const SampleArgs &A, const SampleRow 
 }
 
 // A workgroup a split of a row, a wave a piece: its mass by bins. Rows are split until the card has 1,024
-// workgroups, a row into 16 at most (8 rows of 131,072 fp32: 6.7 us, the kernel after it 9.6). Bound by
+// workgroups, a row into 16 at most (8 rows of 131,072 fp32: 6.9 us, the kernel after it 8.7). Bound by
 // the LDS atomics of neighbours that meet in one bin and, with few rows, by one wave's chain of steps.
 constexpr int NW = 16, NTH = 64 * NW;
 static_assert(NBINS == NTH && NW % BP == 0, "a bin a thread, whole blocks a round");
@@ -977,7 +977,7 @@ __device__ __forceinline__ float far_edge(int b) {   // all in bins up to b are 
 }
 
 // Bound by its chain of a dozen dependent steps between barriers, not by what it reads: 256 rows of
-// 131,072 bf16, whole, 7.8 us; 128 of 50,021, top-k 40, 9.5; 8 of 131,072 fp32 after the nucleus search
+// 131,072 bf16, whole, 7.8 us; 128 of 50,021, top-k 40, 9.6; 8 of 131,072 fp32 after the nucleus search
 // 12; 512 of 32,003, min-p 0.05, with 8 waves each 14 (4 us more with 16).
 // OWN: pieces a wave scans here, 0: sample_scan_kernel's records
 template <class T, int RW, int OWN>
