@@ -142,15 +142,15 @@ def _prepare_adamw(case, seed):
         state |= dict(m=m, v=v)
     if own:
         import snake_amd
-        params, grads = ([x[at:at + s] for at, s in zip(starts, sizes)] for x in (p, g))
-        opt = snake_amd.AdamW(params, grads, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=wds, state_bits=case["bits"],
+        params = [p[at:at + s] for at, s in zip(starts, sizes)]
+        opt = snake_amd.AdamW(params, lr=LR, betas=(B1, B2), eps=EPS, weight_decay=wds, state_bits=case["bits"],
                               max_grad_norm=case["clip"], seed=state["seed"])
         view = {k: torch.as_tensor(x, device="cuda") for k, x in opt.state().items()}
         for name, key in (("m", "m"), ("v", "v"), ("m_scale", "ms"), ("v_scale", "vs")):
             if name in view:
                 view[name].copy_(state[key])
         opt.steps = STEPS
-        state |= dict(opt=opt, view=view)
+        state |= dict(opt=opt, view=view, grads=[g[at:at + s] for at, s in zip(starts, sizes)])
         if case["bits"] == 8:
             state["values"] = [torch.empty(total, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
     return state
@@ -285,7 +285,7 @@ def run(state):
         if not own:
             return _plain_adamw(state)
         opt = state["opt"]
-        opt.step()
+        opt.step(state["grads"])
         out = dict(p=state["p"], m=state["view"]["m"], v=state["view"]["v"])
         if case["bits"] == 8:
             opt.moments(*state["values"])
