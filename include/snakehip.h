@@ -291,7 +291,7 @@ typedef struct snk_adamw_s *snk_adamw;
 typedef struct {
     int32_t struct_size;   /* = sizeof(snk_adamw_cfg_t) = 64 */
     int32_t param_dtype;   /* SNK_F32 / SNK_BF16 / SNK_F16 */
-    int32_t grad_dtype;    /* SNK_F32 / SNK_BF16 / SNK_F16 */
+    int32_t grad_dtype;    /* SNK_F32 / SNK_BF16 / SNK_F16: of the gradients that are bound */
     int32_t copy_dtype;    /* 16-bit type of the optional rounded copies of p, or -1 */
     int32_t state_bits;    /* 32 or 8 */
     float max_grad_norm;   /* 0: no norm; > 0 (may be inf): norm, clipping, and a step whose norm is
@@ -309,12 +309,16 @@ typedef struct {
 int snk_adamw_create(snk_adamw *out, int32_t n, const int64_t *sizes_host, const float *weight_decay_host,
                      const snk_adamw_cfg_t *cfg);
 int snk_adamw_destroy(snk_adamw h);
-/* the tensors' device addresses, contiguous, element-aligned: params (updated), grads, and copies
- * (NULL unless copy_dtype >= 0). Refused where a tensor that is written overlaps another one.
+/* the tensors' device addresses, contiguous, element-aligned: params (updated), grads (NULL: every
+ * step brings its own, snk_adamw_step_grads), and copies (NULL unless copy_dtype >= 0). Refused where a tensor that is written overlaps another one.
  * Enqueued like any work, and kept: later steps (an earlier captured one's replays too) use the last
  * bind. Refused, as snk_adamw_create is, while the stream is being captured. */
 int snk_adamw_bind(snk_adamw h, void *const *params_dev, const void *const *grads_dev, void *const *copies_dev);
 int snk_adamw_step(snk_adamw h, float lr, float grad_scale);
+/* the same step on these gradients of grad_dtype, whatever is bound, which stays: n device addresses,
+ * read by the host during the call (a captured step keeps them, as it does lr and grad_scale).
+ * Refused where one overlaps a parameter or copy. */
+int snk_adamw_step_grads(snk_adamw h, int32_t grad_dtype, const void *const *grads_dev, float lr, float grad_scale);
 /* places in the state layout; starts_host (optional, n): each tensor's */
 int snk_adamw_layout(snk_adamw h, int64_t *total_out, int64_t *starts_host);
 int snk_adamw_state_ptr(snk_adamw h, int32_t which, void **dev_out, int64_t *bytes_out);

@@ -117,6 +117,7 @@ _PROTOS = {
     "snk_adamw_destroy": [vp],
     "snk_adamw_bind": [vp, vp, vp, vp],
     "snk_adamw_step": [vp, f32, f32],
+    "snk_adamw_step_grads": [vp, i32, vp, f32, f32],
     "snk_adamw_layout": [vp, P(i64), vp],
     "snk_adamw_state_ptr": [vp, i32, P(vp), P(i64)],
     "snk_adamw_moments": [vp, i32, vp, vp],
@@ -394,14 +395,14 @@ class Buffer:
 # numpy has no bfloat16: a uint16 DeviceArray holds its bits
 _NP_TYPES = {"float32": "f32", "float16": "f16", "uint16": "bf16", "int32": "i32", "uint8": "u8", "bool": "u8"}
 _torch = None
-_TORCH_TYPES: dict = {}
+TORCH_TYPES: dict = {}
 
 
 def torch_module():
     global _torch
     if _torch is None:
         import torch
-        _TORCH_TYPES.update({torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16", torch.int32: "i32",
+        TORCH_TYPES.update({torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16", torch.int32: "i32",
                              torch.uint8: "u8", torch.bool: "u8"})
         _torch = torch
     return _torch
@@ -420,7 +421,7 @@ def device_buffer(x, what: str, contiguous: bool = True) -> Buffer:
         if contiguous and not x.is_contiguous():
             raise ValueError(f"{what}: a tensor that is not contiguous")
         b.ptr, b.shape, b.device, b.size = x.data_ptr(), x.shape, x.device, x.numel()
-        kind = _TORCH_TYPES.get(x.dtype)
+        kind = TORCH_TYPES.get(x.dtype)
     else:
         raise TypeError(f"{what}: {type(x).__name__} is neither a DeviceArray nor a torch tensor")
     if kind is None:
@@ -431,7 +432,7 @@ def device_buffer(x, what: str, contiguous: bool = True) -> Buffer:
 
 def vector_ptr(x, what: str, kind: str, size: int, device) -> int:
     """Address of a contiguous device tensor of `size` elements of one type, on `device`."""
-    if device is not None and hasattr(x, "data_ptr") and _TORCH_TYPES.get(x.dtype) == kind and x.numel() == size \
+    if device is not None and hasattr(x, "data_ptr") and TORCH_TYPES.get(x.dtype) == kind and x.numel() == size \
             and x.device == device and x.is_contiguous():
         return x.data_ptr()
     b = device_buffer(x, what)   # says what is wrong

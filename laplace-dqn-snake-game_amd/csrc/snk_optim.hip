@@ -210,7 +210,8 @@ __device__ __forceinline__ double sum_group(double v, double *sh) {
 // arrivals costs more, 25 ns a workgroup (27 us for 1,079 of them). W waves a workgroup.
 template <class GT, int W>
 __global__ __launch_bounds__(64 * W) void adamw_norm_kernel(const AdamChunk *__restrict__ chunks, int64_t n_chunks,
-                                                         double *__restrict__ part, AdamCtl *__restrict__ ctl, AdamHyper H) {
+                                                            const void *const *__restrict__ given,
+                                                            double *__restrict__ part, AdamCtl *__restrict__ ctl, AdamHyper H) {
     constexpr int V = 16 / sizeof(GT), N = CH / (64 * V);
     __shared__ double sh[W];
     const int lane = threadIdx.x & 63;
@@ -225,12 +226,12 @@ __global__ __launch_bounds__(64 * W) void adamw_norm_kernel(const AdamChunk *__r
     const GT *g = nullptr;
     int n = 0;
     if (first < n_chunks) {
-        g = (const GT *)chunks[first].g;
+        g = grads_of<GT>(chunks[first], given);
         n = chunks[first].n;
     }
     for (int64_t c = first; c < n_chunks; c += stride) {
         const int64_t next = c + stride < n_chunks ? c + stride : first;
-        const GT *g_next = (const GT *)chunks[next].g;
+        const GT *g_next = grads_of<GT>(chunks[next], given);
         const int n_next = chunks[next].n;
         if (n == CH) {
             Pack<GT, V> q[N];
@@ -283,11 +284,18 @@ __global__ __launch_bounds__(256) void adamw_parts_kernel(const double *__restri
     if (threadIdx.x == 0) ctl->skip = clip_factor(H, sum, ctl->norm, ctl->gmul) ? 0 : 1;
 }
 
+// a chunk's gradients: where the call says, or as bound
+template <class GT>
+__device__ __forceinline__ const GT *grads_of(const AdamChunk &T, const void *const *given) {
+    return given ? (const GT *)given[T.tensor] + T.first : (const GT *)T.g;
+}
+
 struct AdamArgs {
     const AdamChunk *chunks;
     void *m, *v;
     float *ms, *vs;
     AdamCtl *ctl;
+    const void *const *given;   // this step's gradients, an address a tensor (nullptr: the chunks' own)
     const double *part;   // n_part partial sums of the norm (0: no norm, -1: ctl has its results)
     int n_part;
     bool counted;         // the host counts the steps: `step` holds, and ctl is to receive it
@@ -370,7 +378,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamArgs A) {
     mq.template load<NT>(ms + i);   // padded: always whole
     vq.template load<NT>(vs + i);
     const Pack<PT, 4> pq = load4<NT>((const PT *)T.p, i, T.n, whole);
-    const Pack<GT, 4> gq = load4<NT>((const GT *)T.g, i, T.n, whole);
+    const Pack<GT, 4> gq = load4<NT>(grads_of<GT>(T, A.given), i, T.n, whole);
     float gmul;
     if (!grad_factor(A, part, sh, gmul) || mine > last) return;
     float p[4], m[4], v[4];
@@ -415,7 +423,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
         vc = vcs[lane];
     }
     const Pack<PT, 4> pq = load4<NT>((const PT *)T.p, i, T.n, whole);
-    const Pack<GT, 4> gq = load4<NT>((const GT *)T.g, i, T.n, whole);
+    const Pack<GT, 4> gq = load4<NT>(grads_of<GT>(T, A.given), i, T.n, whole);
     const float ms0 = A.ms[block], vs0 = A.vs[block];
     level[threadIdx.x] = v_level((float)threadIdx.x);
     const uint64_t h = splitmix64(key ^ (uint64_t)(block * 64 + lane));
@@ -514,7 +522,7 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(AdamArgs A, int64_t 
 
 // tensor addresses into the device table, by value: safe inside a capture, where a host array
 // would be read again at every replay
-constexpr int BIND_N = 128;
+constexpr int BIND_N = 128, GIVEN_N = 384;   // 3 KB of arguments each
 struct BindArgs {
     void *p[BIND_N], *c[BIND_N];
     const void *g[BIND_N];
@@ -526,6 +534,13 @@ __global__ void adamw_bind_kernel(AdamTensor *__restrict__ tab, BindArgs b, int 
         tab[i].g = b.g[i];
         tab[i].c = b.c[i];
     }
+}
+struct GivenArgs {
+    const void *g[GIVEN_N];
+};
+__global__ __launch_bounds__(GIVEN_N) void adamw_given_kernel(const void **__restrict__ given, GivenArgs b, int n) {
+    const int i = threadIdx.x;
+    if (i < n) given[i] = b.g[i];
 }
 __global__ __launch_bounds__(256) void adamw_chunks_kernel(const AdamTensor *__restrict__ tab, AdamChunk *__restrict__ chunks,
                                                            int64_t n, int psize, int gsize) {
@@ -545,15 +560,23 @@ __global__ void adamw_fill_kernel(uint32_t *__restrict__ p, int64_t n) {
 
 using namespace snk;
 
+struct Span {   // of addresses
+    uintptr_t lo, hi;
+    bool written;
+};
+
 struct snk_adamw_s {
     snk_adamw_cfg_t cfg{};
     int device = 0;
     bool owned = false, bound = false;
+    bool grads_bound = false;
     bool captured = false;   // a step was captured: only the device knows the count
     AdamStep now{};          // the count until then, without a norm
     std::vector<int64_t> size, start;
     int64_t total = 0, n_chunks = 0;
+    std::vector<Span> written;   // the bound parameters and copies, by address
     DevBuf<AdamTensor> tab;
+    DevBuf<const void *> given;  // the last step's own gradients, if it brought any
     DevBuf<AdamChunk> chunks;
     DevBuf<uint8_t> m, v;
     DevBuf<float> ms, vs;
@@ -645,6 +668,7 @@ snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const s
     h->n_chunks = (int64_t)chunks.size();
     SNK_CHECK(h->n_chunks < (int64_t)1 << 31, SNK_ERR_INVALID, "AdamW: too many elements for one handle");
     h->tab = DevBuf<AdamTensor>(n);
+    h->given = DevBuf<const void *>(n);
     h->chunks = DevBuf<AdamChunk>(chunks.size());
     h->m = DevBuf<uint8_t>(h->state_bytes());
     h->v = DevBuf<uint8_t>(h->state_bytes());
@@ -664,27 +688,26 @@ snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const s
 void adamw_free(snk_adamw h) { delete h; }
 void adamw_set_owned(snk_adamw h) { h->owned = true; }
 
+static Span span_of(const void *p, int64_t size, int32_t dtype, bool written, const char *what, int i) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    SNK_CHECK(a && a % dtype_size(dtype) == 0, SNK_ERR_INVALID, "AdamW: %s %d is NULL or not element-aligned", what, i);
+    return Span{a, a + (uintptr_t)size * dtype_size(dtype), written};
+}
+
 void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void *const *copies, hipStream_t s) {
     const int n = (int)h->size.size();
-    SNK_CHECK(params && grads, SNK_ERR_INVALID, "adamw_bind: NULL argument");
+    SNK_CHECK(params, SNK_ERR_INVALID, "adamw_bind: NULL argument");
     check_not_captured(s, "tensors are bound");
     SNK_CHECK((copies != nullptr) == (h->cfg.copy_dtype >= 0), SNK_ERR_INVALID,
               "adamw_bind: copies go with a copy_dtype, and only with one");
-    struct Span {
-        uintptr_t lo, hi;
-        bool written;
-    };
     std::vector<Span> spans;
     auto add = [&](const void *p, int i, int32_t dtype, bool written, const char *what) {
         if (h->size[i] == 0) return;
-        const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-        SNK_CHECK(a && a % dtype_size(dtype) == 0, SNK_ERR_INVALID, "adamw_bind: %s %d is NULL or not element-aligned",
-                  what, i);
-        spans.push_back(Span{a, a + (uintptr_t)h->size[i] * dtype_size(dtype), written});
+        spans.push_back(span_of(p, h->size[i], dtype, written, what, i));
     };
     for (int i = 0; i < n; ++i) {
         add(params[i], i, h->cfg.param_dtype, true, "parameter");
-        add(grads[i], i, h->cfg.grad_dtype, false, "gradient");
+        if (grads) add(grads[i], i, h->cfg.grad_dtype, false, "gradient");
         if (copies) add(copies[i], i, h->cfg.copy_dtype, true, "copy");
     }
     // a tensor that is written must not overlap any other: the chunks run in no order. Swept by
@@ -702,7 +725,7 @@ void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void
         const int k = std::min(BIND_N, n - at);
         for (int i = 0; i < k; ++i) {
             b.p[i] = params[at + i];
-            b.g[i] = grads[at + i];
+            b.g[i] = grads ? grads[at + i] : nullptr;
             b.c[i] = copies ? copies[at + i] : nullptr;
         }
         adamw_bind_kernel<<<1, BIND_N, 0, s>>>(h->tab + at, b, k);
@@ -713,7 +736,10 @@ void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void
             h->tab, h->chunks, h->n_chunks, dtype_size(h->cfg.param_dtype), dtype_size(h->cfg.grad_dtype));
         launch_check("adamw_chunks_kernel");
     }
+    spans.erase(std::remove_if(spans.begin(), spans.end(), [](const Span &x) { return !x.written; }), spans.end());
+    h->written.swap(spans);
     h->bound = true;
+    h->grads_bound = grads != nullptr;
 }
 
 template <class F>
@@ -726,12 +752,40 @@ static void with_type(int32_t d, F &&f) {
         f(_Float16{});
 }
 
-void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s) {
+// this step's own gradients into their table: one launch for up to GIVEN_N tensors
+static void give_grads(snk_adamw h, int32_t dtype, const void *const *grads, hipStream_t s) {
+    const int n = (int)h->size.size();
+    for (int i = 0; i < n; ++i) {
+        if (h->size[i] == 0) continue;
+        const Span x = span_of(grads[i], h->size[i], dtype, false, "gradient", i);
+        // of the written spans, none of which overlap, the first that ends behind x's start
+        const auto w = std::upper_bound(h->written.begin(), h->written.end(), x.lo,
+                                        [](uintptr_t a, const Span &b) { return a < b.hi; });
+        SNK_CHECK(w == h->written.end() || w->lo >= x.hi, SNK_ERR_INVALID, "AdamW: gradient %d overlaps a parameter or copy", i);
+    }
+    for (int at = 0; at < n; at += GIVEN_N) {
+        GivenArgs b{};
+        const int k = std::min(GIVEN_N, n - at);
+        std::copy(grads + at, grads + at + k, b.g);
+        adamw_given_kernel<<<1, GIVEN_N, 0, s>>>(h->given + at, b, k);
+        launch_check("adamw_given_kernel");
+    }
+}
+
+void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s, int32_t grad_dtype, const void *const *grads) {
     SNK_CHECK(h->bound, SNK_ERR_STATE, "AdamW: no tensors are bound");
+    SNK_CHECK(grads || h->grads_bound, SNK_ERR_STATE, "AdamW: no gradients are bound or given");
     SNK_CHECK(lr >= 0 && lr < INFINITY && std::isfinite(grad_scale), SNK_ERR_INVALID, "AdamW: lr %g, grad_scale %g", lr,
               grad_scale);
     const snk_adamw_cfg_t &c = h->cfg;
     AdamArgs A = h->args();
+    if (grads) {
+        SNK_CHECK(dtype_ok(grad_dtype), SNK_ERR_INVALID, "AdamW: unknown element type");
+        give_grads(h, grad_dtype, grads, s);
+        A.given = h->given;
+    } else {
+        grad_dtype = c.grad_dtype;
+    }
     AdamHyper &H = A.H;
     H.b1d = c.beta1;
     H.b2d = c.beta2;
@@ -751,12 +805,12 @@ void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s) {
         const bool eight = h->n_chunks > 4 * FEW_PARTS;
         const int64_t groups = eight ? (h->n_chunks + 7) / 8 : (h->n_chunks + 3) / 4;
         int parts = (int)std::min<int64_t>(groups, groups <= 2 * FEW_PARTS ? FEW_PARTS : NORM_WG);
-        with_type(c.grad_dtype, [&](auto g) {
+        with_type(grad_dtype, [&](auto g) {
             using GT = decltype(g);
             if (eight)
-                adamw_norm_kernel<GT, 8><<<(unsigned)parts, 512, 0, s>>>(h->chunks, h->n_chunks, h->part, h->ctl, H);
+                adamw_norm_kernel<GT, 8><<<(unsigned)parts, 512, 0, s>>>(h->chunks, h->n_chunks, A.given, h->part, h->ctl, H);
             else
-                adamw_norm_kernel<GT, 4><<<(unsigned)parts, 256, 0, s>>>(h->chunks, h->n_chunks, h->part, h->ctl, H);
+                adamw_norm_kernel<GT, 4><<<(unsigned)parts, 256, 0, s>>>(h->chunks, h->n_chunks, A.given, h->part, h->ctl, H);
         });
         launch_check("adamw_norm_kernel");
         if (parts > FEW_PARTS) {
@@ -783,10 +837,10 @@ void adamw_step(snk_adamw h, float lr, float grad_scale, hipStream_t s) {
         }
     }
     if (h->n_chunks == 0) return;
-    const bool nt = h->total * (dtype_size(c.param_dtype) + dtype_size(c.grad_dtype) + c.state_bits / 4) >= NT_FROM;
+    const bool nt = h->total * (dtype_size(c.param_dtype) + dtype_size(grad_dtype) + c.state_bits / 4) >= NT_FROM;
     for (int64_t at = 0; at < h->n_chunks; at += GRID, A.chunks += GRID) {
         with_type(c.param_dtype, [&](auto p) {
-            with_type(c.grad_dtype, [&](auto g) {
+            with_type(grad_dtype, [&](auto g) {
                 using PT = decltype(p);
                 using GT = decltype(g);
                 const unsigned grid = (unsigned)std::min(GRID, h->n_chunks - at);
@@ -838,6 +892,15 @@ extern "C" int snk_adamw_step(snk_adamw h, float lr, float grad_scale) {
         SNK_CHECK(!h->owned, SNK_ERR_STATE, "the AdamW handle belongs to a model: snk_dqn_apply_grad steps it");
         check_device(h);
         adamw_step(h, lr, grad_scale, stream());
+    });
+}
+
+extern "C" int snk_adamw_step_grads(snk_adamw h, int32_t grad_dtype, const void *const *grads, float lr, float grad_scale) {
+    return guard([&] {
+        SNK_CHECK(h && grads, SNK_ERR_INVALID, "NULL argument");
+        SNK_CHECK(!h->owned, SNK_ERR_STATE, "the AdamW handle belongs to a model: snk_dqn_apply_grad steps it");
+        check_device(h);
+        adamw_step(h, lr, grad_scale, stream(), grad_dtype, grads);
     });
 }
 

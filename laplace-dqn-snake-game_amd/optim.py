@@ -8,6 +8,8 @@ or for hundreds.
 from __future__ import annotations
 
 import ctypes as C
+import operator
+import struct
 
 from . import _lib
 from ._lib import DeviceView, call, f32, i64, vp
@@ -23,11 +25,17 @@ class AdamWCfg(C.Structure):
         super().__init__(C.sizeof(self), *args, **kw)
 
 
+_dtype_of = operator.attrgetter("dtype")
+
+
 def _same(buffers, what):
     kinds = {b.dtype for b in buffers}
     if len(kinds) != 1:
         raise ValueError(f"AdamW: the {what} must share one element type, got {sorted(kinds)}")
-    return _lib.DTYPES[kinds.pop()]
+    kind = kinds.pop()
+    if kind not in _lib.DTYPES:
+        raise ValueError(f"AdamW: {what} of type {kind}")
+    return _lib.DTYPES[kind]
 
 
 class _Handle:
@@ -106,7 +114,8 @@ class _Handle:
 
 
 class AdamW(_Handle):
-    """AdamW(params, grads): params and grads are lists of equal lengths and sizes; they (and
+    """AdamW(params): every step(grads) names its gradients, a list of the parameters' length and sizes,
+    new tensors each time if need be. AdamW(params, grads): step() uses these. params, grads (and
     copies) are kept alive and used at these addresses by every step until bind() names others.
 
     weight_decay: one number, or one per tensor. state_bits: 32, or 8 (codes in blocks of 256 with
@@ -114,7 +123,7 @@ class AdamW(_Handle):
     gradient norm and skips a step whose norm is not finite. copies: 16-bit tensors that receive the
     updated parameters too (fp32 master weights with bf16 working weights)."""
 
-    def __init__(self, params, grads, *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01,
+    def __init__(self, params, grads=None, *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay=0.01,
                  state_bits: int = 32, max_grad_norm: float = 0.0, copies=None, seed: int = 0):
         keep = params, grads, copies = self._lists(params, grads, copies)
         ps, gs, cs = self._buffers(params, grads, copies)
@@ -124,10 +133,11 @@ class AdamW(_Handle):
             raise ValueError(f"AdamW: {len(wd)} weight decays for {n} tensors")
         self.lr, self.state_bits, self._n = float(lr), int(state_bits), n
         self._sizes = [b.size for b in ps]
-        self._types = (_same(ps, "params"), _same(gs, "grads"), _same(cs, "copies") if cs else -1)
-        cfg = AdamWCfg(*self._types, self.state_bits, float(max_grad_norm), float(betas[0]), float(betas[1]), float(eps),
+        self._types = self._types_of(ps, gs, cs)
+        cfg = AdamWCfg(self._types[0], max(self._types[1], 0), self._types[2], self.state_bits, float(max_grad_norm), float(betas[0]), float(betas[1]), float(eps),
                        int(seed), 0)
         self._device = ps[0].device
+        self._pack = struct.Struct(f"={n}Q").pack   # a list of addresses
         h = vp()
         self._call("snk_adamw_create", C.byref(h), n, (i64 * n)(*self._sizes), (f32 * n)(*wd), C.byref(cfg))
         self._h = h
@@ -139,14 +149,18 @@ class AdamW(_Handle):
 
     @staticmethod
     def _buffers(params, grads, copies):
-        lists = [[_lib.device_buffer(x, "AdamW") for x in xs] for xs in (params, grads, copies or [])]
+        lists = [[_lib.device_buffer(x, "AdamW") for x in xs or []] for xs in (params, grads, copies)]
         if not lists[0]:
             raise ValueError("AdamW: no tensors")
-        for other in lists[1:] if copies else lists[1:2]:
-            if [b.size for b in other] != [b.size for b in lists[0]]:
+        for xs, other in ((grads, lists[1]), (copies or None, lists[2])):
+            if xs is not None and [b.size for b in other] != [b.size for b in lists[0]]:
                 raise ValueError("AdamW: params, grads (and copies) need the same sizes")
         _lib.same_device([b for bufs in lists for b in bufs])
         return lists
+
+    @staticmethod
+    def _types_of(ps, gs, cs):   # -1: none
+        return _same(ps, "params"), _same(gs, "grads") if gs else -1, _same(cs, "copies") if cs else -1
 
     def _bind(self, ps, gs, cs, keep):
         n = self._n
@@ -155,21 +169,50 @@ class AdamW(_Handle):
         self._call("snk_adamw_bind", self._h, *table)
         self._keep = keep
 
-    def bind(self, params, grads, copies=None) -> None:
-        """Other addresses for the same tensors (new gradients, moved parameters). Not while a graph is
-        captured; graphs captured before use the new addresses from then on."""
+    def bind(self, params, grads=None, copies=None) -> None:
+        """Other addresses for the same tensors (moved parameters, other kept gradients), given as the
+        constructor's were. Not while a graph is captured; graphs captured before use the new addresses
+        from then on."""
         keep = params, grads, copies = self._lists(params, grads, copies)
         ps, gs, cs = self._buffers(params, grads, copies)
         if [b.size for b in ps] != self._sizes:
             raise ValueError("AdamW.bind: the sizes are those of the constructor")
-        if (_same(ps, "params"), _same(gs, "grads"), _same(cs, "copies") if cs else -1) != self._types:
-            raise ValueError("AdamW.bind: the element types are those of the constructor")
+        if self._types_of(ps, gs, cs) != self._types:
+            raise ValueError("AdamW.bind: the element types, and which lists there are, are those of the constructor")
         self._bind(ps, gs, cs, keep)
 
-    def step(self, *, lr: float | None = None, grad_scale: float = 1.0) -> None:
-        """One step on the bound gradients times grad_scale (the inverse of a loss scale).
-        Enqueued; nothing waits for it."""
-        self._call("snk_adamw_step", self._h, self.lr if lr is None else lr, grad_scale)
+    def step(self, grads=None, *, lr: float | None = None, grad_scale: float = 1.0) -> None:
+        """One step on these gradients, or the bound ones, times grad_scale (the inverse of a loss
+        scale). Enqueued; nothing waits for it. A captured step keeps the gradients' addresses, lr and
+        grad_scale."""
+        lr = self.lr if lr is None else lr
+        if grads is not None:
+            dtype, addresses = self._given(grads if isinstance(grads, (list, tuple)) else list(grads))
+            self._call("snk_adamw_step_grads", self._h, dtype, self._pack(*addresses), lr, grad_scale)
+        elif self._types[1] < 0:
+            raise ValueError("AdamW.step: this handle was made without gradients, and none are given")
+        else:
+            self._call("snk_adamw_step", self._h, lr, grad_scale)
+
+    def _given(self, grads):
+        """(element type, addresses) of a step's own gradients. Torch's are looked at a property at a
+        time, by C loops (a step on 261 tensors: 51 us of host time)."""
+        if self._device is not None:
+            tensor = _lib.torch_module().Tensor
+            try:
+                kinds = set(map(_dtype_of, grads))
+                if len(kinds) == 1 and list(map(tensor.numel, grads)) == self._sizes and \
+                        all(map(tensor.is_contiguous, grads)) and set(map(tensor.get_device, grads)) == {self._device.index}:
+                    kind = _lib.DTYPES.get(_lib.TORCH_TYPES.get(kinds.pop()))
+                    if kind is not None:
+                        return kind, map(tensor.data_ptr, grads)
+            except (AttributeError, TypeError):   # not all of them tensors
+                pass
+        bufs = [_lib.device_buffer(g, "AdamW.step") for g in grads]   # says what is wrong
+        if [b.size for b in bufs] != self._sizes:
+            raise ValueError("AdamW.step: the gradients need the parameters' sizes")
+        _lib.same_device(bufs, self._device)
+        return _same(bufs, "grads"), [b.ptr or 0 for b in bufs]
 
     def __del__(self):
         if getattr(self, "_h", None) and _lib._lib is not None:

@@ -89,3 +89,13 @@ def test_reference_bits_are_the_counter_rng():
     got = adamw_ref.bits16(seed, t, 40)
     for i in (0, 1, 5, 39):
         assert got[i] == (devrng.rng_hash(seed, t, i // 4) >> (16 * (i % 4))) & 0xFFFF
+
+
+def test_gradients_may_come_with_the_step():
+    """AdamW(params) and step(grads): what is wrong with this call is the tensor, not the arguments."""
+    import torch
+    with pytest.raises(ValueError, match="GPU"):
+        snake_amd.AdamW([torch.zeros(4)], lr=1e-3)
+    lib, none = snake_amd.load(), (_lib.vp * 1)(None)
+    assert lib.snk_adamw_step_grads(None, 0, none, 1.0, 1.0) == _lib.SNK_ERR_INVALID
+    assert lib.snk_adamw_step_grads(_lib.vp(4096), 0, None, 1.0, 1.0) == _lib.SNK_ERR_INVALID   # before the handle is read

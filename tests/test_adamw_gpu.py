@@ -548,3 +548,121 @@ def test_large_steps(snk, param, grad, bits, copies, n):
             if k != "norm" and (k != "v" or bits == 32):
                 assert torch.equal(st[k][at:at + x.numel()], x), k
     assert canaries(pb, sizes, 3) and canaries(gb, sizes, 1)
+
+
+# ------------------------------------------------------------------ gradients that come with the step
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("ptype,gtype", [("f32", "f32"), ("f32", "bf16"), ("bf16", "f32"), ("f16", "f16")])
+def test_gradients_with_the_step(snk, bits, ptype, gtype):
+    """New tensors every step, at odd addresses too: the formula, and the bits of bound gradients."""
+    gen = torch.Generator(device="cuda").manual_seed(bits)
+    for max_norm in (0.0, 1.0):
+        pbuf, params = views(SIZES, TT[ptype], gen, 0.1, 1)
+        twins = [p.clone() for p in params]
+        opt = snk.AdamW(params, lr=1e-2, betas=(0.9, 0.99), weight_decay=0.1, state_bits=bits, max_grad_norm=max_norm, seed=99)
+        held = [torch.zeros(s, dtype=TT[gtype], device="cuda") for s in SIZES]
+        twin = snk.AdamW(twins, held, lr=1e-2, betas=(0.9, 0.99), weight_decay=0.1, state_bits=bits, max_grad_norm=max_norm,
+                         seed=99)
+        for t in (1, 2, 3):
+            gbuf, grads = views(SIZES, TT[gtype], gen, 0.02, t % 2)
+            for a, b in zip(held, grads):
+                a.copy_(b)
+            check_step(opt, params, grads, SIZES, [0.1] * len(SIZES), t, lambda: opt.step(grads), ptype=ptype, lr=1e-2, b1=0.9,
+                       b2=0.99, eps=1e-8, max_norm=max_norm, seed=99)
+            twin.step()
+            assert canaries(gbuf, SIZES, t % 2)
+        assert canaries(pbuf, SIZES, 1) and all(torch.equal(a, b) for a, b in zip(params, twins))
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 1.0])
+def test_many_gradients_with_the_step(snk, max_norm):
+    """Over 384 tensors: their addresses take several launches; a generator, scaled, with copies."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    sizes = [(i * 37) % 700 for i in range(800)]
+    _, p = views(sizes, torch.float32, gen, 0.1, 1)
+    _, c = views(sizes, torch.bfloat16, gen, 0.0, 1)
+    opt = snk.AdamW(p, weight_decay=0.01, max_grad_norm=max_norm, copies=c)
+    for t in (1, 2):
+        _, g = views(sizes, torch.float16, gen, 3.0, t)
+        check_step(opt, p, g, sizes, [0.01] * 800, t, lambda: opt.step((x for x in g), lr=1e-2, grad_scale=0.125), ptype="f32",
+                   lr=1e-2, b1=0.9, b2=0.999, eps=1e-8, scale=0.125, max_norm=max_norm, copies=c)
+
+
+def test_bound_gradients_stay(snk):
+    """step(grads), of another type too, leaves what is bound."""
+    p = torch.ones(3000, device="cuda")
+    bound, own = torch.full((3000,), 1.0, device="cuda"), torch.full((3000,), -1.0, device="cuda", dtype=torch.bfloat16)
+    opt = snk.AdamW([p], [bound], lr=0.125, betas=(0.0, 0.0), weight_decay=0.0)
+    for call, want in ((lambda: opt.step(), 0.875), (lambda: opt.step([own]), 1.0), (lambda: opt.step(), 0.875)):
+        call()
+        assert torch.allclose(p, torch.full_like(p, want), rtol=0, atol=1e-6)
+
+
+@pytest.mark.parametrize("max_norm", [0.0, 1.0])
+def test_captured_steps_with_gradients(snk, max_norm):
+    """Two captured steps on gradients of their own, replayed in turn with eager steps on others between."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    p0 = torch.randn(70_001, device="cuda", generator=gen)
+    runs = []
+    for captured in (False, True):
+        gen = torch.Generator(device="cuda").manual_seed(7)
+        p = p0.clone()
+        gs = [torch.zeros_like(p0) for _ in range(2)]
+        opt = snk.AdamW([p], state_bits=8, max_grad_norm=max_norm, seed=1)
+        graphs = []
+        if captured:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            for g in gs:
+                graphs.append(torch.cuda.CUDAGraph())
+                with torch.cuda.graph(graphs[-1], stream=side):
+                    opt.step([g])
+        seen = []
+        for i in range(6):
+            for j, g in enumerate(gs):
+                g.copy_(torch.randn(70_001, device="cuda", generator=gen))
+                graphs[j].replay() if captured else opt.step([g])
+                seen.append(p.clone())
+            if i % 2:
+                opt.step([torch.randn(70_001, device="cuda", generator=gen).bfloat16()])
+                torch.cuda.synchronize()
+        assert opt.steps == 15
+        runs.append(seen)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_gradients_of_device_arrays(snk):
+    rng = np.random.default_rng(0)
+    p0, g0 = rng.standard_normal(5000).astype(np.float32), rng.standard_normal(5000).astype(np.float32)
+    p, t = snk.DeviceArray.from_host(p0), torch.from_numpy(p0).cuda()
+    opt, twin = snk.AdamW([p]), snk.AdamW([t])
+    opt.step([snk.DeviceArray.from_host(g0)])
+    twin.step([torch.from_numpy(g0).cuda()])
+    assert np.array_equal(p.numpy(), t.cpu().numpy())
+
+
+def test_refused_gradients(snk):
+    """Each refused call leaves parameters and count as they were."""
+    x = torch.ones(1000, device="cuda")
+    p, g = [x[:300], x[400:900]], [torch.ones(300, device="cuda"), torch.ones(500, device="cuda")]
+    opt = snk.AdamW(p)
+    for bad, error, word in ((None, ValueError, "without gradients"), (g[:1], ValueError, "sizes"), (g[::-1], ValueError, "sizes"),
+                             ([g[0], None], TypeError, "neither"), ([g[0], g[1].half()], ValueError, "one element type"),
+                             ([a.int() for a in g], ValueError, "i32"), ([a.double() for a in g], ValueError, "float64"),
+                             ([a.cpu() for a in g], ValueError, "GPU"), ([], ValueError, "sizes"),
+                             ([g[0], torch.ones(1000, device="cuda")[::2]], ValueError, "contiguous"),
+                             ([g[0], snk.DeviceArray(500, np.float32)], ValueError, "mix"),
+                             ([g[0], x[:500]], snk.SnakeHipError, "overlaps"), ([x[600:900], g[1]], snk.SnakeHipError, "overlaps"),
+                             ([x[301:601], g[1]], snk.SnakeHipError, "overlaps"), ([x[100:400], g[1]], snk.SnakeHipError, "overlaps")):
+        with pytest.raises(error, match=word):
+            opt.step(bad)
+    with pytest.raises(ValueError, match="constructor"):
+        opt.bind(p, g)
+    assert opt.steps == 0 and bool((x == 1).all())
+    opt.bind(p[:1] + [x[500:1000]])
+    opt.step(g)
+    assert opt.steps == 1 and bool((x[:300] < 1).all()) and bool((x[300:500] == 1).all()) and bool((x[500:] < 1).all())
+    with pytest.raises(snk.SnakeHipError, match="belongs"):
+        held = snk.DQNModel(12, 3, n_frames=2).use_adamw()
+        snk._lib.call("snk_adamw_step_grads", held.handle, 0, (C.c_void_p * 10)(), 0.1, 1.0)
