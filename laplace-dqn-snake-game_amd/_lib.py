@@ -365,25 +365,39 @@ class DeviceArray:
 
 
 class DeviceView:
-    """Device memory that another object owns (and that this view keeps alive). torch.as_tensor
-    reads and writes it in place."""
+    """Device memory of a handle, which this view keeps alive. numpy() and upload() take their place
+    among the handle's own calls: on torch's current stream where its tensors are torch's, on the
+    library's otherwise. torch.as_tensor reads and writes the memory in place, in the order of torch's
+    streams: memory of the library's stream is complete when torch gets it, and later calls on it are
+    the caller's to order (snk_synchronize, torch.cuda.synchronize)."""
 
     def __init__(self, ptr: int, n: int, dtype: str, owner):
-        self.ptr, self.shape, self.dtype, self.owner = vp(ptr), (int(n),), np.dtype(dtype), owner
+        self._ptr, self.shape, self.dtype, self.owner = vp(ptr), (int(n),), np.dtype(dtype), owner
         self.nbytes = int(n) * self.dtype.itemsize
 
     @property
+    def ptr(self) -> vp:
+        if self.owner.handle is None:
+            raise ValueError("the handle that this memory belonged to has ended")
+        return self._ptr
+
+    @property
     def __cuda_array_interface__(self):
-        return {"shape": self.shape, "typestr": self.dtype.str, "data": (self.ptr.value or 0, False), "version": 2}
+        at = self.ptr.value or 0
+        if self.owner.device is None:
+            call("snk_synchronize")
+        return {"shape": self.shape, "typestr": self.dtype.str, "data": (at, False), "version": 2}
 
     def numpy(self) -> np.ndarray:
-        return view_numpy(self.ptr.value, self.shape, self.dtype)
+        out = np.empty(self.shape, self.dtype)
+        call_on(self.owner.device, "snk_memcpy_d2h", ptr(out), self.ptr, self.nbytes)
+        return out
 
     def upload(self, a) -> None:
         a = np.ascontiguousarray(a, self.dtype)
         if a.shape != self.shape:
             raise ValueError(f"upload: {a.shape} into {self.shape}")
-        call("snk_memcpy_h2d", self.ptr, ptr(a), self.nbytes)
+        call_on(self.owner.device, "snk_memcpy_h2d", self.ptr, ptr(a), self.nbytes)
 
 
 class Buffer:

@@ -872,7 +872,7 @@ extern "C" int snk_adamw_destroy(snk_adamw h) {
     return guard([&] {
         if (!h) return;
         SNK_CHECK(!h->owned, SNK_ERR_STATE, "the AdamW handle belongs to a model (snk_dqn_use_adamw)");
-        (void)hipStreamSynchronize(stream());
+        (void)hipDeviceSynchronize();   // its steps may be in flight on any stream
         adamw_free(h);
     });
 }

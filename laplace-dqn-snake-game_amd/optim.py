@@ -49,6 +49,11 @@ class _Handle:
     def handle(self):
         return self._h
 
+    @property
+    def device(self):
+        """Whose current stream the calls run on: the tensors' torch device, None for the library's own."""
+        return self._device
+
     def _call(self, name, *args):
         _lib.call_on(self._device, name, *args)
 

@@ -99,3 +99,49 @@ def test_gradients_may_come_with_the_step():
     lib, none = snake_amd.load(), (_lib.vp * 1)(None)
     assert lib.snk_adamw_step_grads(None, 0, none, 1.0, 1.0) == _lib.SNK_ERR_INVALID
     assert lib.snk_adamw_step_grads(_lib.vp(4096), 0, None, 1.0, 1.0) == _lib.SNK_ERR_INVALID   # before the handle is read
+
+
+class _Owner(snake_amd.ModelAdamW):
+    """A handle without a device: what it calls is recorded."""
+
+    def __init__(self, device):
+        self._h, self._device, self.state_bits, self._n = _lib.vp(4096), device, 32, 1
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    seen = []
+
+    def call_on(device, name, *args):
+        seen.append((device, name))
+        if name == "snk_adamw_state_ptr":
+            args[2]._obj.value, args[3]._obj.value = 8192, 16
+    for module in (_lib, snake_amd.optim):
+        monkeypatch.setattr(module, "call", lambda name, *args: call_on(None, name, *args))
+    monkeypatch.setattr(_lib, "call_on", call_on)
+    return seen
+
+
+def test_state_is_reached_on_the_stream_of_the_steps(calls):
+    """Memory that torch's streams order is read and written on torch's stream, the library's on its own."""
+    for device in ("cuda:0", None):
+        view = _Owner(device).state()["m"]
+        del calls[:]
+        view.numpy()
+        view.upload(np.zeros(4))
+        assert calls == [(device, "snk_memcpy_d2h"), (device, "snk_memcpy_h2d")]
+        del calls[:]
+        assert view.__cuda_array_interface__["data"] == (8192, False)
+        assert calls == ([(None, "snk_synchronize")] if device is None else [])
+
+
+def test_views_of_an_ended_state_are_refused(calls):
+    opt = _Owner(None)
+    view = opt.state()["m"]
+    opt._h = None
+    del calls[:]
+    for use in (view.numpy, lambda: view.upload(np.zeros(4)), lambda: view.__cuda_array_interface__,
+                lambda: _lib.device_buffer(view, "x")):
+        with pytest.raises(ValueError, match="ended"):
+            use()
+    assert not calls

@@ -666,3 +666,35 @@ def test_refused_gradients(snk):
     with pytest.raises(snk.SnakeHipError, match="belongs"):
         held = snk.DQNModel(12, 3, n_frames=2).use_adamw()
         snk._lib.call("snk_adamw_step_grads", held.handle, 0, (C.c_void_p * 10)(), 0.1, 1.0)
+
+
+def test_state_after_a_late_step(snk):
+    """The state is read after a step that is still to run on torch's stream, and written after it too."""
+    p, g = torch.zeros(1000, device="cuda"), torch.zeros(1000, device="cuda")
+    opt = snk.AdamW([p], [g], betas=(0.0, 0.0))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for value in (3.0, 5.0):
+            torch.cuda._sleep(20_000_000)
+            g.fill_(value)
+            opt.step()
+            assert np.all(opt.state()["m"].numpy()[:1000] == value)
+        torch.cuda._sleep(20_000_000)
+        opt.step()
+        opt.state()["m"].upload(np.full(opt.total, 9.0, np.float32))
+        assert np.all(opt.state()["m"].numpy() == 9.0)
+        torch.cuda.current_stream().synchronize()
+
+
+def test_torch_gets_a_model_s_finished_state(snk):
+    model = snk.DQNModel(12, 3, n_frames=2, seed=3)
+    opt = model.use_adamw(lr=1e-3, betas=(0.0, 0.9))
+    model.set_params(np.full(model.P, 0.5, np.float32), snk.SNK_NET_GRAD)
+    for _ in range(50):
+        model.apply_grad()
+    m = torch.as_tensor(opt.state()["m"], device="cuda")
+    assert int((m == 0.5).sum()) == model.P
+    view = opt.state()["m"]
+    model.use_rmsprop()
+    with pytest.raises(ValueError, match="ended"):
+        view.numpy()
