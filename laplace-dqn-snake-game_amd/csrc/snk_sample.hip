@@ -1147,8 +1147,12 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             const bool by_q = s.q > 0.0f && s.p >= 1.0f;
             // (never 0, however low the temperature: the top itself is nearer)
             const float near = by_q ? fmaxf((__builtin_amdgcn_logf(s.q) * -0.69315f + 1e-4f) * (float)s.t, 0x1p-120f) : INFINITY;
-            float edge = near;   // candidates are nearer; NaN for two infinities: top itself
-            auto candidate = [&](float v) __attribute__((always_inline)) { return !(top - v >= edge); };
+            // Candidates are nearer; NaN for two infinities: top itself. Without an edge all that is allowed:
+            // a distance may be infinite in fp32 and yet weigh, where the temperature is as large.
+            float edge = near;
+            auto candidate = [&](float v) __attribute__((always_inline)) {
+                return !(top - v >= edge) || (edge == INFINITY && v != -INFINITY);
+            };
             bool dense = false;   // candidates in most groups
             if (W.hard) {
                 edge = far_edge(0);

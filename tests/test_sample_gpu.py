@@ -476,3 +476,31 @@ def test_threads_at_once(snk):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+@pytest.mark.parametrize("rows", [6, 300, 600])
+@pytest.mark.parametrize("n", [7, 300, 3000, 5000, 20000, 70001])
+def test_distances_past_fp32(snk, rows, n):
+    """Logits 6e38 apart weigh e^-2 of each other at a temperature of 3e38: kept as any others are."""
+    x, u = logits(rows, n, "f32", n)
+    u[:6] = torch.tensor([0.0, 0.3, 0.6, 0.9, 0.99, 0.999], device="cuda")
+    x[:] = -3e38
+    x[:, 0] = 3e38
+    x[1, n // 2] = 3e38
+    x[2, : n // 2] = 1e38
+    x[3, 1:4] = -torch.inf
+    x[4] = torch.linspace(-3.4e38, 3.4e38, n, device="cuda")
+    mask = torch.zeros(n, dtype=torch.bool, device="cuda")
+    mask[n - 1] = True
+    for t in (3e38, 1e38, np.float32(np.inf)):
+        t = np.full(rows, t, np.float32) if np.isinf(t) else float(t)
+        for how in (dict(top_k=5), dict(top_k=1500), dict(min_p=0.1), dict(min_p=1e-5), dict(top_p=0.9), dict(top_k=40, top_p=0.8),
+                    dict()):
+            # equal weights put the limits on whole numbers
+            check(snk, x[:6], u[:6], mask=mask, most_left_out=6, temperature=t[:6] if isinstance(t, np.ndarray) else t, **how)
+            dev = torch.as_tensor(t, device="cuda") if isinstance(t, np.ndarray) else t
+            got = snk.sample_logits(x, u, mask=mask, temperature=dev, **how)
+            few = snk.sample_logits(x[:6], u[:6], mask=mask, temperature=dev[:6] if isinstance(t, np.ndarray) else t, **how)
+            assert (got[:6] != few).sum() <= 1, (t, how)   # whole rows' masses are added in another order
+    got = snk.sample_logits(x[:6], u[:6], temperature=3e38, top_k=5)
+    assert got[5] == 4   # of weights 1 and four e^-2, at 0.999
