@@ -281,7 +281,9 @@ int snk_dqn_act_sample(snk_dqn m, snk_env env, const snk_sample_cfg_t *cfg, uint
  *   v is a uint8 b in 0..255, its value sv (b/255)^4, b one of its two neighbours with the chances
  *   that keep the mean (v changes by 1 - b2 a step, less than half a code: rounding to nearest would
  *   freeze it), at least 1 where v > 0. The 16 random bits of place i in step t are field i % 4 of
- *   the counter RNG's hash of (seed, t, i / 4).
+ *   the counter RNG's hash of (seed, t, i / 4). An infinite or NaN m, whose parameter is NaN then, is
+ *   held as 0 (NaN: with a v of 0 or the first code), and an infinite v as the largest finite number:
+ *   no scale is infinite. A large v makes small ones of its block the first code, and their steps small.
  * The step count lives on the device, so a captured step advances at every replay. A handle's
  * steps are ordered by the caller (one stream, or events), like every handle's. */
 typedef struct snk_adamw_s *snk_adamw;

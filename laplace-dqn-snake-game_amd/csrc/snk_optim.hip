@@ -7,6 +7,7 @@
 // owns 256 consecutive elements (the 8-bit block), a lane four of them: 16-byte accesses, and the
 // block's two scales are one wave reduction each.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstddef>
 #include <cstring>
@@ -443,6 +444,18 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamArgs A) {
     store_params<PT, NT>(T, A.H.copy_dtype, i, whole, p);
     mmax = wave_max_nonneg(mmax);
     vmax = wave_max_nonneg(vmax);
+    if (fmaxf(mmax, vmax) == INFINITY) {   // the whole wave, hardly ever: no scale is infinite
+        mmax = vmax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (fabsf(m[e]) == INFINITY) m[e] = v[e] = 0.0f;   // with it the parameter was lost, and no other is
+            if (v[e] == INFINITY) v[e] = FLT_MAX;              // of a finite gradient: its next steps stay small
+            mmax = fmaxf(mmax, fabsf(m[e]));
+            vmax = fmaxf(vmax, v[e]);
+        }
+        mmax = wave_max_nonneg(mmax);
+        vmax = wave_max_nonneg(vmax);
+    }
     // The codes as correctly rounded quotients and roots give them (the same arithmetic anywhere gives
     // the same codes): by one reciprocal a wave, of a scale in the middle of fp32's range.
     float least[4], dm = mmax, dv = vmax;

@@ -698,3 +698,56 @@ def test_torch_gets_a_model_s_finished_state(snk):
     model.use_rmsprop()
     with pytest.raises(ValueError, match="ended"):
         view.numpy()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_lost_element_is_lost_alone(snk, bad):
+    """Without a norm pass an infinite gradient takes one parameter with it; its block's 255 others, whose
+    8-bit scales it must not reach, move as they do beside a gradient of 0."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    p0, g = torch.randn(2000, device="cuda", generator=gen), torch.randn(2000, device="cuda", generator=gen)
+    at, out = 777, []
+    for value in (0.0, bad):
+        p = p0.clone()
+        opt = snk.AdamW([p], state_bits=8, seed=5)
+        for t in range(4):
+            h = g * (1 + t)
+            h[at] = value if t == 1 else 0.0
+            opt.step([h])
+        st = {k: x.numpy() for k, x in opt.state().items()}
+        assert np.all(np.isfinite(st["m_scale"])) and np.all(np.isfinite(st["v_scale"]))
+        st["m"][at] = st["v"][at] = 0
+        out.append((p, st))
+    assert bool(torch.isnan(out[1][0][at]))
+    rest = torch.arange(2000, device="cuda") != at
+    assert torch.equal(out[0][0][rest], out[1][0][rest])
+    for k in ("m", "v", "m_scale", "v_scale"):
+        assert np.array_equal(out[0][1][k], out[1][1][k]), k
+
+
+@pytest.mark.parametrize("max_norm", [0.0, float("inf")])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_square_past_fp32(snk, bits, max_norm):
+    """A finite gradient whose square is not: the norm lets it pass, nothing becomes infinite or NaN, and the
+    parameter takes no step by a second moment that is out of range. (An 8-bit block's other v
+    become the first code of a very large scale: those parameters stand still, finite.)"""
+    p0 = torch.randn(1000, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    p, g = p0.clone(), torch.full((1000,), 0.5, device="cuda")
+    opt = snk.AdamW([p], [g], lr=1e-2, weight_decay=0.0, state_bits=bits, max_grad_norm=max_norm)
+    for t in range(5):
+        g[300] = 2e19 if t == 1 else -1e-3
+        opt.step()
+        if t == 1:
+            before = p[300].clone()
+        if t > 1:
+            assert torch.equal(p[300], before)   # v / (1 - b2^t) is infinite in these steps
+    assert bool(torch.isfinite(p).all()) and opt.steps == 5
+    far = torch.arange(1000, device="cuda") >= 512          # other blocks
+    q = p0.clone()
+    twin = snk.AdamW([q], [torch.full((1000,), 0.5, device="cuda")], lr=1e-2, weight_decay=0.0, state_bits=bits)
+    for t in range(5):
+        twin.step()
+    assert torch.equal(p[far], q[far])
+    if bits == 8:
+        st = opt.state()
+        assert np.all(np.isfinite(st["m_scale"].numpy())) and np.all(np.isfinite(st["v_scale"].numpy()))
