@@ -1147,15 +1147,19 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
             const bool by_q = s.q > 0.0f && s.p >= 1.0f;
             // (never 0, however low the temperature: the top itself is nearer)
             const float near = by_q ? fmaxf((__builtin_amdgcn_logf(s.q) * -0.69315f + 1e-4f) * (float)s.t, 0x1p-120f) : INFINITY;
-            // Candidates are nearer; NaN for two infinities: top itself. Without an edge all that is allowed:
-            // a distance may be infinite in fp32 and yet weigh, where the temperature is as large.
-            float edge = near;
-            auto candidate = [&](float v) __attribute__((always_inline)) {
-                return !(top - v >= edge) || (edge == INFINITY && v != -INFINITY);
+            // Candidates are nearer to the top; NaN for two infinities: top itself. Without an edge all that is
+            // allowed: a distance may be infinite in fp32 and yet weigh, where the temperature is as large, so
+            // 0 stands for the top then.
+            float edge, from;
+            auto set_edge = [&](float e) __attribute__((always_inline)) {
+                edge = e;
+                from = e < INFINITY ? top : 0.0f;
             };
+            set_edge(near);
+            auto candidate = [&](float v) __attribute__((always_inline)) { return !(from - v >= edge); };
             bool dense = false;   // candidates in most groups
             if (W.hard) {
-                edge = far_edge(0);
+                set_edge(far_edge(0));
             } else if (cut) {
                 // the bin that the wanted-th largest of the counted maxima falls in: at least that many
                 // entries are as near
@@ -1187,7 +1191,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
                     const float t = top_of(g);
                     if (t != -INFINITY) atomicAdd(&count[far_bin(top - t)], 1u);
                 }
-                edge = edge_by_counts();
+                set_edge(edge_by_counts());
                 // Too few groups for that many entries, or so few that their maxima leave more than the
                 // list holds: of A groups, W with a larger maximum, -A ln(1 - W/A) entries are expected.
                 // Then by the maxima of 8, read again: one row of 131,072, top-k 2,000, 39 us against 115 by a
@@ -1207,7 +1211,7 @@ __global__ __launch_bounds__(64 * RW) void sample_row_kernel(SampleArgs A) {
                             if (t != -INFINITY) atomicAdd(&count[far_bin(top - t)], 1u);
                         }
                     }
-                    edge = edge_by_counts();
+                    set_edge(edge_by_counts());
                 }
                 // fewer maxima than wanted entries: everything would be a candidate
                 use_list = all >= wanted || n <= LIST || by_q;
