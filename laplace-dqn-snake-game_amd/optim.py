@@ -170,7 +170,6 @@ class AdamW(_Handle):
     def _bind(self, ps, gs, cs, keep):
         n = self._n
         table = [(vp * n)(*[b.ptr for b in bufs]) if bufs else None for bufs in (ps, gs, cs)]
-        self._device = ps[0].device
         self._call("snk_adamw_bind", self._h, *table)
         self._keep = keep
 
@@ -184,6 +183,7 @@ class AdamW(_Handle):
             raise ValueError("AdamW.bind: the sizes are those of the constructor")
         if self._types_of(ps, gs, cs) != self._types:
             raise ValueError("AdamW.bind: the element types, and which lists there are, are those of the constructor")
+        _lib.same_device(ps, self._device)   # another kind's stream would not wait for the steps
         self._bind(ps, gs, cs, keep)
 
     def step(self, grads=None, *, lr: float | None = None, grad_scale: float = 1.0) -> None:

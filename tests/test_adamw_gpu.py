@@ -751,3 +751,22 @@ def test_a_square_past_fp32(snk, bits, max_norm):
     if bits == 8:
         st = opt.state()
         assert np.all(np.isfinite(st["m_scale"].numpy())) and np.all(np.isfinite(st["v_scale"].numpy()))
+
+
+def test_binding_of_another_kind_is_refused(snk):
+    """A handle's calls stay on one stream: torch tensors and DeviceArrays do not follow one another, and a
+    refused bind changes nothing."""
+    p, g, q = (torch.ones(300, device="cuda") for _ in range(3))
+    a, b = (snk.DeviceArray.from_host(np.ones(300, np.float32)) for _ in range(2))
+    opt, own = snk.AdamW([p], [g]), snk.AdamW([a], [b])
+    with pytest.raises(ValueError, match="mix"):
+        opt.bind([a], [b])
+    with pytest.raises(ValueError, match="mix"):
+        own.bind([q], [g])
+    with pytest.raises(snk.SnakeHipError, match="overlaps"):
+        opt.bind([q], [q])
+    assert opt.device == p.device and own.device is None
+    opt.step()
+    own.step()
+    assert opt.steps == own.steps == 1 and bool((q == 1).all())
+    assert np.array_equal(p.cpu().numpy(), a.numpy()) and bool((p < 1).all())
