@@ -121,7 +121,8 @@ class _Handle:
 class AdamW(_Handle):
     """AdamW(params): every step(grads) names its gradients, a list of the parameters' length and sizes,
     new tensors each time if need be. AdamW(params, grads): step() uses these. params, grads (and
-    copies) are kept alive and used at these addresses by every step until bind() names others.
+    copies) are kept alive and used at these addresses by every step until bind() names others (also where
+    a tensor is given other memory, x.data = y: bind it again then).
 
     weight_decay: one number, or one per tensor. state_bits: 32, or 8 (codes in blocks of 256 with
     two fp32 scales each, v rounded stochastically with `seed`). max_grad_norm > 0 clips the global
@@ -171,7 +172,8 @@ class AdamW(_Handle):
         n = self._n
         table = [(vp * n)(*[b.ptr for b in bufs]) if bufs else None for bufs in (ps, gs, cs)]
         self._call("snk_adamw_bind", self._h, *table)
-        self._keep = keep
+        # aliases: a torch tensor's memory may be exchanged under it (x.data = y)
+        self._keep = [[x.detach() if hasattr(x, "detach") else x for x in xs or ()] for xs in keep]
 
     def bind(self, params, grads=None, copies=None) -> None:
         """Other addresses for the same tensors (moved parameters, other kept gradients), given as the

@@ -770,3 +770,18 @@ def test_binding_of_another_kind_is_refused(snk):
     own.step()
     assert opt.steps == own.steps == 1 and bool((q == 1).all())
     assert np.array_equal(p.cpu().numpy(), a.numpy()) and bool((p < 1).all())
+
+
+def test_exchanged_memory_is_kept(snk):
+    """x.data = y takes a parameter's memory away; the handle's steps go on there and nowhere else."""
+    p, g = torch.nn.Parameter(torch.ones(5000, device="cuda")), torch.ones(5000, device="cuda")
+    old = [p.data_ptr(), g.data_ptr()]
+    opt = snk.AdamW([p], [g], lr=0.125, betas=(0.0, 0.0), weight_decay=0.0)
+    p.data, g.data = (torch.full((5000,), 7.0, device="cuda") for _ in range(2))
+    others = [torch.full((5000,), 7.0, device="cuda") for _ in range(12)]   # would take freed places
+    assert not {x.data_ptr() for x in others + [p, g]} & set(old)
+    opt.step()
+    assert opt.steps == 1 and all(bool((x == 7.0).all()) for x in others + [p, g])
+    opt.bind([p], [g])
+    opt.step()
+    assert torch.allclose(p, torch.full_like(p, 7.0 - 0.125), rtol=0, atol=1e-5)
