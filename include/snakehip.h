@@ -326,12 +326,14 @@ int snk_adamw_layout(snk_adamw h, int64_t *total_out, int64_t *starts_host);
 int snk_adamw_state_ptr(snk_adamw h, int32_t which, void **dev_out, int64_t *bytes_out);
 /* the moments' values in the state layout, rounded to dtype, into two arrays; either may be NULL */
 int snk_adamw_moments(snk_adamw h, int32_t dtype, void *m_dev, void *v_dev);
+/* both wait for the stream; refused while it is being captured */
 int snk_adamw_get_steps(snk_adamw h, int64_t *steps_out);
 int snk_adamw_set_steps(snk_adamw h, int64_t steps);
 /* q_net is updated by AdamW from now on, in place of RMSProp: snk_dqn_apply_grad, snk_dqn_update
  * and every trainer path. The layers' weights decay, their biases do not. cfg: param_dtype and
  * grad_dtype SNK_F32, copy_dtype -1. The model owns the handle (out, optional): it is never
- * passed to snk_adamw_destroy or snk_adamw_bind. cfg = NULL: back to RMSProp and its old state. */
+ * passed to snk_adamw_destroy or snk_adamw_bind. cfg = NULL: back to RMSProp and its old state.
+ * Refused while the stream is being captured. */
 int snk_dqn_use_adamw(snk_dqn m, const snk_adamw_cfg_t *cfg, float lr, float weight_decay, snk_adamw *out);
 
 /* ---------------------------------------------------------------- trainer

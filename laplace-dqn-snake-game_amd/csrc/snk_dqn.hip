@@ -503,6 +503,7 @@ extern "C" int snk_dqn_use_adamw(snk_dqn h, const snk_adamw_cfg_t *cfg, float lr
         SNK_CHECK(h, SNK_ERR_INVALID, "NULL argument");
         snk_adamw fresh = nullptr;
         hipStream_t s = stream();
+        adamw_not_captured(s, "the optimizer is chosen");
         if (cfg) {
             SNK_CHECK(cfg->param_dtype == SNK_F32 && cfg->grad_dtype == SNK_F32 && cfg->copy_dtype == -1, SNK_ERR_INVALID,
                       "use_adamw: the model's parameters and gradient are fp32, without copies");

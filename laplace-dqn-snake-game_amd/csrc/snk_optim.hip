@@ -619,14 +619,15 @@ static void check_device(snk_adamw h) {
               dev);
 }
 
-// what a replay would not do again, and what would leave addresses that no replay has brought yet
-static void check_not_captured(hipStream_t s, const char *what) {
+namespace snk {
+
+// what a replay would not do again, what would leave addresses that no replay has brought yet, and what
+// waits for the stream, which would end the capture
+void adamw_not_captured(hipStream_t s, const char *what) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     SNK_HIP(hipStreamIsCapturing(s, &st));
     SNK_CHECK(st == hipStreamCaptureStatusNone, SNK_ERR_STATE, "AdamW: %s while the stream is being captured", what);
 }
-
-namespace snk {
 
 void adamw_reset(snk_adamw h, hipStream_t s) {
     auto zero = [&](void *p, int64_t bytes) {   // a kernel, not hipMemsetAsync: callers may capture
@@ -661,7 +662,7 @@ snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const s
     SNK_CHECK(cfg->max_grad_norm >= 0, SNK_ERR_INVALID, "AdamW: max_grad_norm %g is negative", cfg->max_grad_norm);
     SNK_CHECK(cfg->reserved == 0, SNK_ERR_INVALID, "AdamW: reserved must be 0");
     hipStream_t s = stream();
-    check_not_captured(s, "a handle is made");
+    adamw_not_captured(s, "a handle is made");
     auto h = std::make_unique<snk_adamw_s>();
     h->cfg = *cfg;
     SNK_HIP(hipGetDevice(&h->device));
@@ -710,7 +711,7 @@ static Span span_of(const void *p, int64_t size, int32_t dtype, bool written, co
 void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void *const *copies, hipStream_t s) {
     const int n = (int)h->size.size();
     SNK_CHECK(params, SNK_ERR_INVALID, "adamw_bind: NULL argument");
-    check_not_captured(s, "tensors are bound");
+    adamw_not_captured(s, "tensors are bound");
     SNK_CHECK((copies != nullptr) == (h->cfg.copy_dtype >= 0), SNK_ERR_INVALID,
               "adamw_bind: copies go with a copy_dtype, and only with one");
     std::vector<Span> spans;
@@ -959,6 +960,7 @@ extern "C" int snk_adamw_get_steps(snk_adamw h, int64_t *steps) {
     return guard([&] {
         SNK_CHECK(h && steps, SNK_ERR_INVALID, "NULL argument");
         check_device(h);
+        adamw_not_captured(stream(), "the step count is read");
         AdamCtl ctl{};
         SNK_HIP(hipMemcpyAsync(&ctl, h->ctl.p, sizeof ctl, hipMemcpyDeviceToHost, stream()));
         SNK_HIP(hipStreamSynchronize(stream()));
@@ -970,6 +972,7 @@ extern "C" int snk_adamw_set_steps(snk_adamw h, int64_t steps) {
     return guard([&] {
         SNK_CHECK(h && steps >= 0, SNK_ERR_INVALID, "bad adamw_set_steps arguments");
         check_device(h);
+        adamw_not_captured(stream(), "the step count is set");
         AdamCtl ctl{};
         ctl.t = steps;
         ctl.c1 = 1.0 - std::pow(h->cfg.beta1, (double)steps);

@@ -4,6 +4,7 @@
 
 namespace snk {
 snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const snk_adamw_cfg_t *cfg);
+void adamw_not_captured(hipStream_t s, const char *what);   // throws where s is being captured
 void adamw_free(snk_adamw h);
 void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void *const *copies, hipStream_t s);
 // grads: this step's own, of type grad_dtype; nullptr: as bound

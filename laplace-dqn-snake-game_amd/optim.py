@@ -98,11 +98,11 @@ class _Handle:
         return out
 
     def reset(self) -> None:
-        """Zero moments, step 0."""
+        """Zero moments, step 0. Not while a graph is captured."""
+        self.steps = 0   # first: refused under a capture, which is to record nothing then
         for name, view in self.state().items():
             if name != "norm" and view.nbytes:
                 self._call("snk_memset", view.ptr, 0, view.nbytes)
-        self.steps = 0
 
     def moments(self, m=None, v=None) -> None:
         """The moments' values, written into m and v: [total] arrays of one type, either may be None,

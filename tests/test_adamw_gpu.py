@@ -785,3 +785,35 @@ def test_exchanged_memory_is_kept(snk):
     opt.bind([p], [g])
     opt.step()
     assert torch.allclose(p, torch.full_like(p, 7.0 - 0.125), rtol=0, atol=1e-5)
+
+
+def test_what_waits_is_refused_under_capture(snk):
+    """Step counts, reset and the choice of a model's optimizer; the capture goes on, with nothing of them in it."""
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = snk.AdamW([p], [g], max_grad_norm=1.0)
+    opt.step()
+    assert opt.steps == 1
+    model = snk.DQNModel(12, 3, n_frames=2, seed=3)
+    held = model.use_adamw(lr=1e-3)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        for use in (lambda: opt.steps, lambda: setattr(opt, "steps", 7), opt.reset):
+            with pytest.raises(snk.SnakeHipError, match="captured"):
+                use()
+        snk._lib.call("snk_set_stream", side.cuda_stream)
+        try:
+            for use in (model.use_rmsprop, model.use_adamw, lambda: held.steps, held.reset):
+                with pytest.raises(snk.SnakeHipError, match="captured"):
+                    use()
+        finally:
+            snk._lib.call("snk_set_stream", None)
+        opt.step()
+    moments = opt.state()["m"].numpy()
+    assert opt.steps == 1 and moments.any()
+    for t in (2, 3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert opt.steps == t and np.all(np.abs(opt.state()["m"].numpy()[:300]) > np.abs(moments[:300]))
+    assert held.steps == 0 and model.adamw is held
+    model.use_rmsprop()
