@@ -465,6 +465,12 @@ def same_device(buffers, device="first") -> None:
             raise ValueError("the tensors of one call live on different devices, or mix DeviceArrays and torch tensors")
 
 
+def written(tensors) -> None:
+    """Autograd is told that a list of torch tensors has changed in place: a graph that saved one says so
+    in its backward pass instead of using the new values. After a call_on for a torch device."""
+    _torch_calls[2](tensors)
+
+
 def call_on(device, name: str, *args) -> None:
     """call(), on torch's current stream of `device` where the tensors are torch's (their memory is
     ordered by it); device None: on the library's stream."""
@@ -474,7 +480,7 @@ def call_on(device, name: str, *args) -> None:
     global _torch_calls
     if _torch_calls is None:
         _torch_calls = _find_torch_calls()   # the same for every thread that gets here
-    current, raw_stream = _torch_calls
+    current, raw_stream, _ = _torch_calls
     index = device.index
     if current() != index:
         raise ValueError(f"the tensors live on {device}, the current device is cuda:{current()}")
@@ -498,12 +504,12 @@ _torch_calls = None
 
 
 def _find_torch_calls():
-    """torch's current device and current stream's handle, without the objects (2.8 us a call) where
-    torch offers them so."""
+    """torch's current device and current stream's handle, without the objects (2.8 us a call), and the
+    change of versions, where torch offers them so."""
     t = torch_module()
     device = getattr(t._C, "_cuda_getDevice", None) or t.cuda.current_device
     stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (lambda i: t.cuda.current_stream(i).cuda_stream)
-    return device, stream
+    return device, stream, getattr(t._C, "_increment_version", None) or t.autograd.graph.increment_version
 
 
 def view_numpy(dev_ptr: int, shape, dtype) -> np.ndarray:

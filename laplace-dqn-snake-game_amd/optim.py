@@ -116,6 +116,8 @@ class _Handle:
                 raise ValueError(f"moments: {b.size} elements for {self.total} places")
         _lib.same_device(given, self._device)   # another kind's stream would not wait for the steps
         self._call("snk_adamw_moments", self._h, _same(given, "moments"), *[None if b is None else b.ptr for b in bufs])
+        if self._device is not None:
+            _lib.written([x for x in (m, v) if x is not None])
 
 
 class AdamW(_Handle):
@@ -174,6 +176,10 @@ class AdamW(_Handle):
         self._call("snk_adamw_bind", self._h, *table)
         # aliases: a torch tensor's memory may be exchanged under it (x.data = y)
         self._keep = [[x.detach() if hasattr(x, "detach") else x for x in xs or ()] for xs in keep]
+        if self._device is not None:
+            # a tensor and its views count their changes together: one of each stands for all
+            self._written = list({id(x if x._base is None else x._base): y
+                                  for i in (0, 2) for x, y in zip(keep[i] or (), self._keep[i])}.values())
 
     def bind(self, params, grads=None, copies=None) -> None:
         """Other addresses for the same tensors (moved parameters, other kept gradients), given as the
@@ -200,6 +206,8 @@ class AdamW(_Handle):
             raise ValueError("AdamW.step: this handle was made without gradients, and none are given")
         else:
             self._call("snk_adamw_step", self._h, lr, grad_scale)
+        if self._device is not None:
+            _lib.written(self._written)
 
     def _given(self, grads):
         """(element type, addresses) of a step's own gradients. Torch's are looked at a property at a

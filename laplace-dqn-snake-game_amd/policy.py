@@ -79,7 +79,8 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
             arrays[i] = _lib.vector_ptr(value, what, kind, rows, device)
             numbers[i] = 0 if kind == "i32" else 1.0
     cfg = _CFG.pack(_CFG.size, dtype, *numbers, *arrays)
-    if out is None:
+    made = out is None
+    if made:
         out = _new(device, rows, np.int32)
     o_ptr = _lib.vector_ptr(out, "out", "i32", rows, device)
     p_ptr = None if prob is None else _lib.vector_ptr(prob, "prob", "f32", rows, device)
@@ -92,6 +93,8 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
         _lib.same_device([wb], device)
         w_ptr, w_bytes = wb.ptr, wb.size
     _lib.call_on(device, "snk_sample_logits", b.ptr, rows, n, ld, m_ptr, ldm, u_ptr, cfg, o_ptr, p_ptr, w_ptr, w_bytes)
+    if device is not None and not (made and prob is None):
+        _lib.written((prob,) if made else (out,) if prob is None else (out, prob))
     return out
 
 

@@ -817,3 +817,33 @@ def test_what_waits_is_refused_under_capture(snk):
         assert opt.steps == t and np.all(np.abs(opt.state()["m"].numpy()[:300]) > np.abs(moments[:300]))
     assert held.steps == 0 and model.adamw is held
     model.use_rmsprop()
+
+
+def test_autograd_sees_the_step(snk):
+    """A graph that saved a parameter before the step refuses its backward pass, as after torch's own."""
+    flat = torch.randn(2000, device="cuda")
+    leaf = torch.nn.Parameter(torch.randn(500, device="cuda"))
+    work = torch.zeros(500, dtype=torch.bfloat16, device="cuda")
+    a, b = flat[:700], flat[1000:]
+    g = [torch.randn(x.numel(), device="cuda") for x in (leaf, a, b)]
+    opt = snk.AdamW([leaf, a, b], g)
+    for how in (lambda: opt.step(), lambda: opt.step(g)):
+        x = torch.randn(500, device="cuda", requires_grad=True)
+        before = [t._version for t in (leaf, a, b, flat)]
+        loss, whole = (x * leaf).sum(), (x * flat[:500]).sum()
+        how()
+        assert all(t._version > v for t, v in zip((leaf, a, b, flat), before))
+        for y in (loss, whole):
+            with pytest.raises(RuntimeError, match="inplace"):
+                y.backward()
+        (x * leaf).sum().backward()       # a graph of after the step is fine
+    copied = snk.AdamW([torch.nn.Parameter(torch.randn(500, device="cuda"))], [g[0]], copies=[work])
+    v = work._version
+    copied.step()
+    assert work._version > v
+    out = torch.empty(opt.total, device="cuda")
+    v = out._version
+    opt.moments(None, out)
+    assert out._version > v
+    with torch.inference_mode():          # tensors that count nothing
+        snk.AdamW([torch.ones(9, device="cuda")], [torch.ones(9, device="cuda")]).step()

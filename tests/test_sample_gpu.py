@@ -504,3 +504,16 @@ def test_distances_past_fp32(snk, rows, n):
             assert (got[:6] != few).sum() <= 1, (t, how)   # whole rows' masses are added in another order
     got = snk.sample_logits(x[:6], u[:6], temperature=3e38, top_k=5)
     assert got[5] == 4   # of weights 1 and four e^-2, at 0.999
+
+
+def test_autograd_sees_the_outputs(snk):
+    """An embedding that saved the drawn indices refuses its backward pass after the next draw into them."""
+    x, u = logits(4, 100, "f32", 0)
+    out, prob = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(4, device="cuda")
+    table = torch.randn(100, 8, device="cuda", requires_grad=True)
+    loss = torch.nn.functional.embedding(out, table).sum()
+    versions = out._version, prob._version
+    snk.sample_logits(x, u, out=out, prob=prob)
+    assert out._version > versions[0] and prob._version > versions[1]
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
