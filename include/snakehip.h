@@ -324,7 +324,8 @@ int snk_adamw_step_grads(snk_adamw h, int32_t grad_dtype, const void *const *gra
 /* places in the state layout; starts_host (optional, n): each tensor's */
 int snk_adamw_layout(snk_adamw h, int64_t *total_out, int64_t *starts_host);
 int snk_adamw_state_ptr(snk_adamw h, int32_t which, void **dev_out, int64_t *bytes_out);
-/* the moments' values in the state layout, rounded to dtype, into two arrays; either may be NULL */
+/* the moments' values in the state layout, rounded to dtype, into two arrays, element-aligned, that do
+ * not overlap; either may be NULL */
 int snk_adamw_moments(snk_adamw h, int32_t dtype, void *m_dev, void *v_dev);
 /* both wait for the stream; refused while it is being captured */
 int snk_adamw_get_steps(snk_adamw h, int64_t *steps_out);

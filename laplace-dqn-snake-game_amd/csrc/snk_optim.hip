@@ -943,7 +943,12 @@ extern "C" int snk_adamw_moments(snk_adamw h, int32_t dtype, void *m_dev, void *
         SNK_CHECK(h && dtype_ok(dtype), SNK_ERR_INVALID, "bad adamw_moments arguments");
         check_device(h);
         if (h->total == 0 || (!m_dev && !v_dev)) return;
-        SNK_CHECK(m_dev != v_dev, SNK_ERR_INVALID, "adamw_moments: both moments into one array");
+        const uintptr_t a = reinterpret_cast<uintptr_t>(m_dev), b = reinterpret_cast<uintptr_t>(v_dev);
+        const uintptr_t bytes = (uintptr_t)h->total * dtype_size(dtype);
+        SNK_CHECK(a % dtype_size(dtype) == 0 && b % dtype_size(dtype) == 0, SNK_ERR_INVALID,
+                  "adamw_moments: an array is not element-aligned");
+        SNK_CHECK(!a || !b || a + bytes <= b || b + bytes <= a, SNK_ERR_INVALID,
+                  "adamw_moments: both moments into one array, or arrays that overlap");
         const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(h->total, 1024), 4096);
         with_type(dtype, [&](auto o) {
             using OT = decltype(o);

@@ -847,3 +847,18 @@ def test_autograd_sees_the_step(snk):
     assert out._version > v
     with torch.inference_mode():          # tensors that count nothing
         snk.AdamW([torch.ones(9, device="cuda")], [torch.ones(9, device="cuda")]).step()
+
+
+def test_moments_into_overlapping_arrays_are_refused(snk):
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = snk.AdamW([p], [g])
+    x = torch.full((2 * opt.total,), 7.0, device="cuda")
+    for a, b in ((0, 1), (opt.total - 1, 0), (5, 5)):
+        with pytest.raises(snk.SnakeHipError, match="overlap"):
+            opt.moments(x[a:a + opt.total], x[b:b + opt.total])
+    for m, v in ((x.data_ptr() + 2, None), (None, x.data_ptr() + 1)):
+        with pytest.raises(snk.SnakeHipError, match="aligned"):
+            snk._lib.call("snk_adamw_moments", opt.handle, 0, m, v)
+    assert bool((x == 7.0).all())
+    opt.moments(x[opt.total:], x[:opt.total])
+    assert not bool(x.any())
