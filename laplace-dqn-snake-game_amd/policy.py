@@ -116,7 +116,10 @@ def softmax_actions(game, model, *, temperature: float = 1.0, top_k: int = 0, to
                     seed: int = 0, act: DeviceArray | None = None) -> np.ndarray:
     """Boltzmann exploration for every env, in epsilon_greedy's place: action indices drawn from
     softmax(Q / temperature) under the filters, with the counter RNG's u(seed, env, step)."""
-    act = act if act is not None else DeviceArray(game.n_envs, np.uint8)
+    if act is not None:
+        _lib.vector_ptr(act, "act", "u8", game.n_envs, None)
+    else:
+        act = DeviceArray(game.n_envs, np.uint8)
     cfg = SampleCfg(_lib.SNK_F32, temperature, top_k, top_p, min_p, None, None, None, None)
     call("snk_dqn_act_sample", model.handle, game.handle, C.byref(cfg), int(seed), act.ptr)
     return act.numpy()

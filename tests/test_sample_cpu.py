@@ -1,5 +1,6 @@
 """The sampler's refusals that need no device, and its reference against counted cases (CPU)."""
 import ctypes as C
+import types
 
 import numpy as np
 import pytest
@@ -59,3 +60,24 @@ def test_reference_on_counted_cases():
     assert sample_ref.row(x, 0.5, temperature=0.0)[:2] == (2, 1.0)
     assert sample_ref.row([-np.inf, np.nan], 0.5, mask=[0, 1])[0] == -1
     assert sample_ref.row([1.0, np.inf, np.inf], 0.6)[:2] == (2, 0.5)
+
+
+def _array(n, dtype):
+    """A DeviceArray without memory: only its description is looked at."""
+    a = object.__new__(snake_amd.DeviceArray)
+    a.shape, a.dtype, a.ptr = (n,), np.dtype(dtype), _lib.vp(0)
+    a.nbytes = n * a.dtype.itemsize
+    return a
+
+
+def test_actions_need_their_room(monkeypatch):
+    """softmax_actions writes a byte an env: an array of another size or type is refused before any call."""
+    def never(*args):
+        raise AssertionError("called")
+    monkeypatch.setattr(snake_amd.policy, "call", never)
+    game = model = types.SimpleNamespace(n_envs=300, handle=None)
+    for act in (_array(299, np.uint8), _array(301, np.uint8), _array(300, np.int32), _array(300, np.float32)):
+        with pytest.raises(ValueError, match="act"):
+            snake_amd.softmax_actions(game, model, act=act)
+    with pytest.raises(TypeError):
+        snake_amd.softmax_actions(game, model, act=np.zeros(300, np.uint8))
