@@ -263,7 +263,7 @@ int snk_sample_logits(const void *logits_dev, int64_t rows, int64_t n, int64_t l
                       float *prob_dev, void *ws_dev, int64_t ws_bytes);
 /* the softmax policy over every env's Q values: act_dev [n] action index, drawn with the counter
  * RNG's u(seed, env, step) as epsilon_greedy draws its own; cfg: dtype SNK_F32, the per-row arrays
- * may be given */
+ * may be given. NaN among an env's Q values: action 0 */
 int snk_dqn_act_sample(snk_dqn m, snk_env env, const snk_sample_cfg_t *cfg, uint64_t seed, uint8_t *act_dev);
 
 /* ---------------------------------------------------------------- AdamW

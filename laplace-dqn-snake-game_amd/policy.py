@@ -71,14 +71,7 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
             ldm = 0
         _lib.same_device([mb], device)
         m_ptr = mb.ptr
-    numbers, arrays = [temperature, top_k, top_p, min_p], _NONE
-    for i, value in enumerate(numbers):
-        if value.__class__ is not float and not isinstance(value, (float, int)):
-            what, kind = _SETTINGS[i]
-            arrays = list(arrays)
-            arrays[i] = _lib.vector_ptr(value, what, kind, rows, device)
-            numbers[i] = 0 if kind == "i32" else 1.0
-    cfg = _CFG.pack(_CFG.size, dtype, *numbers, *arrays)
+    cfg = _cfg(dtype, [temperature, top_k, top_p, min_p], rows, device)
     made = out is None
     if made:
         out = _new(device, rows, np.int32)
@@ -98,6 +91,21 @@ def sample_logits(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     return out
 
 
+def _cfg(dtype, settings, rows, device) -> bytes:
+    """snk_sample_cfg_t of numbers, or of device tensors of a value a row."""
+    arrays = _NONE
+    for i, value in enumerate(settings):
+        if value.__class__ is not float and not isinstance(value, (float, int, np.number)):
+            what, kind = _SETTINGS[i]
+            arrays = list(arrays)
+            arrays[i] = _lib.vector_ptr(value, what, kind, rows, device)
+            settings[i] = 0 if kind == "i32" else 1.0
+    try:
+        return _CFG.pack(_CFG.size, dtype, *settings, *arrays)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"temperature, top_k, top_p, min_p = {settings}: {e}") from None
+
+
 def sample_workspace(rows: int, n: int) -> int:
     """Bytes of workspace that sample_logits uses for rows x n logits (0: none)."""
     need = i64(0)
@@ -112,14 +120,15 @@ def _new(device, n, dtype):
     return torch.empty(n, dtype=torch.int32 if dtype is np.int32 else torch.uint8, device=device)
 
 
-def softmax_actions(game, model, *, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
-                    seed: int = 0, act: DeviceArray | None = None) -> np.ndarray:
+def softmax_actions(game, model, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seed: int = 0,
+                    act: DeviceArray | None = None) -> np.ndarray:
     """Boltzmann exploration for every env, in epsilon_greedy's place: action indices drawn from
-    softmax(Q / temperature) under the filters, with the counter RNG's u(seed, env, step)."""
+    softmax(Q / temperature) under the filters (numbers, or DeviceArrays of a value an env), with the
+    counter RNG's u(seed, env, step). NaN among an env's Q values is action 0."""
     if act is not None:
         _lib.vector_ptr(act, "act", "u8", game.n_envs, None)
     else:
         act = DeviceArray(game.n_envs, np.uint8)
-    cfg = SampleCfg(_lib.SNK_F32, temperature, top_k, top_p, min_p, None, None, None, None)
-    call("snk_dqn_act_sample", model.handle, game.handle, C.byref(cfg), int(seed), act.ptr)
+    cfg = _cfg(_lib.SNK_F32, [temperature, top_k, top_p, min_p], game.n_envs, None)
+    call("snk_dqn_act_sample", model.handle, game.handle, cfg, int(seed), act.ptr)
     return act.numpy()

@@ -7,7 +7,7 @@ import pytest
 
 import sample_ref
 import snake_amd
-from snake_amd import _lib
+from snake_amd import _lib, policy
 from snake_amd.policy import SampleCfg
 
 ONE = 4096   # an address that is never read: every call below is refused before a launch
@@ -81,3 +81,36 @@ def test_actions_need_their_room(monkeypatch):
             snake_amd.softmax_actions(game, model, act=act)
     with pytest.raises(TypeError):
         snake_amd.softmax_actions(game, model, act=np.zeros(300, np.uint8))
+
+
+def test_settings_are_numbers_of_any_kind():
+    """numpy's scalars are numbers; one that the library's types cannot hold is refused, not cut off."""
+    want = policy._cfg(0, [0.5, 7, 0.75, 0.25], 3, None)
+    assert want == bytes(SampleCfg(0, 0.5, 7, 0.75, 0.25, None, None, None, None))
+    assert want == policy._cfg(0, [np.float32(0.5), np.int64(7), np.float64(0.75), np.float16(0.25)], 3, None)
+    for bad in ([1.0, 2 ** 32 + 5, 1.0, 0.0], [1.0, -2 ** 31 - 1, 1.0, 0.0], [1.0, 5.5, 1.0, 0.0], [1e39, 0, 1.0, 0.0]):
+        with pytest.raises(ValueError, match="temperature, top_k"):
+            policy._cfg(0, bad, 3, None)
+
+
+def test_actions_take_settings_of_each_env(monkeypatch):
+    seen = []
+    monkeypatch.setattr(policy, "call", lambda name, *args: seen.append((name, args)))
+    game = model = types.SimpleNamespace(n_envs=300, handle=None)
+    act = _array(300, np.uint8)
+    act.numpy = lambda: None
+    t = _array(300, np.float32)
+    t.ptr = _lib.vp(8192)
+    try:
+        snake_amd.softmax_actions(game, model, temperature=t, top_k=2, act=act, seed=9)
+        with pytest.raises(ValueError, match="top_k"):
+            snake_amd.softmax_actions(game, model, top_k=t, act=act)
+        with pytest.raises(ValueError, match="300"):
+            snake_amd.softmax_actions(game, model, temperature=_array(299, np.float32), act=act)
+        with pytest.raises(ValueError, match="top_k"):
+            snake_amd.softmax_actions(game, model, top_k=2 ** 32 + 1, act=act)
+    finally:
+        t.ptr = None
+    (name, args), = seen
+    assert name == "snk_dqn_act_sample" and args[3] == 9
+    assert args[2] == bytes(SampleCfg(0, 1.0, 2, 1.0, 0.0, 8192, None, None, None))

@@ -517,3 +517,22 @@ def test_autograd_sees_the_outputs(snk):
     assert out._version > versions[0] and prob._version > versions[1]
     with pytest.raises(RuntimeError, match="inplace"):
         loss.backward()
+
+
+def test_softmax_actions_with_settings_of_each_env(snk):
+    n, seed = 200, 31
+    rng = np.random.default_rng(2)
+    game = snk.SnakeGame(12, 2, n_envs=n, autoreset=True)
+    model = snk.DQNModel(12, 3, n_frames=2, seed=4)
+    how = dict(temperature=rng.uniform(0.0, 0.2, n).astype(np.float32), top_k=rng.integers(0, 4, n).astype(np.int32),
+               top_p=rng.uniform(0.3, 1, n).astype(np.float32), min_p=rng.uniform(0, 0.5, n).astype(np.float32))
+    q = model.q_env(game)
+    for keys in (list(how), ["temperature"], ["top_k", "min_p"]):
+        dev = {k: snk.DeviceArray.from_host(how[k]) for k in keys}
+        got = snk.softmax_actions(game, model, seed=seed, **dev)
+        for e in range(n):
+            u = devrng.rng_uniform(devrng.rng_hash(seed, e, 0))
+            want, _, margin = sample_ref.row(q[e], u, **{k: how[k][e] for k in keys})
+            assert margin < 1e-9 or got[e] == want
+    model.set_params(np.full(model.P, np.nan, np.float32))
+    assert not snk.softmax_actions(game, model, seed=seed).any()
