@@ -240,4 +240,9 @@ class ModelAdamW(_Handle):
     update step it; use_rmsprop or another use_adamw ends it, and its state()'s memory with it."""
 
     def __init__(self, model, handle, lr, state_bits, n):
-        self._model, self._h, self.lr, self.state_bits, self._n = model, handle, float(lr), int(state_bits), int(n)
+        self._model, self._h, self._lr, self.state_bits, self._n = model, handle, float(lr), int(state_bits), int(n)
+
+    @property
+    def lr(self) -> float:
+        """use_adamw's: another one takes another use_adamw."""
+        return self._lr

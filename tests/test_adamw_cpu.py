@@ -145,3 +145,11 @@ def test_views_of_an_ended_state_are_refused(calls):
         with pytest.raises(ValueError, match="ended"):
             use()
     assert not calls
+
+
+def test_a_model_s_rate_is_use_adamw_s():
+    """Assigning would change nothing: the model holds the rate."""
+    opt = snake_amd.ModelAdamW(None, _lib.vp(4096), 1e-3, 32, 10)
+    assert opt.lr == 1e-3
+    with pytest.raises(AttributeError):
+        opt.lr = 1e-4
