@@ -240,8 +240,13 @@ int snk_dqn_update(snk_dqn m, snk_replay rb, const int64_t *idx_dev, int64_t B, 
  * a row (outside, or NaN: the nearest end). temperature <= 0: the first entry of the order, with
  * probability 1. No allowed entry: index -1, probability 0. An allowed NaN: -1 and NaN. Infinite
  * entries share all the mass. What masked places hold does not matter.
- * Weights and sums are held in 64 bits. An entry lighter than half a unit, 2^-(61 - ceil log2 n) of
- * the largest weight but no finer than 2^-51, is never drawn. Equal calls give equal answers. */
+ * A weight is e^x to 4e-12 of itself, in 64 bits; it is then rounded to whole units of 2^-s of the
+ * row's largest weight, s = min(51, 61 - ceil log2 n), so that sums are exact in any order: an entry
+ * is off by up to half a unit, one lighter than that is never drawn, and S, and with it prob and top_p's
+ * limit, is off by up to n / 2 units (2^-42 of the largest weight for 1,024 entries, 2^-30 for 65,536,
+ * 2^-14 for 2^24). Rows of more than 4,096 entries under no filter add unrounded weights instead, to
+ * 1e-11 of S. Equal calls give equal answers; a row in a call of more or fewer rows may be added in
+ * another order and answer otherwise where u S is that near to the border of two entries. */
 typedef struct {
     int32_t struct_size;   /* = sizeof(snk_sample_cfg_t) = 56 */
     int32_t dtype;         /* of the logits: SNK_F32 / SNK_BF16 / SNK_F16 */

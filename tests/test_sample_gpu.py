@@ -536,3 +536,38 @@ def test_softmax_actions_with_settings_of_each_env(snk):
             assert margin < 1e-9 or got[e] == want
     model.set_params(np.full(model.P, np.nan, np.float32))
     assert not snk.softmax_actions(game, model, seed=seed).any()
+
+
+@pytest.mark.parametrize("n", [5, 900, 3000, 70001, 1 << 22])
+@pytest.mark.parametrize("units", [0.4, 0.6, 1.5, 2.45])
+def test_stated_accuracy(snk, n, units):
+    """One entry that holds nearly all and many of about a unit, where rounding to units shows most: sums,
+    probabilities and answers are within the header's bounds. Each entry is off by half a unit and 4e-12 of
+    itself, so S by n / 2 units and 4e-12 S; the probability's quotient by the two and fp32's half a step;
+    the sum up to the answer, and u S, by S's error each."""
+    s = min(51, 61 - int(np.ceil(np.log2(n))))
+    x = torch.full((1, n), float(np.log(units) - s * np.log(2)), device="cuda")
+    x[0, n // 3] = 0.0
+    w = np.exp(x[0].double().cpu().numpy())
+    upto = np.cumsum(w)          # in order: off by n 2^-53 S at most
+    S = upto[-1]
+    wild = n / 2 * 2.0 ** -s + (4e-12 + n * 2.0 ** -53) * S
+    plain = n > 4096             # unrounded sums without a filter
+    prob = torch.empty(1, device="cuda")
+    for how in (dict(), dict(top_k=n - 1), dict(min_p=1e-30), dict(top_p=0.99999994)):
+        # (entries that are never drawn count in unrounded sums: the answer is off by their mass there)
+        error = (1e-11 + n * 2.0 ** -53) * S if plain and not how and units >= 0.5 else wild
+        # of the small ones, top-p may drop those of the highest indices: a mass of 1 - p, one entry, and the
+        # errors of its limit and of what stays
+        low = S * (1 - float(np.float32(0.99999994))) + w[0] + 2 * error if "top_p" in how else 0.0
+        for u in (0.0, 0.25, 0.5, 0.999, 0.99999, 0.99999994):
+            uu = torch.tensor([u], device="cuda")
+            i = int(snk.sample_logits(x, uu, prob=prob, **how)[0])
+            t = float(uu[0]) * S
+            if "top_k" in how:   # all but the last of the small ones
+                t -= float(uu[0]) * w[-1]
+            assert 0 <= i < n and w[i] >= 0.5 * 2.0 ** -s * (1 - 1e-9)
+            assert upto[i] > t - low - 2 * error and upto[i] - w[i] <= t + low + 2 * error, (how, u, i)
+            kept = S - (w[-1] if "top_k" in how else 0.0) - low
+            p = float(prob[0])
+            assert w[i] / (S + error) * (1 - 2.0 ** -24 - 4e-12) <= p <= w[i] / (kept - error) * (1 + 2.0 ** -24 + 4e-12), (how, u)
