@@ -277,7 +277,8 @@ int snk_dqn_act_sample(snk_dqn m, snk_env env, const snk_sample_cfg_t *cfg, uint
  *   N = sqrt(sum (s g)^2) over all tensors, c = max_grad_norm / N when N is larger, else 1
  *   g' = s c g;  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
  *   p = p - lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + weight_decay p)
- * computed in fp32 (the norm in fp64), p rounded to its type once.
+ * computed in fp32 (the norm in fp64; with 8-bit states the root and the quotient by the hardware's, an
+ * ulp each), p rounded to its type once.
  *
  * State layout: every tensor starts on a multiple of 256 elements, in list order (its start is
  * snk_adamw_layout's); the places between tensors hold zeros. state_bits 32: m and v are floats.

@@ -862,3 +862,45 @@ def test_moments_into_overlapping_arrays_are_refused(snk):
     assert bool((x == 7.0).all())
     opt.moments(x[opt.total:], x[:opt.total])
     assert not bool(x.any())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("max_norm", [0.0, 1.0])
+def test_nothing_to_step(snk, bits, max_norm):
+    """Tensors without elements: steps are counted, the state is empty."""
+    p, g = ([torch.empty(0, device="cuda"), torch.empty(3, 0, device="cuda")] for _ in range(2))
+    opt = snk.AdamW(p, g, state_bits=bits, max_grad_norm=max_norm)
+    opt.step()
+    opt.step([x.bfloat16() for x in g])
+    assert opt.steps == 2 and opt.total == 0 and opt.starts == [0, 0]
+    assert all(x.numpy().size == (k == "norm") for k, x in opt.state().items())
+    assert torch.as_tensor(opt.state()["m"], device="cuda").numel() == 0
+    opt.moments(torch.empty(0, device="cuda"))
+    opt.reset()
+    assert opt.steps == 0
+
+
+def test_a_loop_over_a_module(snk):
+    """As a training loop uses it: autograd's own gradients, new ones every iteration, of parameters of any
+    shape, on a side stream; the updates are the formula's, whatever the gradients' places."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    net = torch.nn.Sequential(torch.nn.Linear(40, 33), torch.nn.Tanh(), torch.nn.Linear(33, 7)).cuda()
+    params = list(net.parameters())
+    sizes = [p.numel() for p in params]
+    opt = snk.AdamW(params, lr=1e-2, weight_decay=[0.1 if p.dim() > 1 else 0.0 for p in params], max_grad_norm=0.5)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    kept = []
+    with torch.cuda.stream(side):
+        for t in range(1, 5):
+            for p in params:
+                p.grad = None
+            x = torch.randn(16, 40, device="cuda", generator=gen)
+            (net(x) ** 2).sum().backward()
+            grads = [p.grad for p in params]
+            kept.append(torch.empty(sizes[0], device="cuda"))   # takes the place of a gradient that was freed
+            check_step(opt, [p.detach() for p in params], grads, sizes, [0.1, 0.0, 0.1, 0.0], t, lambda: opt.step(grads),
+                       ptype="f32", lr=1e-2, b1=0.9, b2=0.999, eps=1e-8, max_norm=0.5)
+            del grads
+        side.synchronize()
+    torch.cuda.current_stream().wait_stream(side)
