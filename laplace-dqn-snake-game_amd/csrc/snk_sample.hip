@@ -140,7 +140,7 @@ __device__ const uint64_t POW2[128] = {
     0x3fefd0765b6e4540ull, 0x3fefdbfdad9cbe14ull, 0x3fefe7c1819e90d8ull, 0x3feff3c22b8f71f1ull,
 };
 
-// e^((x - top) / T) to 3e-12: a u that falls between the sums of two evaluations that near is a one in
+// e^((x - top) / T) by a table and a short polynomial (Tang 1989), to 3e-12: a u that falls between the sums of two evaluations that near is a one in
 // 10^5 event over a row of 10^5 entries. 2^(i + j/128 + f/128), |f| <= 1/2: a table in LDS, a cubic,
 // and the exponent added to the table's: 15 instructions, a quarter of the library's exp. Entries
 // behind 2^-1000 (-inf too) weigh that much: callers leave excluded ones out themselves.

@@ -200,6 +200,8 @@ class AdamW(_Handle):
         grad_scale."""
         lr = self.lr if lr is None else lr
         if grads is not None:
+            if hasattr(grads, "data_ptr"):   # it would be taken apart
+                raise TypeError("AdamW.step: a list of gradients, not a tensor")
             dtype, addresses = self._given(grads if isinstance(grads, (list, tuple)) else list(grads))
             self._call("snk_adamw_step_grads", self._h, dtype, self._pack(*addresses), lr, grad_scale)
         elif self._types[1] < 0:

@@ -647,7 +647,7 @@ def test_refused_gradients(snk):
     x = torch.ones(1000, device="cuda")
     p, g = [x[:300], x[400:900]], [torch.ones(300, device="cuda"), torch.ones(500, device="cuda")]
     opt = snk.AdamW(p)
-    for bad, error, word in ((None, ValueError, "without gradients"), (g[:1], ValueError, "sizes"), (g[::-1], ValueError, "sizes"),
+    for bad, error, word in ((None, ValueError, "without gradients"), (g[0], TypeError, "a list"), (0.1, TypeError, "iterable"), (g[:1], ValueError, "sizes"), (g[::-1], ValueError, "sizes"),
                              ([g[0], None], TypeError, "neither"), ([g[0], g[1].half()], ValueError, "one element type"),
                              ([a.int() for a in g], ValueError, "i32"), ([a.double() for a in g], ValueError, "float64"),
                              ([a.cpu() for a in g], ValueError, "GPU"), ([], ValueError, "sizes"),
