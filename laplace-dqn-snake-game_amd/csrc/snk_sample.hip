@@ -1904,7 +1904,7 @@ static void sample_launch_t(SampleArgs A, uint8_t *ws, hipStream_t s) {
     // a top-k that the groups' maxima bound, so that its candidates are few: 8 rows of 4,096, top-k 40,
     // 11 us against 15, with top-p 0.9 11 against 17. Not for more rows, which that path scans into a
     // workspace: rows of up to 4,096 entries need none. It costs them time (4,096 rows of 4,096 bf16, top-k
-    // 40, 68 us here, rows of 8,192 by the maxima 52; 65,536 rows 976 and 808).
+    // 40, 68 us here, rows of 8,192 by the maxima 52; 65,536 rows 980 and 815).
     const bool by_groups = !many && A.n > 2048 && !A.k_dev && A.top_k > 0 && A.top_k <= A.n / GROUP;
     if (A.n <= WAVE_N && !by_groups) {
         for (; A.row0 < A.rows; A.row0 += GRID) {
