@@ -318,14 +318,16 @@ int snk_adamw_create(snk_adamw *out, int32_t n, const int64_t *sizes_host, const
                      const snk_adamw_cfg_t *cfg);
 int snk_adamw_destroy(snk_adamw h);
 /* the tensors' device addresses, contiguous, element-aligned: params (updated), grads (NULL: every
- * step brings its own, snk_adamw_step_grads), and copies (NULL unless copy_dtype >= 0). Refused where a tensor that is written overlaps another one.
- * Enqueued like any work, and kept: later steps (an earlier captured one's replays too) use the last
- * bind. Refused, as snk_adamw_create is, while the stream is being captured. */
+ * step brings its own, snk_adamw_step_grads; not once they were bound), and copies (NULL unless
+ * copy_dtype >= 0). Refused where a tensor that is written overlaps another one. Enqueued like any
+ * work, and kept: later steps (an earlier captured one's replays too) use the last bind. Refused, as
+ * snk_adamw_create is, while the stream is being captured. */
 int snk_adamw_bind(snk_adamw h, void *const *params_dev, const void *const *grads_dev, void *const *copies_dev);
 int snk_adamw_step(snk_adamw h, float lr, float grad_scale);
 /* the same step on these gradients of grad_dtype, whatever is bound, which stays: n device addresses,
  * read by the host during the call (a captured step keeps them, as it does lr and grad_scale).
- * Refused where one overlaps a parameter or copy. */
+ * Refused where one overlaps a parameter or copy as bound now: what is bound later has to lie apart
+ * from a captured step's gradients too. */
 int snk_adamw_step_grads(snk_adamw h, int32_t grad_dtype, const void *const *grads_dev, float lr, float grad_scale);
 /* places in the state layout; starts_host (optional, n): each tensor's */
 int snk_adamw_layout(snk_adamw h, int64_t *total_out, int64_t *starts_host);

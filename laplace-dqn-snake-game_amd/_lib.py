@@ -417,7 +417,7 @@ def torch_module():
     if _torch is None:
         import torch
         TORCH_TYPES.update({torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16", torch.int32: "i32",
-                             torch.uint8: "u8", torch.bool: "u8"})
+                            torch.uint8: "u8", torch.bool: "u8"})
         _torch = torch
     return _torch
 

@@ -569,14 +569,14 @@ __global__ void adamw_fill_kernel(uint32_t *__restrict__ p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) p[i] = 0;
 }
 
-}  // namespace snk
-
-using namespace snk;
-
-struct Span {   // of addresses
+struct AdamSpan {   // of addresses
     uintptr_t lo, hi;
     bool written;
 };
+
+}  // namespace snk
+
+using namespace snk;
 
 struct snk_adamw_s {
     snk_adamw_cfg_t cfg{};
@@ -587,7 +587,7 @@ struct snk_adamw_s {
     AdamStep now{};          // the count until then, without a norm
     std::vector<int64_t> size, start, first_chunk;
     int64_t total = 0, n_chunks = 0;
-    std::vector<Span> written;   // the bound parameters and copies, by address
+    std::vector<AdamSpan> written;   // the bound parameters and copies, by address
     DevBuf<AdamTensor> tab;
     DevBuf<const void *> bound_grads, given_grads;   // each chunk's: as bound, of the last step that brought its own
     DevBuf<AdamChunk> chunks;
@@ -705,19 +705,21 @@ snk_adamw adamw_create(int32_t n, const int64_t *sizes, const float *wd, const s
 void adamw_free(snk_adamw h) { delete h; }
 void adamw_set_owned(snk_adamw h) { h->owned = true; }
 
-static Span span_of(const void *p, int64_t size, int32_t dtype, bool written, const char *what, int i) {
+static AdamSpan span_of(const void *p, int64_t size, int32_t dtype, bool written, const char *what, int i) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p);
     SNK_CHECK(a && a % dtype_size(dtype) == 0, SNK_ERR_INVALID, "AdamW: %s %d is NULL or not element-aligned", what, i);
-    return Span{a, a + (uintptr_t)size * dtype_size(dtype), written};
+    return AdamSpan{a, a + (uintptr_t)size * dtype_size(dtype), written};
 }
 
 void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void *const *copies, hipStream_t s) {
     const int n = (int)h->size.size();
     SNK_CHECK(params, SNK_ERR_INVALID, "adamw_bind: NULL argument");
     adamw_not_captured(s, "tensors are bound");
+    SNK_CHECK(grads || !h->grads_bound, SNK_ERR_STATE,
+              "adamw_bind: this handle's gradients are bound, and captured steps may read them: bind others");
     SNK_CHECK((copies != nullptr) == (h->cfg.copy_dtype >= 0), SNK_ERR_INVALID,
               "adamw_bind: copies go with a copy_dtype, and only with one");
-    std::vector<Span> spans;
+    std::vector<AdamSpan> spans;
     auto add = [&](const void *p, int i, int32_t dtype, bool written, const char *what) {
         if (h->size[i] == 0) return;
         spans.push_back(span_of(p, h->size[i], dtype, written, what, i));
@@ -729,9 +731,9 @@ void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void
     }
     // a tensor that is written must not overlap any other: the chunks run in no order. Swept by
     // address with the furthest end seen of all spans and of the written ones
-    std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.lo < b.lo; });
+    std::sort(spans.begin(), spans.end(), [](const AdamSpan &a, const AdamSpan &b) { return a.lo < b.lo; });
     uintptr_t end = 0, end_written = 0;
-    for (const Span &x : spans) {
+    for (const AdamSpan &x : spans) {
         SNK_CHECK(x.lo >= end_written && !(x.written && x.lo < end), SNK_ERR_INVALID,
                   "adamw_bind: a parameter or copy overlaps another tensor");
         end = std::max(end, x.hi);
@@ -753,7 +755,7 @@ void adamw_bind(snk_adamw h, void *const *params, const void *const *grads, void
             h->tab, h->chunks, h->bound_grads, h->n_chunks, dtype_size(h->cfg.param_dtype), dtype_size(h->cfg.grad_dtype));
         launch_check("adamw_chunks_kernel");
     }
-    spans.erase(std::remove_if(spans.begin(), spans.end(), [](const Span &x) { return !x.written; }), spans.end());
+    spans.erase(std::remove_if(spans.begin(), spans.end(), [](const AdamSpan &x) { return !x.written; }), spans.end());
     h->written.swap(spans);
     h->bound = true;
     h->grads_bound = grads != nullptr;
@@ -774,10 +776,10 @@ static void give_grads(snk_adamw h, int32_t dtype, const void *const *grads, hip
     const int n = (int)h->size.size();
     for (int i = 0; i < n; ++i) {
         if (h->size[i] == 0) continue;
-        const Span x = span_of(grads[i], h->size[i], dtype, false, "gradient", i);
+        const AdamSpan x = span_of(grads[i], h->size[i], dtype, false, "gradient", i);
         // of the written spans, none of which overlap, the first that ends behind x's start
         const auto w = std::upper_bound(h->written.begin(), h->written.end(), x.lo,
-                                        [](uintptr_t a, const Span &b) { return a < b.hi; });
+                                        [](uintptr_t a, const AdamSpan &b) { return a < b.hi; });
         SNK_CHECK(w == h->written.end() || w->lo >= x.hi, SNK_ERR_INVALID, "AdamW: gradient %d overlaps a parameter or copy", i);
     }
     for (int at = 0; at < n; at += GIVEN_N) {

@@ -142,8 +142,9 @@ class AdamW(_Handle):
         self.lr, self.state_bits, self._n = float(lr), int(state_bits), n
         self._sizes = [b.size for b in ps]
         self._types = self._types_of(ps, gs, cs)
-        cfg = AdamWCfg(self._types[0], max(self._types[1], 0), self._types[2], self.state_bits, float(max_grad_norm), float(betas[0]), float(betas[1]), float(eps),
-                       int(seed), 0)
+        ptype, gtype, ctype = self._types
+        cfg = AdamWCfg(ptype, max(gtype, 0), ctype, self.state_bits, float(max_grad_norm), float(betas[0]), float(betas[1]),
+                       float(eps), int(seed), 0)
         self._device = ps[0].device
         self._pack = struct.Struct(f"={n}Q").pack   # a list of addresses
         h = vp()
@@ -178,8 +179,8 @@ class AdamW(_Handle):
         self._keep = [[x.detach() if hasattr(x, "detach") else x for x in xs or ()] for xs in keep]
         if self._device is not None:
             # a tensor and its views count their changes together: one of each stands for all
-            self._written = list({id(x if x._base is None else x._base): y
-                                  for i in (0, 2) for x, y in zip(keep[i] or (), self._keep[i])}.values())
+            whole = [(x if x._base is None else x._base, y) for i in (0, 2) for x, y in zip(keep[i] or (), self._keep[i])]
+            self._written = list({id(x): y for x, y in whole}.values())
 
     def bind(self, params, grads=None, copies=None) -> None:
         """Other addresses for the same tensors (moved parameters, other kept gradients), given as the
@@ -197,7 +198,7 @@ class AdamW(_Handle):
     def step(self, grads=None, *, lr: float | None = None, grad_scale: float = 1.0) -> None:
         """One step on these gradients, or the bound ones, times grad_scale (the inverse of a loss
         scale). Enqueued; nothing waits for it. A captured step keeps the gradients' addresses, lr and
-        grad_scale."""
+        grad_scale, and needs this handle and the gradients as long as its graph is replayed."""
         lr = self.lr if lr is None else lr
         if grads is not None:
             if hasattr(grads, "data_ptr"):   # it would be taken apart

@@ -904,3 +904,18 @@ def test_a_loop_over_a_module(snk):
             del grads
         side.synchronize()
     torch.cuda.current_stream().wait_stream(side)
+
+
+def test_bound_gradients_are_not_unbound(snk):
+    """A captured step would read at no address."""
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = snk.AdamW([p], [g])
+    where = (C.c_void_p * 1)(p.data_ptr())
+    with pytest.raises(snk.SnakeHipError, match="are bound"):
+        snk._lib.call("snk_adamw_bind", opt.handle, where, None, None)
+    opt.step()
+    assert opt.steps == 1 and bool((p < 1).all())
+    own = snk.AdamW([g])
+    snk._lib.call("snk_adamw_bind", own.handle, (C.c_void_p * 1)(g.data_ptr()), None, None)
+    with pytest.raises(snk.SnakeHipError, match="no gradients"):
+        snk._lib.call("snk_adamw_step", own.handle, 0.1, 1.0)
